@@ -153,6 +153,14 @@ SIGNATURES = {
     "ahip_op_sample": (i, [vp, fp, i, C.c_float, i, C.c_float, C.c_double, ip]),
     "ahip_session_sample": (i, [vp, C.c_float, i, C.c_float, C.c_double, ip]),
     "ahip_attention_decode_noalloc": (i, [vp, vp, vp, vp, i, i, i, i, i, i, vp, vp]),
+    "ahip_kv_q4_bytes": (i, [i, i, i, i64p]),
+    "ahip_kv_q4_store": (i, [vp, i, vp, i64, vp, i64, i, i, vp, vp, vp, i, i, i, vp]),
+    "ahip_kv_q4_load": (i, [vp, i, vp, vp, i, i, i, i, i, vp, i64, vp, i64, vp]),
+    "ahip_attention_q4_workspace": (i, [vp, i, i, i, i, i, i, i, i64p]),
+    "ahip_attention_q4": (i, [vp, i, vp, i64, i, i, i, vp, vp, vp, i, i, i, vp, i64, vp, i64, vp]),
+    "ahip_qk_norm_rope": (i, [vp, i, vp, i64, i, vp, vp, i64, i, vp, i, i, C.c_float, vp, i, i, i, vp, vp, i64, vp,
+                              i64, vp]),
+    "ahip_rope_table": (i, [i, i, C.c_float, vp]),
     "ahip_quantize": (i, [i, fp, i64, vp]),
     "ahip_synth_uniform": (i, [C.c_uint64, C.c_uint64, i64, C.c_float, C.c_float, fp]),
     "ahip_synth_normal": (i, [C.c_uint64, C.c_uint64, i64, C.c_float, fp]),

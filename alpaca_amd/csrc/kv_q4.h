@@ -1,0 +1,100 @@
+// A KV cache held in 4 bits: the format, the layout and the launchers.
+//
+// Values.  Q4_0 blocks of 32 values along the head dimension, with the nibbles
+// and f16 scales ahip_quantize gives: d = m / -8 (m the value of largest
+// magnitude, the first of equals), n = trunc(x * (1 / d) + 8.5) at most 15, and
+// a value reads back as d * (n - 8).  A token whose keys or values of a KV head
+// hold a NaN, an infinity or a magnitude past 65,504 has no such form: its key
+// scales of that head are NaN and its value scales 0, so that a query that sees
+// it gets NaN through its score, one that does not is untouched (0 * finite),
+// and both rows read back as NaN.
+//
+// Layout.  Keys and values in a buffer each: [kv_heads][tiles] tiles of 32
+// tokens, the last one padded; nb = head_dim / 32; 576 nb bytes a tile, 18 for
+// each 32 values.  The quants of a tile lie in the order in which a wave's lanes
+// take them as operands of v_mfma_f32_16x16x32_f16 (lane = 16 g + c), so that the
+// attention loads whole tiles without a gap and unpacks them in place:
+//   keys    [2 halves of 16 tokens][lane: c the token, g a chunk of 8 dims][nb]
+//           words; nibble i of word b is dim 32 b + 8 g + i
+//   values  [nb][lane: c a pair of dims, g a group of 4 tokens][8] bytes; byte e
+//           of (b, g, c) holds dims 32 b + 2 c (low nibble) and + 1 of token
+//           16 (e / 4) + 4 g + {0, 2, 1, 3}[e % 4]
+// (a mask picks nibbles 0 and 4, 1 and 5, ... of a word as pairs of 16 bits; the
+// byte order of the values makes such pairs neighbouring tokens), then
+//   scales  [2 halves][4 groups of 4 tokens][nb][4 tokens] f16
+#pragma once
+
+#include "common.h"
+
+constexpr int kQ4Tile = 32;  // tokens
+constexpr float kQ4Most = 65504.f;
+
+__host__ __device__ constexpr int q4_tile_bytes(int nb) { return 576 * nb; }
+__host__ __device__ constexpr int q4_scales_at(int nb) { return 512 * nb; }
+__host__ __device__ inline int q4_tiles(int capacity) { return (int)(((int64_t)capacity + kQ4Tile - 1) / kQ4Tile); }
+__host__ __device__ inline int64_t q4_head_bytes(int capacity, int nb) {
+    return (int64_t)q4_tiles(capacity) * q4_tile_bytes(nb);
+}
+// Byte offsets inside a tile of token k (0..31).
+__host__ __device__ inline int q4_key_word(int k, int nb, int b, int g) {
+    return 4 * (((k >> 4) * 64 + g * 16 + (k & 15)) * nb + b);
+}
+__host__ __device__ inline int q4_value_byte(int k, int b, int pair) {
+    const int r = k & 3;
+    return b * 512 + (((k >> 2) & 3) * 16 + pair) * 8 + (k >> 4) * 4 + (r == 1 ? 2 : r == 2 ? 1 : r);
+}
+__host__ __device__ inline int q4_scale(int k, int nb, int b) {
+    return q4_scales_at(nb) + 2 * ((((k >> 4) * 4 + ((k >> 2) & 3)) * nb + b) * 4 + (k & 3));
+}
+
+// One layer's cache.
+struct Q4Cache {
+    uint8_t* k = nullptr;
+    uint8_t* v = nullptr;
+    int kv_heads = 0, capacity = 0, nb = 0;
+};
+
+// Rows of `heads` vectors a token, `stride` elements from one token to the next.
+struct HeadRows {
+    const void* p = nullptr;
+    int64_t stride = 0;
+};
+
+// Writes `tokens` rows at positions start.. (*start_dev when set; a range
+// outside the cache then writes nothing).
+hipError_t launch_q4_store(bool f16_rows, HeadRows k, HeadRows v, int tokens, int start, const int* start_dev,
+                           const Q4Cache& c, hipStream_t st);
+// Reads them back; k_out or v_out may be null.
+hipError_t launch_q4_load(bool f16_rows, const Q4Cache& c, int start, int tokens, void* k_out, int64_t k_stride,
+                          void* v_out, int64_t v_stride, hipStream_t st);
+
+// Per-head RMS norm (gain set) and rotation (rope set) of q and k rows.
+struct NormRope {
+    int tokens = 0, heads = 0, kv_heads = 0, hd = 0;
+    HeadRows q, k;
+    void* q_out = nullptr;
+    void* k_out = nullptr;
+    int64_t q_out_stride = 0, k_out_stride = 0;
+    const float* q_gain = nullptr;
+    const float* k_gain = nullptr;
+    float eps = 0.f;
+    const float2* rope = nullptr;  // (cos, sin) [positions][hd / 2]
+    int positions = 0, interleaved = 1, start = 0;
+    const int* position = nullptr;  // a position for each token, instead of start + token
+};
+hipError_t launch_norm_rope(bool f16_rows, const NormRope& a, hipStream_t st);
+
+// Causal attention of `tokens` queries at positions start.. (*start_dev when
+// set) over the cache; partials: q4_attention_partials() floats where splits > 1.
+struct Q4Attention {
+    const void* q = nullptr;
+    void* out = nullptr;
+    int64_t q_stride = 0, out_stride = 0;
+    int tokens = 0, heads = 0, start = 0;
+    const int* start_dev = nullptr;
+    float* partials = nullptr;
+};
+// Parts the keys are split into for `length` positions, and the floats of their partial results.
+int q4_attention_splits(int tokens, int heads, int kv_heads, int hd, int length);
+int64_t q4_attention_partials(int tokens, int heads, int hd, int splits);
+hipError_t launch_q4_attention(bool f16_rows, const Q4Attention& a, const Q4Cache& c, int splits, hipStream_t st);

@@ -431,6 +431,14 @@ static std::vector<float2> rope_table(int positions, int hd, float theta) {
     return t;
 }
 
+extern "C" int ahip_rope_table(int positions, int hd, float theta, float* table) {
+    if (positions < 0 || hd <= 0 || hd % 2 || !(theta > 0) || (positions && !table))
+        return fail(AHIP_ERR_INVALID_ARGUMENT, "rotation table");
+    const auto t = rope_table(positions, hd, theta);
+    std::memcpy(table, t.data(), t.size() * sizeof(float2));
+    return AHIP_OK;
+}
+
 // ------------------------------------------------------------------ model
 
 struct ahip_model {

@@ -28,8 +28,8 @@ _LIVE: "weakref.WeakSet" = weakref.WeakSet()
 
 
 def close_all() -> None:
-    """Closes every session, model and context still open, in that order."""
-    for kind in ("session", "model", "context"):
+    """Closes every session, cache, model and context still open, in that order."""
+    for kind in ("session", "cache", "model", "context"):
         for obj in list(_LIVE):
             if getattr(obj, "_kind", None) == kind:
                 obj.close()
