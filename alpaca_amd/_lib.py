@@ -90,6 +90,19 @@ class StageC(C.Structure):
     _fields_ = [("label", C.c_char * 48), ("seconds", C.c_double), ("dispatches", C.c_int32)]
 
 
+class KVQ4C(C.Structure):
+    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("kv_heads", C.c_int32), ("head_dim", C.c_int32),
+                ("capacity", C.c_int32)]
+
+
+class NormRopeC(C.Structure):
+    _fields_ = ([(x + n, C.c_int64 if "stride" in n else C.c_void_p) for x in "qk"
+                 for n in ("", "_out", "_gain", "_stride", "_out_stride")] +
+                [("rope", C.c_void_p), ("positions", C.c_void_p)] +
+                [(n, C.c_int32) for n in ("dtype", "tokens", "heads", "kv_heads", "head_dim", "rope_positions",
+                                          "interleaved", "start")] + [("eps", C.c_float)])
+
+
 EMIT_FN = C.CFUNCTYPE(C.c_int, C.c_void_p, C.c_int32)
 
 vp, fp, ip, dp = C.c_void_p, C.POINTER(C.c_float), C.POINTER(C.c_int32), C.POINTER(C.c_double)
@@ -154,12 +167,11 @@ SIGNATURES = {
     "ahip_session_sample": (i, [vp, C.c_float, i, C.c_float, C.c_double, ip]),
     "ahip_attention_decode_noalloc": (i, [vp, vp, vp, vp, i, i, i, i, i, i, vp, vp]),
     "ahip_kv_q4_bytes": (i, [i, i, i, i64p]),
-    "ahip_kv_q4_store": (i, [vp, i, vp, i64, vp, i64, i, i, vp, vp, vp, i, i, i, vp]),
-    "ahip_kv_q4_load": (i, [vp, i, vp, vp, i, i, i, i, i, vp, i64, vp, i64, vp]),
-    "ahip_attention_q4_workspace": (i, [vp, i, i, i, i, i, i, i, i64p]),
-    "ahip_attention_q4": (i, [vp, i, vp, i64, i, i, i, vp, vp, vp, i, i, i, vp, i64, vp, i64, vp]),
-    "ahip_qk_norm_rope": (i, [vp, i, vp, i64, i, vp, vp, i64, i, vp, i, i, C.c_float, vp, i, i, i, vp, vp, i64, vp,
-                              i64, vp]),
+    "ahip_kv_q4_store": (i, [vp, vp, i, vp, i64, vp, i64, i, i, vp, vp]),
+    "ahip_kv_q4_load": (i, [vp, vp, i, i, i, vp, i64, vp, i64, vp]),
+    "ahip_attention_q4_workspace": (i, [vp, vp, i, i, i, i, i, i64p]),
+    "ahip_attention_q4": (i, [vp, vp, i, vp, i64, i, i, i, vp, vp, i64, vp, i64, vp]),
+    "ahip_qk_norm_rope": (i, [vp, vp, vp]),
     "ahip_rope_table": (i, [i, i, C.c_float, vp]),
     "ahip_quantize": (i, [i, fp, i64, vp]),
     "ahip_synth_uniform": (i, [C.c_uint64, C.c_uint64, i64, C.c_float, C.c_float, fp]),

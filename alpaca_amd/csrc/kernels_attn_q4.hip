@@ -15,12 +15,22 @@ namespace {
 typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 typedef float f32x2 __attribute__((ext_vector_type(2)));
 
-constexpr int kWaves = 4;        // of a workgroup, each with key tiles of its own
 constexpr float kLog2P = 14.f;   // P enters the products as P 2^14: what is far below the largest stays above f16's subnormals
 
 __device__ __forceinline__ uint32_t bits(f16x2 v) { return __builtin_bit_cast(uint32_t, v); }
 __device__ __forceinline__ f16x2 pair(uint32_t u) { return __builtin_bit_cast(f16x2, u); }
 __device__ __forceinline__ f16x2 round2(float a, float b) { return __builtin_convertvector((f32x2){a, b}, f16x2); }
+// e minus the low (high) half of a pair, in one instruction; exact where the half is e rounded.
+__device__ __forceinline__ float rest_low(f16x2 h, float e) {
+    float d;
+    asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel_hi:[1,0,0]" : "=v"(d) : "v"(bits(h)), "v"(e));
+    return d;
+}
+__device__ __forceinline__ float rest_high(f16x2 h, float e) {
+    float d;
+    asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel:[1,0,0] op_sel_hi:[1,0,0]" : "=v"(d) : "v"(bits(h)), "v"(e));
+    return d;
+}
 __device__ __forceinline__ f16x8 frag(f16x2 a, f16x2 b, f16x2 c, f16x2 d) {
     return {a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
 }
@@ -29,19 +39,36 @@ __device__ __forceinline__ f32x4 mfma(f16x8 a, f16x8 b, f32x4 c) {
 }
 
 // n - 8 of a word's nibbles 0 and 4 (low) or 1 and 5 (high), exactly: 1024 + n
-// and 1024 + 16 n are f16 values with the nibble in their last bits.
-__device__ __forceinline__ f16x2 low_pair(uint32_t w) {
-    return pair((w & 0x000F000Fu) | 0x64006400u) - (f16x2){(f16)1032.f, (f16)1032.f};
-}
-__device__ __forceinline__ f16x2 high_pair(uint32_t w) {
-    const f16x2 x = pair((w & 0x00F000F0u) | 0x64006400u);
-    return __builtin_elementwise_fma(x, (f16x2){(f16)0.0625f, (f16)0.0625f}, (f16x2){(f16)-72.f, (f16)-72.f});
+// and 1024 + 16 n are f16 values with the nibble in their last bits.  The
+// constants in registers (Nibbles(): a scalar and a vector one) let the mask and
+// the bias be one instruction.
+struct Nibbles {
+    uint32_t low = 0x000F000Fu, high = 0x00F000F0u, bias = 0x64006400u;
+    f16x2 sixteenth = {(f16)0.0625f, (f16)0.0625f};
+    __device__ __forceinline__ Nibbles() {
+        asm("" : "+s"(low));
+        asm("" : "+s"(high));
+        asm("" : "+v"(bias));
+    }
+    __device__ __forceinline__ f16x2 lo(uint32_t w) const {
+        return pair((w & low) | bias) - (f16x2){(f16)1032.f, (f16)1032.f};
+    }
+    __device__ __forceinline__ f16x2 hi(uint32_t w) const {
+        return __builtin_elementwise_fma(pair((w & high) | bias), sixteenth, (f16x2){(f16)-72.f, (f16)-72.f});
+    }
+};
+
+// Part i of `parts` of n: [share(n, i, parts), share(n, i + 1, parts)).
+__device__ __forceinline__ int share(int n, int i, int parts) {
+    const int q = (unsigned)n / (unsigned)parts;
+    return q * i + min(i, n - q * parts);
 }
 
 struct SplitArgs {
     Q4Attention a;
     Q4Cache c;
     int G, splits;
+    bool fused;  // the last workgroup of a KV head joins the splits
     float scale_log2;
 };
 
@@ -74,27 +101,197 @@ struct Tile {
     }
 };
 
+// ------------------------------------------------------------------ joining the splits
+// A split leaves (maximum, sum, unnormalised output) of its columns in the
+// workspace.  Few columns (a workgroup's threads hold two dims of each): the last
+// workgroup of a KV head to arrive joins them in the same launch, 3 us of GPU time
+// and as much on the host less than a second one.  Its partial results are
+// written and read with agent-scope accesses, which the L2 caches of all XCDs see;
+// each thread waits for its own to be acknowledged before the count, and the last
+// sets the counter back to zero for the next call.  More columns: a second kernel,
+// which has the whole chip for them.
+struct Joined {
+    float m = -INFINITY, l = 0.f, a = 0.f, b = 0.f;
+};
+// (top is the larger: a maximum that no score has reached weighs 1 where no other
+// has either, so that a NaN is not lost)
+__device__ __forceinline__ float join_weight(float m, float top) { return m == top ? 1.f : __builtin_amdgcn_exp2f(m - top); }
+__device__ __forceinline__ void join_add(Joined& j, float m, float l, float a, float b) {
+    const float top = fmaxf(j.m, m), f = join_weight(j.m, top), w = join_weight(m, top);
+    j.m = top;
+    j.l = j.l * f + l * w;
+    j.a = j.a * f + a * w;
+    j.b = j.b * f + b * w;
+}
+// Two floats, past the caches of an XCD (SHARED) or as usual.
+template <bool SHARED>
+__device__ __forceinline__ void put2(float* p, float a, float b) {
+    if constexpr (SHARED) {
+        const uint64_t u = (uint64_t)__float_as_uint(b) << 32 | __float_as_uint(a);
+        __hip_atomic_store(gptr((uint64_t*)p), u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    } else {
+        *(float2*)p = make_float2(a, b);
+    }
+}
+template <bool SHARED>
+__device__ __forceinline__ float2 get2(const float* p) {
+    if constexpr (!SHARED) return *(const float2*)p;
+    const uint64_t u = __hip_atomic_load(gptr((const uint64_t*)p), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    return make_float2(__uint_as_float((uint32_t)u), __uint_as_float((uint32_t)(u >> 32)));
+}
+// Splits first, first + step, ... < splits of the row at pp, for dims d and d + 1;
+// J of them in a round trip to memory.
+template <int J, bool SHARED>
+__device__ __forceinline__ Joined join(const float* pp, int hd, int d, int first, int step, int splits) {
+    Joined j;
+    for (int s0 = first; s0 < splits; s0 += J * step) {
+        float2 ml[J], o[J];
+#pragma unroll
+        for (int i = 0; i < J; i++) {  // (past the last: that one again, unused)
+            const float* x = pp + (int64_t)min(s0 + i * step, splits - 1) * (hd + 2);
+            ml[i] = get2<SHARED>(x);
+            o[i] = get2<SHARED>(x + 2 + d);
+        }
+        float top = j.m;
+#pragma unroll
+        for (int i = 0; i < J; i++)
+            if (s0 + i * step < splits) top = fmaxf(top, ml[i].x);
+        const float f = join_weight(j.m, top);
+        j.l *= f;
+        j.a *= f;
+        j.b *= f;
+#pragma unroll
+        for (int i = 0; i < J; i++) {
+            if (s0 + i * step >= splits) continue;
+            const float w = join_weight(ml[i].x, top);
+            j.l += w * ml[i].y;
+            j.a += w * o[i].x;
+            j.b += w * o[i].y;
+        }
+        j.m = top;
+    }
+    return j;
+}
+// Groups of threads with every groups-th split each, met in LDS (a float4 a thread):
+// item i of `items` in thread i of each group; the result is group 0's.
+template <int J, bool SHARED>
+__device__ __forceinline__ Joined join_groups(const float* pp, int hd, int d, int group, int groups, int items, int i,
+                                              int splits, float4* js) {
+    Joined j;
+    if (group < groups) j = join<J, SHARED>(pp, hd, d, group, groups, splits);
+    js[threadIdx.x] = make_float4(j.m, j.l, j.a, j.b);
+    __syncthreads();
+    if (group == 0)
+        for (int g = 1; g < groups; g++) {
+            const float4 o = js[i + g * items];
+            join_add(j, o.x, o.y, o.z, o.w);
+        }
+    return j;
+}
+
+// Where column `col` of KV head kvh leaves split 0 (then split by split).
+template <int HD>
+__device__ __forceinline__ float* partial(const SplitArgs& p, int kvh, int col) {
+    const unsigned t = (unsigned)col / (unsigned)p.G, h = kvh * p.G + col - t * p.G;
+    return p.a.partials + ((int64_t)t * p.a.heads + h) * p.splits * (HD + 2);
+}
+
+// Called by the whole workgroup once its partial results are written; `lds` is free.
+template <int HD, typename T>
+__device__ __forceinline__ void count_and_join(const SplitArgs& p, int kvh, int cols, void* lds) {
+    int* last = (int*)lds;
+    __builtin_amdgcn_s_waitcnt(0);
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        int* counter = p.a.counters + kvh;
+        *last = __hip_atomic_fetch_add(counter, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == p.splits - 1;
+        if (*last) __hip_atomic_store(counter, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    }
+    __syncthreads();
+    const bool mine = *last;
+    __syncthreads();  // (*last is read; the joining uses its place)
+    if (!mine) return;
+    const int items = cols * (HD / 2), groups = blockDim.x / items;  // (at least 1: p.fused)
+    const int group = threadIdx.x / items, i = threadIdx.x - group * items, col = i / (HD / 2), d = 2 * (i % (HD / 2));
+    const Joined j = join_groups<8, true>(partial<HD>(p, kvh, col), HD, d, group, groups, items, i, p.splits, (float4*)lds);
+    if (group) return;
+    const unsigned t = (unsigned)col / (unsigned)p.G, h = kvh * p.G + col - t * p.G;
+    T* out = (T*)p.a.out + t * p.a.out_stride + (int64_t)h * HD + d;
+    out[0] = (T)(j.a / j.l);
+    out[1] = (T)(j.b / j.l);
+}
+
+// The joining kernel: GROUPED, a workgroup a query and head; else two dims a thread.
+template <bool GROUPED, int J, typename T>
+__global__ __launch_bounds__(256) void q4_join_kernel(const float* partials, int64_t rows, int heads, int hd,
+                                                      int splits, T* out, int64_t stride) {
+    __shared__ float4 js[GROUPED ? 256 : 1];
+    const int half = hd / 2;
+    int64_t th;
+    int d;
+    Joined j;
+    if constexpr (GROUPED) {
+        th = blockIdx.x;
+        const int group = threadIdx.x / half, i = threadIdx.x - group * half;
+        d = 2 * i;
+        j = join_groups<J, false>(partials + th * splits * (hd + 2), hd, d, group, 256 / half, half, i, splits, js);
+        if (group) return;
+    } else {
+        const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+        th = i / half;
+        if (th >= rows) return;
+        d = 2 * (int)(i - th * half);
+        j = join<J, false>(partials + th * splits * (hd + 2), hd, d, 0, 1, splits);
+    }
+    const int64_t t = th / heads, h = th - t * heads;
+    T* p = out + t * stride + h * hd + d;
+    p[0] = (T)(j.a / j.l);
+    p[1] = (T)(j.b / j.l);
+}
+
 // T float: the scores and outputs to float32 accuracy (the queries and
 // probabilities as two f16 terms, the quants exact and the values exact in two
 // terms).  T f16: queries exact, probabilities and values one f16 term.
+// Up to kMostWaves waves a workgroup, each with key tiles of its own.
+constexpr int kMostWaves = 8;
+template <int NB>
+constexpr int lds_bytes(int waves) {
+    return waves * 16 * (32 * NB + 4 + 2) * 4;
+}
 template <int NB, typename T>
-__global__ __launch_bounds__(64 * kWaves, 2) void q4_attention_kernel(SplitArgs p) {
+__global__ __launch_bounds__(64 * kMostWaves) void q4_attention_kernel(SplitArgs p) {
     constexpr bool EXACT = sizeof(T) == 4;
     constexpr int HD = 32 * NB;
-    __shared__ float xo[kWaves][16][HD + 4];
-    __shared__ float xml[kWaves][2][16];
+    extern __shared__ __align__(16) uint8_t lds[];
+    const int waves = blockDim.x >> 6;
+    float (*xo)[16][HD + 4] = (float (*)[16][HD + 4])lds;
+    float (*xml)[2][16] = (float (*)[2][16])(lds + waves * 16 * (HD + 4) * 4);
     const int lane = threadIdx.x & 63, g = lane >> 4, c16 = lane & 15;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int sp = blockIdx.x % p.splits, kvh = blockIdx.y, col0 = blockIdx.x / p.splits * 16;
+    const Nibbles nib;
+    const int id = blockIdx.x / (unsigned)p.c.kv_heads, kvh = blockIdx.x - id * p.c.kv_heads;
+    const int sp = blockIdx.y, col0 = id * 16;
     const int G = p.G, cols = p.a.tokens * G;
     const int start = p.a.start_dev ? *p.a.start_dev : p.a.start;
     const bool inside = start >= 0 && start <= p.c.capacity - p.a.tokens;
-    const int col = min(col0 + c16, cols - 1), t = col / G, h = kvh * G + col - t * G;
+    const int col = min(col0 + c16, cols - 1), t = col / (unsigned)G, h = kvh * G + col - t * G;
     const int seen = start + t;  // the column's last position
     // the tiles of this column group, and this split's share of them
-    const int first_seen = start + col0 / G, last_seen = start + min(col0 + 15, cols - 1) / G;
+    const int first_seen = start + col0 / (unsigned)G, last_seen = start + min(col0 + 15, cols - 1) / (unsigned)G;
     const int tiles = inside ? last_seen / kQ4Tile + 1 : 0;
-    const int t0 = (int)((int64_t)tiles * sp / p.splits), t1 = (int)((int64_t)tiles * (sp + 1) / p.splits);
+    const int t0 = share(tiles, sp, p.splits), t1 = share(tiles, sp + 1, p.splits);
+
+    const uint8_t* kt = p.c.k + (int64_t)kvh * q4_head_bytes(p.c.capacity, NB);
+    const uint8_t* vt = p.c.v + (int64_t)kvh * q4_head_bytes(p.c.capacity, NB);
+    constexpr int64_t B = q4_tile_bytes(NB);
+    constexpr bool AHEAD = NB <= 4;  // the next tile on its way while one is worked on, where registers allow
+    int j = t0 + wave;
+    Tile<NB> xa, xb;
+    auto load = [&](Tile<NB>& x, int tile) {
+        const int64_t at = min(tile, t1 - 1) * B;  // (past the split's last tile: that one, unused)
+        x.load(kt + at, vt + at, lane);
+    };
+    if (j < t1) load(xa, j);
 
     // queries: block b, dims 8 g + {0, 4, 1, 5, 2, 6, 3, 7} as the keys' nibbles come
     f16x8 qh[NB], ql[EXACT ? NB : 1];
@@ -140,9 +337,6 @@ __global__ __launch_bounds__(64 * kWaves, 2) void q4_attention_kernel(SplitArgs 
     for (int b = 0; b < NB; b++) o[b][0] = o[b][1] = f32x4{0.f, 0.f, 0.f, 0.f};
     const f16x2 one2 = {(f16)1.f, (f16)1.f};
     const f16x8 ones = frag(one2, one2, one2, one2);
-    const uint8_t* kt = p.c.k + (int64_t)kvh * q4_head_bytes(p.c.capacity, NB);
-    const uint8_t* vt = p.c.v + (int64_t)kvh * q4_head_bytes(p.c.capacity, NB);
-
     auto step = [&](Tile<NB>& x, int tile) {
         // S^T(key 16 s + 4 g + r, column c16)
         f32x4 sa[2];
@@ -152,7 +346,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void q4_attention_kernel(SplitArgs 
 #pragma unroll
             for (int b = 0; b < NB; b++) {
                 const uint32_t w = x.k[s][b], w8 = w >> 8;
-                const f16x8 kf = frag(low_pair(w), high_pair(w), low_pair(w8), high_pair(w8));
+                const f16x8 kf = frag(nib.lo(w), nib.hi(w), nib.lo(w8), nib.hi(w8));
                 f32x4 part = mfma(kf, qh[b], f32x4{0.f, 0.f, 0.f, 0.f});
                 if constexpr (EXACT) part = mfma(kf, ql[b], part);
                 const f16x2 d0 = pair(x.ks[s][b].x), d1 = pair(x.ks[s][b].y);
@@ -194,7 +388,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void q4_attention_kernel(SplitArgs 
             const float e0 = __builtin_amdgcn_exp2f(fmaf(sa[i >> 1][2 * (i & 1)], sc, eref));
             const float e1 = __builtin_amdgcn_exp2f(fmaf(sa[i >> 1][2 * (i & 1) + 1], sc, eref));
             ph[i] = round2(e0, e1);
-            if constexpr (EXACT) pl[i] = round2(e0 - (float)ph[i][0], e1 - (float)ph[i][1]);
+            if constexpr (EXACT) pl[i] = round2(rest_low(ph[i], e0), rest_high(ph[i], e1));
         }
         if (__builtin_amdgcn_ballot_w64(m != mn)) {
 #pragma unroll
@@ -219,10 +413,10 @@ __global__ __launch_bounds__(64 * kWaves, 2) void q4_attention_kernel(SplitArgs 
 #pragma unroll
             for (int par = 0; par < 2; par++) {
                 f16x2 n[4], hi[4], lo[4];
-                n[0] = par ? high_pair(w0) : low_pair(w0);
-                n[1] = par ? high_pair(w0 >> 8) : low_pair(w0 >> 8);
-                n[2] = par ? high_pair(w1) : low_pair(w1);
-                n[3] = par ? high_pair(w1 >> 8) : low_pair(w1 >> 8);
+                n[0] = par ? nib.hi(w0) : nib.lo(w0);
+                n[1] = par ? nib.hi(w0 >> 8) : nib.lo(w0 >> 8);
+                n[2] = par ? nib.hi(w1) : nib.lo(w1);
+                n[3] = par ? nib.hi(w1 >> 8) : nib.lo(w1 >> 8);
 #pragma unroll
                 for (int i = 0; i < 4; i++) {
                     hi[i] = n[i] * d[i];
@@ -238,22 +432,19 @@ __global__ __launch_bounds__(64 * kWaves, 2) void q4_attention_kernel(SplitArgs 
             }
         }
     };
-    {
-        constexpr int64_t B = q4_tile_bytes(NB);
-        Tile<NB> x;
-        int j = t0 + wave;
-        if (j < t1) x.load(kt + j * B, vt + j * B, lane);
-        for (; j < t1; j += kWaves) {
-            if constexpr (NB <= 4) {
-                // the next tile on its way while this one is worked on
-                Tile<NB> y = x;
-                const int nx = min(j + kWaves, t1 - 1);
-                x.load(kt + nx * B, vt + nx * B, lane);
-                step(y, j);
-            } else {
-                step(x, j);
-                if (j + kWaves < t1) x.load(kt + (j + kWaves) * B, vt + (j + kWaves) * B, lane);
-            }
+    if constexpr (AHEAD) {
+        if (j + waves < t1) load(xb, j + waves);
+        for (; j < t1; j += 2 * waves) {
+            step(xa, j);
+            if (j + waves >= t1) break;
+            load(xa, j + 2 * waves);
+            step(xb, j + waves);
+            load(xb, j + 3 * waves);
+        }
+    } else {
+        for (; j < t1; j += waves) {
+            step(xa, j);
+            load(xa, j + waves);
         }
     }
 
@@ -268,111 +459,449 @@ __global__ __launch_bounds__(64 * kWaves, 2) void q4_attention_kernel(SplitArgs 
         xml[wave][1][c16] = l[0];
     }
     __syncthreads();
-    for (int i = threadIdx.x; i < 16 * HD; i += 64 * kWaves) {
-        const int qc = i / HD, d = i % HD;
-        if (col0 + qc >= cols) break;
-        const int tt = (col0 + qc) / G;
-        const int64_t hh = kvh * G + col0 + qc - tt * G;
+    const int n = min(16, cols - col0);
+    for (int i = threadIdx.x; i < n * (HD / 2); i += blockDim.x) {
+        const int qc = i / (HD / 2), d = 2 * (i % (HD / 2));
         float mt = xml[0][0][qc];
-#pragma unroll
-        for (int w = 1; w < kWaves; w++) mt = fmaxf(mt, xml[w][0][qc]);
-        float lt = 0.f, ot = 0.f;
-#pragma unroll
-        for (int w = 0; w < kWaves; w++) {
-            const float mw = xml[w][0][qc];
-            const float f = mw == -INFINITY ? (mt == -INFINITY ? 1.f : 0.f) : exp2f(mw - mt);
+        for (int w = 1; w < waves; w++) mt = fmaxf(mt, xml[w][0][qc]);
+        float lt = 0.f, oa = 0.f, ob = 0.f;
+        for (int w = 0; w < waves; w++) {
+            const float f = join_weight(xml[w][0][qc], mt);
             lt += f * xml[w][1][qc];
-            ot += f * xo[w][qc][d];
+            oa += f * xo[w][qc][d];
+            ob += f * xo[w][qc][d + 1];
         }
         if (p.splits == 1) {
-            ((T*)p.a.out)[tt * p.a.out_stride + hh * HD + d] = (T)(ot / lt);
+            const int64_t tt = (col0 + qc) / G, hh = kvh * G + col0 + qc - tt * G;
+            T* out = (T*)p.a.out + tt * p.a.out_stride + hh * HD + d;
+            out[0] = (T)(oa / lt);
+            out[1] = (T)(ob / lt);
         } else {
-            float* pp = p.a.partials + ((tt * (int64_t)p.a.heads + hh) * p.splits + sp) * (HD + 2);
-            pp[2 + d] = ot;
-            if (d == 0) {
-                pp[0] = mt * 0.69314718055994531f;
-                pp[1] = lt;
+            float* pp = partial<HD>(p, kvh, col0 + qc) + sp * (HD + 2);
+            if (p.fused) {
+                put2<true>(pp + 2 + d, oa, ob);
+                if (d == 0) put2<true>(pp, mt, lt);
+            } else {
+                put2<false>(pp + 2 + d, oa, ob);
+                if (d == 0) put2<false>(pp, mt, lt);
             }
         }
     }
+    if (p.fused) count_and_join<HD, T>(p, kvh, cols, lds);
 }
 
-// Joins the splits' (maximum, sum, unnormalised output): one workgroup a query and head.
-constexpr int kMostSplits = 256;
-template <typename T>
-__global__ __launch_bounds__(256) void q4_merge_kernel(const float* partials, int heads, int hd, int splits, T* out,
-                                                       int64_t stride) {
-    __shared__ float w[kMostSplits];
-    __shared__ float red[4];
-    const int64_t th = blockIdx.x, t = th / heads, h = th - t * heads;
-    const float* pp = partials + th * splits * (hd + 2);
-    const int s = threadIdx.x;
-    const float ms = s < splits ? pp[(int64_t)s * (hd + 2)] : -INFINITY;
-    const float ls = s < splits ? pp[(int64_t)s * (hd + 2) + 1] : 0.f;
-    const float wm = wave_max(ms);
-    if ((s & 63) == 0) red[s >> 6] = wm;
-    __syncthreads();
-    const float mx = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
-    // (a split of no key, or of keys without a score, counts for nothing but its NaN)
-    const float f = ms == -INFINITY ? (mx == -INFINITY ? 1.f : 0.f) : expf(ms - mx);
-    w[s] = f;
-    __syncthreads();
-    const float wl = wave_sum(s < splits ? ls * f : 0.f);
-    if ((s & 63) == 0) red[s >> 6] = wl;
-    __syncthreads();
-    const float l = (red[0] + red[1]) + (red[2] + red[3]);
-    for (int d = s; d < hd; d += 256) {
-        float o = 0.f;
-        for (int i = 0; i < splits; i++) o += pp[(int64_t)i * (hd + 2) + 2 + d] * w[i];
-        out[t * stride + h * hd + d] = (T)(o / l);
+// ------------------------------------------------------------------ many columns, f16
+// A workgroup takes 64 CT query columns, 16 CT a wave; the tiles of keys and
+// values are unpacked once for all its waves, into LDS as the fragments that the
+// products read (16 bytes a lane in lane order, so no bank conflicts either
+// way).  NSET sets of four waves take consecutive ranges of the keys and join
+// through LDS at the end.  Two buffers a set: while the waves work on one, they
+// unpack the next tile's words, loaded a step earlier, into the other; one
+// barrier a step.
+template <int NB, int CT, int NSET>
+struct Wide {
+    static constexpr int TPS = NB <= 4 ? 2 : 1;            // tiles a step
+    static constexpr int FRAGS = 2 * NB * TPS;             // of keys, and of values, in a buffer
+    static constexpr int BUF = 2 * FRAGS * 1024;
+    static constexpr int COLS = 64 * CT;
+    static constexpr int JOIN = COLS * (32 * NB + 4) * 4 + COLS * 8;  // a set's outputs and statistics
+    static constexpr int LDS = 2 * NSET * BUF > JOIN ? 2 * NSET * BUF : JOIN;
+};
+
+template <int NB, int CT, int NSET>
+__global__ __launch_bounds__(256 * NSET) __attribute__((amdgpu_waves_per_eu(2, 2))) void q4_attention_wide_kernel(SplitArgs p) {
+    typedef Wide<NB, CT, NSET> W;
+    constexpr int TPS = W::TPS, HD = 32 * NB, STEP = TPS * kQ4Tile;
+    constexpr int ITEMS = NB * TPS;  // (tile, block)
+    constexpr int PER = (ITEMS + 3) / 4;
+    extern __shared__ __align__(16) uint8_t lds[];
+    const int lane = threadIdx.x & 63, g = lane >> 4, c16 = lane & 15;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), set = wave / 4, wl = wave % 4;
+    const int G = p.G, cols = p.a.tokens * G, groups = (cols + W::COLS - 1) / W::COLS;
+    // the longest (last) columns first
+    const Nibbles nib;
+    const int id = blockIdx.x / (unsigned)p.c.kv_heads, kvh = blockIdx.x - id * p.c.kv_heads;
+    const int sp = blockIdx.y, col0 = (groups - 1 - id) * W::COLS;
+    const int start = p.a.start_dev ? *p.a.start_dev : p.a.start;
+    const bool inside = start >= 0 && start <= p.c.capacity - p.a.tokens;
+    const int wcol0 = col0 + wl * 16 * CT;  // the wave's columns
+    const int last_seen = start + min(col0 + W::COLS - 1, cols - 1) / G;
+    const int w_first = start + min(wcol0, cols - 1) / G, w_last = start + min(wcol0 + 16 * CT - 1, cols - 1) / G;
+    const int tiles = inside ? last_seen / kQ4Tile + 1 : 0;
+    const int all = (tiles + TPS - 1) / TPS;  // steps over all the keys
+    const int s0 = share(all, sp, p.splits), s1 = share(all, sp + 1, p.splits);
+    const int per = (s1 - s0 + NSET - 1) / NSET, f0 = s0 + set * per;  // this set's steps: [f0, f0 + count)
+    const int count = max(0, min(s1 - f0, per));
+
+    f16x8 q[CT][NB];
+    int seen[CT];
+#pragma unroll
+    for (int ct = 0; ct < CT; ct++) {
+        const int col = min(wcol0 + 16 * ct + c16, cols - 1), t = col / G, h = kvh * G + col - t * G;
+        seen[ct] = start + t;
+        const f16* qp = (const f16*)p.a.q + (int64_t)t * p.a.q_stride + (int64_t)h * HD + 8 * g;
+#pragma unroll
+        for (int b = 0; b < NB; b++) {
+            const f16 *x = qp + 32 * b;
+            q[ct][b] = f16x8{x[0], x[4], x[1], x[5], x[2], x[6], x[3], x[7]};
+        }
+    }
+    float m[CT];
+    f32x4 o[CT][NB][2], l[CT];
+#pragma unroll
+    for (int ct = 0; ct < CT; ct++) {
+        m[ct] = -INFINITY;
+        l[ct] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int b = 0; b < NB; b++) o[ct][b][0] = o[ct][b][1] = f32x4{0.f, 0.f, 0.f, 0.f};
+    }
+    const f16x2 one2 = {(f16)1.f, (f16)1.f};
+    const f16x8 ones = frag(one2, one2, one2, one2);
+    const uint8_t* kt = p.c.k + (int64_t)kvh * q4_head_bytes(p.c.capacity, NB);
+    const uint8_t* vt = p.c.v + (int64_t)kvh * q4_head_bytes(p.c.capacity, NB);
+    uint8_t* const buf0 = lds + set * 2 * W::BUF;
+
+    // The set's four waves share the (tile, block) items of a step, of the keys and of the values.
+    uint32_t rk[PER][4], rv[PER][6];
+    const uint32_t k_at = lane * 4 * NB, ks_at = q4_scales_at(NB) + ((c16 >> 2) * NB * 4 + (c16 & 3)) * 2;
+    const uint32_t v_at = lane * 8, vs_at = q4_scales_at(NB) + g * NB * 8;
+    auto item = [&](int k, int* tt, int* b) {
+        const int i = wl + 4 * k;
+        *tt = i / NB;
+        *b = i - *tt * NB;
+        return ITEMS % 4 == 0 || i < ITEMS;
+    };
+    auto fetch = [&](int step) {
+#pragma unroll
+        for (int k = 0; k < PER; k++) {
+            int tt, b;
+            if (!item(k, &tt, &b)) continue;
+            // past the last tile: that one again, its columns masked
+            const int64_t at = (int64_t)min(step * TPS + tt, tiles - 1) * q4_tile_bytes(NB);
+            const uint8_t *x = kt + at + b * 4, *y = vt + at + b * 512;
+            const uint8_t *xs = kt + at + b * 8, *ys = vt + at + b * 8;
+#pragma unroll
+            for (int s = 0; s < 2; s++) {
+                rk[k][s] = *(const AS_GLOBAL uint32_t*)(x + (k_at + s * 256 * NB));
+                rk[k][2 + s] = *(const AS_GLOBAL uint16_t*)(xs + (ks_at + s * 32 * NB));
+                const uint2 d = Tile<NB>::load2(ys + (vs_at + s * 32 * NB));
+                rv[k][2 + 2 * s] = d.x;
+                rv[k][3 + 2 * s] = d.y;
+            }
+            const uint2 w = Tile<NB>::load2(y + v_at);
+            rv[k][0] = w.x;
+            rv[k][1] = w.y;
+        }
+    };
+    auto unpack = [&](int step, uint8_t* buf) {
+#pragma unroll
+        for (int k = 0; k < PER; k++) {
+            int tt, b;
+            if (!item(k, &tt, &b)) continue;
+#pragma unroll
+            for (int s = 0; s < 2; s++) {
+                const uint32_t w = rk[k][s], w8 = w >> 8;
+                const f16x2 d = pair(rk[k][2 + s] * 0x10001u);
+                *(f16x8*)(buf + ((tt * 2 + s) * NB + b) * 1024 + lane * 16) =
+                    frag(nib.lo(w) * d, nib.hi(w) * d, nib.lo(w8) * d, nib.hi(w8) * d);
+            }
+            const int key0 = (step * TPS + tt) * kQ4Tile;
+            if (key0 + kQ4Tile - 1 > last_seen) {
+                // positions that may never have been written: values of 0
+#pragma unroll
+                for (int e = 0; e < 8; e++)
+                    if (key0 + 16 * (e >> 2) + 4 * g + (e & 3) > last_seen)
+                        rv[k][2 + (e >> 1)] &= e & 1 ? 0xFFFFu : 0xFFFF0000u;
+            }
+            const uint32_t w0 = rv[k][0], w1 = rv[k][1], u0 = w0 >> 8, u1 = w1 >> 8;
+            const f16x2 d0 = pair(rv[k][2]), d1 = pair(rv[k][3]), d2 = pair(rv[k][4]), d3 = pair(rv[k][5]);
+            uint8_t* v = buf + (W::FRAGS + (tt * NB + b) * 2) * 1024 + lane * 16;
+            *(f16x8*)v = frag(nib.lo(w0) * d0, nib.lo(u0) * d1, nib.lo(w1) * d2, nib.lo(u1) * d3);
+            *(f16x8*)(v + 1024) = frag(nib.hi(w0) * d0, nib.hi(u0) * d1, nib.hi(w1) * d2, nib.hi(u1) * d3);
+        }
+    };
+    auto work = [&](int step, const uint8_t* buf) {
+        const int key0 = step * STEP;
+        if (key0 > w_last) return;
+        f32x4 sa[CT][TPS * 2];
+        // fragments are read a group of NB ahead of the products that take them
+        f16x8 fr[2][NB];
+        auto read = [&](int group) {
+#pragma unroll
+            for (int b = 0; b < NB; b++) fr[group & 1][b] = *(const f16x8*)(buf + (group * NB + b) * 1024 + lane * 16);
+        };
+        read(0);
+#pragma unroll
+        for (int u = 0; u < 2 * TPS; u++) {
+            read(u + 1);  // (after the last keys: the first values)
+#pragma unroll
+            for (int ct = 0; ct < CT; ct++) sa[ct][u] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int b = 0; b < NB; b++)
+#pragma unroll
+                for (int ct = 0; ct < CT; ct++) sa[ct][u] = mfma(fr[u & 1][b], q[ct][b], sa[ct][u]);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        if (key0 + STEP - 1 > w_first) {
+#pragma unroll
+            for (int ct = 0; ct < CT; ct++)
+#pragma unroll
+                for (int u = 0; u < 2 * TPS; u++)
+#pragma unroll
+                    for (int r = 0; r < 4; r++)
+                        if (key0 + 16 * u + 4 * g + r > seen[ct]) sa[ct][u][r] = -INFINITY;
+        }
+        f16x8 pf[CT][TPS];
+#pragma unroll
+        for (int ct = 0; ct < CT; ct++) {
+            float mx = sa[ct][0][0];
+#pragma unroll
+            for (int i = 1; i < 8 * TPS; i++) mx = fmaxf(mx, sa[ct][i >> 2][i & 3]);
+            mx = xor32_combine(xor16_combine(mx, MaxOp()), MaxOp());
+            const float mn = fmaxf(m[ct], mx * p.scale_log2);
+            const float mref = mn == -INFINITY ? 0.f : mn;
+            const float alpha = __builtin_amdgcn_exp2f(m[ct] - mref), eref = kLog2P - mref;
+#pragma unroll
+            for (int tt = 0; tt < TPS; tt++) {
+                f16x2 e[4];
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    const f32x4& x = sa[ct][2 * tt + (i >> 1)];
+                    e[i] = round2(__builtin_amdgcn_exp2f(fmaf(x[2 * (i & 1)], p.scale_log2, eref)),
+                                  __builtin_amdgcn_exp2f(fmaf(x[2 * (i & 1) + 1], p.scale_log2, eref)));
+                }
+                pf[ct][tt] = frag(e[0], e[1], e[2], e[3]);
+            }
+            if (__builtin_amdgcn_ballot_w64(m[ct] != mn)) {
+#pragma unroll
+                for (int b = 0; b < NB; b++) {
+                    o[ct][b][0] *= alpha;
+                    o[ct][b][1] *= alpha;
+                }
+                l[ct] *= alpha;
+                m[ct] = mn;
+            }
+#pragma unroll
+            for (int tt = 0; tt < TPS; tt++) l[ct] = mfma(ones, pf[ct][tt], l[ct]);
+        }
+#pragma unroll
+        for (int u = 0; u < 2 * TPS; u++) {
+            if (u + 1 < 2 * TPS) read(2 * TPS + u + 1);
+#pragma unroll
+            for (int i = 0; i < NB; i++) {
+                const int f = (u & 1) * NB + i;
+#pragma unroll
+                for (int ct = 0; ct < CT; ct++)
+                    o[ct][f >> 1][f & 1] = mfma(fr[(2 * TPS + u) & 1][i], pf[ct][u >> 1], o[ct][f >> 1][f & 1]);
+            }
+            __builtin_amdgcn_sched_barrier(0);
+        }
+    };
+
+    if (tiles > 0 && s1 > s0) {  // (the same for the whole workgroup)
+        const int lastf = all - 1;
+        fetch(min(f0, lastf));
+        unpack(min(f0, lastf), buf0);
+        fetch(min(f0 + 1, lastf));
+        __syncthreads();
+        for (int j = 0; j < per; j++) {
+            if (j + 1 < per) {
+                unpack(min(f0 + j + 1, lastf), buf0 + ((j + 1) & 1) * W::BUF);
+                fetch(min(f0 + j + 2, lastf));
+            }
+            if (j < count) work(f0 + j, buf0 + (j & 1) * W::BUF);
+            __syncthreads();
+        }
+    }
+    // the other sets' results through LDS, [set - 1]
+    float* xo = (float*)lds;
+    float* xml = xo + W::COLS * (HD + 4);
+    auto put_set = [&]() {
+#pragma unroll
+        for (int ct = 0; ct < CT; ct++) {
+            const int c = wl * 16 * CT + 16 * ct + c16;
+#pragma unroll
+            for (int b = 0; b < NB; b++) {
+                float* x = xo + c * (HD + 4) + 32 * b + 8 * g;
+                *(float4*)x = make_float4(o[ct][b][0][0], o[ct][b][1][0], o[ct][b][0][1], o[ct][b][1][1]);
+                *(float4*)(x + 4) = make_float4(o[ct][b][0][2], o[ct][b][1][2], o[ct][b][0][3], o[ct][b][1][3]);
+            }
+            if (g == 0) {
+                xml[2 * c] = m[ct];
+                xml[2 * c + 1] = l[ct][0];
+            }
+        }
+    };
+    for (int s = 1; s < NSET; s++) {
+        if (s > 1) __syncthreads();
+        if (set == s) put_set();
+        __syncthreads();
+        if (set == 0) {
+#pragma unroll
+            for (int ct = 0; ct < CT; ct++) {
+                const int c = wl * 16 * CT + 16 * ct + c16;
+                const float mo = xml[2 * c], mn = fmaxf(m[ct], mo), mref = mn == -INFINITY ? 0.f : mn;
+                // (nothing of a set is lost where neither has a score: a NaN stays)
+                const float fa = m[ct] == mn ? 1.f : __builtin_amdgcn_exp2f(m[ct] - mref);
+                const float fb = mo == mn ? 1.f : __builtin_amdgcn_exp2f(mo - mref);
+                m[ct] = mn;
+                const float lo = xml[2 * c + 1];
+#pragma unroll
+                for (int r = 0; r < 4; r++) l[ct][r] = l[ct][r] * fa + lo * fb;
+#pragma unroll
+                for (int b = 0; b < NB; b++) {
+                    const float* x = xo + c * (HD + 4) + 32 * b + 8 * g;
+#pragma unroll
+                    for (int r = 0; r < 4; r++)
+#pragma unroll
+                        for (int par = 0; par < 2; par++)
+                            o[ct][b][par][r] = o[ct][b][par][r] * fa + x[2 * r + par] * fb;
+                }
+            }
+        }
+    }
+    if (p.splits > 1) {
+        // through LDS, so that the rows of partial results leave whole
+        if (NSET > 1) __syncthreads();  // (the last set's results are read)
+        if (set == 0) put_set();
+        __syncthreads();
+        const int n = min(W::COLS, cols - col0);
+        for (int i = threadIdx.x; i < n * (HD / 2 + 1); i += 256 * NSET) {
+            const int c = i / (HD / 2 + 1), d = 2 * (i - c * (HD / 2 + 1));
+            const float2 v = *(const float2*)(d ? xo + c * (HD + 4) + d - 2 : xml + 2 * c);
+            *(float2*)(partial<HD>(p, kvh, col0 + c) + sp * (HD + 2) + d) = v;
+        }
+        return;
+    }
+    if (set) return;
+#pragma unroll
+    for (int ct = 0; ct < CT; ct++) {
+        const int col = wcol0 + 16 * ct + c16;
+        if (col >= cols) continue;
+        const int t = col / G, h = kvh * G + col - t * G;
+        f16* out = (f16*)p.a.out + t * p.a.out_stride + (int64_t)h * HD + 8 * g;
+        const float inv = 1.0f / l[ct][0];
+#pragma unroll
+        for (int b = 0; b < NB; b++)
+#pragma unroll
+            for (int r = 0; r < 4; r++) {
+                out[32 * b + 2 * r] = (f16)(o[ct][b][0][r] * inv);
+                out[32 * b + 2 * r + 1] = (f16)(o[ct][b][1][r] * inv);
+            }
     }
 }
 
 template <typename T>
-void launch(const SplitArgs& p, dim3 grid, hipStream_t st) {
+hipError_t launch_join(const Q4Attention& a, int hd, int splits, hipStream_t st) {
+    const int64_t rows = (int64_t)a.tokens * a.heads;
+    const unsigned flat = (unsigned)((rows * (hd / 2) + 255) / 256);
+    auto go = [&](auto kernel, unsigned grid) {
+        kernel<<<grid, 256, 0, st>>>(a.partials, rows, a.heads, hd, splits, (T*)a.out, a.out_stride);
+    };
+    if (splits <= 2) go(q4_join_kernel<false, 2, T>, flat);
+    else if (splits <= 4) go(q4_join_kernel<false, 4, T>, flat);
+    else if (splits <= 8) go(q4_join_kernel<false, 8, T>, flat);
+    else go(q4_join_kernel<true, 8, T>, (unsigned)rows);
+    return hipGetLastError();
+}
+
+template <int NB, int CT, int NSET>
+hipError_t launch_wide(const SplitArgs& p, int64_t cols, hipStream_t st) {
+    typedef Wide<NB, CT, NSET> W;
+    auto* kernel = q4_attention_wide_kernel<NB, CT, NSET>;
+    static OncePerDevice once;
+    if (hipError_t e = allow_whole_lds(once, (const void*)kernel)) return e;
+    const dim3 grid((unsigned)((cols + W::COLS - 1) / W::COLS * p.c.kv_heads), p.splits);
+    kernel<<<grid, 256 * NSET, W::LDS, st>>>(p);
+    return hipGetLastError();
+}
+
+template <int NB, typename T>
+hipError_t launch_nb(const SplitArgs& p, const Q4Plan& plan, hipStream_t st) {
+    const int64_t cols = (int64_t)p.a.tokens * p.G;
+    if constexpr (sizeof(T) == 2) {
+        if constexpr (NB <= 4)
+            if (plan.cols == 128) return launch_wide<NB, 2, 2>(p, cols, st);
+        if (plan.cols == 64) return launch_wide<NB, 1, 2>(p, cols, st);
+    }
+    static OncePerDevice once;
+    if (hipError_t e = allow_whole_lds(once, (const void*)q4_attention_kernel<NB, T>)) return e;
+    const dim3 grid((unsigned)((cols + 15) / 16 * p.c.kv_heads), p.splits);
+    q4_attention_kernel<NB, T><<<grid, 64 * plan.waves, lds_bytes<NB>(plan.waves), st>>>(p);
+    return hipGetLastError();
+}
+
+template <typename T>
+hipError_t launch(const SplitArgs& p, const Q4Plan& plan, hipStream_t st) {
     switch (p.c.nb) {
-    case 1: q4_attention_kernel<1, T><<<grid, 64 * kWaves, 0, st>>>(p); break;
-    case 2: q4_attention_kernel<2, T><<<grid, 64 * kWaves, 0, st>>>(p); break;
-    case 3: q4_attention_kernel<3, T><<<grid, 64 * kWaves, 0, st>>>(p); break;
-    case 4: q4_attention_kernel<4, T><<<grid, 64 * kWaves, 0, st>>>(p); break;
-    case 5: q4_attention_kernel<5, T><<<grid, 64 * kWaves, 0, st>>>(p); break;
-    case 6: q4_attention_kernel<6, T><<<grid, 64 * kWaves, 0, st>>>(p); break;
-    case 7: q4_attention_kernel<7, T><<<grid, 64 * kWaves, 0, st>>>(p); break;
-    default: q4_attention_kernel<8, T><<<grid, 64 * kWaves, 0, st>>>(p); break;
+    case 1: return launch_nb<1, T>(p, plan, st);
+    case 2: return launch_nb<2, T>(p, plan, st);
+    case 3: return launch_nb<3, T>(p, plan, st);
+    case 4: return launch_nb<4, T>(p, plan, st);
+    case 5: return launch_nb<5, T>(p, plan, st);
+    case 6: return launch_nb<6, T>(p, plan, st);
+    case 7: return launch_nb<7, T>(p, plan, st);
+    default: return launch_nb<8, T>(p, plan, st);
     }
 }
 
 }  // namespace
 
-int q4_attention_splits(int tokens, int heads, int kv_heads, int hd, int length) {
-    const int64_t groups = ((int64_t)tokens * (heads / kv_heads) + 15) / 16 * kv_heads;
-    const int tiles = (length + kQ4Tile - 1) / kQ4Tile;
-    // about two workgroups a CU, and a tile at least for each wave
-    const int64_t want = 2 * (int64_t)device_cus() / groups, most = (tiles + kWaves - 1) / kWaves;
-    return (int)std::max<int64_t>(1, std::min<int64_t>({want, most, kMostSplits}));
+// How a call runs.  Columns of a workgroup: 16 (every wave key tiles of its own) up
+// to 64 columns, 64 or 128 from there in f16, where unpacking a tile once for all
+// of them pays (64 columns over 8,000 positions, 8 KV heads of 128: 17.2 us either
+// way; 300: 27 us with 64 a workgroup).  128 where workgroups of 128 fill the chip
+// (prompt of 2,048 tokens, 32/8 heads of 128, 63 us against 79; 512 tokens of it 17
+// against 13), at most head dimension 128 (registers).
+//
+// Splits, up to a workgroup a CU over all.  A workgroup alone costs about 5.5 us and
+// nb / 18 us a tile of its keys; joining costs 1.5 us in the same launch, 7 as one
+// of its own.  In the same launch a split has a tile a wave until there are 16 splits
+// (32/8 heads of 128, 4,000 positions: 32.8 us in one, 13.8 in 4, 9.7 in 16, 12.1
+// in 32), then 32 tiles, which hide the waits of 32 splits and more.
+Q4Plan q4_attention_plan(bool f16_rows, int tokens, int heads, int kv_heads, int hd, int length) {
+    Q4Plan r;
+    const int64_t cols = (int64_t)tokens * (heads / kv_heads);
+    const int cus = device_cus(), tiles = q4_tiles(length), work = tiles * (hd / 32);
+    auto groups = [&](int tile) { return (cols + tile - 1) / tile * kv_heads; };
+    auto up = [](int64_t a, int64_t b) { return (int)((a + b - 1) / b); };
+    if (f16_rows && cols > 64) {
+        r.cols = hd <= 128 && groups(128) >= cus ? 128 : 64;
+        const int most = (int)(cus / groups(r.cols));
+        // two sets of waves take 64 keys (32 past head dimension 128) a step each
+        r.splits = tiles <= 48 ? 1 : std::max(1, std::min(most, up(tiles, 8)));
+        return r;
+    }
+    r.cols = 16;
+    const int most = std::max(1, (int)(cus / groups(16)));
+    const int64_t pairs = cols * (hd / 2);  // of dims to join
+    const bool can_fuse = cols <= 16 && pairs <= 512 && kv_heads <= kQ4Counters;
+    if (can_fuse) r.splits = work <= 40 ? 1 : std::min(most, std::max(std::min(16, up(tiles, 4)), up(tiles, 32)));
+    else r.splits = work <= 200 ? 1 : std::min(most, up(work, 64));
+    r.fused = can_fuse && r.splits > 1;
+    // Eight waves where each still has many tiles (131,072 positions in 32 splits: 42.0 us against
+    // 44.2 with four; 4,000 in 16: 10.2 against 9.7) and the chip is not full without them (512
+    // float32 queries, 32/8 heads of 128: 31.9 against 23.1), or for the threads that join.
+    r.waves = (up(tiles, r.splits) >= 16 && groups(16) * r.splits <= cus) || (r.fused && pairs > 256) ? 8 : 4;
+    return r;
 }
 
 int64_t q4_attention_partials(int tokens, int heads, int hd, int splits) {
     return splits > 1 ? (int64_t)tokens * heads * splits * (hd + 2) : 0;
 }
 
-hipError_t launch_q4_attention(bool f16_rows, const Q4Attention& a, const Q4Cache& c, int splits, hipStream_t st) {
+hipError_t launch_q4_attention(bool f16_rows, const Q4Attention& a, const Q4Cache& c, const Q4Plan& plan,
+                               hipStream_t st) {
     if (a.tokens <= 0) return hipSuccess;
     SplitArgs p;
     p.a = a;
     p.c = c;
     p.G = a.heads / c.kv_heads;
-    p.splits = splits;
+    p.splits = plan.splits;
+    p.fused = plan.fused;
     const int hd = 32 * c.nb;
     p.scale_log2 = 1.4426950408889634f / sqrtf((float)hd);
-    const int64_t groups = ((int64_t)a.tokens * p.G + 15) / 16;
-    const dim3 grid((unsigned)(groups * splits), c.kv_heads);
-    if (f16_rows) launch<f16>(p, grid, st);
-    else launch<float>(p, grid, st);
-    if (splits > 1) {
-        const unsigned rows = (unsigned)((int64_t)a.tokens * a.heads);
-        if (f16_rows) q4_merge_kernel<f16><<<rows, 256, 0, st>>>(a.partials, a.heads, hd, splits, (f16*)a.out, a.out_stride);
-        else q4_merge_kernel<float><<<rows, 256, 0, st>>>(a.partials, a.heads, hd, splits, (float*)a.out, a.out_stride);
-    }
-    return hipGetLastError();
+    if (hipError_t e = f16_rows ? launch<f16>(p, plan, st) : launch<float>(p, plan, st)) return e;
+    if (plan.splits == 1 || plan.fused) return hipSuccess;
+    return f16_rows ? launch_join<f16>(a, hd, plan.splits, st) : launch_join<float>(a, hd, plan.splits, st);
 }

@@ -146,53 +146,100 @@ __global__ __launch_bounds__(kBlock) void q4_load_kernel(Q4Cache c, int start, i
 }
 
 // ------------------------------------------------------------------ norm and rotation
-// A wave per (token, head) row: lane l holds pairs l, l + 64 (head_dim up to 256).
-template <typename T>
-__global__ __launch_bounds__(kBlock) void norm_rope_kernel(NormRope a) {
-    const int64_t row = (int64_t)blockIdx.x * (kBlock / 64) + (threadIdx.x >> 6);
-    const int lane = threadIdx.x & 63, all = a.heads + a.kv_heads, half = a.hd / 2;
-    if (row >= (int64_t)a.tokens * all) return;
-    const int64_t t = row / all;
-    const int y = (int)(row - t * all);
-    const bool key = y >= a.heads;
+// One pass over the rows.  A lane holds the values [i V, (i + 1) V) of a head's
+// first half and of its second, V the values of 16 bytes, so that both kinds of
+// pairs, (2 p, 2 p + 1) and (p, p + hd / 2), lie in one lane; L lanes (a power of
+// two, the last ones idle where hd / 2 is none) hold a head and sum its squares
+// among themselves.
+template <typename T, int L, bool ALIGNED>
+__global__ __launch_bounds__(kBlock) void norm_rope_kernel(ahip_norm_rope a) {
+    constexpr int V = 16 / sizeof(T);
+    typedef T vec __attribute__((ext_vector_type(V)));
+    const int64_t row = (int64_t)blockIdx.x * (kBlock / L) + threadIdx.x / L;
+    const unsigned all = a.heads + a.kv_heads;
+    if (row >= (int64_t)a.tokens * all) return;  // (whole groups of L lanes)
+    const unsigned t = (unsigned)row / all, y = (unsigned)row - t * all;  // (at most 2^30 rows)
+    const int i0 = (threadIdx.x % L) * V, half = a.head_dim / 2;
+    const bool key = y >= (unsigned)a.heads, mine = i0 < half;
     const int h = key ? y - a.heads : y;
-    const T* x = (const T*)(key ? a.k.p : a.q.p) + t * (key ? a.k.stride : a.q.stride) + (int64_t)h * a.hd;
-    T* out = (T*)(key ? a.k_out : a.q_out) + t * (key ? a.k_out_stride : a.q_out_stride) + (int64_t)h * a.hd;
+    const T* x = (const T*)(key ? a.k : a.q) + t * (key ? a.k_stride : a.q_stride) + (int64_t)h * 2 * half;
+    T* out = (T*)(key ? a.k_out : a.q_out) + t * (key ? a.k_out_stride : a.q_out_stride) + (int64_t)h * 2 * half;
     const float* gain = key ? a.k_gain : a.q_gain;
-    float u[2] = {0.f, 0.f}, w[2] = {0.f, 0.f};
-    float ss = 0.f;
+    float v[2][V];
 #pragma unroll
-    for (int i = 0; i < 2; i++) {
-        const int p = lane + 64 * i;
-        if (p < half) {
-            u[i] = (float)x[a.interleaved ? 2 * p : p];
-            w[i] = (float)x[a.interleaved ? 2 * p + 1 : p + half];
-            ss += u[i] * u[i] + w[i] * w[i];
+    for (int s = 0; s < 2; s++) {
+        vec r = {};
+        if (mine) {
+            if constexpr (ALIGNED) {
+                r = *(const vec*)(x + s * half + i0);
+            } else {
+#pragma unroll
+                for (int e = 0; e < V; e++) r[e] = x[s * half + i0 + e];
+            }
+        }
+#pragma unroll
+        for (int e = 0; e < V; e++) v[s][e] = (float)r[e];
+    }
+    float f[2][V];  // what each value is scaled by
+    if (gain) {
+        if (mine)
+#pragma unroll
+            for (int s = 0; s < 2; s++)
+#pragma unroll
+                for (int e = 0; e < V; e++) f[s][e] = gain[s * half + i0 + e];
+        float ss = 0.f;
+#pragma unroll
+        for (int e = 0; e < V; e++) ss += v[0][e] * v[0][e] + v[1][e] * v[1][e];
+        const float scale = 1.0f / sqrtf(lane_sum<L>(ss) / (float)(2 * half) + a.eps);
+#pragma unroll
+        for (int s = 0; s < 2; s++)
+#pragma unroll
+            for (int e = 0; e < V; e++) v[s][e] = v[s][e] * scale * f[s][e];
+    }
+    if (!mine) return;
+    if (a.rope) {
+        const int pos = a.positions ? a.positions[t] : a.start + (int)t;
+        const bool known = pos >= 0 && pos < a.rope_positions;
+        const float2* cs = (const float2*)a.rope + (int64_t)(known ? pos : 0) * half;
+        auto turn = [&](float& p, float& q, float2 c) {
+            if (!known) c = {NAN, NAN};  // a position outside the table
+            const float r = p * c.x - q * c.y;
+            q = p * c.y + q * c.x;
+            p = r;
+        };
+        if (a.interleaved) {
+#pragma unroll
+            for (int s = 0; s < 2; s++)
+#pragma unroll
+                for (int e = 0; e < V; e += 2) turn(v[s][e], v[s][e + 1], cs[(s * half + i0 + e) / 2]);
+        } else {
+#pragma unroll
+            for (int e = 0; e < V; e++) turn(v[0][e], v[1][e], cs[i0 + e]);
         }
     }
-    float scale = 1.f;
-    if (gain) scale = 1.0f / sqrtf(wave_sum(ss) / (float)a.hd + a.eps);
-    const int pos = a.position ? a.position[t] : a.start + (int)t;
 #pragma unroll
-    for (int i = 0; i < 2; i++) {
-        const int p = lane + 64 * i;
-        if (p >= half) continue;
-        const int ia = a.interleaved ? 2 * p : p, ib = a.interleaved ? 2 * p + 1 : p + half;
-        float f = u[i], s = w[i];
-        if (gain) {
-            f = f * scale * gain[ia];
-            s = s * scale * gain[ib];
+    for (int s = 0; s < 2; s++) {
+        if constexpr (ALIGNED) {
+            vec r;
+#pragma unroll
+            for (int e = 0; e < V; e++) r[e] = (T)v[s][e];
+            *(vec*)(out + s * half + i0) = r;
+        } else {
+#pragma unroll
+            for (int e = 0; e < V; e++) out[s * half + i0 + e] = (T)v[s][e];
         }
-        if (a.rope) {
-            float2 cs = {NAN, NAN};  // a position outside the table
-            if (pos >= 0 && pos < a.positions) cs = a.rope[(int64_t)pos * half + p];
-            const float ra = f * cs.x - s * cs.y;
-            s = f * cs.y + s * cs.x;
-            f = ra;
-        }
-        out[ia] = (T)f;
-        out[ib] = (T)s;
     }
+}
+
+template <typename T, int L>
+void run_norm_rope(const ahip_norm_rope& a, hipStream_t st) {
+    auto odd = [](const void* p, int64_t stride) { return ((uintptr_t)p | (uintptr_t)(stride * sizeof(T))) & 15; };
+    const bool aligned = !((a.heads ? odd(a.q, a.q_stride) | odd(a.q_out, a.q_out_stride) : 0) |
+                           (a.kv_heads ? odd(a.k, a.k_stride) | odd(a.k_out, a.k_out_stride) : 0));
+    const int64_t rows = (int64_t)a.tokens * (a.heads + a.kv_heads);
+    const unsigned grid = (unsigned)((rows + kBlock / L - 1) / (kBlock / L));
+    if (aligned) norm_rope_kernel<T, L, true><<<grid, kBlock, 0, st>>>(a);
+    else norm_rope_kernel<T, L, false><<<grid, kBlock, 0, st>>>(a);
 }
 
 }  // namespace
@@ -219,11 +266,18 @@ hipError_t launch_q4_load(bool f16_rows, const Q4Cache& c, int start, int tokens
     return hipGetLastError();
 }
 
-hipError_t launch_norm_rope(bool f16_rows, const NormRope& a, hipStream_t st) {
-    const int64_t rows = (int64_t)a.tokens * (a.heads + a.kv_heads);
-    if (rows <= 0) return hipSuccess;
-    const unsigned grid = (unsigned)((rows + kBlock / 64 - 1) / (kBlock / 64));
-    if (f16_rows) norm_rope_kernel<f16><<<grid, kBlock, 0, st>>>(a);
-    else norm_rope_kernel<float><<<grid, kBlock, 0, st>>>(a);
+hipError_t launch_norm_rope(bool f16_rows, const ahip_norm_rope& a, hipStream_t st) {
+    if ((int64_t)a.tokens * (a.heads + a.kv_heads) <= 0) return hipSuccess;
+    const int lanes = a.head_dim / 2 / (f16_rows ? 8 : 4);  // 2 to 32
+    auto go = [&](auto zero) {
+        typedef decltype(zero) T;
+        if (lanes <= 2) run_norm_rope<T, 2>(a, st);
+        else if (lanes <= 4) run_norm_rope<T, 4>(a, st);
+        else if (lanes <= 8) run_norm_rope<T, 8>(a, st);
+        else if (lanes <= 16) run_norm_rope<T, 16>(a, st);
+        else run_norm_rope<T, 32>(a, st);
+    };
+    if (f16_rows) go((f16)0);
+    else go(0.f);
     return hipGetLastError();
 }

@@ -24,6 +24,7 @@
 //   scales  [2 halves][4 groups of 4 tokens][nb][4 tokens] f16
 #pragma once
 
+#include "../../include/alpaca_hip.h"
 #include "common.h"
 
 constexpr int kQ4Tile = 32;  // tokens
@@ -68,24 +69,12 @@ hipError_t launch_q4_store(bool f16_rows, HeadRows k, HeadRows v, int tokens, in
 hipError_t launch_q4_load(bool f16_rows, const Q4Cache& c, int start, int tokens, void* k_out, int64_t k_stride,
                           void* v_out, int64_t v_stride, hipStream_t st);
 
-// Per-head RMS norm (gain set) and rotation (rope set) of q and k rows.
-struct NormRope {
-    int tokens = 0, heads = 0, kv_heads = 0, hd = 0;
-    HeadRows q, k;
-    void* q_out = nullptr;
-    void* k_out = nullptr;
-    int64_t q_out_stride = 0, k_out_stride = 0;
-    const float* q_gain = nullptr;
-    const float* k_gain = nullptr;
-    float eps = 0.f;
-    const float2* rope = nullptr;  // (cos, sin) [positions][hd / 2]
-    int positions = 0, interleaved = 1, start = 0;
-    const int* position = nullptr;  // a position for each token, instead of start + token
-};
-hipError_t launch_norm_rope(bool f16_rows, const NormRope& a, hipStream_t st);
+// Per-head RMS norm and rotation of q and k rows (ahip_qk_norm_rope's arguments, checked).
+hipError_t launch_norm_rope(bool f16_rows, const ahip_norm_rope& a, hipStream_t st);
 
 // Causal attention of `tokens` queries at positions start.. (*start_dev when
-// set) over the cache; partials: q4_attention_partials() floats where splits > 1.
+// set) over the cache; where splits > 1 with q4_attention_partials() floats of
+// partial results and kQ4Counters words, zero before and after every launch.
 struct Q4Attention {
     const void* q = nullptr;
     void* out = nullptr;
@@ -93,8 +82,17 @@ struct Q4Attention {
     int tokens = 0, heads = 0, start = 0;
     const int* start_dev = nullptr;
     float* partials = nullptr;
+    int* counters = nullptr;
 };
-// Parts the keys are split into for `length` positions, and the floats of their partial results.
-int q4_attention_splits(int tokens, int heads, int kv_heads, int hd, int length);
-int64_t q4_attention_partials(int tokens, int heads, int hd, int splits);
-hipError_t launch_q4_attention(bool f16_rows, const Q4Attention& a, const Q4Cache& c, int splits, hipStream_t st);
+constexpr int kQ4Counters = 512;
+// How a call runs: query columns and waves of a workgroup, parts the keys are split into, and
+// whether the last workgroup to arrive joins them.  `length`: the positions that the call may see;
+// the splits do not fall as it grows.
+struct Q4Plan {
+    int cols = 16, waves = 4, splits = 1;
+    bool fused = false;
+};
+Q4Plan q4_attention_plan(bool f16_rows, int tokens, int heads, int kv_heads, int hd, int length);
+int64_t q4_attention_partials(int tokens, int heads, int hd, int splits);  // floats
+hipError_t launch_q4_attention(bool f16_rows, const Q4Attention& a, const Q4Cache& c, const Q4Plan& plan,
+                               hipStream_t st);

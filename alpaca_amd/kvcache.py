@@ -19,49 +19,55 @@ from . import _lib as L
 from .model import HIPContext, _LIVE
 
 DTYPE = {"f32": L.F32, "f16": L.F16}
+WORKSPACE_ZERO = 2048  # AHIP_Q4_WORKSPACE_ZERO
 
 
 class Q4Cache:
     """Keys and values of up to ``capacity`` tokens, Q4_0 blocks along the head dimension."""
 
     def __init__(self, context: HIPContext, kv_heads: int, capacity: int, head_dim: int):
-        n = C.c_int64()
-        L.check(L.lib().ahip_kv_q4_bytes(kv_heads, capacity, head_dim, C.byref(n)))
+        lib, n = L.lib(), C.c_int64()
+        L.check(lib.ahip_kv_q4_bytes(kv_heads, capacity, head_dim, C.byref(n)))
         self.context, self.kv_heads, self.capacity, self.head_dim = context, kv_heads, capacity, head_dim
         self.bytes = 2 * n.value
-        self._k = self._v = self._work = None
-        self._work_bytes = 0
-        self._needs = {}
+        self._ctx = context.handle
+        self._desc = L.KVQ4C(None, None, kv_heads, head_dim, capacity)
+        self._cache = C.byref(self._desc)
+        self._width = kv_heads * head_dim
+        self._store, self._load, self._attention = lib.ahip_kv_q4_store, lib.ahip_kv_q4_load, lib.ahip_attention_q4
+        self._work, self._work_bytes, self._reserved = None, 0, set()
         self._kind = "cache"
         _LIVE.add(self)
-        self._k, self._v = self._malloc(n.value), self._malloc(n.value)
+        self._desc.k, self._desc.v = self._malloc(n.value), self._malloc(n.value)
 
     def _malloc(self, n: int) -> int:
         p = C.c_void_p()
-        L.check(L.lib().ahip_malloc(self.context.handle, n, C.byref(p)))
+        L.check(L.lib().ahip_malloc(self._ctx, n, C.byref(p)))
         return p.value
 
     def store(self, k: int, v: int, tokens: int, start: int = 0, dtype: str = "f32", k_stride: int | None = None,
               v_stride: int | None = None, start_dev: int | None = None, stream=None) -> None:
         """Quantises rows of keys and values into positions start.. (or *start_dev..)."""
-        w = self.kv_heads * self.head_dim
-        L.check(L.lib().ahip_kv_q4_store(self.context.handle, DTYPE[dtype], k, w if k_stride is None else k_stride, v,
-                                         w if v_stride is None else v_stride, tokens, start, start_dev, self._k,
-                                         self._v, self.kv_heads, self.head_dim, self.capacity, stream))
+        rc = self._store(self._ctx, self._cache, DTYPE[dtype], k, self._width if k_stride is None else k_stride, v,
+                         self._width if v_stride is None else v_stride, tokens, start, start_dev, stream)
+        if rc:
+            L.check(rc)
 
     def load(self, k_out: int | None, v_out: int | None, tokens: int, start: int = 0, dtype: str = "f32",
              k_stride: int | None = None, v_stride: int | None = None, stream=None) -> None:
         """The values of positions start.. as rows."""
-        w = self.kv_heads * self.head_dim
-        L.check(L.lib().ahip_kv_q4_load(self.context.handle, DTYPE[dtype], self._k, self._v, self.kv_heads,
-                                        self.head_dim, self.capacity, start, tokens, k_out,
-                                        w if k_stride is None else k_stride, v_out,
-                                        w if v_stride is None else v_stride, stream))
+        rc = self._load(self._ctx, self._cache, DTYPE[dtype], start, tokens, k_out,
+                        self._width if k_stride is None else k_stride, v_out,
+                        self._width if v_stride is None else v_stride, stream)
+        if rc:
+            L.check(rc)
 
-    def workspace_bytes(self, tokens: int, heads: int, start: int = 0, on_device: bool = False) -> int:
+    def workspace_bytes(self, tokens: int, heads: int, start: int = 0, dtype: str = "f32",
+                        on_device: bool = False) -> int:
+        """Bytes of workspace of an attention call with these arguments (on_device: with start_dev)."""
         n = C.c_int64()
-        L.check(L.lib().ahip_attention_q4_workspace(self.context.handle, tokens, heads, self.kv_heads, self.head_dim,
-                                                    start, 1 if on_device else 0, self.capacity, C.byref(n)))
+        L.check(L.lib().ahip_attention_q4_workspace(self._ctx, self._cache, DTYPE[dtype], tokens, heads, start,
+                                                    1 if on_device else 0, C.byref(n)))
         return n.value
 
     def attention(self, q: int, out: int, tokens: int, heads: int, start: int = 0, dtype: str = "f32",
@@ -69,44 +75,49 @@ class Q4Cache:
                   workspace: tuple | None = None, stream=None) -> None:
         """Causal attention of queries at positions start.. (or *start_dev..).
 
-        ``workspace`` is (address, bytes); None takes the cache's own, which
-        grows to what the calls so far needed (an allocation: a call that is
-        captured into a graph, or calls on several streams, pass theirs)."""
-        w = heads * self.head_dim
+        ``workspace`` is (address, bytes), its first WORKSPACE_ZERO bytes cleared
+        once; None takes the cache's own, which grows on the first call of so many
+        tokens and heads to what they need at any position (an allocation: a call
+        that is captured into a graph, or calls on several streams, pass theirs)."""
         if workspace is None:
-            key = (tokens, heads, start, start_dev is not None)
-            need = self._needs.get(key)
-            if need is None:
-                need = self._needs[key] = self.workspace_bytes(tokens, heads, start, start_dev is not None)
-                if len(self._needs) > 1024:
-                    self._needs = {key: need}
-            if need > self._work_bytes:
-                self._grow(need)
-            workspace = (self._work, self._work_bytes)
-        L.check(L.lib().ahip_attention_q4(self.context.handle, DTYPE[dtype], q, w if q_stride is None else q_stride,
-                                          tokens, heads, start, start_dev, self._k, self._v, self.kv_heads,
-                                          self.head_dim, self.capacity, out, w if out_stride is None else out_stride,
-                                          workspace[0], workspace[1], stream))
+            if (tokens, heads, dtype) not in self._reserved:
+                self._reserve(tokens, heads, dtype)
+            work, work_bytes = self._work, self._work_bytes
+        else:
+            work, work_bytes = workspace
+        w = heads * self.head_dim
+        rc = self._attention(self._ctx, self._cache, DTYPE[dtype], q, w if q_stride is None else q_stride, tokens,
+                             heads, start, start_dev, out, w if out_stride is None else out_stride, work, work_bytes,
+                             stream)
+        if rc:
+            L.check(rc)
 
-    def _grow(self, need: int) -> None:
-        if self._work:
-            # hipFree waits for the device: queued calls may still use the old one
-            L.check(L.lib().ahip_free(self.context.handle, self._work))
-            self._work, self._work_bytes = None, 0
-        self._work = self._malloc(need)
-        self._work_bytes = need
+    def _reserve(self, tokens: int, heads: int, dtype: str) -> None:
+        # the need grows with the positions seen, so the capacity's serves all
+        need = self.workspace_bytes(tokens, heads, 0, dtype, True)
+        if need > self._work_bytes:
+            if self._work:
+                # hipFree waits for the device: queued calls may still use the old one
+                L.check(L.lib().ahip_free(self._ctx, self._work))
+                self._work, self._work_bytes = None, 0
+            self._work = self._malloc(need)
+            L.check(L.lib().ahip_memset(self._ctx, self._work, 0, WORKSPACE_ZERO))
+            self._work_bytes = need
+        self._reserved.add((tokens, heads, dtype))
 
     def close(self) -> None:
+        """Frees the cache; calls on it are over."""
         if not getattr(self.context, "handle", None):
             return
-        for p in (self._k, self._v, self._work):
+        for p in (self._desc.k, self._desc.v, self._work):
             if p:
-                L.lib().ahip_free(self.context.handle, p)
-        self._k = self._v = self._work = None
+                L.lib().ahip_free(self._ctx, p)
+        self._desc.k = self._desc.v = self._work = None
         self._work_bytes = 0
+        self._reserved.clear()
 
     def __del__(self):
-        if hasattr(self, "_k"):
+        if hasattr(self, "_desc"):
             self.close()
 
 
@@ -126,8 +137,11 @@ def qk_norm_rope(context: HIPContext, q: int | None, k: int | None, tokens: int,
     """Per-head RMS norm of queries and keys (where a gain is given) and their
     rotation (where a table is), ahip_qk_norm_rope."""
     qw, kw = heads * head_dim, kv_heads * head_dim
-    L.check(L.lib().ahip_qk_norm_rope(
-        context.handle, DTYPE[dtype], q, qw if q_stride is None else q_stride, heads, q_gain, k,
-        kw if k_stride is None else k_stride, kv_heads, k_gain, tokens, head_dim, eps, rope, rope_positions,
-        1 if interleaved else 0, start, positions, q_out, qw if q_out_stride is None else q_out_stride, k_out,
-        kw if k_out_stride is None else k_out_stride, stream))
+    args = L.NormRopeC(q, q_out, q_gain, qw if q_stride is None else q_stride,
+                       qw if q_out_stride is None else q_out_stride, k, k_out, k_gain,
+                       kw if k_stride is None else k_stride, kw if k_out_stride is None else k_out_stride, rope,
+                       positions, DTYPE[dtype], tokens, heads, kv_heads, head_dim, rope_positions,
+                       1 if interleaved else 0, start, eps)
+    rc = L.lib().ahip_qk_norm_rope(context.handle, C.byref(args), stream)
+    if rc:
+        L.check(rc)

@@ -366,7 +366,7 @@ int ahip_attention_decode_noalloc(ahip_context* ctx, const float* q, const void*
  * rows may be part of wider ones ([q | k | v]).  head_dim is a multiple of 32
  * up to 256.
  *
- * k_cache and v_cache are buffers of ahip_kv_q4_bytes each, 16-byte aligned,
+ * A cache's k and v are buffers of ahip_kv_q4_bytes each, 16-byte aligned,
  * laid out for the kernels (in tiles of 32 tokens; ahip_kv_q4_load gives the
  * values).  They need no clearing: only positions that were written are read.
  *
@@ -374,48 +374,63 @@ int ahip_attention_decode_noalloc(ahip_context* ctx, const float* q, const void*
  * token when the kernels run, `start` being ignored: a captured graph then
  * follows it.  A range past the capacity stores nothing, and attends to NaN. */
 
-/* Bytes of k_cache, and of v_cache. */
+typedef struct {
+    void* k;
+    void* v;
+    int32_t kv_heads, head_dim, capacity;
+} ahip_kv_q4;
+/* Bytes of a cache's k, and of its v. */
 int ahip_kv_q4_bytes(int kv_heads, int capacity, int head_dim, int64_t* bytes);
 /* Quantises `tokens` rows of keys and values into positions start.. as
  * ahip_quantize(AHIP_Q4_0) does, bit for bit; other positions keep their bytes.
  * A token whose keys or values of a KV head hold a NaN, an infinity or a
  * magnitude past 65,504 reads back as NaN in that head, keys and values, and
  * gives NaN to the queries that see it and to no others. */
-int ahip_kv_q4_store(ahip_context* ctx, int dtype, const void* k, int64_t k_stride, const void* v, int64_t v_stride,
-                     int tokens, int start, const int32_t* start_dev, void* k_cache, void* v_cache, int kv_heads,
-                     int head_dim, int capacity, ahip_stream* stream);
+int ahip_kv_q4_store(ahip_context* ctx, const ahip_kv_q4* cache, int dtype, const void* k, int64_t k_stride,
+                     const void* v, int64_t v_stride, int tokens, int start, const int32_t* start_dev,
+                     ahip_stream* stream);
 /* The values of positions start.. as rows; k or v may be null. */
-int ahip_kv_q4_load(ahip_context* ctx, int dtype, const void* k_cache, const void* v_cache, int kv_heads, int head_dim,
-                    int capacity, int start, int tokens, void* k, int64_t k_stride, void* v, int64_t v_stride,
-                    ahip_stream* stream);
+int ahip_kv_q4_load(ahip_context* ctx, const ahip_kv_q4* cache, int dtype, int start, int tokens, void* k,
+                    int64_t k_stride, void* v, int64_t v_stride, ahip_stream* stream);
 /* Causal grouped-query attention (as ahip_op_attention) of `tokens` queries at
  * positions start.. over the cache, which already holds their keys and values.
  * q and out rows [heads][head_dim]; out may not overlap q.  With AHIP_F32 the
  * scores, probabilities and sums keep float32 accuracy over the cache's exact
- * values; with AHIP_F16 the probabilities and values enter the products in f16,
- * and sums are float32.  `workspace` (16-byte aligned) holds the partial results
- * of the key ranges: ahip_attention_q4_workspace bytes for the same arguments
- * (on_device: whether start_dev is set), its contents meaningless before and
- * after.  Calls that may run at the same time need workspaces of their own. */
-int ahip_attention_q4_workspace(ahip_context* ctx, int tokens, int heads, int kv_heads, int head_dim, int start,
-                                int on_device, int capacity, int64_t* bytes);
-int ahip_attention_q4(ahip_context* ctx, int dtype, const void* q, int64_t q_stride, int tokens, int heads, int start,
-                      const int32_t* start_dev, const void* k_cache, const void* v_cache, int kv_heads, int head_dim,
-                      int capacity, void* out, int64_t out_stride, void* workspace, int64_t workspace_bytes,
-                      ahip_stream* stream);
+ * values; with AHIP_F16 keys, values and probabilities enter the products rounded
+ * to f16, and sums are float32.  `workspace` (16-byte aligned) holds the partial results
+ * of the key ranges and the counters of their arrival: ahip_attention_q4_workspace
+ * bytes for the same arguments (on_device: whether start_dev is set).  Its first
+ * AHIP_Q4_WORKSPACE_ZERO bytes are zero before its first call, and every call
+ * leaves them so: clear them once, and let one workspace of the largest size serve
+ * any calls that come one after another.  Calls that may run at the same time,
+ * captured graphs among them, need workspaces of their own. */
+#define AHIP_Q4_WORKSPACE_ZERO 2048
+int ahip_attention_q4_workspace(ahip_context* ctx, const ahip_kv_q4* cache, int dtype, int tokens, int heads,
+                                int start, int on_device, int64_t* bytes);
+int ahip_attention_q4(ahip_context* ctx, const ahip_kv_q4* cache, int dtype, const void* q, int64_t q_stride,
+                      int tokens, int heads, int start, const int32_t* start_dev, void* out, int64_t out_stride,
+                      void* workspace, int64_t workspace_bytes, ahip_stream* stream);
 /* RMS norm of every head of q and k over its head_dim values (y = x / sqrt(mean
  * x^2 + eps) * gain), then the rotation (ahip_op_rope), in one pass and float32.
- * q_gain, k_gain: head_dim floats, null for no norm; rope: (cos, sin) pairs
- * [rope_positions][head_dim / 2], as ahip_rope_table makes them, null for no
- * rotation.  Token t has position start + t, or positions[t] where that is set
- * (a token of a position outside the table gets NaN).  heads or kv_heads may be
- * 0.  An output may be its own input with the same stride, or else may not
- * overlap an input. */
-int ahip_qk_norm_rope(ahip_context* ctx, int dtype, const void* q, int64_t q_stride, int heads, const float* q_gain,
-                      const void* k, int64_t k_stride, int kv_heads, const float* k_gain, int tokens, int head_dim,
-                      float eps, const float* rope, int rope_positions, int interleaved, int start,
-                      const int32_t* positions, void* q_out, int64_t q_out_stride, void* k_out, int64_t k_out_stride,
-                      ahip_stream* stream);
+ * A gain of null: no norm; rope null: no rotation.  Token t has position
+ * start + t, or positions[t] where that is set (a token of a position outside
+ * the table gets NaN).  heads or kv_heads may be 0.  An output may be its own
+ * input with the same stride, or else may not overlap an input. */
+typedef struct {
+    const void* q;            /* rows [tokens][heads][head_dim] */
+    void* q_out;
+    const float* q_gain;      /* [head_dim] */
+    int64_t q_stride, q_out_stride;
+    const void* k;            /* rows [tokens][kv_heads][head_dim] */
+    void* k_out;
+    const float* k_gain;
+    int64_t k_stride, k_out_stride;
+    const float* rope;        /* (cos, sin) [rope_positions][head_dim / 2], as ahip_rope_table makes it */
+    const int32_t* positions; /* [tokens], or null */
+    int32_t dtype, tokens, heads, kv_heads, head_dim, rope_positions, interleaved, start;
+    float eps;
+} ahip_norm_rope;
+int ahip_qk_norm_rope(ahip_context* ctx, const ahip_norm_rope* args, ahip_stream* stream);
 /* The table, into host memory: angles in double, rounded once to float (CPUOps.rope,
  * CPUOps.swift:196-201); positions * head_dim floats. */
 int ahip_rope_table(int positions, int head_dim, float theta, float* table);

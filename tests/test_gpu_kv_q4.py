@@ -5,7 +5,7 @@ import pytest
 
 import oracle.oracle as orc
 from alpaca_amd import _lib as L
-from alpaca_amd.kvcache import Q4Cache, qk_norm_rope, rope_table
+from alpaca_amd.kvcache import WORKSPACE_ZERO, Q4Cache, qk_norm_rope, rope_table
 from alpaca_amd.tensor import Q4_0
 from tests import q4_reference as ref
 
@@ -113,7 +113,7 @@ def test_positions_that_are_not_written_keep_their_bytes(hip_ctx):
     cache = Q4Cache(hip_ctx, 3, 100, 96)
     with ref.Device(hip_ctx) as dev:
         store(dev, cache, k, v, 0, "f32")
-        before = [dev.get(p, cache.bytes // 2, np.uint8) for p in (cache._k, cache._v)]
+        before = [dev.get(p, cache.bytes // 2, np.uint8) for p in (cache._desc.k, cache._desc.v)]
         for start, n in ((37, 1), (50, 20), (0, 2), (99, 1), (64, 32)):
             a, b = rows(rng, n, 3, 96, "f32"), rows(rng, n, 3, 96, "f32")
             store(dev, cache, a, b, start, "f32")
@@ -122,7 +122,7 @@ def test_positions_that_are_not_written_keep_their_bytes(hip_ctx):
             assert all(equal(g, w) for g, w in zip(got, want)), (start, n)
         # the padding behind the last position is never written
         cache.store(dev.put(k), dev.put(v), 100, 0)
-        after = [dev.get(p, cache.bytes // 2, np.uint8) for p in (cache._k, cache._v)]
+        after = [dev.get(p, cache.bytes // 2, np.uint8) for p in (cache._desc.k, cache._desc.v)]
     assert all(np.array_equal(a, b) for a, b in zip(before, after))
 
 
@@ -266,7 +266,7 @@ def test_attention_never_reads_positions_past_its_own(hip_ctx, dtype):
     for tail in (0, 1, np.nan):
         cache = Q4Cache(hip_ctx, 2, 300, 64)
         with ref.Device(hip_ctx) as dev:
-            for p in (cache._k, cache._v):
+            for p in (cache._desc.k, cache._desc.v):
                 L.check(L.lib().ahip_memset(hip_ctx.handle, p, 0xFF, cache.bytes // 2))
             if tail != 0:
                 store(dev, cache, k * tail, v * tail, 0, "f32")
@@ -304,7 +304,8 @@ def test_attention_twice_gives_the_same_bits(hip_ctx):
         store(dev, cache, k, v, 0, "f32")
         a = run_attention(dev, cache, q, 2997, "f32")
         need = cache.workspace_bytes(3, 8, 2997)
-        mine = (dev.empty(need, 0xFF), need)  # another workspace, its bytes NaN
+        mine = (dev.empty(need, 0xFF), need)  # another workspace, its bytes NaN but for the counters
+        L.check(L.lib().ahip_memset(hip_ctx.handle, mine[0], 0, min(need, WORKSPACE_ZERO)))
         b = run_attention(dev, cache, q, 2997, "f32", workspace=mine)
         if need:
             with pytest.raises(L.InvalidArgument, match="workspace"):
@@ -409,7 +410,7 @@ def test_a_layer_s_steps_together_on_a_stream(hip_ctx):
     with ref.Device(hip_ctx) as dev:
         p, g, tab, out = dev.put(qkv), dev.put(gain), dev.put(table), dev.empty(cap * H * hd * 4)
         work = max(cache.workspace_bytes(n, H, sum(lens[:i])) for i, n in enumerate(lens))
-        ws = (dev.empty(max(work, 1)), work)
+        ws = (dev.empty(max(work, 1), 0), work)
         at = 0
         for n in lens:
             row = p + at * w * 4

@@ -33,9 +33,12 @@ def test_cache_bytes():
     refused(L.lib().ahip_kv_q4_bytes(1, 1, 64, None), "null")
 
 
-def store(ctx=ctx, dtype=F32, k=P, ks=128, v=P, vs=128, tokens=4, start=0, start_dev=None, kc=P, vc=P, kv_heads=2,
-          hd=64, cap=100):
-    return L.lib().ahip_kv_q4_store(ctx, dtype, k, ks, v, vs, tokens, start, start_dev, kc, vc, kv_heads, hd, cap, None)
+def cache(kc=P, vc=P, kv_heads=2, hd=64, cap=100):
+    return C.byref(L.KVQ4C(kc, vc, kv_heads, hd, cap))
+
+
+def store(ctx=ctx, dtype=F32, k=P, ks=128, v=P, vs=128, tokens=4, start=0, start_dev=None, **c):
+    return L.lib().ahip_kv_q4_store(ctx, cache(**c), dtype, k, ks, v, vs, tokens, start, start_dev, None)
 
 
 def test_store_refusals():
@@ -62,8 +65,8 @@ def test_store_refusals():
     assert store(tokens=0, k=None, v=None) == 0  # nothing to do
 
 
-def load(ctx=ctx, dtype=F32, kc=P, vc=P, kv_heads=2, hd=64, cap=100, start=0, tokens=4, k=P, ks=128, v=P, vs=128):
-    return L.lib().ahip_kv_q4_load(ctx, dtype, kc, vc, kv_heads, hd, cap, start, tokens, k, ks, v, vs, None)
+def load(ctx=ctx, dtype=F32, start=0, tokens=4, k=P, ks=128, v=P, vs=128, **c):
+    return L.lib().ahip_kv_q4_load(ctx, cache(**c), dtype, start, tokens, k, ks, v, vs, None)
 
 
 def test_load_refusals():
@@ -77,10 +80,10 @@ def test_load_refusals():
     assert load(tokens=0) == 0 and load(k=None, v=None) == 0
 
 
-def attention(ctx=ctx, dtype=F32, q=P, qs=256, tokens=4, heads=4, start=10, start_dev=None, kc=P, vc=P, kv_heads=2,
-              hd=64, cap=100, out=P, os=256, ws=None, wb=0):
-    return L.lib().ahip_attention_q4(ctx, dtype, q, qs, tokens, heads, start, start_dev, kc, vc, kv_heads, hd, cap, out,
-                                     os, ws, wb, None)
+def attention(ctx=ctx, dtype=F32, q=P, qs=256, tokens=4, heads=4, start=10, start_dev=None, out=P, os=256, ws=None,
+              wb=0, **c):
+    return L.lib().ahip_attention_q4(ctx, cache(**c), dtype, q, qs, tokens, heads, start, start_dev, out, os, ws, wb,
+                                     None)
 
 
 def test_attention_refusals():
@@ -108,25 +111,32 @@ def test_attention_refusals():
 
 def test_workspace_refusals():
     n = C.c_int64()
-    f = L.lib().ahip_attention_q4_workspace
-    refused(f(None, 1, 4, 2, 64, 0, 0, 100, C.byref(n)), "null")
-    refused(f(ctx, 1, 4, 2, 64, 0, 0, 100, None), "null")
-    refused(f(ctx, 1, 5, 2, 64, 0, 0, 100, C.byref(n)), "multiple")
-    refused(f(ctx, 1, 4, 2, 65, 0, 0, 100, C.byref(n)), "head dimension")
-    refused(f(ctx, 1, 4, 2, 64, 100, 0, 100, C.byref(n)), "capacity")
-    refused(f(ctx, 101, 4, 2, 64, 0, 1, 100, C.byref(n)), "more tokens")
+
+    def f(ctx=ctx, dtype=F32, tokens=1, heads=4, start=0, on_device=0, n=n, **c):
+        return L.lib().ahip_attention_q4_workspace(ctx, cache(**c), dtype, tokens, heads, start, on_device,
+                                                   None if n is None else C.byref(n))
+    refused(f(ctx=None), "null")
+    refused(f(n=None), "null")
+    refused(f(dtype=L.Q4_0), "rows must be")
+    refused(f(heads=5), "multiple")
+    refused(f(hd=65), "head dimension")
+    refused(f(start=100), "capacity")
+    refused(f(tokens=101, on_device=1), "more tokens")
+    refused(L.lib().ahip_attention_q4_workspace(ctx, None, F32, 1, 4, 0, 0, C.byref(n)), "null cache")
     n.value = 7
-    assert f(ctx, 0, 4, 2, 64, 0, 0, 100, C.byref(n)) == 0 and n.value == 0
+    assert f(tokens=0) == 0 and n.value == 0
 
 
 def norm_rope(ctx=ctx, dtype=F32, q=P, qs=256, heads=4, qg=P, k=P, ks=128, kv_heads=2, kg=P, tokens=4, hd=64, eps=1e-5,
               rope=P, positions=100, start=0, pos=None, qo=P, qos=256, ko=P, kos=128):
-    return L.lib().ahip_qk_norm_rope(ctx, dtype, q, qs, heads, qg, k, ks, kv_heads, kg, tokens, hd, eps, rope,
-                                     positions, 1, start, pos, qo, qos, ko, kos, None)
+    a = L.NormRopeC(q, qo, qg, qs, qos, k, ko, kg, ks, kos, rope, pos, dtype, tokens, heads, kv_heads, hd, positions,
+                    1, start, eps)
+    return L.lib().ahip_qk_norm_rope(ctx, C.byref(a), None)
 
 
 def test_norm_rope_refusals():
     refused(norm_rope(ctx=None), "null context")
+    refused(L.lib().ahip_qk_norm_rope(ctx, None, None), "null arguments")
     refused(norm_rope(dtype=L.Q8_0), "rows must be")
     refused(norm_rope(hd=72), "head dimension")
     refused(norm_rope(heads=-1), "head counts")
