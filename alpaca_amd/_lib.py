@@ -15,7 +15,7 @@ SHIM_CODE_OBJECT = os.path.join(HERE, "shim_kernels.hsaco")
 
 OK, NO_DEVICE, MODULE_LOAD, MISSING_KERNEL, ALLOC, COMMAND_FAILED, UNSUPPORTED, INVALID_ARGUMENT, BUSY, GGUF = range(10)
 F32, F16, Q8_0, Q4_0 = 0, 1, 2, 3
-KV_F16, KV_F32 = 0, 1
+KV_F16, KV_F32, KV_Q4_0 = 0, 1, 2
 GEMM_EXACT, GEMM_FAST, GEMM_FAST_F16 = 0, 1, 2
 
 STATUS_NAMES = {
@@ -159,6 +159,7 @@ SIGNATURES = {
     "ahip_op_linear_add": (i, [vp, fp, i, i, i, vp, i, i, fp]),
     "ahip_op_gate_up_silu": (i, [vp, fp, i, i, i, vp, vp, i, i, fp]),
     "ahip_op_rope": (i, [vp, fp, i, i, i, i, C.c_float, i]),
+    "ahip_op_qk_norm_rope": (i, [vp, fp, i, fp, fp, i, fp, i, i, C.c_float, i, C.c_float, i]),
     "ahip_op_attention": (i, [vp, fp, i, i, i, fp, fp, i, i, i, i, i, fp]),
     "ahip_op_embed": (i, [vp, ip, i, i, vp, i, i, fp]),
     "ahip_op_dequantize": (i, [vp, i, vp, i64, fp]),

@@ -886,8 +886,13 @@ Q4Plan q4_attention_plan(bool f16_rows, int tokens, int heads, int kv_heads, int
     return r;
 }
 
-int64_t q4_attention_partials(int tokens, int heads, int hd, int splits) {
-    return splits > 1 ? (int64_t)tokens * heads * splits * (hd + 2) : 0;
+int64_t q4_attention_workspace(int tokens, int heads, int hd, const Q4Plan& plan) {
+    return plan.splits > 1 ? kQ4Counters * 4 + (int64_t)tokens * heads * plan.splits * (hd + 2) * 4 : 0;
+}
+
+void q4_set_workspace(Q4Attention& a, void* workspace) {
+    a.counters = (int*)workspace;
+    a.partials = (float*)((uint8_t*)workspace + kQ4Counters * 4);
 }
 
 hipError_t launch_q4_attention(bool f16_rows, const Q4Attention& a, const Q4Cache& c, const Q4Plan& plan,

@@ -140,10 +140,6 @@ static Q4Plan plan_of(const ahip_kv_q4* c, int dtype, int tokens, int heads, int
 }
 
 static_assert(kQ4Counters * 4 == AHIP_Q4_WORKSPACE_ZERO, "the counters at the front of a workspace");
-// The counters, always at the front, then the partial results.
-static int64_t workspace_need(int tokens, int heads, int hd, int splits) {
-    return splits > 1 ? kQ4Counters * 4 + q4_attention_partials(tokens, heads, hd, splits) * 4 : 0;
-}
 
 extern "C" int ahip_attention_q4_workspace(ahip_context* ctx, const ahip_kv_q4* cache, int dtype, int tokens,
                                            int heads, int start, int on_device, int64_t* bytes) {
@@ -157,8 +153,8 @@ extern "C" int ahip_attention_q4_workspace(ahip_context* ctx, const ahip_kv_q4* 
     if (tokens == 0) return AHIP_OK;
     hipStream_t st;
     if (int rc = stream_of(ctx, nullptr, &st)) return rc;  // (the device's CU count)
-    *bytes = workspace_need(tokens, heads, cache->head_dim,
-                            plan_of(cache, dtype, tokens, heads, start, on_device).splits);
+    *bytes = q4_attention_workspace(tokens, heads, cache->head_dim,
+                                    plan_of(cache, dtype, tokens, heads, start, on_device));
     return AHIP_OK;
 }
 
@@ -178,7 +174,7 @@ extern "C" int ahip_attention_q4(ahip_context* ctx, const ahip_kv_q4* cache, int
     hipStream_t st;
     if (int rc = stream_of(ctx, stream, &st)) return rc;
     const Q4Plan plan = plan_of(cache, dtype, tokens, heads, start, start_dev);
-    const int64_t need = workspace_need(tokens, heads, cache->head_dim, plan.splits);
+    const int64_t need = q4_attention_workspace(tokens, heads, cache->head_dim, plan);
     if (need && (!workspace || workspace_bytes < need || ((uintptr_t)workspace & 15)))
         return bad("the attention needs " + std::to_string(need) + " bytes of 16-byte aligned workspace, got " +
                    std::to_string(workspace ? workspace_bytes : 0));
@@ -191,8 +187,7 @@ extern "C" int ahip_attention_q4(ahip_context* ctx, const ahip_kv_q4* cache, int
     a.heads = heads;
     a.start = start;
     a.start_dev = start_dev;
-    a.counters = (int*)workspace;
-    a.partials = (float*)((uint8_t*)workspace + kQ4Counters * 4);
+    q4_set_workspace(a, workspace);
     return launched(launch_q4_attention(dtype == AHIP_F16, a, cache_of(cache), plan, st));
 }
 

@@ -65,6 +65,17 @@ struct HeadRows {
 // outside the cache then writes nothing).
 hipError_t launch_q4_store(bool f16_rows, HeadRows k, HeadRows v, int tokens, int start, const int* start_dev,
                            const Q4Cache& c, hipStream_t st);
+// A session's rows [q | k | v] (interleaved pairs): q rotated in place or, with q16 set, into
+// f16 rows [heads][hd]; k rotated and v written at positions start.. .
+struct Q4Queries {
+    float* q = nullptr;
+    int64_t stride = 0;
+    int heads = 0;
+    const float2* rope = nullptr;  // (cos, sin) [positions][hd / 2]
+    f16* q16 = nullptr;
+};
+hipError_t launch_q4_append(const Q4Queries& q, int tokens, int start, const int* start_dev, const Q4Cache& c,
+                            hipStream_t st);
 // Reads them back; k_out or v_out may be null.
 hipError_t launch_q4_load(bool f16_rows, const Q4Cache& c, int start, int tokens, void* k_out, int64_t k_stride,
                           void* v_out, int64_t v_stride, hipStream_t st);
@@ -93,6 +104,8 @@ struct Q4Plan {
     bool fused = false;
 };
 Q4Plan q4_attention_plan(bool f16_rows, int tokens, int heads, int kv_heads, int hd, int length);
-int64_t q4_attention_partials(int tokens, int heads, int hd, int splits);  // floats
+// Bytes of a launch's workspace, the counters first; 0 for one part.
+int64_t q4_attention_workspace(int tokens, int heads, int hd, const Q4Plan& plan);
+void q4_set_workspace(Q4Attention& a, void* workspace);
 hipError_t launch_q4_attention(bool f16_rows, const Q4Attention& a, const Q4Cache& c, const Q4Plan& plan,
                                hipStream_t st);

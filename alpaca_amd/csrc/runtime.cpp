@@ -25,6 +25,7 @@
 #include "../../include/alpaca_hip.h"
 #include "common.h"
 #include "host.h"
+#include "kv_q4.h"
 
 // ------------------------------------------------------------------ errors
 
@@ -625,16 +626,30 @@ extern "C" int ahip_model_prefill_cache_bytes(const ahip_model* m, int64_t* byte
 // ------------------------------------------------------------------ session
 
 struct SessionSizes {
-    int64_t kv_per_layer, x, qkv, q16, ctx, ffn, partials, logits;
+    int64_t kv_per_layer, x, qkv, q16, ctx, ffn, partials, logits, q4_work;
     int64_t total;
 };
 
 static constexpr int kMaxSplits = 65;
 
-static SessionSizes session_sizes(const ahip_llama_config& c, int capacity, int max_batch, int kv_f16) {
+// The largest workspace that the attention over a 4-bit cache takes in calls of up to max_batch tokens.
+static int64_t q4_session_workspace(const ahip_llama_config& c, int capacity, int max_batch) {
+    int64_t most = 0;
+    for (int n = 1; n <= std::min(max_batch, capacity); n++)
+        for (bool f16_rows : {false, true})
+            most = std::max(most, q4_attention_workspace(n, c.head_count, c.head_dim,
+                                                         q4_attention_plan(f16_rows, n, c.head_count, c.kv_head_count,
+                                                                           c.head_dim, capacity)));
+    return (most + 255) / 256 * 256;
+}
+
+static SessionSizes session_sizes(const ahip_llama_config& c, int capacity, int max_batch, int kv_precision) {
     SessionSizes s{};
     const int64_t B = max_batch, QW = (int64_t)c.head_count * c.head_dim, KW = (int64_t)c.kv_head_count * c.head_dim;
-    s.kv_per_layer = (int64_t)capacity * KW * (kv_f16 ? 2 : 4);
+    const bool q4 = kv_precision == AHIP_KV_Q4_0;
+    s.kv_per_layer = q4 ? (int64_t)c.kv_head_count * q4_head_bytes(capacity, c.head_dim / 32)
+                        : (int64_t)capacity * KW * (kv_precision == AHIP_KV_F16 ? 2 : 4);
+    s.q4_work = q4 ? 2 * q4_session_workspace(c, capacity, max_batch) : 0;  // one for each stream of a split prefill
     s.x = B * c.hidden_size;
     s.qkv = B * (QW + 2 * KW);
     s.q16 = B * QW;
@@ -644,14 +659,16 @@ static SessionSizes session_sizes(const ahip_llama_config& c, int capacity, int 
     s.logits = c.vocab_size;
     // the f16 activation buffers hold two planes (the two-term activations' hi and lo)
     s.total = 2 * c.layer_count * s.kv_per_layer + 4 * (2 * s.x + s.qkv + s.ctx + s.ffn + s.partials + s.logits) +
-              4 * (s.x + s.q16 + s.ctx + s.ffn) + 4 * ((int64_t)capacity + 9 + capacity);
+              4 * (s.x + s.q16 + s.ctx + s.ffn) + 4 * ((int64_t)capacity + 9 + capacity) + s.q4_work;
     return s;
 }
 
 extern "C" int ahip_session_byte_count(const ahip_llama_config* config, int capacity, int max_batch, int kv_precision,
                                        int64_t* bytes) {
     if (!config || !bytes || capacity <= 0 || max_batch <= 0) return fail(AHIP_ERR_INVALID_ARGUMENT, "bad argument");
-    *bytes = session_sizes(*config, capacity, max_batch, kv_precision == AHIP_KV_F16).total;
+    if (kv_precision == AHIP_KV_Q4_0)
+        if (int rc = validate_config(config)) return rc;
+    *bytes = session_sizes(*config, capacity, max_batch, kv_precision).total;
     return AHIP_OK;
 }
 
@@ -666,6 +683,9 @@ static void split_stream_release(int device);  // below, with the split prefill
 struct ahip_session {
     ahip_model* m = nullptr;
     int capacity = 0, max_batch = 0, kv_f16 = 1, fast = 1;
+    bool kv_q4 = false;         // the cache in 4 bits (kv_q4.h), kc / vc its buffers
+    DevBuf q4_work;             // its attention's workspaces, one for each stream of a split prefill
+    int64_t q4_work_bytes = 0;  // of each
     int two_term = 1;  // fast prefill with two-term activations (AHIP_GEMM_FAST); 0: one f16 term (FAST_F16)
     int lo_terms = 0;  // with two_term: which operands carry the second term (kLo* bits)
     bool lo_all_rows = false;  // second terms on every row, not only the last row's tiles
@@ -1159,7 +1179,8 @@ extern "C" int ahip_session_create(ahip_model* m, int capacity, int max_batch, i
     if (!m || !out) return fail(AHIP_ERR_INVALID_ARGUMENT, "null argument");
     drop_stale_error();
     if (capacity <= 0 || max_batch <= 0) return fail(AHIP_ERR_INVALID_ARGUMENT, "capacity and maxBatch must be positive");
-    if (kv_precision != AHIP_KV_F16 && kv_precision != AHIP_KV_F32) return fail(AHIP_ERR_INVALID_ARGUMENT, "bad kv precision");
+    if (kv_precision != AHIP_KV_F16 && kv_precision != AHIP_KV_F32 && kv_precision != AHIP_KV_Q4_0)
+        return fail(AHIP_ERR_INVALID_ARGUMENT, "bad kv precision");
     if (gemm_precision != AHIP_GEMM_EXACT && gemm_precision != AHIP_GEMM_FAST && gemm_precision != AHIP_GEMM_FAST_F16)
         return fail(AHIP_ERR_INVALID_ARGUMENT, "bad gemm precision");
     const ahip_llama_config& c = m->c;
@@ -1171,6 +1192,7 @@ extern "C" int ahip_session_create(ahip_model* m, int capacity, int max_batch, i
     s->capacity = capacity;
     s->max_batch = max_batch;
     s->kv_f16 = kv_precision == AHIP_KV_F16;
+    s->kv_q4 = kv_precision == AHIP_KV_Q4_0;
     s->fast = gemm_precision != AHIP_GEMM_EXACT;
     s->two_term = gemm_precision == AHIP_GEMM_FAST;
     s->lo_terms = s->two_term ? lo_terms_for(c) : 0;
@@ -1194,12 +1216,17 @@ extern "C" int ahip_session_create(ahip_model* m, int capacity, int max_batch, i
         s->prefill_f32_gemm = g && !std::strcmp(g, "f32");
     }
     HIP_OR(hipStreamCreateWithFlags(&s->stream, hipStreamNonBlocking), "hipStreamCreate");
-    const SessionSizes z = session_sizes(c, capacity, max_batch, s->kv_f16);
+    const SessionSizes z = session_sizes(c, capacity, max_batch, kv_precision);
     for (int l = 0; l < c.layer_count; l++) {
         s->kc.emplace_back(new DevBuf());
         s->vc.emplace_back(new DevBuf());
         if (int rc = s->kc.back()->alloc(z.kv_per_layer)) return rc;
         if (int rc = s->vc.back()->alloc(z.kv_per_layer)) return rc;
+    }
+    if (z.q4_work) {
+        s->q4_work_bytes = z.q4_work / 2;
+        if (int rc = s->q4_work.alloc(z.q4_work)) return rc;
+        HIP_OR(hipMemset(s->q4_work.p, 0, z.q4_work), "hipMemset");
     }
     struct A { DevBuf* b; int64_t n; };
     for (A a : {A{&s->x, z.x * 4}, A{&s->xn, z.x * 4}, A{&s->xh, z.x * 4}, A{&s->qkv, z.qkv * 4}, A{&s->qh, z.q16 * 4},
@@ -1214,7 +1241,7 @@ extern "C" int ahip_session_create(ahip_model* m, int capacity, int max_batch, i
     HIP_OR(hipHostGetDevicePointer((void**)&s->emitted_mapped, s->emitted_host, 0), "hipHostGetDevicePointer");
     HIP_OR(hipHostGetDevicePointer((void**)&s->logits_mapped, s->logits_host, 0), "hipHostGetDevicePointer");
     HIP_OR(hipHostGetDevicePointer((void**)&s->tokens_mapped, s->tokens_host, 0), "hipHostGetDevicePointer");
-    s->dec_split = attention_decode_supported(c.head_count, c.kv_head_count, c.head_dim) &&
+    s->dec_split = !s->kv_q4 && attention_decode_supported(c.head_count, c.kv_head_count, c.head_dim) &&
                    attention_decode_session_split_len(capacity, c.head_count, c.kv_head_count) > 0;
     if (s->dec_split) {
         s->dec_split_len = attention_decode_session_split_len(capacity, c.head_count, c.kv_head_count);
@@ -1260,6 +1287,48 @@ struct BusyGuard {
 };
 
 
+// A layer's cache of a session with a 4-bit one, and its attention of n float32 or f16 rows
+// at positions pos.. (*pos_dev.. when set): `part` is the split prefill's stream.
+static Q4Cache q4_cache(const ahip_session* s, int li) {
+    Q4Cache c;
+    c.k = (uint8_t*)s->kc[li]->p;
+    c.v = (uint8_t*)s->vc[li]->p;
+    c.kv_heads = s->m->c.kv_head_count;
+    c.capacity = s->capacity;
+    c.nb = s->m->c.head_dim / 32;
+    return c;
+}
+static hipError_t q4_attend(ahip_session* s, int li, bool f16_rows, const void* q, int64_t q_stride, int n, int pos,
+                            const int* pos_dev, void* out, int part, hipStream_t st) {
+    const ahip_llama_config& c = s->m->c;
+    const Q4Plan plan = q4_attention_plan(f16_rows, n, c.head_count, c.kv_head_count, c.head_dim,
+                                          pos_dev ? s->capacity : pos + n);
+    if (q4_attention_workspace(n, c.head_count, c.head_dim, plan) > s->q4_work_bytes) return hipErrorInvalidValue;
+    Q4Attention a;
+    a.q = q;
+    a.q_stride = q_stride;
+    a.out = out;
+    a.out_stride = (int64_t)c.head_count * c.head_dim;
+    a.tokens = n;
+    a.heads = c.head_count;
+    a.start = pos;
+    a.start_dev = pos_dev;
+    q4_set_workspace(a, s->q4_work.as<uint8_t>() + part * s->q4_work_bytes);
+    return launch_q4_attention(f16_rows, a, q4_cache(s, li), plan, st);
+}
+// q4_append of n rows of the stacked projection, the queries in place or (q16) into f16.
+static hipError_t q4_append(ahip_session* s, int li, float* qkv, int n, int pos, const int* pos_dev, f16* q16,
+                            hipStream_t st) {
+    const ahip_llama_config& c = s->m->c;
+    Q4Queries q;
+    q.q = qkv;
+    q.stride = (int64_t)(c.head_count + 2 * c.kv_head_count) * c.head_dim;
+    q.heads = c.head_count;
+    q.rope = s->m->rope.as<float2>();
+    q.q16 = q16;
+    return launch_q4_append(q, n, pos, pos_dev, q4_cache(s, li), st);
+}
+
 // One decoder layer for a single token (the fused decode path,
 // MetalLlamaModel.swift:344-356): 5 launches -- QKV GEMV with RMSNorm prologue
 // and RoPE + KV-store epilogue; split-K attention; Wo GEMV merging the splits
@@ -1292,10 +1361,20 @@ static int encode_decode_layer(ahip_session* s, int li, int pos, const int* pos_
     rope.kc = kc;
     rope.vc = vc;
     rope.kv_f16 = s->kv_f16;
-    LAUNCH(launch_gemv_ex(L.qkv.m, nullptr, in, &rope, qkv, GEMV_QKV_ROPE, st));
+    if (s->kv_q4) {
+        // a block of the cache is quantised by its largest value: after the product, in its own kernel
+        LAUNCH(launch_gemv_ex(L.qkv.m, nullptr, in, nullptr, qkv, GEMV_STORE, st));
+        s->stage("rope + kv store");
+        LAUNCH(q4_append(s, li, qkv, 1, pos, pos_dev, nullptr, st));
+    } else {
+        LAUNCH(launch_gemv_ex(L.qkv.m, nullptr, in, &rope, qkv, GEMV_QKV_ROPE, st));
+    }
     s->stage("attention");
     GemvInput att;
-    if (s->dec_split) {
+    if (s->kv_q4) {
+        LAUNCH(q4_attend(s, li, false, qkv, LDQKV, 1, pos, pos_dev, s->ctx.as<float>(), 0, st));
+        att.x = s->ctx.as<float>();
+    } else if (s->dec_split) {
         // eager calls launch only the splits the context covers; graph replays cover the capacity
         const int splits = pos_dev ? s->dec_splits : (pos + s->dec_split_len) / s->dec_split_len;
         LAUNCH(launch_attention_decode(qkv, kc, vc, s->kv_f16, s->capacity, c.head_count, c.kv_head_count, hd, pos + 1,
@@ -1414,6 +1493,8 @@ static int encode_mfma_layer(ahip_session* s, int li, int row0, int n, int pos, 
     const DevMatrix& wqkv = L.pre(L.qkv, L.qkv16);
     hipError_t fused = hipErrorNotSupported;
     const bool rope_fused = flash && s->fuse_qkv_rope;
+    // the attention of a 4-bit cache: one f16 term of everything, or float32
+    const bool q4_f16 = s->kv_q4 && !s->two_term;
     QkvRope o;
     if (rope_fused) {
         // RoPE and the KV append in the GEMM epilogue (q/k/v never reach HBM as f32)
@@ -1454,7 +1535,10 @@ static int encode_mfma_layer(ahip_session* s, int li, int row0, int n, int pos, 
         if (fused == hipErrorNotSupported)
             LAUNCH(launch_gemm_mfma(xh, xhlo_qkv, H, n, wqkv, nullptr, qkv, nullptr, nullptr, LDQKV, GEMM_STORE, st));
     }
-    if (fused == hipErrorNotSupported) {
+    if (s->kv_q4) {
+        s->stage("rope + kv store");
+        LAUNCH(q4_append(s, li, qkv, n, pos, nullptr, q4_f16 ? qh : nullptr, st));
+    } else if (fused == hipErrorNotSupported) {
         s->stage("rope + kv store");
         LAUNCH(launch_rope_store(qkv, LDQKV, n, c.head_count, c.kv_head_count, hd, pos, rope, 1, flash ? 0 : 1,
                                  flash ? qh : nullptr, flash ? qhlo : nullptr, kc, vc, s->kv_f16, s->capacity, st));
@@ -1478,6 +1562,11 @@ static int encode_mfma_layer(ahip_session* s, int li, int row0, int n, int pos, 
                                       c.kv_head_count, hd, pos, nullptr, ctxh, ctxhlo, st, p_terms,
                                       all ? 0 : n - 1, tail0, exact_last ? s->last_arrive.as<unsigned>() : nullptr,
                                       exact_last ? s->last_part.as<float>() : nullptr));
+    } else if (q4_f16) {
+        LAUNCH(q4_attend(s, li, true, qh, QW, n, pos, nullptr, ctxh, st == s->stream ? 0 : 1, st));
+    } else if (s->kv_q4) {
+        LAUNCH(q4_attend(s, li, false, qkv, LDQKV, n, pos, nullptr, ctx, st == s->stream ? 0 : 1, st));
+        LAUNCH(launch_f32_to_f16(ctx, ctxh, ctxhlo, (int64_t)n * QW, st));
     } else {
         LAUNCH(launch_attention_generic(qkv, LDQKV, kc, vc, s->kv_f16, s->capacity, n, c.head_count, c.kv_head_count,
                                         hd, pos, 1, nullptr, ctx, st));
@@ -1623,7 +1712,7 @@ static int encode_chunk(ahip_session* s, const int32_t* dtok, int n, int pos, bo
     // Calls of 2 to 15 tokens keep float32 activations in every mode: the fast modes'
     // on bf16 MFMA without loss (launch_gemm_small), summed in its order; with a
     // float32 cache, the setting that numerics are checked in, in the reference's.
-    const bool few = s->fast && n < 16 && s->kv_f16 && !s->prefill_f32_gemm;
+    const bool few = s->fast && n < 16 && (s->kv_f16 || s->kv_q4) && !s->prefill_f32_gemm;
     if (mfma && n >= env_int("ALPACA_HIP_SPLIT_MIN", kSplitPrefillMin) && !s->profiling && env_int("ALPACA_HIP_PREFILL_STREAMS", 2) >= 2 &&
         prefill_split_pays(n, QW + 2 * KW)) {
         if (!s->part_stream[1]) s->part_stream[1] = split_stream_acquire(m->device);
@@ -1680,15 +1769,20 @@ static int encode_chunk(ahip_session* s, const int32_t* dtok, int n, int pos, bo
                 return launch_gemm_f32(rows.xf, w.cols, n, w, up, y, ldy, mode == GEMM_QKV_ROPE ? GEMM_STORE : mode, st);
             };
             LAUNCH(gemm("qkv projections", x, &L.attn_norm, L.qkv.m, nullptr, qkv, LDQKV,
-                        s->fuse_qkv_rope ? GEMM_QKV_ROPE : GEMM_STORE));
-            if (!roped) {
+                        s->fuse_qkv_rope && !s->kv_q4 ? GEMM_QKV_ROPE : GEMM_STORE));
+            if (s->kv_q4) {
+                s->stage("rope + kv store");
+                LAUNCH(q4_append(s, li, qkv, n, pos, nullptr, nullptr, st));
+            } else if (!roped) {
                 s->stage("rope + kv store");
                 LAUNCH(launch_rope_store(qkv, LDQKV, n, c.head_count, c.kv_head_count, hd, pos, rope, 1, flash ? 0 : 1,
                                          flash ? s->qh.as<f16>() : nullptr, flash ? qhlo : nullptr, kc, vc, s->kv_f16,
                                          s->capacity, st));
             }
             s->stage("attention");
-            if (flash) {
+            if (s->kv_q4) {
+                LAUNCH(q4_attend(s, li, false, qkv, LDQKV, n, pos, nullptr, s->ctx.as<float>(), 0, st));
+            } else if (flash) {
                 LAUNCH(launch_flash_attention(s->qh.as<f16>(), qhlo, QW, (const f16*)kc, (const f16*)vc, s->capacity,
                                               n, c.head_count, c.kv_head_count, hd, pos, s->ctx.as<float>(), nullptr,
                                               nullptr, st, s->two_term && (s->lo_terms & kLoP) ? 2 : 1));
@@ -1796,7 +1890,7 @@ static int encode_greedy_step(ahip_session* s) {
 // per token so the host issues one launch per token instead of ~150.
 static bool capture_greedy_graph(ahip_session* s) {
     if (s->greedy_graph) return true;
-    if (s->graph_failed || !s->dec_split) return false;
+    if (s->graph_failed || !(s->dec_split || s->kv_q4)) return false;
     hipGraph_t g = nullptr;
     if (hipStreamBeginCapture(s->stream, hipStreamCaptureModeThreadLocal) != hipSuccess) {
         s->graph_failed = true;
@@ -1853,7 +1947,7 @@ extern "C" int ahip_session_decode_greedy(ahip_session* s, int32_t start, int ma
             if (int r = pdec_launch(s, false, true)) return r;
         } else if (use_graph) {
             HIP_OR(hipGraphLaunch(s->greedy_graph, st), "hipGraphLaunch");
-        } else if (s->dec_split) {
+        } else if (s->dec_split || s->kv_q4) {
             if (int r = encode_greedy_step(s)) return r;
         } else {
             // generic attention needs host-side positions
@@ -2176,6 +2270,91 @@ extern "C" int ahip_op_rope(ahip_context* ctx, float* x, int tokens, int heads, 
     });
 }
 
+// ahip_op_attention over a cache in 4 bits: in f16 as the fast_f16 prefill does, else in float32.
+static int op_attention_q4(ahip_context* ctx, const float* q, int tokens, int heads, int hd, const float* keys,
+                           const float* values, int capacity, int kv_heads, int start, int precision, float* out) {
+    return with_ctx(ctx, [&](hipStream_t st) -> int {
+        DevBuf rows[2], cache[2], dq, dout, work;
+        const int64_t width = (int64_t)kv_heads * hd, cells = (int64_t)kv_heads * q4_head_bytes(capacity, hd / 32);
+        const size_t qn = (size_t)tokens * heads * hd;
+        if (int rc = upload(rows[0], keys, (size_t)(capacity * width * 4), st)) return rc;
+        if (int rc = upload(rows[1], values, (size_t)(capacity * width * 4), st)) return rc;
+        for (DevBuf& b : cache)
+            if (int rc = b.alloc((size_t)cells)) return rc;
+        Q4Cache c;
+        c.k = cache[0].as<uint8_t>();
+        c.v = cache[1].as<uint8_t>();
+        c.kv_heads = kv_heads;
+        c.capacity = capacity;
+        c.nb = hd / 32;
+        LAUNCH(launch_q4_store(false, {rows[0].p, width}, {rows[1].p, width}, capacity, 0, nullptr, c, st));
+        const bool half = precision == AHIP_GEMM_FAST_F16 && tokens >= 16;
+        const Q4Plan plan = q4_attention_plan(half, tokens, heads, kv_heads, hd, start + tokens);
+        const int64_t need = q4_attention_workspace(tokens, heads, hd, plan);
+        if (int rc = work.alloc((size_t)need)) return rc;
+        if (need) HIP_OR(hipMemsetAsync(work.p, 0, kQ4Counters * 4, st), "clear workspace");
+        std::vector<uint16_t> h(half ? qn : 0);
+        for (size_t i = 0; i < h.size(); i++) h[i] = f32_to_f16_bits(q[i]);
+        if (int rc = upload(dq, half ? (const void*)h.data() : q, qn * (half ? 2 : 4), st)) return rc;
+        if (int rc = dout.alloc(qn * (half ? 2 : 4))) return rc;
+        Q4Attention a;
+        a.q = dq.p;
+        a.out = dout.p;
+        a.q_stride = a.out_stride = (int64_t)heads * hd;
+        a.tokens = tokens;
+        a.heads = heads;
+        a.start = start;
+        q4_set_workspace(a, work.p);
+        LAUNCH(launch_q4_attention(half, a, c, plan, st));
+        if (!half) return download(out, dout, qn * 4, st);
+        if (int rc = download(h.data(), dout, qn * 2, st)) return rc;
+        for (size_t i = 0; i < qn; i++) out[i] = f16_bits_to_f32(h[i]);
+        return AHIP_OK;
+    });
+}
+
+// ahip_qk_norm_rope on host rows, in place.
+extern "C" int ahip_op_qk_norm_rope(ahip_context* ctx, float* q, int heads, const float* q_gain, float* k,
+                                    int kv_heads, const float* k_gain, int tokens, int hd, float eps, int start,
+                                    float theta, int interleaved) {
+    if (tokens < 0 || heads < 0 || kv_heads < 0 || start < 0 || (tokens && ((heads && !q) || (kv_heads && !k))))
+        return fail(AHIP_ERR_INVALID_ARGUMENT, "norm and rope shapes");
+    if (hd <= 0 || hd % 32 || hd > 256) return fail(AHIP_ERR_INVALID_ARGUMENT, "head dimension must be a multiple of 32 up to 256");
+    if (!(theta > 0)) return fail(AHIP_ERR_INVALID_ARGUMENT, "ropeTheta must be positive");
+    if (tokens > (1 << 28) || start > (1 << 28)) return fail(AHIP_ERR_INVALID_ARGUMENT, "implausibly large position");
+    return with_ctx(ctx, [&](hipStream_t st) -> int {
+        if (tokens == 0) return AHIP_OK;
+        auto table = rope_table(start + tokens, hd, theta);
+        DevBuf dt, dq, dk, dgq, dgk;
+        const size_t qb = (size_t)tokens * heads * hd * 4, kb = (size_t)tokens * kv_heads * hd * 4;
+        if (int rc = upload(dt, table.data(), table.size() * sizeof(float2), st)) return rc;
+        if (int rc = upload(dq, q, qb, st)) return rc;
+        if (int rc = upload(dk, k, kb, st)) return rc;
+        if (int rc = upload(dgq, q_gain, q_gain ? (size_t)hd * 4 : 0, st)) return rc;
+        if (int rc = upload(dgk, k_gain, k_gain ? (size_t)hd * 4 : 0, st)) return rc;
+        ahip_norm_rope a{};
+        a.q = a.q_out = dq.p;
+        a.k = a.k_out = dk.p;
+        a.q_gain = q_gain ? dgq.as<float>() : nullptr;
+        a.k_gain = k_gain ? dgk.as<float>() : nullptr;
+        a.q_stride = a.q_out_stride = (int64_t)heads * hd;
+        a.k_stride = a.k_out_stride = (int64_t)kv_heads * hd;
+        a.rope = dt.as<float>();
+        a.dtype = AHIP_F32;
+        a.tokens = tokens;
+        a.heads = heads;
+        a.kv_heads = kv_heads;
+        a.head_dim = hd;
+        a.rope_positions = start + tokens;
+        a.interleaved = interleaved;
+        a.start = start;
+        a.eps = eps;
+        if (int rc = ahip_qk_norm_rope(ctx, &a, nullptr)) return rc;
+        if (int rc = download(q, dq, qb, st)) return rc;
+        return download(k, dk, kb, st);
+    });
+}
+
 extern "C" int ahip_op_attention(ahip_context* ctx, const float* q, int tokens, int heads, int hd, const float* keys,
                                  const float* values, int capacity, int kv_heads, int start, int kv_precision,
                                  int precision, float* out) {
@@ -2184,6 +2363,8 @@ extern "C" int ahip_op_attention(ahip_context* ctx, const float* q, int tokens, 
         return fail(AHIP_ERR_INVALID_ARGUMENT, "attention shapes");
     if (hd % 32 || hd > 256) return fail(AHIP_ERR_INVALID_ARGUMENT, "head dimension must be a multiple of 32 up to 256");
     const bool f16kv = kv_precision == AHIP_KV_F16;
+    if (kv_precision == AHIP_KV_Q4_0) return op_attention_q4(ctx, q, tokens, heads, hd, keys, values, capacity, kv_heads,
+                                                             start, precision, out);
     return with_ctx(ctx, [&](hipStream_t st) -> int {
         // Cache rows [capacity][kv_heads][hd] -> [kv_heads][capacity][hd] in the cache format.
         const size_t ne = (size_t)capacity * kv_heads * hd;

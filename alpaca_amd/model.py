@@ -18,7 +18,7 @@ from . import _lib as L
 from .tensor import QTensor
 
 # Handles still open when the interpreter exits are closed by an atexit hook
-# (sessions, then models, then contexts), which runs at the start of
+# (sessions and caches, then models, then contexts), which runs at the start of
 # interpreter finalization, while the library and the HIP runtime are intact.
 # Left to finalizers at module teardown they may not be released at all, and
 # the HIP runtime then frees the session's streams, events and mapped host
@@ -93,7 +93,7 @@ class LlamaConfig:
                               self.rms_norm_eps, self.rope_theta, 1 if self.rope_interleaved else 0)
 
 
-KV = {"f16": L.KV_F16, "f32": L.KV_F32}
+KV = {"f16": L.KV_F16, "f32": L.KV_F32, "q4_0": L.KV_Q4_0}
 GEMM = {"exact": L.GEMM_EXACT, "fast": L.GEMM_FAST, "fast-f16": L.GEMM_FAST_F16}
 
 

@@ -99,6 +99,21 @@ class HIPOps:
         L.check(L.lib().ahip_op_rope(self.h, _fp(v), t, h, hd, start_position, theta, 1 if interleaved else 0))
         return v
 
+    def qk_norm_rope(self, q, k, start_position: int, theta: float, q_gain=None, k_gain=None, eps: float = 1e-5,
+                     interleaved: bool = True):
+        """Per-head RMS norm (where a gain [hd] is given) and RoPE of q [tokens, heads, hd] and k [tokens, kv_heads, hd]."""
+        q, k = _f32(q).copy(), _f32(k).copy()
+        if q.ndim != 3 or k.ndim != 3 or q.shape[0] != k.shape[0] or q.shape[2] != k.shape[2]:
+            raise L.InvalidArgument(L.INVALID_ARGUMENT, f"qkNormRope shapes q {q.shape} k {k.shape}")
+        t, h, hd = q.shape
+        gains = [None if g is None else _f32(g) for g in (q_gain, k_gain)]
+        if any(g is not None and g.shape != (hd,) for g in gains):
+            raise L.InvalidArgument(L.INVALID_ARGUMENT, "qkNormRope gain shape")
+        gq, gk = (None if g is None else _fp(g) for g in gains)
+        L.check(L.lib().ahip_op_qk_norm_rope(self.h, _fp(q), h, gq, _fp(k), k.shape[1], gk, t, hd, eps, start_position,
+                                             theta, 1 if interleaved else 0))
+        return q, k
+
     def attention(self, q, keys, values, start_position: int, kv: str = "f16", precision: str = "exact"):
         """q [tokens, heads, hd]; keys/values [capacity, kv_heads, hd] -> [tokens, heads, hd]."""
         q, k, v = _f32(q), _f32(keys), _f32(values)

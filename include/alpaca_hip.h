@@ -43,8 +43,12 @@ typedef enum {
  * in its low nibble and element j+16 in its high nibble; value = d*(nib-8). */
 typedef enum { AHIP_F32 = 0, AHIP_F16 = 1, AHIP_Q8_0 = 2, AHIP_Q4_0 = 3 } ahip_dtype;
 
-/* KVPrecision, Sources/AlpacaMetal/Backend/KernelEncoder.swift:9-17. */
-typedef enum { AHIP_KV_F16 = 0, AHIP_KV_F32 = 1 } ahip_kv_precision;
+/* KVPrecision, Sources/AlpacaMetal/Backend/KernelEncoder.swift:9-17, and a
+ * cache in 4 bits, which the reference does not have: Q4_0 blocks along the head
+ * dimension, 18 bytes where f16 takes 64 (see ahip_kv_q4_store).  Its attention
+ * is float32 over the cache's exact values, in the fast_f16 prefill f16; decode
+ * runs as a step of several kernels, replayed as a graph by the greedy chain. */
+typedef enum { AHIP_KV_F16 = 0, AHIP_KV_F32 = 1, AHIP_KV_Q4_0 = 2 } ahip_kv_precision;
 
 /* GEMMPrecision, KernelEncoder.swift:41-48: exact = float32 operands (the
  * SIMT GEMMs and float32 attention); fast = f16 MFMA with float32
@@ -322,6 +326,11 @@ int ahip_op_gate_up_silu(ahip_context* ctx, const float* x, int m, int k, int dt
 /* RoPE in place on x[tokens, heads, hd] (MetalOps.rope, :107-114). */
 int ahip_op_rope(ahip_context* ctx, float* x, int tokens, int heads, int head_dim, int start, float theta,
                  int interleaved);
+/* ahip_qk_norm_rope in place on q[tokens, heads, hd] and k[tokens, kv_heads, hd]
+ * (no counterpart in the reference); a null gain: no norm. */
+int ahip_op_qk_norm_rope(ahip_context* ctx, float* q, int heads, const float* q_gain, float* k, int kv_heads,
+                         const float* k_gain, int tokens, int head_dim, float eps, int start, float theta,
+                         int interleaved);
 /* Causal GQA attention (MetalOps.attention, :116-148).  q [tokens, heads, hd];
  * keys/values [capacity, kv_heads, hd] f32, stored into the cache format
  * selected by kv_precision; out [tokens, heads, hd]. */
