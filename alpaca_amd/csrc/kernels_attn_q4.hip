@@ -58,16 +58,30 @@ struct Nibbles {
     }
 };
 
+// Division of 0 <= n < 2^31 by a divisor that the host knows: with 2^s >= d,
+// m = floor(2^(31 + s) / d) + 1 has m d = 2^(31 + s) + e, 0 < e <= d <= 2^s, so
+// n m / 2^(31 + s) exceeds n / d by less than n / 2^31 / d < 1 / d and has its floor.
+struct Divisor {
+    unsigned d = 1, m = 0, s = 0;
+    Divisor() = default;
+    explicit Divisor(unsigned v) : d(v) {
+        while ((1u << s) < d) s++;
+        m = (unsigned)((1ull << (31 + s)) / d + 1);  // (d = 1: 2^31 + 1)
+    }
+    __device__ __forceinline__ int operator()(int n) const { return (int)(__umulhi((unsigned)n << 1, m) >> s); }
+};
+
 // Part i of `parts` of n: [share(n, i, parts), share(n, i + 1, parts)).
-__device__ __forceinline__ int share(int n, int i, int parts) {
-    const int q = (unsigned)n / (unsigned)parts;
-    return q * i + min(i, n - q * parts);
+__device__ __forceinline__ int share(int n, int i, const Divisor& parts) {
+    const int q = parts(n);
+    return q * i + min(i, n - q * (int)parts.d);
 }
 
 struct SplitArgs {
     Q4Attention a;
     Q4Cache c;
     int G, splits;
+    Divisor by_group, by_heads, by_splits;
     bool fused;  // the last workgroup of a KV head joins the splits
     float scale_log2;
 };
@@ -192,7 +206,7 @@ __device__ __forceinline__ Joined join_groups(const float* pp, int hd, int d, in
 // Where column `col` of KV head kvh leaves split 0 (then split by split).
 template <int HD>
 __device__ __forceinline__ float* partial(const SplitArgs& p, int kvh, int col) {
-    const unsigned t = (unsigned)col / (unsigned)p.G, h = kvh * p.G + col - t * p.G;
+    const int t = p.by_group(col), h = kvh * p.G + col - t * p.G;
     return p.a.partials + ((int64_t)t * p.a.heads + h) * p.splits * (HD + 2);
 }
 
@@ -215,7 +229,7 @@ __device__ __forceinline__ void count_and_join(const SplitArgs& p, int kvh, int 
     const int group = threadIdx.x / items, i = threadIdx.x - group * items, col = i / (HD / 2), d = 2 * (i % (HD / 2));
     const Joined j = join_groups<8, true>(partial<HD>(p, kvh, col), HD, d, group, groups, items, i, p.splits, (float4*)lds);
     if (group) return;
-    const unsigned t = (unsigned)col / (unsigned)p.G, h = kvh * p.G + col - t * p.G;
+    const int t = p.by_group(col), h = kvh * p.G + col - t * p.G;
     T* out = (T*)p.a.out + t * p.a.out_stride + (int64_t)h * HD + d;
     out[0] = (T)(j.a / j.l);
     out[1] = (T)(j.b / j.l);
@@ -252,6 +266,59 @@ __global__ __launch_bounds__(256) void q4_join_kernel(const float* partials, int
 // T float: the scores and outputs to float32 accuracy (the queries and
 // probabilities as two f16 terms, the quants exact and the values exact in two
 // terms).  T f16: queries exact, probabilities and values one f16 term.
+// A column's queries as the lane takes them, at q its dims 8 g of block 0: block b,
+// dims 8 g + {0, 4, 1, 5, 2, 6, 3, 7} as the keys' nibbles come.  float: scaled into
+// [-1, 1] by a power of two, so that two f16 terms hold any float32 range.  Returns what
+// the products are to be scaled by for scores in base 2.
+template <int NB, typename T>
+__device__ __forceinline__ float load_queries(const T* q, float scale_log2, f16x8 (&qh)[NB],
+                                              f16x8 (&ql)[sizeof(T) == 4 ? NB : 1]) {
+    constexpr int at[8] = {0, 4, 1, 5, 2, 6, 3, 7};
+    T x[NB][8];
+#pragma unroll
+    for (int b = 0; b < NB; b++)
+#pragma unroll
+        for (int e = 0; e < 8; e++) x[b][e] = q[32 * b + e];
+    if constexpr (sizeof(T) == 2) {
+#pragma unroll
+        for (int b = 0; b < NB; b++)
+#pragma unroll
+            for (int e = 0; e < 8; e++) qh[b][e] = x[b][at[e]];
+        return scale_log2;
+    } else {
+        float most = 0.f;
+#pragma unroll
+        for (int b = 0; b < NB; b++)
+#pragma unroll
+            for (int e = 0; e < 8; e++) most = fmaxf(most, fabsf(x[b][e]));
+        most = xor32_combine(xor16_combine(most, MaxOp()), MaxOp());
+        // (the bounds keep the scale itself, and a masked score's product with it, a number)
+        const int ex = most > 0.f && most < INFINITY ? max(-100, min(__builtin_amdgcn_frexp_expf(most), 120)) : 0;
+        const float down = ldexpf(1.f, -ex);
+#pragma unroll
+        for (int b = 0; b < NB; b++) {
+            f16x2 hi[4], lo[4];
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const float u = x[b][at[2 * i]] * down, v = x[b][at[2 * i + 1]] * down;
+                hi[i] = round2(u, v);
+                lo[i] = round2(rest_low(hi[i], u), rest_high(hi[i], v));
+            }
+            qh[b] = frag(hi[0], hi[1], hi[2], hi[3]);
+            ql[b] = frag(lo[0], lo[1], lo[2], lo[3]);
+        }
+        return ldexpf(scale_log2, ex);
+    }
+}
+// A key's four scores of a block, in the units of the block's quants, added scaled.
+__device__ __forceinline__ void add_scaled(f32x4& s, f32x4 part, uint2 d) {
+    const f16x2 d0 = pair(d.x), d1 = pair(d.y);
+    s[0] = fmaf((float)d0[0], part[0], s[0]);
+    s[1] = fmaf((float)d0[1], part[1], s[1]);
+    s[2] = fmaf((float)d1[0], part[2], s[2]);
+    s[3] = fmaf((float)d1[1], part[3], s[3]);
+}
+
 // Up to kMostWaves waves a workgroup, each with key tiles of its own.
 constexpr int kMostWaves = 8;
 template <int NB>
@@ -269,17 +336,17 @@ __global__ __launch_bounds__(64 * kMostWaves) void q4_attention_kernel(SplitArgs
     const int lane = threadIdx.x & 63, g = lane >> 4, c16 = lane & 15;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const Nibbles nib;
-    const int id = blockIdx.x / (unsigned)p.c.kv_heads, kvh = blockIdx.x - id * p.c.kv_heads;
+    const int id = p.by_heads(blockIdx.x), kvh = blockIdx.x - id * p.c.kv_heads;
     const int sp = blockIdx.y, col0 = id * 16;
     const int G = p.G, cols = p.a.tokens * G;
     const int start = p.a.start_dev ? *p.a.start_dev : p.a.start;
     const bool inside = start >= 0 && start <= p.c.capacity - p.a.tokens;
-    const int col = min(col0 + c16, cols - 1), t = col / (unsigned)G, h = kvh * G + col - t * G;
+    const int col = min(col0 + c16, cols - 1), t = p.by_group(col), h = kvh * G + col - t * G;
     const int seen = start + t;  // the column's last position
     // the tiles of this column group, and this split's share of them
-    const int first_seen = start + col0 / (unsigned)G, last_seen = start + min(col0 + 15, cols - 1) / (unsigned)G;
+    const int first_seen = start + p.by_group(col0), last_seen = start + p.by_group(min(col0 + 15, cols - 1));
     const int tiles = inside ? last_seen / kQ4Tile + 1 : 0;
-    const int t0 = share(tiles, sp, p.splits), t1 = share(tiles, sp + 1, p.splits);
+    const int t0 = share(tiles, sp, p.by_splits), t1 = share(tiles, sp + 1, p.by_splits);
 
     const uint8_t* kt = p.c.k + (int64_t)kvh * q4_head_bytes(p.c.capacity, NB);
     const uint8_t* vt = p.c.v + (int64_t)kvh * q4_head_bytes(p.c.capacity, NB);
@@ -293,43 +360,9 @@ __global__ __launch_bounds__(64 * kMostWaves) void q4_attention_kernel(SplitArgs
     };
     if (j < t1) load(xa, j);
 
-    // queries: block b, dims 8 g + {0, 4, 1, 5, 2, 6, 3, 7} as the keys' nibbles come
     f16x8 qh[NB], ql[EXACT ? NB : 1];
-    float sc = p.scale_log2;
-    {
-        const T* q = (const T*)p.a.q + (int64_t)t * p.a.q_stride + (int64_t)h * HD + 8 * g;
-        T x[NB][8];
-#pragma unroll
-        for (int b = 0; b < NB; b++)
-#pragma unroll
-            for (int e = 0; e < 8; e++) x[b][e] = q[32 * b + e];
-        constexpr int at[8] = {0, 4, 1, 5, 2, 6, 3, 7};
-        if constexpr (EXACT) {
-            // the column scaled into [-1, 1] by a power of two, so that its two terms hold any float32 range
-            float most = 0.f;
-#pragma unroll
-            for (int b = 0; b < NB; b++)
-#pragma unroll
-                for (int e = 0; e < 8; e++) most = fmaxf(most, fabsf(x[b][e]));
-            most = xor32_combine(xor16_combine(most, MaxOp()), MaxOp());
-            // (the bounds keep the scale itself, and a masked score's product with it, a number)
-            const int ex = most > 0.f && most < INFINITY ? max(-100, min(__builtin_amdgcn_frexp_expf(most), 120)) : 0;
-            sc = ldexpf(sc, ex);
-#pragma unroll
-            for (int b = 0; b < NB; b++)
-#pragma unroll
-                for (int e = 0; e < 8; e++) {
-                    const float v = ldexpf(x[b][at[e]], -ex);
-                    qh[b][e] = (f16)v;
-                    ql[b][e] = (f16)(v - (float)qh[b][e]);
-                }
-        } else {
-#pragma unroll
-            for (int b = 0; b < NB; b++)
-#pragma unroll
-                for (int e = 0; e < 8; e++) qh[b][e] = x[b][at[e]];
-        }
-    }
+    const float sc = load_queries<NB, T>((const T*)p.a.q + (int64_t)t * p.a.q_stride + (int64_t)h * HD + 8 * g,
+                                         p.scale_log2, qh, ql);
 
     float m = -INFINITY;
     f32x4 o[NB][2], l = {0.f, 0.f, 0.f, 0.f};
@@ -349,11 +382,7 @@ __global__ __launch_bounds__(64 * kMostWaves) void q4_attention_kernel(SplitArgs
                 const f16x8 kf = frag(nib.lo(w), nib.hi(w), nib.lo(w8), nib.hi(w8));
                 f32x4 part = mfma(kf, qh[b], f32x4{0.f, 0.f, 0.f, 0.f});
                 if constexpr (EXACT) part = mfma(kf, ql[b], part);
-                const f16x2 d0 = pair(x.ks[s][b].x), d1 = pair(x.ks[s][b].y);
-                sa[s][0] = fmaf((float)d0[0], part[0], sa[s][0]);
-                sa[s][1] = fmaf((float)d0[1], part[1], sa[s][1]);
-                sa[s][2] = fmaf((float)d1[0], part[2], sa[s][2]);
-                sa[s][3] = fmaf((float)d1[1], part[3], sa[s][3]);
+                add_scaled(sa[s], part, x.ks[s][b]);
             }
         }
         const int key0 = tile * kQ4Tile;
@@ -459,20 +488,20 @@ __global__ __launch_bounds__(64 * kMostWaves) void q4_attention_kernel(SplitArgs
         xml[wave][1][c16] = l[0];
     }
     __syncthreads();
-    const int n = min(16, cols - col0);
+    const int n = min(16, cols - col0), had = max(1, min(waves, t1 - t0));  // (a wave without a tile adds nothing)
     for (int i = threadIdx.x; i < n * (HD / 2); i += blockDim.x) {
         const int qc = i / (HD / 2), d = 2 * (i % (HD / 2));
         float mt = xml[0][0][qc];
-        for (int w = 1; w < waves; w++) mt = fmaxf(mt, xml[w][0][qc]);
+        for (int w = 1; w < had; w++) mt = fmaxf(mt, xml[w][0][qc]);
         float lt = 0.f, oa = 0.f, ob = 0.f;
-        for (int w = 0; w < waves; w++) {
+        for (int w = 0; w < had; w++) {
             const float f = join_weight(xml[w][0][qc], mt);
             lt += f * xml[w][1][qc];
             oa += f * xo[w][qc][d];
             ob += f * xo[w][qc][d + 1];
         }
         if (p.splits == 1) {
-            const int64_t tt = (col0 + qc) / G, hh = kvh * G + col0 + qc - tt * G;
+            const int64_t tt = p.by_group(col0 + qc), hh = kvh * G + col0 + qc - tt * G;
             T* out = (T*)p.a.out + tt * p.a.out_stride + hh * HD + d;
             out[0] = (T)(oa / lt);
             out[1] = (T)(ob / lt);
@@ -490,7 +519,7 @@ __global__ __launch_bounds__(64 * kMostWaves) void q4_attention_kernel(SplitArgs
     if (p.fused) count_and_join<HD, T>(p, kvh, cols, lds);
 }
 
-// ------------------------------------------------------------------ many columns, f16
+// ------------------------------------------------------------------ many columns
 // A workgroup takes 64 CT query columns, 16 CT a wave; the tiles of keys and
 // values are unpacked once for all its waves, into LDS as the fragments that the
 // products read (16 bytes a lane in lane order, so no bank conflicts either
@@ -498,19 +527,29 @@ __global__ __launch_bounds__(64 * kMostWaves) void q4_attention_kernel(SplitArgs
 // through LDS at the end.  Two buffers a set: while the waves work on one, they
 // unpack the next tile's words, loaded a step earlier, into the other; one
 // barrier a step.
-template <int NB, int CT, int NSET>
+//
+// T f16: the keys' and values' fragments hold d (n - 8) rounded to f16, as an f16
+// cache holds them, and the products run through without another instruction.
+// T float: the keys' fragments hold n - 8 and the products are scaled block by
+// block; the values have a second fragment with what the first one's rounding left.
+template <int NB, int CT, int NSET, typename T>
 struct Wide {
-    static constexpr int TPS = NB <= 4 ? 2 : 1;            // tiles a step
-    static constexpr int FRAGS = 2 * NB * TPS;             // of keys, and of values, in a buffer
-    static constexpr int BUF = 2 * FRAGS * 1024;
+    static constexpr bool EXACT = sizeof(T) == 4;
+    static constexpr int TPS = NB <= 4 && !EXACT ? 2 : 1;    // tiles a step
+    static constexpr int KF = 2 * NB * TPS;                  // fragments of keys in a buffer,
+    static constexpr int VT = EXACT ? 2 : 1;                 // and of values, in VT terms
+    static constexpr int SCALES = (KF + KF * VT) * 1024;     // EXACT: the keys' scales, a tile's as in the cache
+    static constexpr int BUF = SCALES + (EXACT ? TPS * 64 * NB : 0);
     static constexpr int COLS = 64 * CT;
     static constexpr int JOIN = COLS * (32 * NB + 4) * 4 + COLS * 8;  // a set's outputs and statistics
     static constexpr int LDS = 2 * NSET * BUF > JOIN ? 2 * NSET * BUF : JOIN;
+    static constexpr bool FITS = LDS <= 160 << 10;
 };
 
-template <int NB, int CT, int NSET>
+template <int NB, int CT, int NSET, typename T>
 __global__ __launch_bounds__(256 * NSET) __attribute__((amdgpu_waves_per_eu(2, 2))) void q4_attention_wide_kernel(SplitArgs p) {
-    typedef Wide<NB, CT, NSET> W;
+    typedef Wide<NB, CT, NSET, T> W;
+    constexpr bool EXACT = W::EXACT;
     constexpr int TPS = W::TPS, HD = 32 * NB, STEP = TPS * kQ4Tile;
     constexpr int ITEMS = NB * TPS;  // (tile, block)
     constexpr int PER = (ITEMS + 3) / 4;
@@ -518,33 +557,31 @@ __global__ __launch_bounds__(256 * NSET) __attribute__((amdgpu_waves_per_eu(2, 2
     const int lane = threadIdx.x & 63, g = lane >> 4, c16 = lane & 15;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), set = wave / 4, wl = wave % 4;
     const int G = p.G, cols = p.a.tokens * G, groups = (cols + W::COLS - 1) / W::COLS;
-    // the longest (last) columns first
     const Nibbles nib;
-    const int id = blockIdx.x / (unsigned)p.c.kv_heads, kvh = blockIdx.x - id * p.c.kv_heads;
+    // the longest (last) columns first
+    const int id = p.by_heads(blockIdx.x), kvh = blockIdx.x - id * p.c.kv_heads;
     const int sp = blockIdx.y, col0 = (groups - 1 - id) * W::COLS;
     const int start = p.a.start_dev ? *p.a.start_dev : p.a.start;
     const bool inside = start >= 0 && start <= p.c.capacity - p.a.tokens;
     const int wcol0 = col0 + wl * 16 * CT;  // the wave's columns
-    const int last_seen = start + min(col0 + W::COLS - 1, cols - 1) / G;
-    const int w_first = start + min(wcol0, cols - 1) / G, w_last = start + min(wcol0 + 16 * CT - 1, cols - 1) / G;
+    const int last_seen = start + p.by_group(min(col0 + W::COLS - 1, cols - 1));
+    const int w_first = start + p.by_group(min(wcol0, cols - 1));
+    const int w_last = start + p.by_group(min(wcol0 + 16 * CT - 1, cols - 1));
     const int tiles = inside ? last_seen / kQ4Tile + 1 : 0;
     const int all = (tiles + TPS - 1) / TPS;  // steps over all the keys
-    const int s0 = share(all, sp, p.splits), s1 = share(all, sp + 1, p.splits);
+    const int s0 = share(all, sp, p.by_splits), s1 = share(all, sp + 1, p.by_splits);
     const int per = (s1 - s0 + NSET - 1) / NSET, f0 = s0 + set * per;  // this set's steps: [f0, f0 + count)
     const int count = max(0, min(s1 - f0, per));
 
-    f16x8 q[CT][NB];
+    f16x8 q[CT][NB], ql[CT][EXACT ? NB : 1];
     int seen[CT];
+    float sc[CT];
 #pragma unroll
     for (int ct = 0; ct < CT; ct++) {
-        const int col = min(wcol0 + 16 * ct + c16, cols - 1), t = col / G, h = kvh * G + col - t * G;
+        const int col = min(wcol0 + 16 * ct + c16, cols - 1), t = p.by_group(col), h = kvh * G + col - t * G;
         seen[ct] = start + t;
-        const f16* qp = (const f16*)p.a.q + (int64_t)t * p.a.q_stride + (int64_t)h * HD + 8 * g;
-#pragma unroll
-        for (int b = 0; b < NB; b++) {
-            const f16 *x = qp + 32 * b;
-            q[ct][b] = f16x8{x[0], x[4], x[1], x[5], x[2], x[6], x[3], x[7]};
-        }
+        sc[ct] = load_queries<NB, T>((const T*)p.a.q + (int64_t)t * p.a.q_stride + (int64_t)h * HD + 8 * g, p.scale_log2,
+                                     q[ct], ql[ct]);
     }
     float m[CT];
     f32x4 o[CT][NB][2], l[CT];
@@ -601,9 +638,16 @@ __global__ __launch_bounds__(256 * NSET) __attribute__((amdgpu_waves_per_eu(2, 2
 #pragma unroll
             for (int s = 0; s < 2; s++) {
                 const uint32_t w = rk[k][s], w8 = w >> 8;
-                const f16x2 d = pair(rk[k][2 + s] * 0x10001u);
-                *(f16x8*)(buf + ((tt * 2 + s) * NB + b) * 1024 + lane * 16) =
-                    frag(nib.lo(w) * d, nib.hi(w) * d, nib.lo(w8) * d, nib.hi(w8) * d);
+                f16x2 n[4] = {nib.lo(w), nib.hi(w), nib.lo(w8), nib.hi(w8)};
+                if constexpr (!EXACT) {
+                    const f16x2 d = pair(rk[k][2 + s] * 0x10001u);
+#pragma unroll
+                    for (int i = 0; i < 4; i++) n[i] *= d;
+                } else if (g == 0) {
+                    *(uint16_t*)(buf + W::SCALES + (((tt * 2 + s) * 4 + (c16 >> 2)) * NB + b) * 8 + (c16 & 3) * 2) =
+                        (uint16_t)rk[k][2 + s];
+                }
+                *(f16x8*)(buf + ((tt * 2 + s) * NB + b) * 1024 + lane * 16) = frag(n[0], n[1], n[2], n[3]);
             }
             const int key0 = (step * TPS + tt) * kQ4Tile;
             if (key0 + kQ4Tile - 1 > last_seen) {
@@ -613,11 +657,20 @@ __global__ __launch_bounds__(256 * NSET) __attribute__((amdgpu_waves_per_eu(2, 2
                     if (key0 + 16 * (e >> 2) + 4 * g + (e & 3) > last_seen)
                         rv[k][2 + (e >> 1)] &= e & 1 ? 0xFFFFu : 0xFFFF0000u;
             }
-            const uint32_t w0 = rv[k][0], w1 = rv[k][1], u0 = w0 >> 8, u1 = w1 >> 8;
-            const f16x2 d0 = pair(rv[k][2]), d1 = pair(rv[k][3]), d2 = pair(rv[k][4]), d3 = pair(rv[k][5]);
-            uint8_t* v = buf + (W::FRAGS + (tt * NB + b) * 2) * 1024 + lane * 16;
-            *(f16x8*)v = frag(nib.lo(w0) * d0, nib.lo(u0) * d1, nib.lo(w1) * d2, nib.lo(u1) * d3);
-            *(f16x8*)(v + 1024) = frag(nib.hi(w0) * d0, nib.hi(u0) * d1, nib.hi(w1) * d2, nib.hi(u1) * d3);
+            const uint32_t w[4] = {rv[k][0], rv[k][0] >> 8, rv[k][1], rv[k][1] >> 8};
+            uint8_t* v = buf + (W::KF + (tt * NB + b) * 2 * W::VT) * 1024 + lane * 16;
+#pragma unroll
+            for (int par = 0; par < 2; par++) {
+                f16x2 hi[4], lo[4];
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    const f16x2 n = par ? nib.hi(w[i]) : nib.lo(w[i]), d = pair(rv[k][2 + i]);
+                    hi[i] = n * d;
+                    if constexpr (EXACT) lo[i] = __builtin_elementwise_fma(n, d, -hi[i]);
+                }
+                *(f16x8*)(v + par * W::VT * 1024) = frag(hi[0], hi[1], hi[2], hi[3]);
+                if constexpr (EXACT) *(f16x8*)(v + (par * W::VT + 1) * 1024) = frag(lo[0], lo[1], lo[2], lo[3]);
+            }
         }
     };
     auto work = [&](int step, const uint8_t* buf) {
@@ -634,12 +687,25 @@ __global__ __launch_bounds__(256 * NSET) __attribute__((amdgpu_waves_per_eu(2, 2
 #pragma unroll
         for (int u = 0; u < 2 * TPS; u++) {
             read(u + 1);  // (after the last keys: the first values)
+            uint2 d[EXACT ? NB : 1];
+            if constexpr (EXACT) {
+#pragma unroll
+                for (int b = 0; b < NB; b++) d[b] = *(const uint2*)(buf + W::SCALES + ((u * 4 + g) * NB + b) * 8);
+            }
 #pragma unroll
             for (int ct = 0; ct < CT; ct++) sa[ct][u] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
             for (int b = 0; b < NB; b++)
 #pragma unroll
-                for (int ct = 0; ct < CT; ct++) sa[ct][u] = mfma(fr[u & 1][b], q[ct][b], sa[ct][u]);
+                for (int ct = 0; ct < CT; ct++) {
+                    if constexpr (EXACT) {
+                        f32x4 part = mfma(fr[u & 1][b], q[ct][b], f32x4{0.f, 0.f, 0.f, 0.f});
+                        part = mfma(fr[u & 1][b], ql[ct][b], part);
+                        add_scaled(sa[ct][u], part, d[b]);
+                    } else {
+                        sa[ct][u] = mfma(fr[u & 1][b], q[ct][b], sa[ct][u]);
+                    }
+                }
             __builtin_amdgcn_sched_barrier(0);
         }
         if (key0 + STEP - 1 > w_first) {
@@ -651,26 +717,29 @@ __global__ __launch_bounds__(256 * NSET) __attribute__((amdgpu_waves_per_eu(2, 2
                     for (int r = 0; r < 4; r++)
                         if (key0 + 16 * u + 4 * g + r > seen[ct]) sa[ct][u][r] = -INFINITY;
         }
-        f16x8 pf[CT][TPS];
+        f16x8 pf[CT][TPS], pg[CT][EXACT ? TPS : 1];
 #pragma unroll
         for (int ct = 0; ct < CT; ct++) {
             float mx = sa[ct][0][0];
 #pragma unroll
             for (int i = 1; i < 8 * TPS; i++) mx = fmaxf(mx, sa[ct][i >> 2][i & 3]);
             mx = xor32_combine(xor16_combine(mx, MaxOp()), MaxOp());
-            const float mn = fmaxf(m[ct], mx * p.scale_log2);
+            const float mn = fmaxf(m[ct], mx * sc[ct]);
             const float mref = mn == -INFINITY ? 0.f : mn;
             const float alpha = __builtin_amdgcn_exp2f(m[ct] - mref), eref = kLog2P - mref;
 #pragma unroll
             for (int tt = 0; tt < TPS; tt++) {
-                f16x2 e[4];
+                f16x2 e[4], r[4];
 #pragma unroll
                 for (int i = 0; i < 4; i++) {
                     const f32x4& x = sa[ct][2 * tt + (i >> 1)];
-                    e[i] = round2(__builtin_amdgcn_exp2f(fmaf(x[2 * (i & 1)], p.scale_log2, eref)),
-                                  __builtin_amdgcn_exp2f(fmaf(x[2 * (i & 1) + 1], p.scale_log2, eref)));
+                    const float a = __builtin_amdgcn_exp2f(fmaf(x[2 * (i & 1)], sc[ct], eref));
+                    const float b = __builtin_amdgcn_exp2f(fmaf(x[2 * (i & 1) + 1], sc[ct], eref));
+                    e[i] = round2(a, b);
+                    if constexpr (EXACT) r[i] = round2(rest_low(e[i], a), rest_high(e[i], b));
                 }
                 pf[ct][tt] = frag(e[0], e[1], e[2], e[3]);
+                if constexpr (EXACT) pg[ct][tt] = frag(r[0], r[1], r[2], r[3]);
             }
             if (__builtin_amdgcn_ballot_w64(m[ct] != mn)) {
 #pragma unroll
@@ -682,17 +751,26 @@ __global__ __launch_bounds__(256 * NSET) __attribute__((amdgpu_waves_per_eu(2, 2
                 m[ct] = mn;
             }
 #pragma unroll
-            for (int tt = 0; tt < TPS; tt++) l[ct] = mfma(ones, pf[ct][tt], l[ct]);
+            for (int tt = 0; tt < TPS; tt++) {
+                l[ct] = mfma(ones, pf[ct][tt], l[ct]);
+                if constexpr (EXACT) l[ct] = mfma(ones, pg[ct][tt], l[ct]);
+            }
         }
+        constexpr int VG = 2 * TPS * W::VT;  // groups of the values' fragments: (tile, block, parity, term)
 #pragma unroll
-        for (int u = 0; u < 2 * TPS; u++) {
-            if (u + 1 < 2 * TPS) read(2 * TPS + u + 1);
+        for (int u = 0; u < VG; u++) {
+            if (u + 1 < VG) read(2 * TPS + u + 1);
 #pragma unroll
             for (int i = 0; i < NB; i++) {
-                const int f = (u & 1) * NB + i;
+                const int at = u * NB + i, f = at / W::VT, tt = f / (2 * NB), d = f % (2 * NB);
+                const f16x8 v = fr[(2 * TPS + u) & 1][i];
 #pragma unroll
-                for (int ct = 0; ct < CT; ct++)
-                    o[ct][f >> 1][f & 1] = mfma(fr[(2 * TPS + u) & 1][i], pf[ct][u >> 1], o[ct][f >> 1][f & 1]);
+                for (int ct = 0; ct < CT; ct++) {
+                    f32x4& x = o[ct][d >> 1][d & 1];
+                    x = mfma(v, pf[ct][tt], x);
+                    if constexpr (EXACT)
+                        if (at % W::VT == 0) x = mfma(v, pg[ct][tt], x);
+                }
             }
             __builtin_amdgcn_sched_barrier(0);
         }
@@ -713,7 +791,7 @@ __global__ __launch_bounds__(256 * NSET) __attribute__((amdgpu_waves_per_eu(2, 2
             __syncthreads();
         }
     }
-    // the other sets' results through LDS, [set - 1]
+    // the other sets' results through LDS
     float* xo = (float*)lds;
     float* xml = xo + W::COLS * (HD + 4);
     auto put_set = [&]() {
@@ -740,10 +818,7 @@ __global__ __launch_bounds__(256 * NSET) __attribute__((amdgpu_waves_per_eu(2, 2
 #pragma unroll
             for (int ct = 0; ct < CT; ct++) {
                 const int c = wl * 16 * CT + 16 * ct + c16;
-                const float mo = xml[2 * c], mn = fmaxf(m[ct], mo), mref = mn == -INFINITY ? 0.f : mn;
-                // (nothing of a set is lost where neither has a score: a NaN stays)
-                const float fa = m[ct] == mn ? 1.f : __builtin_amdgcn_exp2f(m[ct] - mref);
-                const float fb = mo == mn ? 1.f : __builtin_amdgcn_exp2f(mo - mref);
+                const float mo = xml[2 * c], mn = fmaxf(m[ct], mo), fa = join_weight(m[ct], mn), fb = join_weight(mo, mn);
                 m[ct] = mn;
                 const float lo = xml[2 * c + 1];
 #pragma unroll
@@ -778,15 +853,15 @@ __global__ __launch_bounds__(256 * NSET) __attribute__((amdgpu_waves_per_eu(2, 2
     for (int ct = 0; ct < CT; ct++) {
         const int col = wcol0 + 16 * ct + c16;
         if (col >= cols) continue;
-        const int t = col / G, h = kvh * G + col - t * G;
-        f16* out = (f16*)p.a.out + t * p.a.out_stride + (int64_t)h * HD + 8 * g;
+        const int t = p.by_group(col), h = kvh * G + col - t * G;
+        T* out = (T*)p.a.out + t * p.a.out_stride + (int64_t)h * HD + 8 * g;
         const float inv = 1.0f / l[ct][0];
 #pragma unroll
         for (int b = 0; b < NB; b++)
 #pragma unroll
             for (int r = 0; r < 4; r++) {
-                out[32 * b + 2 * r] = (f16)(o[ct][b][0][r] * inv);
-                out[32 * b + 2 * r + 1] = (f16)(o[ct][b][1][r] * inv);
+                out[32 * b + 2 * r] = (T)(o[ct][b][0][r] * inv);
+                out[32 * b + 2 * r + 1] = (T)(o[ct][b][1][r] * inv);
             }
     }
 }
@@ -805,10 +880,11 @@ hipError_t launch_join(const Q4Attention& a, int hd, int splits, hipStream_t st)
     return hipGetLastError();
 }
 
-template <int NB, int CT, int NSET>
+template <int NB, int CT, int NSET, typename T>
 hipError_t launch_wide(const SplitArgs& p, int64_t cols, hipStream_t st) {
-    typedef Wide<NB, CT, NSET> W;
-    auto* kernel = q4_attention_wide_kernel<NB, CT, NSET>;
+    typedef Wide<NB, CT, NSET, T> W;
+    static_assert(W::FITS, "LDS");
+    auto* kernel = q4_attention_wide_kernel<NB, CT, NSET, T>;
     static OncePerDevice once;
     if (hipError_t e = allow_whole_lds(once, (const void*)kernel)) return e;
     const dim3 grid((unsigned)((cols + W::COLS - 1) / W::COLS * p.c.kv_heads), p.splits);
@@ -816,14 +892,21 @@ hipError_t launch_wide(const SplitArgs& p, int64_t cols, hipStream_t st) {
     return hipGetLastError();
 }
 
+// Columns of a workgroup of the wide kernel at most, for nb blocks a head: as registers and LDS allow,
+// and in float32, where its barriers cost small heads more than unpacking does (512 queries at 3,584
+// positions, 32/32 heads of 64: 78 us against 65 with a wave's tiles its own), from head dimension 128.
+constexpr int wide_columns(int nb, bool exact) {
+    return exact ? (nb == 4 ? 128 : nb > 4 && nb <= 6 ? 64 : 16) : nb <= 4 ? 128 : 64;
+}
+
 template <int NB, typename T>
 hipError_t launch_nb(const SplitArgs& p, const Q4Plan& plan, hipStream_t st) {
     const int64_t cols = (int64_t)p.a.tokens * p.G;
-    if constexpr (sizeof(T) == 2) {
-        if constexpr (NB <= 4)
-            if (plan.cols == 128) return launch_wide<NB, 2, 2>(p, cols, st);
-        if (plan.cols == 64) return launch_wide<NB, 1, 2>(p, cols, st);
-    }
+    constexpr int most = wide_columns(NB, sizeof(T) == 4);
+    if constexpr (most >= 128)
+        if (plan.cols == 128) return launch_wide<NB, 2, 2, T>(p, cols, st);
+    if constexpr (most >= 64)
+        if (plan.cols == 64) return launch_wide<NB, 1, 2, T>(p, cols, st);
     static OncePerDevice once;
     if (hipError_t e = allow_whole_lds(once, (const void*)q4_attention_kernel<NB, T>)) return e;
     const dim3 grid((unsigned)((cols + 15) / 16 * p.c.kv_heads), p.splits);
@@ -865,8 +948,11 @@ Q4Plan q4_attention_plan(bool f16_rows, int tokens, int heads, int kv_heads, int
     const int cus = device_cus(), tiles = q4_tiles(length), work = tiles * (hd / 32);
     auto groups = [&](int tile) { return (cols + tile - 1) / tile * kv_heads; };
     auto up = [](int64_t a, int64_t b) { return (int)((a + b - 1) / b); };
-    if (f16_rows && cols > 64) {
-        r.cols = hd <= 128 && groups(128) >= cus ? 128 : 64;
+    const int wide = wide_columns(hd / 32, !f16_rows);
+    // (float32 from a full chip on: 1,024 queries of 32/8 heads of 128 55 us against 59, 2,048 108
+    // against 164, 256 13.4 against 11.3)
+    if (cols > 64 && wide > 16 && (f16_rows || groups(64) >= cus)) {
+        r.cols = wide == 128 && groups(128) >= cus ? 128 : 64;
         const int most = (int)(cus / groups(r.cols));
         // two sets of waves take 64 keys (32 past head dimension 128) a step each
         r.splits = tiles <= 48 ? 1 : std::max(1, std::min(most, up(tiles, 8)));
@@ -903,6 +989,9 @@ hipError_t launch_q4_attention(bool f16_rows, const Q4Attention& a, const Q4Cach
     p.c = c;
     p.G = a.heads / c.kv_heads;
     p.splits = plan.splits;
+    p.by_group = Divisor(p.G);
+    p.by_heads = Divisor(c.kv_heads);
+    p.by_splits = Divisor(plan.splits);
     p.fused = plan.fused;
     const int hd = 32 * c.nb;
     p.scale_log2 = 1.4426950408889634f / sqrtf((float)hd);
