@@ -12,6 +12,7 @@ order and without waiting.
 from __future__ import annotations
 
 import ctypes as C
+import struct
 
 import numpy as np
 
@@ -20,6 +21,8 @@ from .model import HIPContext, _LIVE
 
 DTYPE = {"f32": L.F32, "f16": L.F16}
 WORKSPACE_ZERO = 2048  # AHIP_Q4_WORKSPACE_ZERO
+# ahip_norm_rope's bytes (L.NormRopeC), packed in a third of the time that the structure's 21 fields take
+_NORM_ROPE = struct.Struct("@PPPqqPPPqqPPiiiiiiiif4x").pack
 
 
 class Q4Cache:
@@ -137,11 +140,11 @@ def qk_norm_rope(context: HIPContext, q: int | None, k: int | None, tokens: int,
     """Per-head RMS norm of queries and keys (where a gain is given) and their
     rotation (where a table is), ahip_qk_norm_rope."""
     qw, kw = heads * head_dim, kv_heads * head_dim
-    args = L.NormRopeC(q, q_out, q_gain, qw if q_stride is None else q_stride,
-                       qw if q_out_stride is None else q_out_stride, k, k_out, k_gain,
-                       kw if k_stride is None else k_stride, kw if k_out_stride is None else k_out_stride, rope,
-                       positions, DTYPE[dtype], tokens, heads, kv_heads, head_dim, rope_positions,
-                       1 if interleaved else 0, start, eps)
-    rc = L.lib().ahip_qk_norm_rope(context.handle, C.byref(args), stream)
+    args = _NORM_ROPE(q or 0, q_out or 0, q_gain or 0, qw if q_stride is None else q_stride,
+                      qw if q_out_stride is None else q_out_stride, k or 0, k_out or 0, k_gain or 0,
+                      kw if k_stride is None else k_stride, kw if k_out_stride is None else k_out_stride, rope or 0,
+                      positions or 0, DTYPE[dtype], tokens, heads, kv_heads, head_dim, rope_positions,
+                      1 if interleaved else 0, start, eps)
+    rc = L.lib().ahip_qk_norm_rope(context.handle, args, stream)
     if rc:
         L.check(rc)

@@ -304,13 +304,204 @@ def test_attention_twice_gives_the_same_bits(hip_ctx):
         store(dev, cache, k, v, 0, "f32")
         a = run_attention(dev, cache, q, 2997, "f32")
         need = cache.workspace_bytes(3, 8, 2997)
+        assert need > WORKSPACE_ZERO  # (the keys are split over workgroups)
         mine = (dev.empty(need, 0xFF), need)  # another workspace, its bytes NaN but for the counters
-        L.check(L.lib().ahip_memset(hip_ctx.handle, mine[0], 0, min(need, WORKSPACE_ZERO)))
+        L.check(L.lib().ahip_memset(hip_ctx.handle, mine[0], 0, WORKSPACE_ZERO))
         b = run_attention(dev, cache, q, 2997, "f32", workspace=mine)
-        if need:
-            with pytest.raises(L.InvalidArgument, match="workspace"):
-                run_attention(dev, cache, q, 2997, "f32", workspace=(mine[0], need - 1))
+        with pytest.raises(L.InvalidArgument, match="workspace"):
+            run_attention(dev, cache, q, 2997, "f32", workspace=(mine[0], need - 1))
     assert np.array_equal(a.view(np.uint32), b.view(np.uint32))
+
+
+def check_heads(got, q, kd, vd, start, dtype, heads, label):
+    """As check_attention, for some of the query heads."""
+    G = q.shape[1] // kd.shape[1]
+    for h in heads:
+        one, kv = slice(h, h + 1), slice(h // G, h // G + 1)
+        check_attention(got[:, one], q[:, one], kd[:, kv], vd[:, kv], start, dtype, (*label, h))
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16"])
+@pytest.mark.parametrize("heads,kv_heads,hd,tokens,start", [
+    (128, 128, 128, 250, 37),  # a chip full of workgroups of 128 columns
+    (64, 64, 160, 250, 3), (64, 64, 192, 197, 60), (70, 70, 128, 129, 0), (64, 64, 256, 250, 0), (96, 32, 64, 350, 31),
+    (600, 600, 32, 1, 2100), (16, 1, 32, 1, 5000), (8, 1, 128, 1, 5000)])
+def test_attention_of_many_heads(hip_ctx, heads, kv_heads, hd, tokens, start, dtype):
+    """Calls that fill the chip, at every width of a workgroup; many KV heads and long caches for few queries."""
+    rng = np.random.default_rng(heads + hd)
+    n = start + tokens
+    k, v = rows(rng, n, kv_heads, hd, "f32"), rows(rng, n, kv_heads, hd, "f32")
+    q = rows(rng, tokens, heads, hd, dtype, 3)
+    cache = Q4Cache(hip_ctx, kv_heads, n + 13, hd)
+    with ref.Device(hip_ctx) as dev:
+        for p in (cache._desc.k, cache._desc.v):  # what was never written is NaN
+            L.check(L.lib().ahip_memset(hip_ctx.handle, p, 0xFF, cache.bytes // 2))
+        store(dev, cache, k, v, 0, "f32")
+        got = run_attention(dev, cache, q, start, dtype)
+        on_device = run_attention(dev, cache, q, 0, dtype, start_dev=dev.put(np.array([start], np.int32)))
+    cache.close()
+    kd, vd = ref.q4_rows(k, v)
+    for x in (got, on_device):
+        check_heads(x, q, kd, vd, start, dtype, [0, heads // 2, heads - 1], (hd, tokens))
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16"])
+@pytest.mark.parametrize("hd", [128, 160])
+def test_a_token_without_a_form_in_a_long_prompt(hip_ctx, hd, dtype):
+    rng = np.random.default_rng(16)
+    H, T, hit = 64, 250, 131
+    k, v = rows(rng, T, H, hd, "f32"), rows(rng, T, H, hd, "f32")
+    q = rows(rng, T, H, hd, dtype)
+    clean = ref.q4_rows(k, v)
+    v[hit, 5, 9] = np.nan
+    cache = Q4Cache(hip_ctx, H, T, hd)
+    with ref.Device(hip_ctx) as dev:
+        store(dev, cache, k, v, 0, "f32")
+        got = run_attention(dev, cache, q, 0, dtype)
+    bad = np.zeros(got.shape, bool)
+    bad[hit:, 5] = True
+    assert np.array_equal(np.isnan(got), bad)
+    check_heads(got[:hit], q[:hit], *[x[:hit] for x in clean], 0, dtype, [5], (hd, "before"))
+    check_heads(got, q, *clean, 0, dtype, [4, 6], (hd, "beside"))
+
+
+def test_one_workspace_serves_calls_of_every_shape_in_turn(hip_ctx):
+    """Joined in one launch or in two, or not split: each leaves the workspace as the next needs it."""
+    rng = np.random.default_rng(17)
+    n = 6000
+    k, v = rows(rng, n, 2, 64, "f32"), rows(rng, n, 2, 64, "f32")
+    cache = Q4Cache(hip_ctx, 2, n, 64)
+    shapes = [(1, 8, 5999), (64, 8, 5900), (1, 2, 200), (3, 4, 4000), (700, 8, 5300), (1, 32, 2000), (1, 8, 5999)] * 2
+    with ref.Device(hip_ctx) as dev:
+        store(dev, cache, k, v, 0, "f32")
+        need = max(cache.workspace_bytes(T, H, at) for T, H, at in shapes)
+        one = dev.empty(need)
+        L.check(L.lib().ahip_memset(hip_ctx.handle, one, 0, WORKSPACE_ZERO))
+        for T, H, at in shapes:
+            q = rows(rng, T, H, 64, "f32")
+            a = run_attention(dev, cache, q, at, "f32", workspace=(one, need))
+            b = run_attention(dev, cache, q, at, "f32")
+            assert np.isfinite(a).all() and np.array_equal(a.view(np.uint32), b.view(np.uint32)), (T, H, at)
+        assert not dev.get(one, WORKSPACE_ZERO, np.uint8).any()
+
+
+def test_two_streams_with_workspaces_of_their_own(hip_ctx):
+    import ctypes as C
+    rng = np.random.default_rng(18)
+    n, T, H = 5000, 1, 12
+    k, v = rows(rng, n, 3, 64, "f32"), rows(rng, n, 3, 64, "f32")
+    cache = Q4Cache(hip_ctx, 3, n, 64)
+    streams = [C.c_void_p() for _ in range(2)]
+    for s in streams:
+        L.check(L.lib().ahip_stream_create(hip_ctx.handle, C.byref(s)))
+    with ref.Device(hip_ctx) as dev:
+        store(dev, cache, k, v, 0, "f32")
+        need = cache.workspace_bytes(T, H, n - 1)
+        assert need
+        qs = [rows(rng, T, H, 64, "f32") for _ in streams]
+        want = [run_attention(dev, cache, q, n - 1, "f32") for q in qs]
+        ws, outs, qp = [(dev.empty(need, 0), need) for _ in streams], [dev.empty(T * H * 64 * 4) for _ in streams], \
+            [dev.put(q) for q in qs]
+        for _ in range(50):
+            for s, w, o, q in zip(streams, ws, outs, qp):
+                cache.attention(q, o, T, H, n - 1, workspace=w, stream=s)
+        for s in streams:
+            L.check(L.lib().ahip_stream_synchronize(s))
+        for o, w in zip(outs, want):
+            assert np.array_equal(dev.get(o, w.shape, np.float32).view(np.uint32), w.view(np.uint32))
+    for s in streams:
+        L.check(L.lib().ahip_stream_destroy(s))
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16"])
+def test_rows_at_any_element_and_stride(hip_ctx, dtype):
+    """Rows one element past a wide load's alignment, strides odd: the same bits as of aligned rows."""
+    rng = np.random.default_rng(19)
+    T, H, KVH, hd, size = 37, 6, 2, 64, NP[dtype]().nbytes
+    w, wk = H * hd, KVH * hd
+    q, k, v = rows(rng, T, H, hd, dtype), rows(rng, T, KVH, hd, dtype), rows(rng, T, KVH, hd, dtype)
+    table, gain = rope_table(T, hd, 1e4), (1 + 0.1 * rng.standard_normal(hd)).astype(np.float32)
+
+    def shifted(dev, x):
+        flat, stride = padded(x, 1)
+        return dev.put(np.concatenate([np.zeros(1, x.dtype), flat.reshape(-1)])) + size, stride
+
+    def taken(dev, p, width):
+        return dev.get(p, (T, width + 1), NP[dtype])[:, :width]
+
+    with ref.Device(hip_ctx) as dev:
+        got = []
+        for odd in (False, True):
+            cache = Q4Cache(hip_ctx, KVH, T, hd)
+            put = shifted if odd else (lambda dev, x: (dev.put(x), x[0].size))
+            (qp, qs), (kp, ks), (vp, vs) = put(dev, q), put(dev, k), put(dev, v)
+            g, tab = dev.put(gain), dev.put(table)
+            o = [dev.empty((T + 1) * (n + 1) * size) + (size if odd else 0) for n in (w, wk, wk, wk, w)]
+            n = 1 if odd else 0
+            qk_norm_rope(hip_ctx, qp, kp, T, H, KVH, hd, o[0], o[1], dtype, g, g, 1e-6, tab, T, q_stride=qs,
+                         k_stride=ks, q_out_stride=w + n, k_out_stride=wk + n)
+            cache.store(kp, vp, T, 0, dtype, ks, vs)
+            cache.load(o[2], o[3], T, 0, dtype, wk + n, wk + n)
+            cache.attention(qp, o[4], T, H, 0, dtype, qs, w + n)
+            got.append([taken(dev, p, n) if odd else dev.get(p, (T, n), NP[dtype])
+                        for p, n in zip(o, (w, wk, wk, wk, w))])
+    for a, b in zip(*got):
+        assert np.isfinite(a.astype(np.float64)).all() and np.array_equal(a, b)
+
+
+def test_offsets_past_32_bits(hip_ctx):
+    """A head's cache of 4.8 GB, and rows 4 GiB elements apart.
+
+    All keys but 40 are zeros, of score 0; the query scores 60 or more with one of the 40, so that the others' share
+    is below 2^25 e^-60 < 2^-61 and the 40 alone, closed up, are the reference."""
+    rng = np.random.default_rng(20)
+    cap, hd, n = 1 << 25, 256, 40
+    at = np.array([5, (1 << 24) - 7, cap - 20])  # 12, 12 and 16 rows from there
+    sizes = (12, 12, 16)
+    k, v = rows(rng, n, 2, hd, "f16"), rows(rng, n, 2, hd, "f16")
+    q = (k[-1:] * 8).astype(np.float32)  # the last key's own: a score near 8 * 256 / 16 = 128
+    far = 1 << 31
+    cache = Q4Cache(hip_ctx, 2, cap, hd)
+    assert cache.bytes // 4 > 1 << 32
+    with ref.Device(hip_ctx) as dev:
+        for p in (cache._desc.k, cache._desc.v):
+            L.check(L.lib().ahip_memset(hip_ctx.handle, p, 0, cache.bytes // 2))
+        a = 0
+        for start, m in zip(at, sizes):
+            store(dev, cache, k[a:a + m], v[a:a + m], int(start), "f16")
+            a += m
+        kd, vd = ref.q4_rows(k.astype(np.float32), v.astype(np.float32))
+        a = 0
+        for start, m in zip(at, sizes):
+            got = load(dev, cache, int(start) - 2 if a else 0, m + 2 if a else m, "f32")
+            if a:
+                assert all((g[:2] == 0).all() for g in got)
+                assert equal(got[0][2:], kd[a:a + m]) and equal(got[1][2:], vd[a:a + m])
+            a += m
+        # the last 4 positions are behind the query's
+        got = run_attention(dev, cache, q, cap - 5, "f32")
+        q2 = (k[-5:-4] * 8).astype(np.float32)
+        own = run_attention(dev, cache, q2, cap - 5, "f32")
+        # three rows of two heads, 2^31 elements (4 GiB of f16) from one to the next
+        w = 2 * hd
+        src, dst = dev.empty(2 * (2 * far + w)), dev.empty(2 * (2 * far + w))
+        for i in range(3):
+            L.check(L.lib().ahip_memcpy_htod(hip_ctx.handle, src + 2 * far * i, k[i:i + 1].ctypes.data, 2 * w))
+        cache.store(src, src, 3, 100, "f16", far, far)
+        cache.load(dst, None, 3, 100, "f16", far, far)
+        for i in range(3):
+            assert np.array_equal(dev.get(dst + 2 * far * i, (2, hd), np.float16), kd[i].astype(np.float16)), i
+        qk_norm_rope(hip_ctx, src, None, 3, 2, 0, hd, dst, None, "f16", q_stride=far, q_out_stride=far)
+        for i in range(3):
+            assert np.array_equal(dev.get(dst + 2 * far * i, (2, hd), np.float16), k[i]), i
+        cache.attention(src, dst, 3, 2, 0, "f16", far, far)  # positions 0 to 2: zeros
+        for i in range(3):
+            assert not dev.get(dst + 2 * far * i, (2, hd), np.float16).any(), i
+    cache.close()
+    score = (kd[:n - 4, :] * q2[0]).sum(-1).max(0) / 16
+    assert (score > 60).all()
+    check_attention(own, q2, kd[:n - 4], vd[:n - 4], n - 5, "f32", "far")
+    assert np.isfinite(got).all()
 
 
 # ---------------------------------------------------------------- norm and rotation

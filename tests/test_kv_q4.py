@@ -176,3 +176,10 @@ def test_the_reference_reads_back_what_the_quantiser_writes():
     x = (np.random.default_rng(2).standard_normal((50, 3, 64)) * 3).astype(np.float32)
     want = orc.dequantize(orc.Q4_0, quantize(x, Q4_0), x.size).reshape(x.shape)
     assert np.array_equal(ref.q4_values(x), want.astype(np.float64))
+
+
+def test_the_packed_arguments_are_the_structure_s_bytes():
+    from alpaca_amd import kvcache
+    values = [P + 64 * i for i in range(3)] + [7, 8] + [P + 4096 + 64 * i for i in range(3)] + [9, 10, P + 16, P + 32, 1,
+                                                                                        2, 3, 4, 64, 5, 1, 6, 1e-5]
+    assert kvcache._NORM_ROPE(*values) == bytes(L.NormRopeC(*values))
