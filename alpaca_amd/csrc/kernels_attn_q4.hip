@@ -31,6 +31,10 @@ __device__ __forceinline__ float rest_high(f16x2 h, float e) {
     asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel:[1,0,0] op_sel_hi:[1,0,0]" : "=v"(d) : "v"(bits(h)), "v"(e));
     return d;
 }
+// An f16 value times e, in one instruction (the product with 0 added, which no product of a
+// number differs from but -0).  Not written as assembly: e comes from a matrix product or an
+// exponential, whose waits the compiler places only before instructions that it knows.
+__device__ __forceinline__ float times(f16 h, float e) { return fmaf((float)h, e, 0.f); }
 __device__ __forceinline__ f16x8 frag(f16x2 a, f16x2 b, f16x2 c, f16x2 d) {
     return {a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
 }
@@ -270,9 +274,12 @@ __global__ __launch_bounds__(256) void q4_join_kernel(const float* partials, int
 // dims 8 g + {0, 4, 1, 5, 2, 6, 3, 7} as the keys' nibbles come.  float: scaled into
 // [-1, 1] by a power of two, so that two f16 terms hold any float32 range.  Returns what
 // the products are to be scaled by for scores in base 2.
-template <int NB, typename T>
+struct Same {
+    __device__ __forceinline__ float operator()(float x) const { return x; }
+};
+template <int NB, typename T, typename Over = Same>
 __device__ __forceinline__ float load_queries(const T* q, float scale_log2, f16x8 (&qh)[NB],
-                                              f16x8 (&ql)[sizeof(T) == 4 ? NB : 1]) {
+                                              f16x8 (&ql)[sizeof(T) == 4 ? NB : 1], Over over = Same()) {
     constexpr int at[8] = {0, 4, 1, 5, 2, 6, 3, 7};
     T x[NB][8];
 #pragma unroll
@@ -291,7 +298,7 @@ __device__ __forceinline__ float load_queries(const T* q, float scale_log2, f16x
         for (int b = 0; b < NB; b++)
 #pragma unroll
             for (int e = 0; e < 8; e++) most = fmaxf(most, fabsf(x[b][e]));
-        most = xor32_combine(xor16_combine(most, MaxOp()), MaxOp());
+        most = over(xor32_combine(xor16_combine(most, MaxOp()), MaxOp()));
         // (the bounds keep the scale itself, and a masked score's product with it, a number)
         const int ex = most > 0.f && most < INFINITY ? max(-100, min(__builtin_amdgcn_frexp_expf(most), 120)) : 0;
         const float down = ldexpf(1.f, -ex);
@@ -325,6 +332,46 @@ template <int NB>
 constexpr int lds_bytes(int waves) {
     return waves * 16 * (32 * NB + 4 + 2) * 4;
 }
+// Joins the waves' results of columns col0.., left in LDS: outputs xo[wave][column][dim], then
+// (maximum, sum) xml[wave][2][column].  `tiles`: how many the waves shared.
+template <int NB, typename T>
+__device__ __forceinline__ void join_waves(const SplitArgs& p, int kvh, int sp, int col0, int cols, int tiles,
+                                           uint8_t* lds) {
+    constexpr int HD = 32 * NB;
+    const int waves = blockDim.x >> 6, G = p.G;
+    float (*xo)[16][HD + 4] = (float (*)[16][HD + 4])lds;
+    float (*xml)[2][16] = (float (*)[2][16])(lds + waves * 16 * (HD + 4) * 4);
+    const int n = min(16, cols - col0), had = max(1, min(waves, tiles));  // (a wave without a tile adds nothing)
+    for (int i = threadIdx.x; i < n * (HD / 2); i += blockDim.x) {
+        const int qc = i / (HD / 2), d = 2 * (i % (HD / 2));
+        float mt = xml[0][0][qc];
+        for (int w = 1; w < had; w++) mt = fmaxf(mt, xml[w][0][qc]);
+        float lt = 0.f, oa = 0.f, ob = 0.f;
+        for (int w = 0; w < had; w++) {
+            const float f = join_weight(xml[w][0][qc], mt);
+            lt += f * xml[w][1][qc];
+            oa += f * xo[w][qc][d];
+            ob += f * xo[w][qc][d + 1];
+        }
+        if (p.splits == 1) {
+            const int64_t tt = p.by_group(col0 + qc), hh = kvh * G + col0 + qc - tt * G;
+            T* out = (T*)p.a.out + tt * p.a.out_stride + hh * HD + d;
+            out[0] = (T)(oa / lt);
+            out[1] = (T)(ob / lt);
+        } else {
+            float* pp = partial<HD>(p, kvh, col0 + qc) + sp * (HD + 2);
+            if (p.fused) {
+                put2<true>(pp + 2 + d, oa, ob);
+                if (d == 0) put2<true>(pp, mt, lt);
+            } else {
+                put2<false>(pp + 2 + d, oa, ob);
+                if (d == 0) put2<false>(pp, mt, lt);
+            }
+        }
+    }
+    if (p.fused) count_and_join<HD, T>(p, kvh, cols, lds);
+}
+
 template <int NB, typename T>
 __global__ __launch_bounds__(64 * kMostWaves) void q4_attention_kernel(SplitArgs p) {
     constexpr bool EXACT = sizeof(T) == 4;
@@ -488,35 +535,225 @@ __global__ __launch_bounds__(64 * kMostWaves) void q4_attention_kernel(SplitArgs
         xml[wave][1][c16] = l[0];
     }
     __syncthreads();
-    const int n = min(16, cols - col0), had = max(1, min(waves, t1 - t0));  // (a wave without a tile adds nothing)
-    for (int i = threadIdx.x; i < n * (HD / 2); i += blockDim.x) {
-        const int qc = i / (HD / 2), d = 2 * (i % (HD / 2));
-        float mt = xml[0][0][qc];
-        for (int w = 1; w < had; w++) mt = fmaxf(mt, xml[w][0][qc]);
-        float lt = 0.f, oa = 0.f, ob = 0.f;
-        for (int w = 0; w < had; w++) {
-            const float f = join_weight(xml[w][0][qc], mt);
-            lt += f * xml[w][1][qc];
-            oa += f * xo[w][qc][d];
-            ob += f * xo[w][qc][d + 1];
+    join_waves<NB, T>(p, kvh, sp, col0, cols, t1 - t0, lds);
+}
+
+// ------------------------------------------------------------------ few columns
+// Single tokens: up to few_columns(NB) = CP query columns, and all blocks of the head in
+// the 16 columns of a product.  Column CP b + c holds query c's block b, zeros standing
+// for the other blocks, so that one accumulator takes all blocks' scores, a lane scales
+// its own block's only, and a sum over the columns CP apart gives the score.  The
+// values' scales go into the probabilities the same way (a column has one block's), so
+// that values enter as n - 8, exactly, and of the products with each block's values a
+// lane keeps its own block's.  Bound by the vector instructions, two thirds of them the
+// unpacking, close to memory: 131,072 positions, 32/8 heads of 128, 35.7 us in float32
+// (4.2 TB/s) and 31.0 in f16, against 41.9 and 35 with a column a query; 8,000 positions,
+// 9/3 heads of 64, 8.2 us against 10.3.  Three tiles ahead instead of two: 37.2 us.
+// The probabilities times scales are held as P 2^14 d / 2^E, E the largest scale's
+// exponent so far, kept as the maximum of the softmax is.
+constexpr int few_columns(int nb) { return nb == 1 ? 16 : nb == 2 ? 8 : nb <= 4 ? 4 : 2; }
+
+typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
+
+template <int N>
+__device__ __forceinline__ float row_rotated(float x) {  // of 16 lanes
+    return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), 0x120 | N, 0xf, 0xf, true));
+}
+// Over the lanes of a row that are CP apart; the same bits in each.
+template <int CP, typename Op>
+__device__ __forceinline__ float over_slots(float x, Op op) {
+    if constexpr (CP <= 8) x = op(x, row_rotated<8>(x));
+    if constexpr (CP <= 4) x = op(x, row_rotated<4>(x));
+    if constexpr (CP <= 2) x = op(x, row_rotated<2>(x));
+    return x;
+}
+
+template <int NB>
+struct FewTile {
+    uint32_t k[2][NB];
+    uint2 v[NB], ks[2], vs[2];  // (the scales: of the lane's own block)
+    __device__ __forceinline__ void load(const uint8_t* kt, const uint8_t* vt, int lane, int scales_at) {
+#pragma unroll
+        for (int s = 0; s < 2; s++) {
+            const uint32_t* kw = (const uint32_t*)(kt + (s * 64 + lane) * 4 * NB);
+#pragma unroll
+            for (int b = 0; b < NB; b++) k[s][b] = gptr(kw)[b];
+            ks[s] = Tile<NB>::load2(kt + scales_at + s * 32 * NB);
+            vs[s] = Tile<NB>::load2(vt + scales_at + s * 32 * NB);
         }
-        if (p.splits == 1) {
-            const int64_t tt = p.by_group(col0 + qc), hh = kvh * G + col0 + qc - tt * G;
-            T* out = (T*)p.a.out + tt * p.a.out_stride + hh * HD + d;
-            out[0] = (T)(oa / lt);
-            out[1] = (T)(ob / lt);
-        } else {
-            float* pp = partial<HD>(p, kvh, col0 + qc) + sp * (HD + 2);
-            if (p.fused) {
-                put2<true>(pp + 2 + d, oa, ob);
-                if (d == 0) put2<true>(pp, mt, lt);
-            } else {
-                put2<false>(pp + 2 + d, oa, ob);
-                if (d == 0) put2<false>(pp, mt, lt);
+#pragma unroll
+        for (int b = 0; b < NB; b++) v[b] = Tile<NB>::load2(vt + b * 512 + lane * 8);
+    }
+};
+
+template <int NB, typename T>
+__global__ __launch_bounds__(64 * kMostWaves) void q4_attention_few_kernel(SplitArgs p) {
+    constexpr bool EXACT = sizeof(T) == 4;
+    constexpr int HD = 32 * NB, CP = few_columns(NB);
+    extern __shared__ __align__(16) uint8_t lds[];
+    const int waves = blockDim.x >> 6;
+    const int lane = threadIdx.x & 63, g = lane >> 4, slot = (lane & 15) / CP, cc = lane % CP, own = min(slot, NB - 1);
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const Nibbles nib;
+    const int kvh = blockIdx.x, sp = blockIdx.y, G = p.G, cols = p.a.tokens * G;  // (at most CP)
+    const int start = p.a.start_dev ? *p.a.start_dev : p.a.start;
+    const bool inside = start >= 0 && start <= p.c.capacity - p.a.tokens;
+    const int col = min(cc, cols - 1), t = p.by_group(col), h = kvh * G + col - t * G;
+    const int seen = start + t, last_seen = start + p.a.tokens - 1;
+    const int tiles = inside ? last_seen / kQ4Tile + 1 : 0;
+    const int t0 = share(tiles, sp, p.by_splits), t1 = share(tiles, sp + 1, p.by_splits);
+
+    const uint8_t* kt = p.c.k + (int64_t)kvh * q4_head_bytes(p.c.capacity, NB);
+    const uint8_t* vt = p.c.v + (int64_t)kvh * q4_head_bytes(p.c.capacity, NB);
+    const int scales_at = q4_scales_at(NB) + (g * NB + own) * 8;
+    constexpr int AHEAD = 2;  // tiles on their way or at work
+    FewTile<NB> x[AHEAD];
+    auto load = [&](FewTile<NB>& y, int tile) {
+        const int64_t at = min(tile, t1 - 1) * q4_tile_bytes(NB);  // (past the split's last tile: that one, unused)
+        y.load(kt + at, vt + at, lane, scales_at);
+    };
+    int j = t0 + wave;
+    if (j < t1)
+#pragma unroll
+        for (int i = 0; i < AHEAD - 1; i++) load(x[i], j + i * waves);
+
+    f16x8 qh[NB], ql[EXACT ? NB : 1], mine[2][1];
+    const float sc = load_queries<1, T>((const T*)p.a.q + (int64_t)t * p.a.q_stride + (int64_t)h * HD + 32 * own + 8 * g,
+                                        p.scale_log2, mine[0], mine[1],
+                                        [](float most) { return over_slots<CP>(most, MaxOp()); });
+    const f16x8 zero = {};
+#pragma unroll
+    for (int b = 0; b < NB; b++) {
+        qh[b] = slot == b ? mine[0][0] : zero;
+        if constexpr (EXACT) ql[b] = slot == b ? mine[1][0] : zero;
+    }
+
+    float m = -INFINITY, l = 0.f;
+    int E = -14;  // every scale so far is below 2^E,
+    u16x2 limit = {0x3FF, 0x3FF};  // the largest of these
+    f32x4 o[NB][2];
+#pragma unroll
+    for (int b = 0; b < NB; b++) o[b][0] = o[b][1] = f32x4{0.f, 0.f, 0.f, 0.f};
+    auto step = [&](FewTile<NB>& y, int tile) {
+        f32x4 sa[2];
+#pragma unroll
+        for (int s = 0; s < 2; s++) sa[s] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int b = 0; b < NB; b++)
+#pragma unroll
+            for (int s = 0; s < 2; s++) {
+                const uint32_t w = y.k[s][b], w8 = w >> 8;
+                const f16x8 kf = frag(nib.lo(w), nib.hi(w), nib.lo(w8), nib.hi(w8));
+                sa[s] = mfma(kf, qh[b], sa[s]);
+                if constexpr (EXACT) sa[s] = mfma(kf, ql[b], sa[s]);
+            }
+#pragma unroll
+        for (int s = 0; s < 2; s++) {
+            const f16x2 d0 = pair(y.ks[s].x), d1 = pair(y.ks[s].y);
+            sa[s] = f32x4{times(d0[0], sa[s][0]), times(d0[1], sa[s][1]), times(d1[0], sa[s][2]), times(d1[1], sa[s][3])};
+#pragma unroll
+            for (int r = 0; r < 4; r++) sa[s][r] = over_slots<CP>(sa[s][r], AddOp());
+        }
+        const int key0 = tile * kQ4Tile;
+        if (key0 + kQ4Tile - 1 > start) {
+#pragma unroll
+            for (int s = 0; s < 2; s++) {
+                uint32_t keep[2] = {0u, 0u};
+#pragma unroll
+                for (int r = 0; r < 4; r++) {
+                    const int key = key0 + 16 * s + 4 * g + r;
+                    if (key > seen) sa[s][r] = -INFINITY;
+                    if (key <= last_seen) keep[r >> 1] |= 0xFFFFu << (16 * (r & 1));
+                }
+                // positions that may never have been written: values of 0
+                y.vs[s].x &= keep[0];
+                y.vs[s].y &= keep[1];
             }
         }
+        const uint32_t dv[4] = {y.vs[0].x, y.vs[0].y, y.vs[1].x, y.vs[1].y};
+        u16x2 most = limit;
+#pragma unroll
+        for (int i = 0; i < 4; i++) most = __builtin_elementwise_max(most, __builtin_bit_cast(u16x2, dv[i] & 0x7FFF7FFFu));
+        float mx = sa[0][0];
+#pragma unroll
+        for (int i = 1; i < 8; i++) mx = fmaxf(mx, sa[i >> 2][i & 3]);
+        mx = xor32_combine(xor16_combine(mx, MaxOp()), MaxOp());
+        const float mn = fmaxf(m, mx * sc);
+        const float mref = mn == -INFINITY ? 0.f : mn;
+        if (__builtin_amdgcn_ballot_w64(m != mn || __builtin_bit_cast(uint32_t, most) != __builtin_bit_cast(uint32_t, limit))) {
+            float top = (float)max(most[0], most[1]);  // f16 bits, in order for what is not negative
+            top = xor32_combine(xor16_combine(top, MaxOp()), MaxOp());
+            const int now = ((int)top >> 10) - 14;
+            const float alpha = __builtin_amdgcn_exp2f(m - mref + (float)(E - now));
+            limit[0] = limit[1] = (uint16_t)((int)top | 0x3FF);
+            E = now;
+#pragma unroll
+            for (int b = 0; b < NB; b++) {
+                o[b][0] *= alpha;
+                o[b][1] *= alpha;
+            }
+            l *= alpha;
+            m = mn;
+        }
+        const float eref = kLog2P - mref - (float)E;
+        f16x2 ph[4], pl[EXACT ? 4 : 1];
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const f16x2 d = pair(dv[i]);
+            const float e0 = __builtin_amdgcn_exp2f(fmaf(sa[i >> 1][2 * (i & 1)], sc, eref));
+            const float e1 = __builtin_amdgcn_exp2f(fmaf(sa[i >> 1][2 * (i & 1) + 1], sc, eref));
+            l += e0 + e1;
+            const float w0 = times(d[0], e0), w1 = times(d[1], e1);
+            ph[i] = round2(w0, w1);
+            if constexpr (EXACT) pl[i] = round2(rest_low(ph[i], w0), rest_high(ph[i], w1));
+        }
+        const f16x8 pf = frag(ph[0], ph[1], ph[2], ph[3]);
+        f16x8 pg;
+        if constexpr (EXACT) pg = frag(pl[0], pl[1], pl[2], pl[3]);
+#pragma unroll
+        for (int b = 0; b < NB; b++) {
+            const uint32_t w0 = y.v[b].x, w1 = y.v[b].y, w08 = w0 >> 8, w18 = w1 >> 8;
+            const f16x8 even = frag(nib.lo(w0), nib.lo(w08), nib.lo(w1), nib.lo(w18));
+            const f16x8 odd = frag(nib.hi(w0), nib.hi(w08), nib.hi(w1), nib.hi(w18));
+            o[b][0] = mfma(even, pf, o[b][0]);
+            o[b][1] = mfma(odd, pf, o[b][1]);
+            if constexpr (EXACT) {
+                o[b][0] = mfma(even, pg, o[b][0]);
+                o[b][1] = mfma(odd, pg, o[b][1]);
+            }
+        }
+    };
+    for (; j < t1; j += AHEAD * waves) {
+#pragma unroll
+        for (int i = 0; i < AHEAD; i++) {
+            if (j + i * waves >= t1) break;
+            load(x[(i + AHEAD - 1) % AHEAD], j + (i + AHEAD - 1) * waves);
+            step(x[i], j + i * waves);
+        }
     }
-    if (p.fused) count_and_join<HD, T>(p, kvh, cols, lds);
+
+    // o[own][par][r] = O(column cc, dim 32 own + 2 (4 g + r) + par) / 2^E
+    float (*xo)[16][HD + 4] = (float (*)[16][HD + 4])lds;
+    float (*xml)[2][16] = (float (*)[2][16])(lds + waves * 16 * (HD + 4) * 4);
+    l = xor32_combine(xor16_combine(l, AddOp()), AddOp());
+#pragma unroll
+    for (int b = 1; b < NB; b++)
+        if (slot == b) {
+            o[0][0] = o[b][0];
+            o[0][1] = o[b][1];
+        }
+    if (slot < NB) {
+        const float up = ldexpf(1.f, E);
+#pragma unroll
+        for (int r = 0; r < 4; r++)
+            *(float2*)&xo[wave][cc][32 * slot + 2 * (4 * g + r)] = make_float2(o[0][0][r] * up, o[0][1][r] * up);
+        if (lane < CP) {
+            xml[wave][0][cc] = m;
+            xml[wave][1][cc] = l * up;
+        }
+    }
+    __syncthreads();
+    join_waves<NB, T>(p, kvh, sp, 0, cols, t1 - t0, lds);
 }
 
 // ------------------------------------------------------------------ many columns
@@ -907,9 +1144,15 @@ hipError_t launch_nb(const SplitArgs& p, const Q4Plan& plan, hipStream_t st) {
         if (plan.cols == 128) return launch_wide<NB, 2, 2, T>(p, cols, st);
     if constexpr (most >= 64)
         if (plan.cols == 64) return launch_wide<NB, 1, 2, T>(p, cols, st);
+    const dim3 grid((unsigned)((cols + 15) / 16 * p.c.kv_heads), p.splits);
+    if (cols <= few_columns(NB)) {
+        static OncePerDevice once;
+        if (hipError_t e = allow_whole_lds(once, (const void*)q4_attention_few_kernel<NB, T>)) return e;
+        q4_attention_few_kernel<NB, T><<<grid, 64 * plan.waves, lds_bytes<NB>(plan.waves), st>>>(p);
+        return hipGetLastError();
+    }
     static OncePerDevice once;
     if (hipError_t e = allow_whole_lds(once, (const void*)q4_attention_kernel<NB, T>)) return e;
-    const dim3 grid((unsigned)((cols + 15) / 16 * p.c.kv_heads), p.splits);
     q4_attention_kernel<NB, T><<<grid, 64 * plan.waves, lds_bytes<NB>(plan.waves), st>>>(p);
     return hipGetLastError();
 }
@@ -941,7 +1184,8 @@ hipError_t launch(const SplitArgs& p, const Q4Plan& plan, hipStream_t st) {
 // nb / 18 us a tile of its keys; joining costs 1.5 us in the same launch, 7 as one
 // of its own.  In the same launch a split has a tile a wave until there are 16 splits
 // (32/8 heads of 128, 4,000 positions: 32.8 us in one, 13.8 in 4, 9.7 in 16, 12.1
-// in 32), then 32 tiles, which hide the waits of 32 splits and more.
+// in 32), then 32 tiles, which hide the waits of 32 splits and more, or 16 of more than
+// 4 blocks (4/2 heads of 256, 30,000 positions: 15.4 us in 64, 17.5 in 32).
 Q4Plan q4_attention_plan(bool f16_rows, int tokens, int heads, int kv_heads, int hd, int length) {
     Q4Plan r;
     const int64_t cols = (int64_t)tokens * (heads / kv_heads);
@@ -962,7 +1206,7 @@ Q4Plan q4_attention_plan(bool f16_rows, int tokens, int heads, int kv_heads, int
     const int most = std::max(1, (int)(cus / groups(16)));
     const int64_t pairs = cols * (hd / 2);  // of dims to join
     const bool can_fuse = cols <= 16 && pairs <= 512 && kv_heads <= kQ4Counters;
-    if (can_fuse) r.splits = work <= 40 ? 1 : std::min(most, std::max(std::min(16, up(tiles, 4)), up(tiles, 32)));
+    if (can_fuse) r.splits = work <= 40 ? 1 : std::min(most, std::max(std::min(16, up(tiles, 4)), up(tiles, hd > 128 ? 16 : 32)));
     else r.splits = work <= 200 ? 1 : std::min(most, up(work, 64));
     r.fused = can_fuse && r.splits > 1;
     // Eight waves where each still has many tiles (131,072 positions in 32 splits: 42.0 us against

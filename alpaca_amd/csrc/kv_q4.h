@@ -30,7 +30,7 @@
 constexpr int kQ4Tile = 32;  // tokens
 constexpr float kQ4Most = 65504.f;
 
-__host__ __device__ constexpr int q4_tile_bytes(int nb) { return 576 * nb; }
+__host__ __device__ constexpr int64_t q4_tile_bytes(int nb) { return 576 * nb; }  // (64 bits: a tile index times it may need them)
 __host__ __device__ constexpr int q4_scales_at(int nb) { return 512 * nb; }
 __host__ __device__ inline int q4_tiles(int capacity) { return (int)(((int64_t)capacity + kQ4Tile - 1) / kQ4Tile); }
 __host__ __device__ inline int64_t q4_head_bytes(int capacity, int nb) {
