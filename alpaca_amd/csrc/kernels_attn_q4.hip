@@ -86,7 +86,6 @@ struct SplitArgs {
     Q4Cache c;
     int G, splits;
     Divisor by_group, by_heads, by_splits;
-    bool fused;  // the last workgroup of a KV head joins the splits
     float scale_log2;
 };
 
@@ -121,9 +120,9 @@ struct Tile {
 
 // ------------------------------------------------------------------ joining the splits
 // A split leaves (maximum, sum, unnormalised output) of its columns in the
-// workspace.  Few columns (a workgroup's threads hold two dims of each): the last
-// workgroup of a KV head to arrive joins them in the same launch, 3 us of GPU time
-// and as much on the host less than a second one.  Its partial results are
+// workspace.  Up to 16 columns a workgroup: the last workgroup of a group of columns
+// to arrive joins them in the same launch, 3 us of GPU time and as much on the host
+// less than a second one.  Its partial results are
 // written and read with agent-scope accesses, which the L2 caches of all XCDs see;
 // each thread waits for its own to be acknowledged before the count, and the last
 // sets the counter back to zero for the next call.  More columns: a second kernel,
@@ -141,16 +140,12 @@ __device__ __forceinline__ void join_add(Joined& j, float m, float l, float a, f
     j.a = j.a * f + a * w;
     j.b = j.b * f + b * w;
 }
-// Two floats, past the caches of an XCD (SHARED) or as usual.
-template <bool SHARED>
+// Two floats past the caches of an XCD.
 __device__ __forceinline__ void put2(float* p, float a, float b) {
-    if constexpr (SHARED) {
-        const uint64_t u = (uint64_t)__float_as_uint(b) << 32 | __float_as_uint(a);
-        __hip_atomic_store(gptr((uint64_t*)p), u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    } else {
-        *(float2*)p = make_float2(a, b);
-    }
+    const uint64_t u = (uint64_t)__float_as_uint(b) << 32 | __float_as_uint(a);
+    __hip_atomic_store(gptr((uint64_t*)p), u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
+// And back (SHARED), or from an earlier launch.
 template <bool SHARED>
 __device__ __forceinline__ float2 get2(const float* p) {
     if constexpr (!SHARED) return *(const float2*)p;
@@ -214,14 +209,15 @@ __device__ __forceinline__ float* partial(const SplitArgs& p, int kvh, int col) 
     return p.a.partials + ((int64_t)t * p.a.heads + h) * p.splits * (HD + 2);
 }
 
-// Called by the whole workgroup once its partial results are written; `lds` is free.
+// Called by the whole workgroup once its partial results of columns [col0, col0 + n) are
+// written; `lds` is free.
 template <int HD, typename T>
-__device__ __forceinline__ void count_and_join(const SplitArgs& p, int kvh, int cols, void* lds) {
+__device__ __forceinline__ void count_and_join(const SplitArgs& p, int kvh, int col0, int n, void* lds) {
     int* last = (int*)lds;
     __builtin_amdgcn_s_waitcnt(0);
     __syncthreads();
     if (threadIdx.x == 0) {
-        int* counter = p.a.counters + kvh;
+        int* counter = p.a.counters + blockIdx.x;
         *last = __hip_atomic_fetch_add(counter, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == p.splits - 1;
         if (*last) __hip_atomic_store(counter, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     }
@@ -229,14 +225,24 @@ __device__ __forceinline__ void count_and_join(const SplitArgs& p, int kvh, int 
     const bool mine = *last;
     __syncthreads();  // (*last is read; the joining uses its place)
     if (!mine) return;
-    const int items = cols * (HD / 2), groups = blockDim.x / items;  // (at least 1: p.fused)
-    const int group = threadIdx.x / items, i = threadIdx.x - group * items, col = i / (HD / 2), d = 2 * (i % (HD / 2));
+    auto put = [&](int col, int d, const Joined& j) {
+        const int t = p.by_group(col), h = kvh * p.G + col - t * p.G;
+        T* out = (T*)p.a.out + t * p.a.out_stride + (int64_t)h * HD + d;
+        out[0] = (T)(j.a / j.l);
+        out[1] = (T)(j.b / j.l);
+    };
+    const int items = n * (HD / 2);
+    if (2 * items > (int)blockDim.x) {
+        for (int i = threadIdx.x; i < items; i += blockDim.x) {
+            const int col = col0 + i / (HD / 2), d = 2 * (i % (HD / 2));
+            put(col, d, join<8, true>(partial<HD>(p, kvh, col), HD, d, 0, 1, p.splits));
+        }
+        return;
+    }
+    const int groups = blockDim.x / items, group = threadIdx.x / items, i = threadIdx.x - group * items;
+    const int col = col0 + i / (HD / 2), d = 2 * (i % (HD / 2));
     const Joined j = join_groups<8, true>(partial<HD>(p, kvh, col), HD, d, group, groups, items, i, p.splits, (float4*)lds);
-    if (group) return;
-    const int t = p.by_group(col), h = kvh * p.G + col - t * p.G;
-    T* out = (T*)p.a.out + t * p.a.out_stride + (int64_t)h * HD + d;
-    out[0] = (T)(j.a / j.l);
-    out[1] = (T)(j.b / j.l);
+    if (group == 0) put(col, d, j);
 }
 
 // The joining kernel: GROUPED, a workgroup a query and head; else two dims a thread.
@@ -360,16 +366,11 @@ __device__ __forceinline__ void join_waves(const SplitArgs& p, int kvh, int sp, 
             out[1] = (T)(ob / lt);
         } else {
             float* pp = partial<HD>(p, kvh, col0 + qc) + sp * (HD + 2);
-            if (p.fused) {
-                put2<true>(pp + 2 + d, oa, ob);
-                if (d == 0) put2<true>(pp, mt, lt);
-            } else {
-                put2<false>(pp + 2 + d, oa, ob);
-                if (d == 0) put2<false>(pp, mt, lt);
-            }
+            put2(pp + 2 + d, oa, ob);
+            if (d == 0) put2(pp, mt, lt);
         }
     }
-    if (p.fused) count_and_join<HD, T>(p, kvh, cols, lds);
+    if (p.splits > 1) count_and_join<HD, T>(p, kvh, col0, n, lds);
 }
 
 template <int NB, typename T>
@@ -1196,12 +1197,15 @@ hipError_t launch(const SplitArgs& p, const Q4Plan& plan, hipStream_t st) {
 // (prompt of 2,048 tokens, 32/8 heads of 128, 63 us against 79; 512 tokens of it 17
 // against 13), at most head dimension 128 (registers).
 //
-// Splits, up to a workgroup a CU over all.  A workgroup alone costs about 5.5 us and
-// nb / 18 us a tile of its keys; joining costs 1.5 us in the same launch, 7 as one
-// of its own.  In the same launch a split has a tile a wave until there are 16 splits
-// (32/8 heads of 128, 4,000 positions: 32.8 us in one, 13.8 in 4, 9.7 in 16, 12.1
-// in 32), then 32 tiles, which hide the waits of 32 splits and more, or 16 of more than
-// 4 blocks (4/2 heads of 256, 30,000 positions: 15.4 us in 64, 17.5 in 32).
+// Splits, up to a workgroup a CU over all.  A workgroup alone costs about 4 us and
+// nb / 18 us a tile of its keys; joining costs 1.5 us in the same launch (4 with 16
+// full columns), 7 as one of its own.  In the same launch a split has a tile a wave
+// until there are 16 splits (32/8 heads of 128, one token at 4,000: 32.8 us in one,
+// 13.8 in 4, 9.7 in 16, 12.1 in 32; 37 at 1,021, 15/5 heads of 64: 8.5 in one, 8.0
+// in 7), then 32 tiles, which hide the waits of 32 splits and more, or 16 of more than
+// 4 blocks (4/2 heads of 256, 30,000 positions: 15.4 us in 64, 17.5 in 32).  Two or
+// three splits pay over long caches only (64 queries of 32/8 heads of 128 at 1,000:
+// 13.9 in two, 13.5 in one; 37 of 15/5 heads of 64 at 8,000: 22.6 and 34.6).
 Q4Plan q4_attention_plan(bool f16_rows, int tokens, int heads, int kv_heads, int hd, int length) {
     Q4Plan r;
     const int64_t cols = (int64_t)tokens * (heads / kv_heads);
@@ -1219,16 +1223,13 @@ Q4Plan q4_attention_plan(bool f16_rows, int tokens, int heads, int kv_heads, int
         return r;
     }
     r.cols = 16;
-    const int most = std::max(1, (int)(cus / groups(16)));
-    const int64_t pairs = cols * (hd / 2);  // of dims to join
-    const bool can_fuse = cols <= 16 && pairs <= 512 && kv_heads <= kQ4Counters;
-    if (can_fuse) r.splits = work <= 40 ? 1 : std::min(most, std::max(std::min(16, up(tiles, 4)), up(tiles, hd > 128 ? 16 : 32)));
-    else r.splits = work <= 200 ? 1 : std::min(most, up(work, 64));
-    r.fused = can_fuse && r.splits > 1;
+    const int most = groups(16) <= kQ4Counters ? std::max(1, (int)(cus / groups(16))) : 1;
+    r.splits = work <= 40 ? 1 : std::min(most, std::max(std::min(16, up(tiles, 4)), up(tiles, hd > 128 ? 16 : 32)));
+    if (r.splits < 4 && work <= 200) r.splits = 1;
     // Eight waves where each still has many tiles (131,072 positions in 32 splits: 42.0 us against
     // 44.2 with four; 4,000 in 16: 10.2 against 9.7) and the chip is not full without them (512
     // float32 queries, 32/8 heads of 128: 31.9 against 23.1), or for the threads that join.
-    r.waves = (up(tiles, r.splits) >= 16 && groups(16) * r.splits <= cus) || (r.fused && pairs > 256) ? 8 : 4;
+    r.waves = (up(tiles, r.splits) >= 16 && groups(16) * r.splits <= cus) || (r.splits > 1 && cols * (hd / 2) > 256) ? 8 : 4;
     return r;
 }
 
@@ -1252,10 +1253,9 @@ hipError_t launch_q4_attention(bool f16_rows, const Q4Attention& a, const Q4Cach
     p.by_group = Divisor(p.G);
     p.by_heads = Divisor(c.kv_heads);
     p.by_splits = Divisor(plan.splits);
-    p.fused = plan.fused;
     const int hd = 32 * c.nb;
     p.scale_log2 = 1.4426950408889634f / sqrtf((float)hd);
     if (hipError_t e = f16_rows ? launch<f16>(p, plan, st) : launch<float>(p, plan, st)) return e;
-    if (plan.splits == 1 || plan.fused) return hipSuccess;
+    if (plan.splits == 1 || plan.cols == 16) return hipSuccess;
     return f16_rows ? launch_join<f16>(a, hd, plan.splits, st) : launch_join<float>(a, hd, plan.splits, st);
 }

@@ -96,12 +96,11 @@ struct Q4Attention {
     int* counters = nullptr;
 };
 constexpr int kQ4Counters = 512;
-// How a call runs: query columns and waves of a workgroup, parts the keys are split into, and
-// whether the last workgroup to arrive joins them.  `length`: the positions that the call may see;
-// the splits do not fall as it grows.
+// How a call runs: query columns of a workgroup, its waves (16 columns only), and parts the keys
+// are split into.  `length`: the positions that the call may see; the splits do not fall as it
+// grows, and the rest does not depend on it but for the waves.
 struct Q4Plan {
     int cols = 16, waves = 4, splits = 1;
-    bool fused = false;
 };
 Q4Plan q4_attention_plan(bool f16_rows, int tokens, int heads, int kv_heads, int hd, int length);
 // Bytes of a launch's workspace, the counters first; 0 for one part.
