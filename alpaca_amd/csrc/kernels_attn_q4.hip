@@ -335,19 +335,19 @@ __device__ __forceinline__ void add_scaled(f32x4& s, f32x4 part, uint2 d) {
 // Up to kMostWaves waves a workgroup, each with key tiles of its own.
 constexpr int kMostWaves = 8;
 template <int NB>
-constexpr int lds_bytes(int waves) {
-    return waves * 16 * (32 * NB + 4 + 2) * 4;
+constexpr int lds_bytes(int waves, int cols) {
+    return waves * cols * (32 * NB + 4 + 2) * 4;
 }
 // Joins the waves' results of columns col0.., left in LDS: outputs xo[wave][column][dim], then
 // (maximum, sum) xml[wave][2][column].  `tiles`: how many the waves shared.
-template <int NB, typename T>
+template <int NB, int COLS, typename T>
 __device__ __forceinline__ void join_waves(const SplitArgs& p, int kvh, int sp, int col0, int cols, int tiles,
                                            uint8_t* lds) {
     constexpr int HD = 32 * NB;
     const int waves = blockDim.x >> 6, G = p.G;
-    float (*xo)[16][HD + 4] = (float (*)[16][HD + 4])lds;
-    float (*xml)[2][16] = (float (*)[2][16])(lds + waves * 16 * (HD + 4) * 4);
-    const int n = min(16, cols - col0), had = max(1, min(waves, tiles));  // (a wave without a tile adds nothing)
+    float (*xo)[COLS][HD + 4] = (float (*)[COLS][HD + 4])lds;
+    float (*xml)[2][COLS] = (float (*)[2][COLS])(lds + waves * COLS * (HD + 4) * 4);
+    const int n = min(COLS, cols - col0), had = max(1, min(waves, tiles));  // (a wave without a tile adds nothing)
     for (int i = threadIdx.x; i < n * (HD / 2); i += blockDim.x) {
         const int qc = i / (HD / 2), d = 2 * (i % (HD / 2));
         float mt = xml[0][0][qc];
@@ -373,26 +373,24 @@ __device__ __forceinline__ void join_waves(const SplitArgs& p, int kvh, int sp, 
     if (p.splits > 1) count_and_join<HD, T>(p, kvh, col0, n, lds);
 }
 
-template <int NB, typename T>
+template <int NB, int CT, typename T>
 __global__ __launch_bounds__(64 * kMostWaves) void q4_attention_kernel(SplitArgs p) {
     constexpr bool EXACT = sizeof(T) == 4;
-    constexpr int HD = 32 * NB;
+    constexpr int HD = 32 * NB, COLS = 16 * CT;
     extern __shared__ __align__(16) uint8_t lds[];
     const int waves = blockDim.x >> 6;
-    float (*xo)[16][HD + 4] = (float (*)[16][HD + 4])lds;
-    float (*xml)[2][16] = (float (*)[2][16])(lds + waves * 16 * (HD + 4) * 4);
+    float (*xo)[COLS][HD + 4] = (float (*)[COLS][HD + 4])lds;
+    float (*xml)[2][COLS] = (float (*)[2][COLS])(lds + waves * COLS * (HD + 4) * 4);
     const int lane = threadIdx.x & 63, g = lane >> 4, c16 = lane & 15;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const Nibbles nib;
     const int id = p.by_heads(blockIdx.x), kvh = blockIdx.x - id * p.c.kv_heads;
-    const int sp = blockIdx.y, col0 = id * 16;
+    const int sp = blockIdx.y, col0 = id * COLS;
     const int G = p.G, cols = p.a.tokens * G;
     const int start = p.a.start_dev ? *p.a.start_dev : p.a.start;
     const bool inside = start >= 0 && start <= p.c.capacity - p.a.tokens;
-    const int col = min(col0 + c16, cols - 1), t = p.by_group(col), h = kvh * G + col - t * G;
-    const int seen = start + t;  // the column's last position
     // the tiles of this column group, and this split's share of them
-    const int first_seen = start + p.by_group(col0), last_seen = start + p.by_group(min(col0 + 15, cols - 1));
+    const int first_seen = start + p.by_group(col0), last_seen = start + p.by_group(min(col0 + COLS - 1, cols - 1));
     const int tiles = inside ? last_seen / kQ4Tile + 1 : 0;
     const int t0 = share(tiles, sp, p.by_splits), t1 = share(tiles, sp + 1, p.by_splits);
 
@@ -408,29 +406,40 @@ __global__ __launch_bounds__(64 * kMostWaves) void q4_attention_kernel(SplitArgs
     };
     if (j < t1) load(xa, j);
 
-    f16x8 qh[NB], ql[EXACT ? NB : 1];
-    const float sc = load_queries<NB, T>((const T*)p.a.q + (int64_t)t * p.a.q_stride + (int64_t)h * HD + 8 * g,
-                                         p.scale_log2, qh, ql);
-
-    float m = -INFINITY;
-    f32x4 o[NB][2], l = {0.f, 0.f, 0.f, 0.f};
+    f16x8 qh[CT][NB], ql[CT][EXACT ? NB : 1];
+    float sc[CT], m[CT];
+    int seen[CT];  // a column's last position
+    f32x4 o[CT][NB][2], l[CT];
 #pragma unroll
-    for (int b = 0; b < NB; b++) o[b][0] = o[b][1] = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int ct = 0; ct < CT; ct++) {
+        const int col = min(col0 + 16 * ct + c16, cols - 1), t = p.by_group(col), h = kvh * G + col - t * G;
+        seen[ct] = start + t;
+        sc[ct] = load_queries<NB, T>((const T*)p.a.q + (int64_t)t * p.a.q_stride + (int64_t)h * HD + 8 * g, p.scale_log2,
+                                     qh[ct], ql[ct]);
+        m[ct] = -INFINITY;
+        l[ct] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int b = 0; b < NB; b++) o[ct][b][0] = o[ct][b][1] = f32x4{0.f, 0.f, 0.f, 0.f};
+    }
     const f16x2 one2 = {(f16)1.f, (f16)1.f};
     const f16x8 ones = frag(one2, one2, one2, one2);
     auto step = [&](Tile<NB>& x, int tile) {
         // S^T(key 16 s + 4 g + r, column c16)
-        f32x4 sa[2];
+        f32x4 sa[CT][2];
 #pragma unroll
         for (int s = 0; s < 2; s++) {
-            sa[s] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int ct = 0; ct < CT; ct++) sa[ct][s] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
             for (int b = 0; b < NB; b++) {
                 const uint32_t w = x.k[s][b], w8 = w >> 8;
                 const f16x8 kf = frag(nib.lo(w), nib.hi(w), nib.lo(w8), nib.hi(w8));
-                f32x4 part = mfma(kf, qh[b], f32x4{0.f, 0.f, 0.f, 0.f});
-                if constexpr (EXACT) part = mfma(kf, ql[b], part);
-                add_scaled(sa[s], part, x.ks[s][b]);
+#pragma unroll
+                for (int ct = 0; ct < CT; ct++) {
+                    f32x4 part = mfma(kf, qh[ct][b], f32x4{0.f, 0.f, 0.f, 0.f});
+                    if constexpr (EXACT) part = mfma(kf, ql[ct][b], part);
+                    add_scaled(sa[ct][s], part, x.ks[s][b]);
+                }
             }
         }
         const int key0 = tile * kQ4Tile;
@@ -441,7 +450,9 @@ __global__ __launch_bounds__(64 * kMostWaves) void q4_attention_kernel(SplitArgs
 #pragma unroll
                 for (int r = 0; r < 4; r++) {
                     const int key = key0 + 16 * s + 4 * g + r;
-                    if (key > seen) sa[s][r] = -INFINITY;
+#pragma unroll
+                    for (int ct = 0; ct < CT; ct++)
+                        if (key > seen[ct]) sa[ct][s][r] = -INFINITY;
                     if (key <= last_seen) keep[r >> 1] |= 0xFFFFu << (16 * (r & 1));
                 }
                 // positions that may never have been written: values of 0, since 0 times what lies there may be NaN
@@ -452,36 +463,40 @@ __global__ __launch_bounds__(64 * kMostWaves) void q4_attention_kernel(SplitArgs
                 }
             }
         }
-        float mx = sa[0][0];
+        f16x8 pf[CT], pg[CT];
 #pragma unroll
-        for (int i = 1; i < 8; i++) mx = fmaxf(mx, sa[i >> 2][i & 3]);
-        mx = xor32_combine(xor16_combine(mx, MaxOp()), MaxOp());
-        const float mn = fmaxf(m, mx * sc);  // (sc > 0)
-        const float mref = mn == -INFINITY ? 0.f : mn;
-        const float alpha = __builtin_amdgcn_exp2f(m - mref), eref = kLog2P - mref;
-        f16x2 ph[4], pl[EXACT ? 4 : 1];
+        for (int ct = 0; ct < CT; ct++) {
+            const f32x4(&x)[2] = sa[ct];
+            float mx = x[0][0];
 #pragma unroll
-        for (int i = 0; i < 4; i++) {
-            const float e0 = __builtin_amdgcn_exp2f(fmaf(sa[i >> 1][2 * (i & 1)], sc, eref));
-            const float e1 = __builtin_amdgcn_exp2f(fmaf(sa[i >> 1][2 * (i & 1) + 1], sc, eref));
-            ph[i] = round2(e0, e1);
-            if constexpr (EXACT) pl[i] = round2(rest_low(ph[i], e0), rest_high(ph[i], e1));
-        }
-        if (__builtin_amdgcn_ballot_w64(m != mn)) {
+            for (int i = 1; i < 8; i++) mx = fmaxf(mx, x[i >> 2][i & 3]);
+            mx = xor32_combine(xor16_combine(mx, MaxOp()), MaxOp());
+            const float mn = fmaxf(m[ct], mx * sc[ct]);  // (sc > 0)
+            const float mref = mn == -INFINITY ? 0.f : mn;
+            const float alpha = __builtin_amdgcn_exp2f(m[ct] - mref), eref = kLog2P - mref;
+            f16x2 ph[4], pl[EXACT ? 4 : 1];
 #pragma unroll
-            for (int b = 0; b < NB; b++) {
-                o[b][0] *= alpha;
-                o[b][1] *= alpha;
+            for (int i = 0; i < 4; i++) {
+                const float e0 = __builtin_amdgcn_exp2f(fmaf(x[i >> 1][2 * (i & 1)], sc[ct], eref));
+                const float e1 = __builtin_amdgcn_exp2f(fmaf(x[i >> 1][2 * (i & 1) + 1], sc[ct], eref));
+                ph[i] = round2(e0, e1);
+                if constexpr (EXACT) pl[i] = round2(rest_low(ph[i], e0), rest_high(ph[i], e1));
             }
-            l *= alpha;
-            m = mn;
-        }
-        const f16x8 pf = frag(ph[0], ph[1], ph[2], ph[3]);
-        f16x8 pg;
-        l = mfma(ones, pf, l);
-        if constexpr (EXACT) {
-            pg = frag(pl[0], pl[1], pl[2], pl[3]);
-            l = mfma(ones, pg, l);
+            if (__builtin_amdgcn_ballot_w64(m[ct] != mn)) {
+#pragma unroll
+                for (int b = 0; b < NB; b++) {
+                    o[ct][b][0] *= alpha;
+                    o[ct][b][1] *= alpha;
+                }
+                l[ct] *= alpha;
+                m[ct] = mn;
+            }
+            pf[ct] = frag(ph[0], ph[1], ph[2], ph[3]);
+            l[ct] = mfma(ones, pf[ct], l[ct]);
+            if constexpr (EXACT) {
+                pg[ct] = frag(pl[0], pl[1], pl[2], pl[3]);
+                l[ct] = mfma(ones, pg[ct], l[ct]);
+            }
         }
 #pragma unroll
         for (int b = 0; b < NB; b++) {
@@ -501,10 +516,14 @@ __global__ __launch_bounds__(64 * kMostWaves) void q4_attention_kernel(SplitArgs
                     if constexpr (EXACT) lo[i] = __builtin_elementwise_fma(n[i], d[i], -hi[i]);
                 }
                 const f16x8 vh = frag(hi[0], hi[1], hi[2], hi[3]);
-                o[b][par] = mfma(vh, pf, o[b][par]);
-                if constexpr (EXACT) {
-                    o[b][par] = mfma(vh, pg, o[b][par]);
-                    o[b][par] = mfma(frag(lo[0], lo[1], lo[2], lo[3]), pf, o[b][par]);
+#pragma unroll
+                for (int ct = 0; ct < CT; ct++) {
+                    f32x4& y = o[ct][b][par];
+                    y = mfma(vh, pf[ct], y);
+                    if constexpr (EXACT) {
+                        y = mfma(vh, pg[ct], y);
+                        y = mfma(frag(lo[0], lo[1], lo[2], lo[3]), pf[ct], y);
+                    }
                 }
             }
         }
@@ -525,18 +544,22 @@ __global__ __launch_bounds__(64 * kMostWaves) void q4_attention_kernel(SplitArgs
         }
     }
 
-    // o[b][par][r] = O(column c16, dim 32 b + 2 (4 g + r) + par)
+    // o[ct][b][par][r] = O(column 16 ct + c16, dim 32 b + 2 (4 g + r) + par)
 #pragma unroll
-    for (int b = 0; b < NB; b++)
+    for (int ct = 0; ct < CT; ct++) {
+        const int c = 16 * ct + c16;
 #pragma unroll
-        for (int r = 0; r < 4; r++)
-            *(float2*)&xo[wave][c16][32 * b + 2 * (4 * g + r)] = make_float2(o[b][0][r], o[b][1][r]);
-    if (g == 0) {
-        xml[wave][0][c16] = m;
-        xml[wave][1][c16] = l[0];
+        for (int b = 0; b < NB; b++)
+#pragma unroll
+            for (int r = 0; r < 4; r++)
+                *(float2*)&xo[wave][c][32 * b + 2 * (4 * g + r)] = make_float2(o[ct][b][0][r], o[ct][b][1][r]);
+        if (g == 0) {
+            xml[wave][0][c] = m[ct];
+            xml[wave][1][c] = l[ct][0];
+        }
     }
     __syncthreads();
-    join_waves<NB, T>(p, kvh, sp, col0, cols, t1 - t0, lds);
+    join_waves<NB, COLS, T>(p, kvh, sp, col0, cols, t1 - t0, lds);
 }
 
 // ------------------------------------------------------------------ few columns
@@ -754,7 +777,7 @@ __global__ __launch_bounds__(64 * kMostWaves) void q4_attention_few_kernel(Split
         }
     }
     __syncthreads();
-    join_waves<NB, T>(p, kvh, sp, 0, cols, t1 - t0, lds);
+    join_waves<NB, 16, T>(p, kvh, sp, 0, cols, t1 - t0, lds);
 }
 
 // ------------------------------------------------------------------ many columns
@@ -1146,6 +1169,15 @@ hipError_t launch_wide(const SplitArgs& p, int64_t cols, hipStream_t st) {
     return hipGetLastError();
 }
 
+template <auto* kernel, int NB, int COLS>
+hipError_t launch_waves(const SplitArgs& p, const Q4Plan& plan, int64_t cols, hipStream_t st) {
+    static OncePerDevice once;
+    if (hipError_t e = allow_whole_lds(once, (const void*)kernel)) return e;
+    const dim3 grid((unsigned)((cols + COLS - 1) / COLS * p.c.kv_heads), p.splits);
+    kernel<<<grid, 64 * plan.waves, lds_bytes<NB>(plan.waves, COLS), st>>>(p);
+    return hipGetLastError();
+}
+
 // Columns of a workgroup of the wide kernel at most, for nb blocks a head: as registers and LDS allow,
 // and in float32, where its barriers cost small heads more than unpacking does (512 queries at 3,584
 // positions, 32/32 heads of 64: 78 us against 65 with a wave's tiles its own), from head dimension 128.
@@ -1161,17 +1193,10 @@ hipError_t launch_nb(const SplitArgs& p, const Q4Plan& plan, hipStream_t st) {
         if (plan.cols == 128) return launch_wide<NB, 2, 2, T>(p, cols, st);
     if constexpr (most >= 64)
         if (plan.cols == 64) return launch_wide<NB, 1, 2, T>(p, cols, st);
-    const dim3 grid((unsigned)((cols + 15) / 16 * p.c.kv_heads), p.splits);
-    if (cols <= few_columns(NB)) {
-        static OncePerDevice once;
-        if (hipError_t e = allow_whole_lds(once, (const void*)q4_attention_few_kernel<NB, T>)) return e;
-        q4_attention_few_kernel<NB, T><<<grid, 64 * plan.waves, lds_bytes<NB>(plan.waves), st>>>(p);
-        return hipGetLastError();
-    }
-    static OncePerDevice once;
-    if (hipError_t e = allow_whole_lds(once, (const void*)q4_attention_kernel<NB, T>)) return e;
-    q4_attention_kernel<NB, T><<<grid, 64 * plan.waves, lds_bytes<NB>(plan.waves), st>>>(p);
-    return hipGetLastError();
+    if constexpr (NB <= 3 && sizeof(T) == 4)
+        if (plan.cols == 32) return launch_waves<q4_attention_kernel<NB, 2, T>, NB, 32>(p, plan, cols, st);
+    if (cols <= few_columns(NB)) return launch_waves<q4_attention_few_kernel<NB, T>, NB, 16>(p, plan, cols, st);
+    return launch_waves<q4_attention_kernel<NB, 1, T>, NB, 16>(p, plan, cols, st);
 }
 
 template <typename T>
@@ -1190,7 +1215,7 @@ hipError_t launch(const SplitArgs& p, const Q4Plan& plan, hipStream_t st) {
 
 }  // namespace
 
-// How a call runs.  Columns of a workgroup: 16 (every wave key tiles of its own) up
+// How a call runs.  Columns of a workgroup: 16 or 32 (every wave key tiles of its own) up
 // to 64 columns, 64 or 128 from there in f16, where unpacking a tile once for all
 // of them pays (64 columns over 8,000 positions, 8 KV heads of 128: 17.2 us either
 // way; 300: 27 us with 64 a workgroup).  128 where workgroups of 128 fill the chip
@@ -1223,13 +1248,17 @@ Q4Plan q4_attention_plan(bool f16_rows, int tokens, int heads, int kv_heads, int
         return r;
     }
     r.cols = 16;
-    const int most = groups(16) <= kQ4Counters ? std::max(1, (int)(cus / groups(16))) : 1;
+    // 32 a workgroup, its waves unpacking a tile for both halves, where they are four times the CUs:
+    // 4,000 float32 queries of 15/5 heads of 64 108 us against 122, 2,048 40.1 against 41.1, 777 14.7
+    // against 12.4; at most 3 blocks a head (registers).
+    if (!f16_rows && hd <= 96 && groups(32) >= 4 * cus) r.cols = 32;
+    const int most = groups(r.cols) <= kQ4Counters ? std::max(1, (int)(cus / groups(r.cols))) : 1;
     r.splits = work <= 40 ? 1 : std::min(most, std::max(std::min(16, up(tiles, 4)), up(tiles, hd > 128 ? 16 : 32)));
     if (r.splits < 4 && work <= 200) r.splits = 1;
     // Eight waves where each still has many tiles (131,072 positions in 32 splits: 42.0 us against
     // 44.2 with four; 4,000 in 16: 10.2 against 9.7) and the chip is not full without them (512
     // float32 queries, 32/8 heads of 128: 31.9 against 23.1), or for the threads that join.
-    r.waves = (up(tiles, r.splits) >= 16 && groups(16) * r.splits <= cus) || (r.splits > 1 && cols * (hd / 2) > 256) ? 8 : 4;
+    r.waves = (up(tiles, r.splits) >= 16 && groups(r.cols) * r.splits <= cus) || (r.splits > 1 && cols * (hd / 2) > 256) ? 8 : 4;
     return r;
 }
 
@@ -1256,6 +1285,6 @@ hipError_t launch_q4_attention(bool f16_rows, const Q4Attention& a, const Q4Cach
     const int hd = 32 * c.nb;
     p.scale_log2 = 1.4426950408889634f / sqrtf((float)hd);
     if (hipError_t e = f16_rows ? launch<f16>(p, plan, st) : launch<float>(p, plan, st)) return e;
-    if (plan.splits == 1 || plan.cols == 16) return hipSuccess;
+    if (plan.splits == 1 || plan.cols <= 32) return hipSuccess;
     return f16_rows ? launch_join<f16>(a, hd, plan.splits, st) : launch_join<float>(a, hd, plan.splits, st);
 }
