@@ -784,7 +784,7 @@ __global__ __launch_bounds__(64 * kMostWaves) void q4_attention_few_kernel(Split
 // A workgroup takes 64 CT query columns, 16 CT a wave; the tiles of keys and
 // values are unpacked once for all its waves, into LDS as the fragments that the
 // products read (16 bytes a lane in lane order, so no bank conflicts either
-// way).  NSET sets of four waves take consecutive ranges of the keys and join
+// way).  NSET (2 or 4) sets of four waves take consecutive ranges of the keys and join
 // through LDS at the end.  Two buffers a set: while the waves work on one, they
 // unpack the next tile's words, loaded a step earlier, into the other; one
 // barrier a step.
@@ -808,7 +808,7 @@ struct Wide {
 };
 
 template <int NB, int CT, int NSET, typename T>
-__global__ __launch_bounds__(256 * NSET) __attribute__((amdgpu_waves_per_eu(2, 2))) void q4_attention_wide_kernel(SplitArgs p) {
+__global__ __launch_bounds__(256 * NSET) __attribute__((amdgpu_waves_per_eu(NSET, NSET))) void q4_attention_wide_kernel(SplitArgs p) {
     typedef Wide<NB, CT, NSET, T> W;
     constexpr bool EXACT = W::EXACT;
     constexpr int TPS = W::TPS, HD = 32 * NB, STEP = TPS * kQ4Tile;
@@ -1143,6 +1143,9 @@ __global__ __launch_bounds__(256 * NSET) __attribute__((amdgpu_waves_per_eu(2, 2
     }
 }
 
+// Whether workgroups of 64 columns may have four sets of waves, as LDS and registers allow.
+constexpr bool four_sets(int nb, bool exact) { return nb <= 2 && !exact; }
+
 template <typename T>
 hipError_t launch_join(const Q4Attention& a, int hd, int splits, hipStream_t st) {
     const int64_t rows = (int64_t)a.tokens * a.heads;
@@ -1192,7 +1195,11 @@ hipError_t launch_nb(const SplitArgs& p, const Q4Plan& plan, hipStream_t st) {
     if constexpr (most >= 128)
         if (plan.cols == 128) return launch_wide<NB, 2, 2, T>(p, cols, st);
     if constexpr (most >= 64)
-        if (plan.cols == 64) return launch_wide<NB, 1, 2, T>(p, cols, st);
+        if (plan.cols == 64) {
+            if constexpr (four_sets(NB, sizeof(T) == 4))
+                if (plan.waves == 16) return launch_wide<NB, 1, 4, T>(p, cols, st);
+            return launch_wide<NB, 1, 2, T>(p, cols, st);
+        }
     if constexpr (NB <= 3 && sizeof(T) == 4)
         if (plan.cols == 32) return launch_waves<q4_attention_kernel<NB, 2, T>, NB, 32>(p, plan, cols, st);
     if (cols <= few_columns(NB)) return launch_waves<q4_attention_few_kernel<NB, T>, NB, 16>(p, plan, cols, st);
@@ -1218,9 +1225,11 @@ hipError_t launch(const SplitArgs& p, const Q4Plan& plan, hipStream_t st) {
 // How a call runs.  Columns of a workgroup: 16 or 32 (every wave key tiles of its own) up
 // to 64 columns, 64 or 128 from there in f16, where unpacking a tile once for all
 // of them pays (64 columns over 8,000 positions, 8 KV heads of 128: 17.2 us either
-// way; 300: 27 us with 64 a workgroup).  128 where workgroups of 128 fill the chip
-// (prompt of 2,048 tokens, 32/8 heads of 128, 63 us against 79; 512 tokens of it 17
-// against 13), at most head dimension 128 (registers).
+// way; 300: 27 us with 64 a workgroup).  128, at most head dimension 128 (registers),
+// where workgroups of 128 fill the chip and the longest does not outlast a CU's share of
+// the work by half (f16, 32/8 heads of 128, us with 128 and 64: 2,048 queries 54 and 79,
+// 1,500 35.7 and 47.1, 1,024 26.4 and 24.2, 1,024 at 1,000 45.1 and 50.2; 4,096 of 9/3
+// heads of 64 56.3 and 51.2).
 //
 // Splits, up to a workgroup a CU over all.  A workgroup alone costs about 4 us and
 // nb / 18 us a tile of its keys; joining costs 1.5 us in the same launch (4 with 16
@@ -1238,13 +1247,20 @@ Q4Plan q4_attention_plan(bool f16_rows, int tokens, int heads, int kv_heads, int
     auto groups = [&](int tile) { return (cols + tile - 1) / tile * kv_heads; };
     auto up = [](int64_t a, int64_t b) { return (int)((a + b - 1) / b); };
     const int wide = wide_columns(hd / 32, !f16_rows);
-    // (float32 from a full chip on: 1,024 queries of 32/8 heads of 128 55 us against 59, 2,048 108
-    // against 164, 256 13.4 against 11.3)
+    // (float32 from a full chip on: 1,024 queries of 32/8 heads of 128 37.5 us against 49 with 16
+    // columns, 2,048 105 against 143, 512 18.8 against 20.9)
     if (cols > 64 && wide > 16 && (f16_rows || groups(64) >= cus)) {
-        r.cols = wide == 128 && groups(128) >= cus ? 128 : 64;
+        // the longest workgroup of 128 against a CU's share of the work: the columns see `length`
+        // positions at most, half of their tokens fewer on average
+        const int64_t seen = length - tokens / 2;
+        const bool even = 2 * 128 * cus * (int64_t)length <= 3 * cols * kv_heads * seen;
+        r.cols = wide == 128 && groups(128) >= cus && even ? 128 : 64;
         const int most = (int)(cus / groups(r.cols));
-        // two sets of waves take 64 keys (32 past head dimension 128) a step each
+        // a set of waves takes 64 keys (32 past head dimension 128) a step
         r.splits = tiles <= 48 ? 1 : std::max(1, std::min(most, up(tiles, 8)));
+        // Four sets where each has many steps (32/32 heads of 64, f16: 512 queries at 3,584 33.3 us
+        // against 37.0, 300 at 1,000 15.0 against 14.9, at 300 10.0 against 8.5 of 9/3 heads).
+        r.waves = r.cols == 64 && four_sets(hd / 32, !f16_rows) && seen / kQ4Tile / r.splits >= 48 ? 16 : 8;
         return r;
     }
     r.cols = 16;

@@ -96,9 +96,8 @@ struct Q4Attention {
     int* counters = nullptr;
 };
 constexpr int kQ4Counters = 512;
-// How a call runs: query columns of a workgroup, its waves (16 columns only), and parts the keys
-// are split into.  `length`: the positions that the call may see; the splits do not fall as it
-// grows, and the rest does not depend on it but for the waves.
+// How a call runs: query columns of a workgroup, its waves, and parts the keys are split into.
+// `length`: the positions that the call may see.  A call's workspace does not shrink as it grows.
 struct Q4Plan {
     int cols = 16, waves = 4, splits = 1;
 };
