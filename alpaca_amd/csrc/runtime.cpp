@@ -419,24 +419,26 @@ static int half_copy(const OwnedMatrix& w, OwnedMatrix& h, hipStream_t st) {
 
 // RoPE (cos, sin) for positions [0, positions): frequencies and angles in
 // double, rounded once to float (CPUOps.rope, CPUOps.swift:196-201).
-static std::vector<float2> rope_table(int positions, int hd, float theta) {
+static void rope_rows(int first, int positions, int hd, float theta, float2* t) {
     const int half = hd / 2;
-    std::vector<float2> t((size_t)positions * half);
     std::vector<double> freq(half);
     for (int i = 0; i < half; i++) freq[i] = std::pow((double)theta, -2.0 * (double)i / (double)hd);
     for (int p = 0; p < positions; p++)
         for (int i = 0; i < half; i++) {
-            const double a = (double)p * freq[i];
+            const double a = (double)(first + p) * freq[i];
             t[(size_t)p * half + i] = make_float2((float)std::cos(a), (float)std::sin(a));
         }
+}
+static std::vector<float2> rope_table(int positions, int hd, float theta) {
+    std::vector<float2> t((size_t)positions * (hd / 2));
+    rope_rows(0, positions, hd, theta, t.data());
     return t;
 }
 
 extern "C" int ahip_rope_table(int positions, int hd, float theta, float* table) {
-    if (positions < 0 || hd <= 0 || hd % 2 || !(theta > 0) || (positions && !table))
+    if (positions < 0 || hd <= 0 || hd % 2 || hd > 1 << 16 || !(theta > 0) || (positions && !table))
         return fail(AHIP_ERR_INVALID_ARGUMENT, "rotation table");
-    const auto t = rope_table(positions, hd, theta);
-    std::memcpy(table, t.data(), t.size() * sizeof(float2));
+    rope_rows(0, positions, hd, theta, (float2*)table);
     return AHIP_OK;
 }
 
@@ -1226,7 +1228,8 @@ extern "C" int ahip_session_create(ahip_model* m, int capacity, int max_batch, i
     if (z.q4_work) {
         s->q4_work_bytes = z.q4_work / 2;
         if (int rc = s->q4_work.alloc(z.q4_work)) return rc;
-        HIP_OR(hipMemset(s->q4_work.p, 0, z.q4_work), "hipMemset");
+        HIP_OR(hipMemsetAsync(s->q4_work.p, 0, z.q4_work, s->stream), "hipMemset");
+        HIP_OR(hipStreamSynchronize(s->stream), "hipMemset");  // (the split prefill's other stream uses it too)
     }
     struct A { DevBuf* b; int64_t n; };
     for (A a : {A{&s->x, z.x * 4}, A{&s->xn, z.x * 4}, A{&s->xh, z.x * 4}, A{&s->qkv, z.qkv * 4}, A{&s->qh, z.q16 * 4},
@@ -2293,7 +2296,12 @@ static int op_attention_q4(ahip_context* ctx, const float* q, int tokens, int he
         const int64_t need = q4_attention_workspace(tokens, heads, hd, plan);
         if (int rc = work.alloc((size_t)need)) return rc;
         if (need) HIP_OR(hipMemsetAsync(work.p, 0, kQ4Counters * 4, st), "clear workspace");
-        std::vector<uint16_t> h(half ? qn : 0);
+        std::vector<uint16_t> h;
+        try {
+            h.resize(half ? qn : 0);
+        } catch (const std::bad_alloc&) {
+            return fail(AHIP_ERR_ALLOC, "out of host memory for f16 queries");
+        }
         for (size_t i = 0; i < h.size(); i++) h[i] = f32_to_f16_bits(q[i]);
         if (int rc = upload(dq, half ? (const void*)h.data() : q, qn * (half ? 2 : 4), st)) return rc;
         if (int rc = dout.alloc(qn * (half ? 2 : 4))) return rc;
@@ -2324,7 +2332,13 @@ extern "C" int ahip_op_qk_norm_rope(ahip_context* ctx, float* q, int heads, cons
     if (tokens > (1 << 28) || start > (1 << 28)) return fail(AHIP_ERR_INVALID_ARGUMENT, "implausibly large position");
     return with_ctx(ctx, [&](hipStream_t st) -> int {
         if (tokens == 0) return AHIP_OK;
-        auto table = rope_table(start + tokens, hd, theta);
+        std::vector<float2> table;
+        try {
+            table.resize((size_t)tokens * (hd / 2));
+        } catch (const std::bad_alloc&) {
+            return fail(AHIP_ERR_ALLOC, "out of host memory for the rotation table");
+        }
+        rope_rows(start, tokens, hd, theta, table.data());
         DevBuf dt, dq, dk, dgq, dgk;
         const size_t qb = (size_t)tokens * heads * hd * 4, kb = (size_t)tokens * kv_heads * hd * 4;
         if (int rc = upload(dt, table.data(), table.size() * sizeof(float2), st)) return rc;
@@ -2345,9 +2359,8 @@ extern "C" int ahip_op_qk_norm_rope(ahip_context* ctx, float* q, int heads, cons
         a.heads = heads;
         a.kv_heads = kv_heads;
         a.head_dim = hd;
-        a.rope_positions = start + tokens;
+        a.rope_positions = tokens;  // (the table starts at `start`)
         a.interleaved = interleaved;
-        a.start = start;
         a.eps = eps;
         if (int rc = ahip_qk_norm_rope(ctx, &a, nullptr)) return rc;
         if (int rc = download(q, dq, qb, st)) return rc;

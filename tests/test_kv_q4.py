@@ -167,6 +167,8 @@ def test_rotation_table_is_the_double_angle_rounded_once():
     np.testing.assert_allclose(t[..., 1], np.sin(a), rtol=0, atol=6.1e-8)
     with pytest.raises(L.InvalidArgument):
         rope_table(4, 64, 0.0)
+    for bad in ((-1, 64), (4, 0), (4, 63), (1, 1 << 20)):  # (refused before the table is written)
+        refused(L.lib().ahip_rope_table(*bad, 1e4, None if bad[0] < 0 else P), "rotation table")
     assert rope_table(0, 64, 1e4).shape == (0, 32, 2)
 
 
