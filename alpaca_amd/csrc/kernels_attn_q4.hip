@@ -85,7 +85,7 @@ struct SplitArgs {
     Q4Attention a;
     Q4Cache c;
     int G, splits;
-    Divisor by_group, by_heads, by_splits;
+    Divisor by_group, by_heads, by_splits, by_cus;
     float scale_log2;
 };
 
@@ -784,7 +784,7 @@ __global__ __launch_bounds__(64 * kMostWaves) void q4_attention_few_kernel(Split
 // A workgroup takes 64 CT query columns, 16 CT a wave; the tiles of keys and
 // values are unpacked once for all its waves, into LDS as the fragments that the
 // products read (16 bytes a lane in lane order, so no bank conflicts either
-// way).  NSET (2 or 4) sets of four waves take consecutive ranges of the keys and join
+// way).  NSET (1, 2 or 4) sets of four waves take consecutive ranges of the keys and join
 // through LDS at the end.  Two buffers a set: while the waves work on one, they
 // unpack the next tile's words, loaded a step earlier, into the other; one
 // barrier a step.
@@ -808,7 +808,7 @@ struct Wide {
 };
 
 template <int NB, int CT, int NSET, typename T>
-__global__ __launch_bounds__(256 * NSET) __attribute__((amdgpu_waves_per_eu(NSET, NSET))) void q4_attention_wide_kernel(SplitArgs p) {
+__global__ __launch_bounds__(256 * NSET) __attribute__((amdgpu_waves_per_eu(NSET == 4 ? 4 : 2, NSET == 4 ? 4 : 2))) void q4_attention_wide_kernel(SplitArgs p) {
     typedef Wide<NB, CT, NSET, T> W;
     constexpr bool EXACT = W::EXACT;
     constexpr int TPS = W::TPS, HD = 32 * NB, STEP = TPS * kQ4Tile;
@@ -819,8 +819,14 @@ __global__ __launch_bounds__(256 * NSET) __attribute__((amdgpu_waves_per_eu(NSET
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), set = wave / 4, wl = wave % 4;
     const int G = p.G, cols = p.a.tokens * G, groups = (cols + W::COLS - 1) / W::COLS;
     const Nibbles nib;
-    // the longest (last) columns first
-    const int id = p.by_heads(blockIdx.x), kvh = blockIdx.x - id * p.c.kv_heads;
+    // The longest (last) columns first.  One set: the chip holds two workgroups a CU and hands CU c
+    // the workgroups c and c + CUs first, so every other CUs' worth comes in reverse, short beside long.
+    int bx = blockIdx.x;
+    if constexpr (NSET == 1) {
+        const int cus = p.by_cus.d, from = p.by_cus(bx) * cus;
+        if (p.by_cus(bx) & 1) bx = from + min(cus, (int)gridDim.x - from) - 1 - (bx - from);
+    }
+    const int id = p.by_heads(bx), kvh = bx - id * p.c.kv_heads;
     const int sp = blockIdx.y, col0 = (groups - 1 - id) * W::COLS;
     const int start = p.a.start_dev ? *p.a.start_dev : p.a.start;
     const bool inside = start >= 0 && start <= p.c.capacity - p.a.tokens;
@@ -1143,7 +1149,9 @@ __global__ __launch_bounds__(256 * NSET) __attribute__((amdgpu_waves_per_eu(NSET
     }
 }
 
-// Whether workgroups of 64 columns may have four sets of waves, as LDS and registers allow.
+// Whether workgroups of the many-column kernel may have one set of waves, and of 64 columns four, as
+// LDS and registers allow.
+constexpr bool one_set(int nb) { return nb <= 6; }
 constexpr bool four_sets(int nb, bool exact) { return nb <= 2 && !exact; }
 
 template <typename T>
@@ -1193,9 +1201,12 @@ hipError_t launch_nb(const SplitArgs& p, const Q4Plan& plan, hipStream_t st) {
     const int64_t cols = (int64_t)p.a.tokens * p.G;
     constexpr int most = wide_columns(NB, sizeof(T) == 4);
     if constexpr (most >= 128)
-        if (plan.cols == 128) return launch_wide<NB, 2, 2, T>(p, cols, st);
+        if (plan.cols == 128)
+            return plan.waves == 4 ? launch_wide<NB, 2, 1, T>(p, cols, st) : launch_wide<NB, 2, 2, T>(p, cols, st);
     if constexpr (most >= 64)
         if (plan.cols == 64) {
+            if constexpr (one_set(NB) && most == 64)
+                if (plan.waves == 4) return launch_wide<NB, 1, 1, T>(p, cols, st);
             if constexpr (four_sets(NB, sizeof(T) == 4))
                 if (plan.waves == 16) return launch_wide<NB, 1, 4, T>(p, cols, st);
             return launch_wide<NB, 1, 2, T>(p, cols, st);
@@ -1260,7 +1271,13 @@ Q4Plan q4_attention_plan(bool f16_rows, int tokens, int heads, int kv_heads, int
         r.splits = tiles <= 48 ? 1 : std::max(1, std::min(most, up(tiles, 8)));
         // Four sets where each has many steps (32/32 heads of 64, f16: 512 queries at 3,584 33.3 us
         // against 37.0, 300 at 1,000 15.0 against 14.9, at 300 10.0 against 8.5 of 9/3 heads).
-        r.waves = r.cols == 64 && four_sets(hd / 32, !f16_rows) && seen / kQ4Tile / r.splits >= 48 ? 16 : 8;
+        // One set, two workgroups a CU, which do not wait for each other, where enough of the columns
+        // keep the last CU's second one at work (f16, 32/8 heads of 128, us with one and two sets: 8,192
+        // queries 604 and 655, 4,000 160 and 177, 2,400 74 and 80, 2,048 63 and 54, 2,048 at 3,000 158
+        // and 165; float32: 3,000 182 and 222; 4,000 of 16/8 heads of 256 259 and 242), at the greatest
+        // width (64 columns of small heads: 800 at 3,000, 32/32 heads of 64, 59.4 and 56.0).
+        if (one_set(hd / 32) && r.cols == wide && 8 * groups(r.cols) * seen >= 9 * cus * (int64_t)length) r.waves = 4;
+        else r.waves = r.cols == 64 && four_sets(hd / 32, !f16_rows) && seen / kQ4Tile / r.splits >= 48 ? 16 : 8;
         return r;
     }
     r.cols = 16;
@@ -1298,6 +1315,7 @@ hipError_t launch_q4_attention(bool f16_rows, const Q4Attention& a, const Q4Cach
     p.by_group = Divisor(p.G);
     p.by_heads = Divisor(c.kv_heads);
     p.by_splits = Divisor(plan.splits);
+    p.by_cus = Divisor(device_cus());
     const int hd = 32 * c.nb;
     p.scale_log2 = 1.4426950408889634f / sqrtf((float)hd);
     if (hipError_t e = f16_rows ? launch<f16>(p, plan, st) : launch<float>(p, plan, st)) return e;

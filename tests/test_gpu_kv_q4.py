@@ -327,6 +327,7 @@ def check_heads(got, q, kd, vd, start, dtype, heads, label):
     (64, 64, 160, 250, 3), (64, 64, 192, 197, 60), (70, 70, 128, 129, 0), (64, 64, 256, 250, 0), (96, 32, 64, 350, 31),
     (300, 300, 64, 128, 21), (256, 256, 96, 150, 33), (400, 200, 32, 90, 5),  # and 32 of float32
     (130, 130, 64, 70, 1600),  # four sets of waves in f16
+    (200, 200, 128, 250, 700), (180, 180, 160, 130, 300), (340, 340, 64, 129, 200),  # and one
     (600, 600, 32, 1, 2100), (16, 1, 32, 1, 5000), (8, 1, 128, 1, 5000)])
 def test_attention_of_many_heads(hip_ctx, heads, kv_heads, hd, tokens, start, dtype):
     """Calls that fill the chip, at every width of a workgroup; many KV heads and long caches for few queries."""
