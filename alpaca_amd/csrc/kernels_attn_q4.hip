@@ -120,13 +120,11 @@ struct Tile {
 
 // ------------------------------------------------------------------ joining the splits
 // A split leaves (maximum, sum, unnormalised output) of its columns in the
-// workspace.  Up to 16 columns a workgroup: the last workgroup of a group of columns
-// to arrive joins them in the same launch, 3 us of GPU time and as much on the host
-// less than a second one.  Its partial results are
-// written and read with agent-scope accesses, which the L2 caches of all XCDs see;
-// each thread waits for its own to be acknowledged before the count, and the last
-// sets the counter back to zero for the next call.  More columns: a second kernel,
-// which has the whole chip for them.
+// workspace, and the last workgroup of a group of columns to arrive joins them in the
+// same launch, 3 us of GPU time and as much on the host less than a second one.  The
+// partial results are written and read with agent-scope accesses, which the L2 caches
+// of all XCDs see; each thread waits for its own to be acknowledged before the count,
+// and the last sets the counter back to zero for the next call.
 struct Joined {
     float m = -INFINITY, l = 0.f, a = 0.f, b = 0.f;
 };
@@ -140,21 +138,18 @@ __device__ __forceinline__ void join_add(Joined& j, float m, float l, float a, f
     j.a = j.a * f + a * w;
     j.b = j.b * f + b * w;
 }
-// Two floats past the caches of an XCD.
+// Two floats past the caches of an XCD, and back.
 __device__ __forceinline__ void put2(float* p, float a, float b) {
     const uint64_t u = (uint64_t)__float_as_uint(b) << 32 | __float_as_uint(a);
     __hip_atomic_store(gptr((uint64_t*)p), u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
-// And back (SHARED), or from an earlier launch.
-template <bool SHARED>
 __device__ __forceinline__ float2 get2(const float* p) {
-    if constexpr (!SHARED) return *(const float2*)p;
     const uint64_t u = __hip_atomic_load(gptr((const uint64_t*)p), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     return make_float2(__uint_as_float((uint32_t)u), __uint_as_float((uint32_t)(u >> 32)));
 }
 // Splits first, first + step, ... < splits of the row at pp, for dims d and d + 1;
 // J of them in a round trip to memory.
-template <int J, bool SHARED>
+template <int J>
 __device__ __forceinline__ Joined join(const float* pp, int hd, int d, int first, int step, int splits) {
     Joined j;
     for (int s0 = first; s0 < splits; s0 += J * step) {
@@ -162,8 +157,8 @@ __device__ __forceinline__ Joined join(const float* pp, int hd, int d, int first
 #pragma unroll
         for (int i = 0; i < J; i++) {  // (past the last: that one again, unused)
             const float* x = pp + (int64_t)min(s0 + i * step, splits - 1) * (hd + 2);
-            ml[i] = get2<SHARED>(x);
-            o[i] = get2<SHARED>(x + 2 + d);
+            ml[i] = get2(x);
+            o[i] = get2(x + 2 + d);
         }
         float top = j.m;
 #pragma unroll
@@ -187,11 +182,11 @@ __device__ __forceinline__ Joined join(const float* pp, int hd, int d, int first
 }
 // Groups of threads with every groups-th split each, met in LDS (a float4 a thread):
 // item i of `items` in thread i of each group; the result is group 0's.
-template <int J, bool SHARED>
+template <int J>
 __device__ __forceinline__ Joined join_groups(const float* pp, int hd, int d, int group, int groups, int items, int i,
                                               int splits, float4* js) {
     Joined j;
-    if (group < groups) j = join<J, SHARED>(pp, hd, d, group, groups, splits);
+    if (group < groups) j = join<J>(pp, hd, d, group, groups, splits);
     js[threadIdx.x] = make_float4(j.m, j.l, j.a, j.b);
     __syncthreads();
     if (group == 0)
@@ -235,51 +230,25 @@ __device__ __forceinline__ void count_and_join(const SplitArgs& p, int kvh, int 
     if (2 * items > (int)blockDim.x) {
         for (int i = threadIdx.x; i < items; i += blockDim.x) {
             const int col = col0 + i / (HD / 2), d = 2 * (i % (HD / 2));
-            put(col, d, join<8, true>(partial<HD>(p, kvh, col), HD, d, 0, 1, p.splits));
+            put(col, d, join<8>(partial<HD>(p, kvh, col), HD, d, 0, 1, p.splits));
         }
         return;
     }
     const int groups = blockDim.x / items, group = threadIdx.x / items, i = threadIdx.x - group * items;
     const int col = col0 + i / (HD / 2), d = 2 * (i % (HD / 2));
-    const Joined j = join_groups<8, true>(partial<HD>(p, kvh, col), HD, d, group, groups, items, i, p.splits, (float4*)lds);
+    const Joined j = join_groups<8>(partial<HD>(p, kvh, col), HD, d, group, groups, items, i, p.splits, (float4*)lds);
     if (group == 0) put(col, d, j);
-}
-
-// The joining kernel: GROUPED, a workgroup a query and head; else two dims a thread.
-template <bool GROUPED, int J, typename T>
-__global__ __launch_bounds__(256) void q4_join_kernel(const float* partials, int64_t rows, int heads, int hd,
-                                                      int splits, T* out, int64_t stride) {
-    __shared__ float4 js[GROUPED ? 256 : 1];
-    const int half = hd / 2;
-    int64_t th;
-    int d;
-    Joined j;
-    if constexpr (GROUPED) {
-        th = blockIdx.x;
-        const int group = threadIdx.x / half, i = threadIdx.x - group * half;
-        d = 2 * i;
-        j = join_groups<J, false>(partials + th * splits * (hd + 2), hd, d, group, 256 / half, half, i, splits, js);
-        if (group) return;
-    } else {
-        const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-        th = i / half;
-        if (th >= rows) return;
-        d = 2 * (int)(i - th * half);
-        j = join<J, false>(partials + th * splits * (hd + 2), hd, d, 0, 1, splits);
-    }
-    const int64_t t = th / heads, h = th - t * heads;
-    T* p = out + t * stride + h * hd + d;
-    p[0] = (T)(j.a / j.l);
-    p[1] = (T)(j.b / j.l);
 }
 
 // T float: the scores and outputs to float32 accuracy (the queries and
 // probabilities as two f16 terms, the quants exact and the values exact in two
-// terms).  T f16: queries exact, probabilities and values one f16 term.
+// terms).  T f16: queries and keys exact, probabilities and values one f16 term.
+//
 // A column's queries as the lane takes them, at q its dims 8 g of block 0: block b,
 // dims 8 g + {0, 4, 1, 5, 2, 6, 3, 7} as the keys' nibbles come.  float: scaled into
-// [-1, 1] by a power of two, so that two f16 terms hold any float32 range.  Returns what
-// the products are to be scaled by for scores in base 2.
+// [-1, 1] by a power of two (`over` of the largest among the lane's rows), so that two f16
+// terms hold any float32 range.  Returns what the products are to be scaled by for scores in
+// base 2.
 struct Same {
     __device__ __forceinline__ float operator()(float x) const { return x; }
 };
@@ -789,18 +758,21 @@ __global__ __launch_bounds__(64 * kMostWaves) void q4_attention_few_kernel(Split
 // unpack the next tile's words, loaded a step earlier, into the other; one
 // barrier a step.
 //
-// T f16: the keys' and values' fragments hold d (n - 8) rounded to f16, as an f16
-// cache holds them, and the products run through without another instruction.
-// T float: the keys' fragments hold n - 8 and the products are scaled block by
-// block; the values have a second fragment with what the first one's rounding left.
+// The keys' fragments hold n - 8 and the products are scaled block by block, which keeps
+// the keys exact; rounded to f16 in the fragments, d (n - 8) costs no vector instruction
+// a score and is a fifth faster (2,048 f16 queries, 32/8 heads of 128: 54 us against 67),
+// but doubles the error of the f16 outputs (4e-4 of the norm against 2.8e-4, of which
+// the output's own rounding is 2e-4; queries of 3 times the keys' size).  The values'
+// fragments hold d (n - 8), T f16 rounded to f16, T float with a second fragment of
+// what the first one's rounding left.
 template <int NB, int CT, int NSET, typename T>
 struct Wide {
     static constexpr bool EXACT = sizeof(T) == 4;
     static constexpr int TPS = NB <= 4 && !EXACT ? 2 : 1;    // tiles a step
     static constexpr int KF = 2 * NB * TPS;                  // fragments of keys in a buffer,
     static constexpr int VT = EXACT ? 2 : 1;                 // and of values, in VT terms
-    static constexpr int SCALES = (KF + KF * VT) * 1024;     // EXACT: the keys' scales, a tile's as in the cache
-    static constexpr int BUF = SCALES + (EXACT ? TPS * 64 * NB : 0);
+    static constexpr int SCALES = (KF + KF * VT) * 1024;     // the keys' scales, a tile's as in the cache
+    static constexpr int BUF = SCALES + TPS * 64 * NB;
     static constexpr int COLS = 64 * CT;
     static constexpr int JOIN = COLS * (32 * NB + 4) * 4 + COLS * 8;  // a set's outputs and statistics
     static constexpr int LDS = 2 * NSET * BUF > JOIN ? 2 * NSET * BUF : JOIN;
@@ -827,7 +799,7 @@ __global__ __launch_bounds__(256 * NSET) __attribute__((amdgpu_waves_per_eu(NSET
         if (p.by_cus(bx) & 1) bx = from + min(cus, (int)gridDim.x - from) - 1 - (bx - from);
     }
     const int id = p.by_heads(bx), kvh = bx - id * p.c.kv_heads;
-    const int sp = blockIdx.y, col0 = (groups - 1 - id) * W::COLS;
+    const int col0 = (groups - 1 - id) * W::COLS;
     const int start = p.a.start_dev ? *p.a.start_dev : p.a.start;
     const bool inside = start >= 0 && start <= p.c.capacity - p.a.tokens;
     const int wcol0 = col0 + wl * 16 * CT;  // the wave's columns
@@ -836,9 +808,8 @@ __global__ __launch_bounds__(256 * NSET) __attribute__((amdgpu_waves_per_eu(NSET
     const int w_last = start + p.by_group(min(wcol0 + 16 * CT - 1, cols - 1));
     const int tiles = inside ? last_seen / kQ4Tile + 1 : 0;
     const int all = (tiles + TPS - 1) / TPS;  // steps over all the keys
-    const int s0 = share(all, sp, p.by_splits), s1 = share(all, sp + 1, p.by_splits);
-    const int per = (s1 - s0 + NSET - 1) / NSET, f0 = s0 + set * per;  // this set's steps: [f0, f0 + count)
-    const int count = max(0, min(s1 - f0, per));
+    const int per = (all + NSET - 1) / NSET, f0 = set * per;  // this set's steps: [f0, f0 + count)
+    const int count = max(0, min(all - f0, per));
 
     f16x8 q[CT][NB], ql[CT][EXACT ? NB : 1];
     int seen[CT];
@@ -905,16 +876,11 @@ __global__ __launch_bounds__(256 * NSET) __attribute__((amdgpu_waves_per_eu(NSET
 #pragma unroll
             for (int s = 0; s < 2; s++) {
                 const uint32_t w = rk[k][s], w8 = w >> 8;
-                f16x2 n[4] = {nib.lo(w), nib.hi(w), nib.lo(w8), nib.hi(w8)};
-                if constexpr (!EXACT) {
-                    const f16x2 d = pair(rk[k][2 + s] * 0x10001u);
-#pragma unroll
-                    for (int i = 0; i < 4; i++) n[i] *= d;
-                } else if (g == 0) {
+                if (g == 0)
                     *(uint16_t*)(buf + W::SCALES + (((tt * 2 + s) * 4 + (c16 >> 2)) * NB + b) * 8 + (c16 & 3) * 2) =
                         (uint16_t)rk[k][2 + s];
-                }
-                *(f16x8*)(buf + ((tt * 2 + s) * NB + b) * 1024 + lane * 16) = frag(n[0], n[1], n[2], n[3]);
+                *(f16x8*)(buf + ((tt * 2 + s) * NB + b) * 1024 + lane * 16) =
+                    frag(nib.lo(w), nib.hi(w), nib.lo(w8), nib.hi(w8));
             }
             const int key0 = (step * TPS + tt) * kQ4Tile;
             if (key0 + kQ4Tile - 1 > last_seen) {
@@ -951,30 +917,34 @@ __global__ __launch_bounds__(256 * NSET) __attribute__((amdgpu_waves_per_eu(NSET
             for (int b = 0; b < NB; b++) fr[group & 1][b] = *(const f16x8*)(buf + (group * NB + b) * 1024 + lane * 16);
         };
         read(0);
+        // a group's products are scaled while the next group's run, where registers allow
+        constexpr int LAG = NB <= 3 && !EXACT ? 1 : 0;
+        f32x4 part[2][CT][NB];
+        uint2 d[2][NB];
+        auto scale = [&](int u) {
+#pragma unroll
+            for (int ct = 0; ct < CT; ct++) {
+                sa[ct][u] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int b = 0; b < NB; b++) add_scaled(sa[ct][u], part[u & 1][ct][b], d[u & 1][b]);
+            }
+        };
 #pragma unroll
         for (int u = 0; u < 2 * TPS; u++) {
             read(u + 1);  // (after the last keys: the first values)
-            uint2 d[EXACT ? NB : 1];
-            if constexpr (EXACT) {
 #pragma unroll
-                for (int b = 0; b < NB; b++) d[b] = *(const uint2*)(buf + W::SCALES + ((u * 4 + g) * NB + b) * 8);
-            }
-#pragma unroll
-            for (int ct = 0; ct < CT; ct++) sa[ct][u] = f32x4{0.f, 0.f, 0.f, 0.f};
+            for (int b = 0; b < NB; b++) d[u & 1][b] = *(const uint2*)(buf + W::SCALES + ((u * 4 + g) * NB + b) * 8);
 #pragma unroll
             for (int b = 0; b < NB; b++)
 #pragma unroll
                 for (int ct = 0; ct < CT; ct++) {
-                    if constexpr (EXACT) {
-                        f32x4 part = mfma(fr[u & 1][b], q[ct][b], f32x4{0.f, 0.f, 0.f, 0.f});
-                        part = mfma(fr[u & 1][b], ql[ct][b], part);
-                        add_scaled(sa[ct][u], part, d[b]);
-                    } else {
-                        sa[ct][u] = mfma(fr[u & 1][b], q[ct][b], sa[ct][u]);
-                    }
+                    part[u & 1][ct][b] = mfma(fr[u & 1][b], q[ct][b], f32x4{0.f, 0.f, 0.f, 0.f});
+                    if constexpr (EXACT) part[u & 1][ct][b] = mfma(fr[u & 1][b], ql[ct][b], part[u & 1][ct][b]);
                 }
+            if (u >= LAG) scale(u - LAG);
             __builtin_amdgcn_sched_barrier(0);
         }
+        if (LAG) scale(2 * TPS - 1);
         if (key0 + STEP - 1 > w_first) {
 #pragma unroll
             for (int ct = 0; ct < CT; ct++)
@@ -1043,7 +1013,7 @@ __global__ __launch_bounds__(256 * NSET) __attribute__((amdgpu_waves_per_eu(NSET
         }
     };
 
-    if (tiles > 0 && s1 > s0) {  // (the same for the whole workgroup)
+    if (tiles > 0) {  // (the same for the whole workgroup)
         const int lastf = all - 1;
         fetch(min(f0, lastf));
         unpack(min(f0, lastf), buf0);
@@ -1118,19 +1088,6 @@ __global__ __launch_bounds__(256 * NSET) __attribute__((amdgpu_waves_per_eu(NSET
             }
         }
     }
-    if (p.splits > 1) {
-        // through LDS, so that the rows of partial results leave whole
-        if (NSET > 1) __syncthreads();  // (the last set's results are read)
-        if (set == 0) put_set();
-        __syncthreads();
-        const int n = min(W::COLS, cols - col0);
-        for (int i = threadIdx.x; i < n * (HD / 2 + 1); i += 256 * NSET) {
-            const int c = i / (HD / 2 + 1), d = 2 * (i - c * (HD / 2 + 1));
-            const float2 v = *(const float2*)(d ? xo + c * (HD + 4) + d - 2 : xml + 2 * c);
-            *(float2*)(partial<HD>(p, kvh, col0 + c) + sp * (HD + 2) + d) = v;
-        }
-        return;
-    }
     if (set) return;
 #pragma unroll
     for (int ct = 0; ct < CT; ct++) {
@@ -1154,20 +1111,6 @@ __global__ __launch_bounds__(256 * NSET) __attribute__((amdgpu_waves_per_eu(NSET
 constexpr bool one_set(int nb) { return nb <= 6; }
 constexpr bool four_sets(int nb, bool exact) { return nb <= 2 && !exact; }
 
-template <typename T>
-hipError_t launch_join(const Q4Attention& a, int hd, int splits, hipStream_t st) {
-    const int64_t rows = (int64_t)a.tokens * a.heads;
-    const unsigned flat = (unsigned)((rows * (hd / 2) + 255) / 256);
-    auto go = [&](auto kernel, unsigned grid) {
-        kernel<<<grid, 256, 0, st>>>(a.partials, rows, a.heads, hd, splits, (T*)a.out, a.out_stride);
-    };
-    if (splits <= 2) go(q4_join_kernel<false, 2, T>, flat);
-    else if (splits <= 4) go(q4_join_kernel<false, 4, T>, flat);
-    else if (splits <= 8) go(q4_join_kernel<false, 8, T>, flat);
-    else go(q4_join_kernel<true, 8, T>, (unsigned)rows);
-    return hipGetLastError();
-}
-
 template <int NB, int CT, int NSET, typename T>
 hipError_t launch_wide(const SplitArgs& p, int64_t cols, hipStream_t st) {
     typedef Wide<NB, CT, NSET, T> W;
@@ -1175,7 +1118,7 @@ hipError_t launch_wide(const SplitArgs& p, int64_t cols, hipStream_t st) {
     auto* kernel = q4_attention_wide_kernel<NB, CT, NSET, T>;
     static OncePerDevice once;
     if (hipError_t e = allow_whole_lds(once, (const void*)kernel)) return e;
-    const dim3 grid((unsigned)((cols + W::COLS - 1) / W::COLS * p.c.kv_heads), p.splits);
+    const dim3 grid((unsigned)((cols + W::COLS - 1) / W::COLS * p.c.kv_heads));
     kernel<<<grid, 256 * NSET, W::LDS, st>>>(p);
     return hipGetLastError();
 }
@@ -1233,65 +1176,60 @@ hipError_t launch(const SplitArgs& p, const Q4Plan& plan, hipStream_t st) {
 
 }  // namespace
 
-// How a call runs.  Columns of a workgroup: 16 or 32 (every wave key tiles of its own) up
-// to 64 columns, 64 or 128 from there in f16, where unpacking a tile once for all
-// of them pays (64 columns over 8,000 positions, 8 KV heads of 128: 17.2 us either
-// way; 300: 27 us with 64 a workgroup).  128, at most head dimension 128 (registers),
-// where workgroups of 128 fill the chip and the longest does not outlast a CU's share of
-// the work by half (f16, 32/8 heads of 128, us with 128 and 64: 2,048 queries 54 and 79,
-// 1,500 35.7 and 47.1, 1,024 26.4 and 24.2, 1,024 at 1,000 45.1 and 50.2; 4,096 of 9/3
-// heads of 64 56.3 and 51.2).
+// How a call runs.  Columns of a workgroup: 16 or 32 (every wave key tiles of its own)
+// until workgroups of 64 fill the chip (half of it, f16 heads of 96 and 128), 64 or 128
+// from there, where unpacking a tile once for all of them pays, us with 64 or 128 and 16:
+// f16, 32/32 heads of 64, 512 queries at 3,584 37.9 and 49.7, 300 at 1,000 16.7 and 15.9;
+// 32/8 heads of 128, 512 queries 13.5 and 18.4, 300 10.7 and 12.5, 100 7.0 and 6.0; 16/8
+// heads of 192, 400 queries 16.1 and 13.3; float32, 32/8 heads of 128, 2,048 queries 105
+// and 143, 1,024 37.5 and 49, 512 18.8 and 20.9.
 //
 // Splits, up to a workgroup a CU over all.  A workgroup alone costs about 4 us and
-// nb / 18 us a tile of its keys; joining costs 1.5 us in the same launch (4 with 16
-// full columns), 7 as one of its own.  In the same launch a split has a tile a wave
-// until there are 16 splits (32/8 heads of 128, one token at 4,000: 32.8 us in one,
-// 13.8 in 4, 9.7 in 16, 12.1 in 32; 37 at 1,021, 15/5 heads of 64: 8.5 in one, 8.0
-// in 7), then 32 tiles, which hide the waits of 32 splits and more, or 16 of more than
-// 4 blocks (4/2 heads of 256, 30,000 positions: 15.4 us in 64, 17.5 in 32).  Two or
-// three splits pay over long caches only (64 queries of 32/8 heads of 128 at 1,000:
-// 13.9 in two, 13.5 in one; 37 of 15/5 heads of 64 at 8,000: 22.6 and 34.6).
+// nb / 18 us a tile of its keys; joining costs 1.5 us (4 with 16 full columns).  A split
+// has a tile a wave until there are 16 splits (32/8 heads of 128, one token at 4,000:
+// 32.8 us in one, 13.8 in 4, 9.7 in 16, 12.1 in 32; 37 at 1,021, 15/5 heads of 64: 8.5 in
+// one, 8.0 in 7), then 32 tiles, which hide the waits of 32 splits and more, or 16 of
+// more than 4 blocks (4/2 heads of 256, 30,000 positions: 15.4 us in 64, 17.5 in 32).
+// Two or three splits pay over long caches only (64 queries of 32/8 heads of 128 at
+// 1,000: 13.9 in two, 13.5 in one; 37 of 15/5 heads of 64 at 8,000: 22.6 and 34.6).
 Q4Plan q4_attention_plan(bool f16_rows, int tokens, int heads, int kv_heads, int hd, int length) {
     Q4Plan r;
     const int64_t cols = (int64_t)tokens * (heads / kv_heads);
-    const int cus = device_cus(), tiles = q4_tiles(length), work = tiles * (hd / 32);
+    const int cus = device_cus(), nb = hd / 32, tiles = q4_tiles(length), work = tiles * nb;
     auto groups = [&](int tile) { return (cols + tile - 1) / tile * kv_heads; };
     auto up = [](int64_t a, int64_t b) { return (int)((a + b - 1) / b); };
-    const int wide = wide_columns(hd / 32, !f16_rows);
-    // (float32 from a full chip on: 1,024 queries of 32/8 heads of 128 37.5 us against 49 with 16
-    // columns, 2,048 105 against 143, 512 18.8 against 20.9)
-    if (cols > 64 && wide > 16 && (f16_rows || groups(64) >= cus)) {
-        // the longest workgroup of 128 against a CU's share of the work: the columns see `length`
-        // positions at most, half of their tokens fewer on average
+    const int wide = wide_columns(nb, !f16_rows);
+    if (cols > 64 && wide > 16 && groups(64) >= (f16_rows && (nb == 3 || nb == 4) ? cus / 2 : cus)) {
+        // 128 columns where workgroups of 128 fill the chip and the longest does not outlast a CU's
+        // share of the work by half (the columns see `length` positions at most, half of their tokens
+        // fewer on average): f16, 32/8 heads of 128, us with 128 and 64: 2,048 queries 67 and 87, 1,500
+        // 44.7 and 56.0, 1,024 at 1,000 57 and 61, 1,024 32.6 and 27.9; 4,096 of 9/3 heads of 64 66.6
+        // and 55.7.
         const int64_t seen = length - tokens / 2;
         const bool even = 2 * 128 * cus * (int64_t)length <= 3 * cols * kv_heads * seen;
         r.cols = wide == 128 && groups(128) >= cus && even ? 128 : 64;
-        const int most = (int)(cus / groups(r.cols));
-        // a set of waves takes 64 keys (32 past head dimension 128) a step
-        r.splits = tiles <= 48 ? 1 : std::max(1, std::min(most, up(tiles, 8)));
-        // Four sets where each has many steps (32/32 heads of 64, f16: 512 queries at 3,584 33.3 us
-        // against 37.0, 300 at 1,000 15.0 against 14.9, at 300 10.0 against 8.5 of 9/3 heads).
-        // One set, two workgroups a CU, which do not wait for each other, where enough of the columns
-        // keep the last CU's second one at work (f16, 32/8 heads of 128, us with one and two sets: 8,192
-        // queries 604 and 655, 4,000 160 and 177, 2,400 74 and 80, 2,048 63 and 54, 2,048 at 3,000 158
-        // and 165; float32: 3,000 182 and 222; 4,000 of 16/8 heads of 256 259 and 242), at the greatest
-        // width (64 columns of small heads: 800 at 3,000, 32/32 heads of 64, 59.4 and 56.0).
-        if (one_set(hd / 32) && r.cols == wide && 8 * groups(r.cols) * seen >= 9 * cus * (int64_t)length) r.waves = 4;
-        else r.waves = r.cols == 64 && four_sets(hd / 32, !f16_rows) && seen / kQ4Tile / r.splits >= 48 ? 16 : 8;
+        // One set of waves, two workgroups a CU, which do not wait for each other, at the greatest
+        // width where enough of the columns keep the last CU's second one at work (f16, 32/8 heads of
+        // 128, us with one and two sets: 8,192 queries 691 and 842, 4,000 189 and 225, 2,400 84 and 100,
+        // 2,048 71 and 67; float32: 3,000 182 and 222).  Four sets of 64 columns where each has many
+        // steps (32/32 heads of 64: 512 queries at 3,584 37.9 us against 45.6; 300 at 300 of 9/3 heads
+        // 10.8 against 9.9).
+        if (one_set(nb) && r.cols == wide && 8 * groups(r.cols) * seen >= 9 * cus * (int64_t)length) r.waves = 4;
+        else r.waves = r.cols == 64 && four_sets(nb, !f16_rows) && seen / kQ4Tile >= 48 ? 16 : 8;
         return r;
     }
-    r.cols = 16;
     // 32 a workgroup, its waves unpacking a tile for both halves, where they are four times the CUs:
     // 4,000 float32 queries of 15/5 heads of 64 108 us against 122, 2,048 40.1 against 41.1, 777 14.7
     // against 12.4; at most 3 blocks a head (registers).
-    if (!f16_rows && hd <= 96 && groups(32) >= 4 * cus) r.cols = 32;
+    r.cols = !f16_rows && nb <= 3 && groups(32) >= 4 * cus ? 32 : 16;
     const int most = groups(r.cols) <= kQ4Counters ? std::max(1, (int)(cus / groups(r.cols))) : 1;
-    r.splits = work <= 40 ? 1 : std::min(most, std::max(std::min(16, up(tiles, 4)), up(tiles, hd > 128 ? 16 : 32)));
+    r.splits = work <= 40 ? 1 : std::min(most, std::max(std::min(16, up(tiles, 4)), up(tiles, nb > 4 ? 16 : 32)));
     if (r.splits < 4 && work <= 200) r.splits = 1;
     // Eight waves where each still has many tiles (131,072 positions in 32 splits: 42.0 us against
     // 44.2 with four; 4,000 in 16: 10.2 against 9.7) and the chip is not full without them (512
     // float32 queries, 32/8 heads of 128: 31.9 against 23.1), or for the threads that join.
-    r.waves = (up(tiles, r.splits) >= 16 && groups(r.cols) * r.splits <= cus) || (r.splits > 1 && cols * (hd / 2) > 256) ? 8 : 4;
+    const int64_t here = groups(r.cols) * r.splits;
+    r.waves = (up(tiles, r.splits) >= 16 && here <= cus) || (r.splits > 1 && cols * (hd / 2) > 256) ? 8 : 4;
     return r;
 }
 
@@ -1316,9 +1254,6 @@ hipError_t launch_q4_attention(bool f16_rows, const Q4Attention& a, const Q4Cach
     p.by_heads = Divisor(c.kv_heads);
     p.by_splits = Divisor(plan.splits);
     p.by_cus = Divisor(device_cus());
-    const int hd = 32 * c.nb;
-    p.scale_log2 = 1.4426950408889634f / sqrtf((float)hd);
-    if (hipError_t e = f16_rows ? launch<f16>(p, plan, st) : launch<float>(p, plan, st)) return e;
-    if (plan.splits == 1 || plan.cols <= 32) return hipSuccess;
-    return f16_rows ? launch_join<f16>(a, hd, plan.splits, st) : launch_join<float>(a, hd, plan.splits, st);
+    p.scale_log2 = 1.4426950408889634f / sqrtf(32.f * c.nb);
+    return f16_rows ? launch<f16>(p, plan, st) : launch<float>(p, plan, st);
 }

@@ -405,8 +405,9 @@ int ahip_kv_q4_load(ahip_context* ctx, const ahip_kv_q4* cache, int dtype, int s
  * positions start.. over the cache, which already holds their keys and values.
  * q and out rows [heads][head_dim]; out may not overlap q.  With AHIP_F32 the
  * scores, probabilities and sums keep float32 accuracy over the cache's exact
- * values; with AHIP_F16 keys, values and probabilities enter the products rounded
- * to f16 (keys and values exactly in calls of few queries), and sums are float32.
+ * values; with AHIP_F16 keys enter the products exactly, values and probabilities
+ * rounded to f16 (in calls of few queries their products with the values' scales),
+ * and sums are float32.
  * `workspace` (16-byte aligned) holds the partial results of the key ranges and the counters of their arrival: ahip_attention_q4_workspace
  * bytes for the same arguments (on_device: whether start_dev is set).  Its first
  * AHIP_Q4_WORKSPACE_ZERO bytes are zero before its first call, and every call

@@ -78,9 +78,8 @@ def attention(q, k, v, start, dtype):
     of magnitudes; the probability as much as its score, and the exponential's 2^-22; numerator and denominator
     both.  The probabilities enter the products as two f16 terms of p * 2^14, p against the largest of the row: past
     the terms' 2^-22 they are off by half of f16's smallest step, 2^-25 * 2^-14, each.  The sums over the keys lose
-    a half step of the sum of magnitudes for every key.  In f16 the key (d (n - 8) has up to 15 bits), the probability
-    and the value each lose half an f16 step, the key of its score's magnitudes and so of numerator and denominator,
-    and so does the output."""
+    a half step of the sum of magnitudes for every key.  In f16 the keys are exact; the probability (of numerator and
+    denominator) and the value each lose half an f16 step, and so does the output."""
     T, H, hd = q.shape
     G = H // k.shape[1]
     out, bound = np.empty(q.shape), np.empty(q.shape)
@@ -96,7 +95,7 @@ def attention(q, k, v, start, dtype):
             rel = 2 * ((hd + 16) * EPS32 * size + 2.0 ** -22) + (n + 64) * EPS32
             small = n * 2.0 ** -39 * np.abs(vh[:n]).max()
             if dtype == "f16":
-                rel, small = rel + 2 * EPS16 * size + 3 * EPS16, small + EPS16 * np.abs(out[t, h]) + 2.0 ** -24
+                rel, small = rel + 3 * EPS16, small + EPS16 * np.abs(out[t, h]) + 2.0 ** -24
             bound[t, h] = rel * (p @ np.abs(vh[:n])) + small
     return out, bound
 
