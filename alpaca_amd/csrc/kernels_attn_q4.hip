@@ -1027,10 +1027,10 @@ __global__ __launch_bounds__(256 * NSET) __attribute__((amdgpu_waves_per_eu(NSET
         auto now = [&](int j) {
             if (j < count) work(f0 + j, buf0 + (j & 1) * W::BUF);
         };
-        // One set unpacks while the other, on the same SIMDs, is at its products, where a step is a
-        // tile (1,024 f16 queries, 8/8 heads of 256: 34.5 us against 36.9; 2,048 of float32, 32/8 heads
-        // of 128: 105 against 107); with two tiles a step it costs (2,048 of f16: 56.6 against 54.2).
-        if (W::TPS == 1 && (set & 1)) {
+        // Of two sets one unpacks while the other, on the same SIMDs, is at its products (2,048 float32
+        // queries, 32/8 heads of 128: 103.6 us against 107.0, of f16 64.9 against 65.5; 4,000 of f16, 16/8
+        // heads of 256: 288 against 298); of four sets it costs (37.4 against 38.9 so).
+        if (NSET == 2 && set) {
             for (int j = 0; j < per; j++) {
                 now(j);
                 next(j);
