@@ -538,7 +538,7 @@ __global__ __launch_bounds__(64 * kMostWaves) void q4_attention_kernel(SplitArgs
 // its own block's only, and a sum over the columns CP apart gives the score.  The
 // values' scales go into the probabilities the same way (a column has one block's), so
 // that values enter as n - 8, exactly, and of the products with each block's values a
-// lane keeps its own block's.  Bound by the vector instructions, two thirds of them the
+// lane keeps its own block's.  Bound by the vector instructions, over half of them the
 // unpacking, close to memory: 131,072 positions, 32/8 heads of 128, 35.7 us in float32
 // (4.2 TB/s) and 31.0 in f16, against 41.9 and 35 with a column a query; 8,000 positions,
 // 9/3 heads of 64, 8.2 us against 10.3.  Three tiles ahead instead of two: 37.2 us.
@@ -1186,9 +1186,9 @@ hipError_t launch(const SplitArgs& p, const Q4Plan& plan, hipStream_t st) {
 //
 // Splits, up to a workgroup a CU over all.  A workgroup alone costs about 4 us and
 // nb / 18 us a tile of its keys; joining costs 1.5 us (4 with 16 full columns).  A split
-// has a tile a wave until there are 16 splits (32/8 heads of 128, one token at 4,000:
-// 32.8 us in one, 13.8 in 4, 9.7 in 16, 12.1 in 32; 37 at 1,021, 15/5 heads of 64: 8.5 in
-// one, 8.0 in 7), then 32 tiles, which hide the waits of 32 splits and more, or 16 of
+// has a tile a wave until there are 16 splits (one token at 4,000, 32/8 heads of 128: 9.3
+// us in 8 and in 16, 11.5 in 32; at 8,000, 9/3 heads of 64: 9.6 in 8, 7.7 in 16, 9.2 in 48;
+// 37 at 1,021, 15/5 heads of 64: 8.5 in one, 8.0 in 7), then 32 tiles, which hide the waits of 32 splits and more, or 16 of
 // more than 4 blocks (4/2 heads of 256, 30,000 positions: 15.4 us in 64, 17.5 in 32).
 // Two or three splits pay over long caches only (64 queries of 32/8 heads of 128 at
 // 1,000: 13.9 in two, 13.5 in one; 37 of 15/5 heads of 64 at 8,000: 22.6 and 34.6).
@@ -1225,9 +1225,10 @@ Q4Plan q4_attention_plan(bool f16_rows, int tokens, int heads, int kv_heads, int
     const int most = groups(r.cols) <= kQ4Counters ? std::max(1, (int)(cus / groups(r.cols))) : 1;
     r.splits = work <= 40 ? 1 : std::min(most, std::max(std::min(16, up(tiles, 4)), up(tiles, nb > 4 ? 16 : 32)));
     if (r.splits < 4 && work <= 200) r.splits = 1;
-    // Eight waves where each still has many tiles (131,072 positions in 32 splits: 42.0 us against
-    // 44.2 with four; 4,000 in 16: 10.2 against 9.7) and the chip is not full without them (512
-    // float32 queries, 32/8 heads of 128: 31.9 against 23.1), or for the threads that join.
+    // Eight waves where each still has many tiles (131,072 positions in 32 splits: 33.1 us against
+    // 36.6 with four; 1,000 in 8: 7.4 against 6.9) and the chip is not full without them (512
+    // float32 queries, 32/8 heads of 128, in this kernel: 31.9 against 23.1), or for the threads that
+    // join (16 queries of 32/8 heads of 128 at 4,000 in 8 splits: 14.2 against 15.8).
     const int64_t here = groups(r.cols) * r.splits;
     r.waves = (up(tiles, r.splits) >= 16 && here <= cus) || (r.splits > 1 && cols * (hd / 2) > 256) ? 8 : 4;
     return r;
