@@ -542,11 +542,14 @@ __global__ __launch_bounds__(64 * kMostWaves) void q4_attention_kernel(SplitArgs
 // unpacking, close to memory: 131,072 positions, 32/8 heads of 128, 35.7 us in float32
 // (4.2 TB/s) and 31.0 in f16, against 41.9 and 35 with a column a query; 8,000 positions,
 // 9/3 heads of 64, 8.2 us against 10.3.  Three tiles ahead instead of two: 37.2 us.
-// The probabilities times scales are held as P 2^14 d / 2^E, E the largest scale's
-// exponent so far, kept as the maximum of the softmax is.
+// The probabilities times scales are held as P 2^14 d / 2^E, E kept as the maximum of
+// the softmax is, so that the largest of the block's so far lies in [2^13, 2^15) and
+// f16's smallest step is 2^-37 of it or less, whatever the scales of tokens that have no
+// weight.  (E as the largest scale's exponent is known before the exponentials and 2.5%
+// faster, 31.7 us against 32.5 on one card, but with values of 1e-5 beside one of 6e4 at a
+// weight of e^-60 it loses 6e-3 of a float32 output.)
+constexpr int kLeastE = -80;  // a sum of weights over any cache stays a number
 constexpr int few_columns(int nb) { return nb == 1 ? 16 : nb == 2 ? 8 : nb <= 4 ? 4 : 2; }
-
-typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
 
 template <int N>
 __device__ __forceinline__ float row_rotated(float x) {  // of 16 lanes
@@ -622,8 +625,8 @@ __global__ __launch_bounds__(64 * kMostWaves) void q4_attention_few_kernel(Split
     }
 
     float m = -INFINITY, l = 0.f;
-    int E = -14;  // every scale so far is below 2^E,
-    u16x2 limit = {0x3FF, 0x3FF};  // the largest of these
+    int E = 0;         // the exponent that P 2^14 d is held against,
+    float peak = 0.f;  // and its largest so far (of this lane), which E keeps at 2^13 or above, below 2^15
     f32x4 o[NB][2];
 #pragma unroll
     for (int b = 0; b < NB; b++) o[b][0] = o[b][1] = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -663,23 +666,33 @@ __global__ __launch_bounds__(64 * kMostWaves) void q4_attention_few_kernel(Split
                 y.vs[s].y &= keep[1];
             }
         }
-        const uint32_t dv[4] = {y.vs[0].x, y.vs[0].y, y.vs[1].x, y.vs[1].y};
-        u16x2 most = limit;
-#pragma unroll
-        for (int i = 0; i < 4; i++) most = __builtin_elementwise_max(most, __builtin_bit_cast(u16x2, dv[i] & 0x7FFF7FFFu));
         float mx = sa[0][0];
 #pragma unroll
         for (int i = 1; i < 8; i++) mx = fmaxf(mx, sa[i >> 2][i & 3]);
         mx = xor32_combine(xor16_combine(mx, MaxOp()), MaxOp());
         const float mn = fmaxf(m, mx * sc);
         const float mref = mn == -INFINITY ? 0.f : mn;
-        if (__builtin_amdgcn_ballot_w64(m != mn || __builtin_bit_cast(uint32_t, most) != __builtin_bit_cast(uint32_t, limit))) {
-            float top = (float)max(most[0], most[1]);  // f16 bits, in order for what is not negative
-            top = xor32_combine(xor16_combine(top, MaxOp()), MaxOp());
-            const int now = ((int)top >> 10) - 14;
-            const float alpha = __builtin_amdgcn_exp2f(m - mref + (float)(E - now));
-            limit[0] = limit[1] = (uint16_t)((int)top | 0x3FF);
-            E = now;
+        const float eref = kLog2P - mref - (float)E;
+        const uint32_t dv[4] = {y.vs[0].x, y.vs[0].y, y.vs[1].x, y.vs[1].y};
+        float w[8], sum = 0.f, top = 0.f;
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            const float e = __builtin_amdgcn_exp2f(fmaf(sa[i >> 2][i & 3], sc, eref));
+            sum += e;
+            w[i] = times(pair(dv[i >> 1])[i & 1], e);
+            top = fmaxf(top, fabsf(w[i]));  // (a NaN is not taken)
+        }
+        if (__builtin_amdgcn_ballot_w64(m != mn || top > 32768.f)) {
+            const float down = __builtin_amdgcn_exp2f(m - mref);
+            peak = fmaxf(peak * down, top);
+            peak = xor32_combine(xor16_combine(peak, MaxOp()), MaxOp());
+            const int by = peak > 0.f ? max(__builtin_amdgcn_frexp_expf(peak) - 14, kLeastE - E) : 0;
+            const float f = ldexpf(1.f, -by), alpha = down * f;
+            E += by;
+            peak *= f;
+            sum *= f;
+#pragma unroll
+            for (int i = 0; i < 8; i++) w[i] *= f;
 #pragma unroll
             for (int b = 0; b < NB; b++) {
                 o[b][0] *= alpha;
@@ -687,18 +700,15 @@ __global__ __launch_bounds__(64 * kMostWaves) void q4_attention_few_kernel(Split
             }
             l *= alpha;
             m = mn;
+        } else {
+            peak = fmaxf(peak, top);
         }
-        const float eref = kLog2P - mref - (float)E;
+        l += sum;
         f16x2 ph[4], pl[EXACT ? 4 : 1];
 #pragma unroll
         for (int i = 0; i < 4; i++) {
-            const f16x2 d = pair(dv[i]);
-            const float e0 = __builtin_amdgcn_exp2f(fmaf(sa[i >> 1][2 * (i & 1)], sc, eref));
-            const float e1 = __builtin_amdgcn_exp2f(fmaf(sa[i >> 1][2 * (i & 1) + 1], sc, eref));
-            l += e0 + e1;
-            const float w0 = times(d[0], e0), w1 = times(d[1], e1);
-            ph[i] = round2(w0, w1);
-            if constexpr (EXACT) pl[i] = round2(rest_low(ph[i], w0), rest_high(ph[i], w1));
+            ph[i] = round2(w[2 * i], w[2 * i + 1]);
+            if constexpr (EXACT) pl[i] = round2(rest_low(ph[i], w[2 * i]), rest_high(ph[i], w[2 * i + 1]));
         }
         const f16x8 pf = frag(ph[0], ph[1], ph[2], ph[3]);
         f16x8 pg;

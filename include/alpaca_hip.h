@@ -404,10 +404,12 @@ int ahip_kv_q4_load(ahip_context* ctx, const ahip_kv_q4* cache, int dtype, int s
 /* Causal grouped-query attention (as ahip_op_attention) of `tokens` queries at
  * positions start.. over the cache, which already holds their keys and values.
  * q and out rows [heads][head_dim]; out may not overlap q.  With AHIP_F32 the
- * scores, probabilities and sums keep float32 accuracy over the cache's exact
- * values; with AHIP_F16 keys enter the products exactly, values and probabilities
- * rounded to f16 (in calls of few queries their products with the values' scales),
- * and sums are float32.
+ * scores and sums keep float32 accuracy over the cache's exact values, and a
+ * probability is held to 2^-22 of itself or 2^-39 of its row's largest, whichever
+ * is more (in calls of few queries its product with the value's scale, to 2^-22 of
+ * itself or 2^-38 of the largest such product so far); with AHIP_F16 keys enter
+ * the products exactly, values and probabilities rounded to f16 (in calls of few
+ * queries their products with the values' scales), and sums are float32.
  * `workspace` (16-byte aligned) holds the partial results of the key ranges and the counters of their arrival: ahip_attention_q4_workspace
  * bytes for the same arguments (on_device: whether start_dev is set).  Its first
  * AHIP_Q4_WORKSPACE_ZERO bytes are zero before its first call, and every call
