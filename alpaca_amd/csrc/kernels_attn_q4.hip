@@ -1205,6 +1205,7 @@ hipError_t launch(const SplitArgs& p, const Q4Plan& plan, hipStream_t st) {
 Q4Plan q4_attention_plan(bool f16_rows, int tokens, int heads, int kv_heads, int hd, int length) {
     Q4Plan r;
     const int64_t cols = (int64_t)tokens * (heads / kv_heads);
+    if (cols <= 0) return r;  // (nothing runs)
     const int cus = device_cus(), nb = hd / 32, tiles = q4_tiles(length), work = tiles * nb;
     auto groups = [&](int tile) { return (cols + tile - 1) / tile * kv_heads; };
     auto up = [](int64_t a, int64_t b) { return (int)((a + b - 1) / b); };

@@ -123,3 +123,12 @@ def test_session_logits(hip_ctx, prec, dtype):
 def test_session_logits_of_many_queries(hip_ctx, prec, heads, kv_heads, hd):
     """Chunks that the many-column attention takes (16,384 queries), then a few tokens."""
     check(hip_ctx, (512, 1, 2), prec, heads, kv_heads, hd, 2, 515, Q8_0)
+
+
+@pytest.mark.parametrize("prec", ["fast-f16", "fast"])
+@pytest.mark.parametrize("least,tokens", [(500, 502), (512, 530)])
+def test_session_logits_of_a_prompt_on_two_streams(hip_ctx, monkeypatch, least, tokens, prec):
+    """From position 13, so that the halves meet inside a tile of the cache: an empty one and 502 tokens (they meet at
+    multiples of 256), 256 and 274."""
+    monkeypatch.setenv("ALPACA_HIP_SPLIT_MIN", str(least))
+    check(hip_ctx, (13, tokens), prec, 32, 8, 64, 2, 13 + tokens, Q8_0)
