@@ -41,7 +41,12 @@ class Q4Cache:
         self._work, self._work_bytes, self._reserved = None, 0, set()
         self._kind = "cache"
         _LIVE.add(self)
-        self._desc.k, self._desc.v = self._malloc(n.value), self._malloc(n.value)
+        try:
+            self._desc.k = self._malloc(n.value)
+            self._desc.v = self._malloc(n.value)
+        except L.HIPError:
+            self.close()
+            raise
 
     def _malloc(self, n: int) -> int:
         p = C.c_void_p()
