@@ -108,6 +108,7 @@ class Q4Cache:
                 # hipFree waits for the device: queued calls may still use the old one
                 L.check(L.lib().ahip_free(self._ctx, self._work))
                 self._work, self._work_bytes = None, 0
+                self._reserved.clear()  # (none has one should the next fail)
             self._work = self._malloc(need)
             L.check(L.lib().ahip_memset(self._ctx, self._work, 0, WORKSPACE_ZERO))
             self._work_bytes = need

@@ -81,3 +81,16 @@ def test_a_cache_that_cannot_be_allocated_keeps_nothing(made, fails):
     assert len(a.held) == 2
     cache.close()
     assert not a.held
+
+
+def test_a_workspace_that_cannot_grow_is_allocated_by_the_next_call(made):
+    a, ctx = made([4])
+    cache = Q4Cache(ctx, 2, 64, 64)
+    cache.attention(1 << 10, 1 << 12, 1, 4)
+    with pytest.raises(L.HIPError):
+        cache.attention(1 << 10, 1 << 12, 8, 4)
+    cache.attention(1 << 10, 1 << 12, 1, 4)  # a shape that ran before
+    cache.attention(1 << 10, 1 << 12, 8, 4)
+    assert sorted(a.held.values())[-1] == 8 * 4096 and len(a.held) == 3
+    cache.close()
+    assert not a.held
