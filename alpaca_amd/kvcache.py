@@ -33,7 +33,6 @@ class Q4Cache:
         L.check(lib.ahip_kv_q4_bytes(kv_heads, capacity, head_dim, C.byref(n)))
         self.context, self.kv_heads, self.capacity, self.head_dim = context, kv_heads, capacity, head_dim
         self.bytes = 2 * n.value
-        self._ctx = context.handle
         self._desc = L.KVQ4C(None, None, kv_heads, head_dim, capacity)
         self._cache = C.byref(self._desc)
         self._width = kv_heads * head_dim
@@ -50,13 +49,14 @@ class Q4Cache:
 
     def _malloc(self, n: int) -> int:
         p = C.c_void_p()
-        L.check(L.lib().ahip_malloc(self._ctx, n, C.byref(p)))
+        L.check(L.lib().ahip_malloc(self.context.handle, n, C.byref(p)))
         return p.value
 
     def store(self, k: int, v: int, tokens: int, start: int = 0, dtype: str = "f32", k_stride: int | None = None,
               v_stride: int | None = None, start_dev: int | None = None, stream=None) -> None:
         """Quantises rows of keys and values into positions start.. (or *start_dev..)."""
-        rc = self._store(self._ctx, self._cache, DTYPE[dtype], k, self._width if k_stride is None else k_stride, v,
+        rc = self._store(self.context.handle, self._cache, DTYPE[dtype], k,
+                         self._width if k_stride is None else k_stride, v,
                          self._width if v_stride is None else v_stride, tokens, start, start_dev, stream)
         if rc:
             L.check(rc)
@@ -64,7 +64,7 @@ class Q4Cache:
     def load(self, k_out: int | None, v_out: int | None, tokens: int, start: int = 0, dtype: str = "f32",
              k_stride: int | None = None, v_stride: int | None = None, stream=None) -> None:
         """The values of positions start.. as rows."""
-        rc = self._load(self._ctx, self._cache, DTYPE[dtype], start, tokens, k_out,
+        rc = self._load(self.context.handle, self._cache, DTYPE[dtype], start, tokens, k_out,
                         self._width if k_stride is None else k_stride, v_out,
                         self._width if v_stride is None else v_stride, stream)
         if rc:
@@ -74,8 +74,8 @@ class Q4Cache:
                         on_device: bool = False) -> int:
         """Bytes of workspace of an attention call with these arguments (on_device: with start_dev)."""
         n = C.c_int64()
-        L.check(L.lib().ahip_attention_q4_workspace(self._ctx, self._cache, DTYPE[dtype], tokens, heads, start,
-                                                    1 if on_device else 0, C.byref(n)))
+        L.check(L.lib().ahip_attention_q4_workspace(self.context.handle, self._cache, DTYPE[dtype], tokens, heads,
+                                                    start, 1 if on_device else 0, C.byref(n)))
         return n.value
 
     def attention(self, q: int, out: int, tokens: int, heads: int, start: int = 0, dtype: str = "f32",
@@ -94,9 +94,9 @@ class Q4Cache:
         else:
             work, work_bytes = workspace
         w = heads * self.head_dim
-        rc = self._attention(self._ctx, self._cache, DTYPE[dtype], q, w if q_stride is None else q_stride, tokens,
-                             heads, start, start_dev, out, w if out_stride is None else out_stride, work, work_bytes,
-                             stream)
+        rc = self._attention(self.context.handle, self._cache, DTYPE[dtype], q, w if q_stride is None else q_stride,
+                             tokens, heads, start, start_dev, out, w if out_stride is None else out_stride, work,
+                             work_bytes, stream)
         if rc:
             L.check(rc)
 
@@ -106,21 +106,19 @@ class Q4Cache:
         if need > self._work_bytes:
             if self._work:
                 # hipFree waits for the device: queued calls may still use the old one
-                L.check(L.lib().ahip_free(self._ctx, self._work))
+                L.check(L.lib().ahip_free(self.context.handle, self._work))
                 self._work, self._work_bytes = None, 0
                 self._reserved.clear()  # (none has one should the next fail)
             self._work = self._malloc(need)
-            L.check(L.lib().ahip_memset(self._ctx, self._work, 0, WORKSPACE_ZERO))
+            L.check(L.lib().ahip_memset(self.context.handle, self._work, 0, WORKSPACE_ZERO))
             self._work_bytes = need
         self._reserved.add((tokens, heads, dtype))
 
     def close(self) -> None:
-        """Frees the cache; calls on it are over."""
-        if not getattr(self.context, "handle", None):
-            return
+        """Frees the cache (as its context's close does); calls on it are refused."""
         for p in (self._desc.k, self._desc.v, self._work):
-            if p:
-                L.lib().ahip_free(self._ctx, p)
+            if p and getattr(self.context, "handle", None):
+                L.lib().ahip_free(self.context.handle, p)
         self._desc.k = self._desc.v = self._work = None
         self._work_bytes = 0
         self._reserved.clear()

@@ -57,6 +57,9 @@ class HIPContext:
 
     def close(self) -> None:
         if getattr(self, "handle", None):
+            for obj in list(_LIVE):
+                if getattr(obj, "_kind", None) == "cache" and obj.context is self:
+                    obj.close()
             L.lib().ahip_context_destroy(self.handle)
             self.handle = None
 

@@ -36,6 +36,8 @@ class Allocator:
         return 0
 
     def ahip_attention_q4_workspace(self, ctx, cache, dtype, tokens, heads, start, on_device, n):
+        if not ctx:
+            return L.INVALID_ARGUMENT
         C.cast(n, C.POINTER(C.c_int64))[0] = 4096 * tokens
         return 0
 
@@ -94,3 +96,33 @@ def test_a_workspace_that_cannot_grow_is_allocated_by_the_next_call(made):
     assert sorted(a.held.values())[-1] == 8 * 4096 and len(a.held) == 3
     cache.close()
     assert not a.held
+
+
+def test_a_closed_context_frees_its_caches_and_refuses_their_calls(made):
+    _, ctx = made()
+    b, other = made()
+    caches = [Q4Cache(other, 2, 64, 64) for _ in range(2)]
+    caches[0].attention(1 << 10, 1 << 12, 1, 4)
+    assert len(b.held) == 5
+    ctx.close()
+    assert len(b.held) == 5  # another context's
+    other.close()
+    assert not b.held and b.contexts == 2
+    for cache in caches:
+        for call in (lambda: cache.store(1 << 10, 1 << 10, 1), lambda: cache.load(1 << 10, None, 1),
+                     lambda: cache.attention(1 << 10, 1 << 12, 1, 4),
+                     lambda: cache.attention(1 << 10, 1 << 12, 1, 4, workspace=(1 << 20, 1 << 20)),
+                     lambda: cache.workspace_bytes(1, 4)):
+            with pytest.raises(L.InvalidArgument):
+                call()
+        cache.close()  # (again: nothing)
+
+
+def test_a_closed_cache_refuses_its_calls(made):
+    a, ctx = made()
+    cache = Q4Cache(ctx, 2, 64, 64)
+    cache.close()
+    assert not a.held
+    for call in (lambda: cache.store(1 << 10, 1 << 10, 1), lambda: cache.load(1 << 10, None, 1)):
+        with pytest.raises(L.InvalidArgument):
+            call()
