@@ -421,13 +421,16 @@ static int half_copy(const OwnedMatrix& w, OwnedMatrix& h, hipStream_t st) {
 // double, rounded once to float (CPUOps.rope, CPUOps.swift:196-201).
 static void rope_rows(int first, int positions, int hd, float theta, float2* t) {
     const int half = hd / 2;
-    std::vector<double> freq(half);
-    for (int i = 0; i < half; i++) freq[i] = std::pow((double)theta, -2.0 * (double)i / (double)hd);
-    for (int p = 0; p < positions; p++)
-        for (int i = 0; i < half; i++) {
-            const double a = (double)(first + p) * freq[i];
-            t[(size_t)p * half + i] = make_float2((float)std::cos(a), (float)std::sin(a));
-        }
+    for (int i0 = 0; i0 < half; i0 += 128) {  // (pairs at a time: no allocation)
+        double freq[128];
+        const int n = std::min(128, half - i0);
+        for (int i = 0; i < n; i++) freq[i] = std::pow((double)theta, -2.0 * (double)(i0 + i) / (double)hd);
+        for (int p = 0; p < positions; p++)
+            for (int i = 0; i < n; i++) {
+                const double a = (double)(first + p) * freq[i];
+                t[(size_t)p * half + i0 + i] = make_float2((float)std::cos(a), (float)std::sin(a));
+            }
+    }
 }
 static std::vector<float2> rope_table(int positions, int hd, float theta) {
     std::vector<float2> t((size_t)positions * (hd / 2));
