@@ -15,12 +15,16 @@ def run(body):
         def no_more_memory():
             used = int(open("/proc/self/statm").read().split()[0]) * resource.getpagesize()
             resource.setrlimit(resource.RLIMIT_AS, (used, resource.getrlimit(resource.RLIMIT_AS)[1]))
-            kept = []  # what the allocator still holds in pieces of the size asked for
+            # what the allocator still holds in large pieces
             malloc = C.CDLL(None).malloc
             malloc.restype, malloc.argtypes = C.c_void_p, [C.c_size_t]
             for size in (1 << 22, 1 << 20, 1 << 18, 1 << 16):
                 while malloc(size):
                     pass
+
+        def memory_again():
+            hard = resource.getrlimit(resource.RLIMIT_AS)[1]
+            resource.setrlimit(resource.RLIMIT_AS, (hard, hard))
     """) + textwrap.dedent(body) + "\nprint('done', flush=True)\n"
     r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=120)
     assert r.returncode == 0 and r.stdout.endswith("done\n"), (r.returncode, r.stdout, r.stderr[-2000:])
@@ -33,5 +37,6 @@ def test_rotation_table():
         assert lib.ahip_rope_table(3, 1 << 16, 1e4, want.ctypes.data) == 0
         no_more_memory()
         rc = lib.ahip_rope_table(3, 1 << 16, 1e4, table.ctypes.data)
+        memory_again()
         assert rc == 0 and (table == want).all()
     """)
