@@ -2375,7 +2375,7 @@ extern "C" int ahip_op_attention(ahip_context* ctx, const float* q, int tokens, 
                                  const float* values, int capacity, int kv_heads, int start, int kv_precision,
                                  int precision, float* out) {
     if (tokens <= 0 || heads <= 0 || kv_heads <= 0 || heads % kv_heads || hd <= 0 || start < 0 ||
-        start + tokens > capacity || !q || !keys || !values || !out)
+        (int64_t)start + tokens > capacity || !q || !keys || !values || !out)
         return fail(AHIP_ERR_INVALID_ARGUMENT, "attention shapes");
     if (hd % 32 || hd > 256) return fail(AHIP_ERR_INVALID_ARGUMENT, "head dimension must be a multiple of 32 up to 256");
     const bool f16kv = kv_precision == AHIP_KV_F16;
