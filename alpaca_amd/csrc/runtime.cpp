@@ -640,7 +640,9 @@ static constexpr int kMaxSplits = 65;
 // The largest workspace that the attention over a 4-bit cache takes in calls of up to max_batch tokens.
 static int64_t q4_session_workspace(const ahip_llama_config& c, int capacity, int max_batch) {
     int64_t most = 0;
-    for (int n = 1; n <= std::min(max_batch, capacity); n++)
+    // (one part, and no workspace, from more groups of at most 128 columns than there are counters)
+    const int tokens = std::min({max_batch, capacity, 128 * kQ4Counters / c.head_count + 1});
+    for (int n = 1; n <= tokens; n++)
         for (bool f16_rows : {false, true})
             most = std::max(most, q4_attention_workspace(n, c.head_count, c.head_dim,
                                                          q4_attention_plan(f16_rows, n, c.head_count, c.kv_head_count,
