@@ -545,9 +545,9 @@ __global__ __launch_bounds__(64 * kMostWaves) void q4_attention_kernel(SplitArgs
 // The probabilities times scales are held as P 2^14 d / 2^E, E kept as the maximum of
 // the softmax is, so that the largest of the block's so far lies in [2^13, 2^15) and
 // f16's smallest step is 2^-37 of it or less, whatever the scales of tokens that have no
-// weight.  (E as the largest scale's exponent is known before the exponentials and 2.5%
-// faster, 31.7 us against 32.5 on one card, but with values of 1e-5 beside one of 6e4 at a
-// weight of e^-60 it loses 6e-3 of a float32 output.)
+// weight.  (E as the largest scale's exponent is known before the exponentials, but costs
+// as much, within 1%, and with values of 1e-5 beside one of 6e4 at a weight of e^-60 it
+// loses 6e-3 of a float32 output.)
 constexpr int kLeastE = -80;  // a sum of weights over any cache stays a number
 constexpr int few_columns(int nb) { return nb == 1 ? 16 : nb == 2 ? 8 : nb <= 4 ? 4 : 2; }
 
@@ -626,7 +626,7 @@ __global__ __launch_bounds__(64 * kMostWaves) void q4_attention_few_kernel(Split
 
     float m = -INFINITY, l = 0.f;
     int E = 0;         // the exponent that P 2^14 d is held against,
-    float peak = 0.f;  // and its largest so far (of this lane), which E keeps at 2^13 or above, below 2^15
+    float peak = 0.f;  // and its largest when E was last chosen, in [2^13, 2^14); from 2^15 on E is chosen again
     f32x4 o[NB][2];
 #pragma unroll
     for (int b = 0; b < NB; b++) o[b][0] = o[b][1] = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -700,8 +700,6 @@ __global__ __launch_bounds__(64 * kMostWaves) void q4_attention_few_kernel(Split
             }
             l *= alpha;
             m = mn;
-        } else {
-            peak = fmaxf(peak, top);
         }
         l += sum;
         f16x2 ph[4], pl[EXACT ? 4 : 1];
