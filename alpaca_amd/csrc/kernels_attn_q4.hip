@@ -240,9 +240,11 @@ __device__ __forceinline__ void count_and_join(const SplitArgs& p, int kvh, int 
     if (group == 0) put(col, d, j);
 }
 
-// T float: the scores and outputs to float32 accuracy (the queries and
-// probabilities as two f16 terms, the quants exact and the values exact in two
-// terms).  T f16: queries and keys exact, probabilities and values one f16 term.
+// T float: the queries and probabilities as two f16 terms, the quants exact and the
+// values exact in two terms.  A probability below 2^-17 of its row's largest loses bits
+// (half of f16's smallest step is 2^-39 of that), which shows in an output 2^-15 the size
+// of that key's value.  T f16: queries and keys exact, probabilities and values one f16
+// term.
 //
 // A column's queries as the lane takes them, at q its dims 8 g of block 0: block b,
 // dims 8 g + {0, 4, 1, 5, 2, 6, 3, 7} as the keys' nibbles come.  float: scaled into
@@ -539,9 +541,10 @@ __global__ __launch_bounds__(64 * kMostWaves) void q4_attention_kernel(SplitArgs
 // values' scales go into the probabilities the same way (a column has one block's), so
 // that values enter as n - 8, exactly, and of the products with each block's values a
 // lane keeps its own block's.  Bound by the vector instructions, over half of them the
-// unpacking, close to memory: 131,072 positions, 32/8 heads of 128, 35.7 us in float32
-// (4.2 TB/s) and 31.0 in f16, against 41.9 and 35 with a column a query; 8,000 positions,
-// 9/3 heads of 64, 8.2 us against 10.3.  Three tiles ahead instead of two: 37.2 us.
+// unpacking, close to memory: 131,072 positions, 32/8 heads of 128, 31.8 to 36 us over
+// cards in float32 (4.2 to 4.7 TB/s) and 29.0 to 31.0 in f16; on one card 35.7 and 31.0
+// against 41.9 and 35 with a column a query, and 37.2 in float32 with three tiles ahead
+// instead of two; 8,000 positions, 9/3 heads of 64, 8.2 us against 10.3.
 // The probabilities times scales are held as P 2^14 d / 2^E, E kept as the maximum of
 // the softmax is, so that the largest of the block's so far lies in [2^13, 2^15) and
 // f16's smallest step is 2^-37 of it or less, whatever the scales of tokens that have no
@@ -1196,8 +1199,9 @@ hipError_t launch(const SplitArgs& p, const Q4Plan& plan, hipStream_t st) {
 // nb / 18 us a tile of its keys; joining costs 1.5 us (4 with 16 full columns).  A split
 // has a tile a wave until there are 16 splits (one token at 4,000, 32/8 heads of 128: 9.3
 // us in 8 and in 16, 11.5 in 32; at 8,000, 9/3 heads of 64: 9.6 in 8, 7.7 in 16, 9.2 in 48;
-// 37 at 1,021, 15/5 heads of 64: 8.5 in one, 8.0 in 7), then 32 tiles, which hide the waits of 32 splits and more, or 16 of
-// more than 4 blocks (4/2 heads of 256, 30,000 positions: 15.4 us in 64, 17.5 in 32).
+// 37 at 1,021, 15/5 heads of 64: 8.5 in one, 8.0 in 7), then 32 tiles, which hide the
+// waits of 32 splits and more, or 16 of more than 4 blocks (4/2 heads of 256, 30,000
+// positions: 15.4 us in 64, 17.5 in 32).
 // Two or three splits pay over long caches only (64 queries of 32/8 heads of 128 at
 // 1,000: 13.9 in two, 13.5 in one; 37 of 15/5 heads of 64 at 8,000: 22.6 and 34.6).
 Q4Plan q4_attention_plan(bool f16_rows, int tokens, int heads, int kv_heads, int hd, int length) {
@@ -1235,7 +1239,7 @@ Q4Plan q4_attention_plan(bool f16_rows, int tokens, int heads, int kv_heads, int
     r.splits = work <= 40 ? 1 : std::min(most, std::max(std::min(16, up(tiles, 4)), up(tiles, nb > 4 ? 16 : 32)));
     if (r.splits < 4 && work <= 200) r.splits = 1;
     // Eight waves where each still has many tiles (131,072 positions in 32 splits: 33.1 us against
-    // 36.6 with four; 1,000 in 8: 7.4 against 6.9) and the chip is not full without them (512
+    // 36.6 with four, one card; 1,000 in 8: 7.4 against 6.9) and the chip is not full without them (512
     // float32 queries, 32/8 heads of 128, in this kernel: 31.9 against 23.1), or for the threads that
     // join (16 queries of 32/8 heads of 128 at 4,000 in 8 splits: 14.2 against 15.8).
     const int64_t here = groups(r.cols) * r.splits;

@@ -40,10 +40,6 @@ __host__ __device__ inline int64_t q4_head_bytes(int capacity, int nb) {
 __host__ __device__ inline int q4_key_word(int k, int nb, int b, int g) {
     return 4 * (((k >> 4) * 64 + g * 16 + (k & 15)) * nb + b);
 }
-__host__ __device__ inline int q4_value_byte(int k, int b, int pair) {
-    const int r = k & 3;
-    return b * 512 + (((k >> 2) & 3) * 16 + pair) * 8 + (k >> 4) * 4 + (r == 1 ? 2 : r == 2 ? 1 : r);
-}
 __host__ __device__ inline int q4_scale(int k, int nb, int b) {
     return q4_scales_at(nb) + 2 * ((((k >> 4) * 4 + ((k >> 2) & 3)) * nb + b) * 4 + (k & 3));
 }
@@ -84,8 +80,8 @@ hipError_t launch_q4_load(bool f16_rows, const Q4Cache& c, int start, int tokens
 hipError_t launch_norm_rope(bool f16_rows, const ahip_norm_rope& a, hipStream_t st);
 
 // Causal attention of `tokens` queries at positions start.. (*start_dev when
-// set) over the cache; where splits > 1 with q4_attention_partials() floats of
-// partial results and kQ4Counters words, zero before and after every launch.
+// set) over the cache; where splits > 1 with a workspace of q4_attention_workspace()
+// bytes: kQ4Counters words, zero before and after every launch, and the parts' results.
 struct Q4Attention {
     const void* q = nullptr;
     void* out = nullptr;

@@ -403,15 +403,20 @@ int ahip_kv_q4_load(ahip_context* ctx, const ahip_kv_q4* cache, int dtype, int s
                     int64_t k_stride, void* v, int64_t v_stride, ahip_stream* stream);
 /* Causal grouped-query attention (as ahip_op_attention) of `tokens` queries at
  * positions start.. over the cache, which already holds their keys and values.
- * q and out rows [heads][head_dim]; out may not overlap q.  With AHIP_F32 the
- * scores and sums keep float32 accuracy over the cache's exact values, and a
- * probability is held to 2^-22 of itself or 2^-39 of its row's largest, whichever
- * is more (in calls of few queries its product with the value's scale, to 2^-22 of
- * itself or 2^-38 of the largest such product so far); with AHIP_F16 keys enter
- * the products exactly, values and probabilities rounded to f16 (in calls of few
- * queries their products with the values' scales), and sums are float32.
- * `workspace` (16-byte aligned) holds the partial results of the key ranges and the counters of their arrival: ahip_attention_q4_workspace
- * bytes for the same arguments (on_device: whether start_dev is set).  Its first
+ * q and out rows [heads][head_dim]; out may not overlap q.
+ *
+ * With AHIP_F32 the cached keys and values enter the products exactly, sums are
+ * float32, and two operands are held as two f16 terms: a query's value, to 2^-22
+ * of itself or 2^-24 of the largest in its head, whichever is more, and a
+ * probability, to 2^-22 of itself or 2^-39 of its row's largest (in calls of few
+ * queries its product with the value's scale, to 2^-22 of itself or 2^-38 of the
+ * largest such product so far).  With AHIP_F16 queries and keys enter exactly,
+ * values and probabilities rounded to f16 (in calls of few queries their products
+ * with the values' scales), and sums are float32.
+ *
+ * `workspace` (16-byte aligned) holds the partial results of the key ranges and
+ * the counters of their arrival: ahip_attention_q4_workspace bytes for the same
+ * arguments (on_device: whether start_dev is set).  Its first
  * AHIP_Q4_WORKSPACE_ZERO bytes are zero before its first call, and every call
  * leaves them so: clear them once, and let one workspace of the largest size serve
  * any calls that come one after another.  Calls that may run at the same time,
