@@ -303,6 +303,27 @@ __device__ __forceinline__ void add_scaled(f32x4& s, f32x4 part, uint2 d) {
     s[3] = fmaf((float)d1[1], part[3], s[3]);
 }
 
+// What comes off the exponents of a step: kLog2P - mref, mref the maximum so far in base 2
+// (0 for none), mx the step's own largest score.  A maximum is the rounded product of a
+// score with `sc`, and x sc - mref, rounded once, keeps what that rounding left: the same
+// for every key, so that it cancels, but past kLargeScore it would take P out of f16's
+// range.  From there on the scores are taken from the step's largest first, exactly 0 for
+// that one, and only the maxima are rounded.
+constexpr float kLargeScore = 8388608.f;  // 2^23: half a step is 2^-1
+template <int N>
+__device__ __forceinline__ float exponent_base(f32x4 (&x)[N], float mx, float mref, float sc) {
+#pragma clang fp contract(off)
+    float base = kLog2P - mref;
+    const bool large = fabsf(mref) > kLargeScore;
+    if (__builtin_amdgcn_ballot_w64(large)) {
+        const float top = large && mx != -INFINITY ? mx : 0.f;  // (a step of masked keys: 0)
+#pragma unroll
+        for (int i = 0; i < N; i++) x[i] -= top;
+        if (large) base = kLog2P + (top * sc - mref);
+    }
+    return base;
+}
+
 // Up to kMostWaves waves a workgroup, each with key tiles of its own.
 constexpr int kMostWaves = 8;
 template <int NB>
@@ -437,14 +458,14 @@ __global__ __launch_bounds__(64 * kMostWaves) void q4_attention_kernel(SplitArgs
         f16x8 pf[CT], pg[CT];
 #pragma unroll
         for (int ct = 0; ct < CT; ct++) {
-            const f32x4(&x)[2] = sa[ct];
+            f32x4(&x)[2] = sa[ct];
             float mx = x[0][0];
 #pragma unroll
             for (int i = 1; i < 8; i++) mx = fmaxf(mx, x[i >> 2][i & 3]);
             mx = xor32_combine(xor16_combine(mx, MaxOp()), MaxOp());
             const float mn = fmaxf(m[ct], mx * sc[ct]);  // (sc > 0)
             const float mref = mn == -INFINITY ? 0.f : mn;
-            const float alpha = __builtin_amdgcn_exp2f(m[ct] - mref), eref = kLog2P - mref;
+            const float alpha = __builtin_amdgcn_exp2f(m[ct] - mref), eref = exponent_base(x, mx, mref, sc[ct]);
             f16x2 ph[4], pl[EXACT ? 4 : 1];
 #pragma unroll
             for (int i = 0; i < 4; i++) {
@@ -675,7 +696,7 @@ __global__ __launch_bounds__(64 * kMostWaves) void q4_attention_few_kernel(Split
         mx = xor32_combine(xor16_combine(mx, MaxOp()), MaxOp());
         const float mn = fmaxf(m, mx * sc);
         const float mref = mn == -INFINITY ? 0.f : mn;
-        const float eref = kLog2P - mref - (float)E;
+        const float eref = exponent_base(sa, mx, mref, sc) - (float)E;
         const uint32_t dv[4] = {y.vs[0].x, y.vs[0].y, y.vs[1].x, y.vs[1].y};
         float w[8], sum = 0.f, top = 0.f;
 #pragma unroll
@@ -930,6 +951,9 @@ __global__ __launch_bounds__(256 * NSET) __attribute__((amdgpu_waves_per_eu(NSET
         read(0);
         // a group's products are scaled while the next group's run, where registers allow
         constexpr int LAG = NB <= 3 && !EXACT ? 1 : 0;
+        // heads of 256: the first values only behind the softmax, ahead of which 39 registers spill
+        // (4,000 queries of 16/8 heads: 287 us against 444)
+        constexpr bool LATE = NB == 8;
         f32x4 part[2][CT][NB];
         uint2 d[2][NB];
         auto scale = [&](int u) {
@@ -942,7 +966,7 @@ __global__ __launch_bounds__(256 * NSET) __attribute__((amdgpu_waves_per_eu(NSET
         };
 #pragma unroll
         for (int u = 0; u < 2 * TPS; u++) {
-            read(u + 1);  // (after the last keys: the first values)
+            if (!LATE || u + 1 < 2 * TPS) read(u + 1);  // (after the last keys: the first values)
 #pragma unroll
             for (int b = 0; b < NB; b++) d[u & 1][b] = *(const uint2*)(buf + W::SCALES + ((u * 4 + g) * NB + b) * 8);
 #pragma unroll
@@ -974,7 +998,7 @@ __global__ __launch_bounds__(256 * NSET) __attribute__((amdgpu_waves_per_eu(NSET
             mx = xor32_combine(xor16_combine(mx, MaxOp()), MaxOp());
             const float mn = fmaxf(m[ct], mx * sc[ct]);
             const float mref = mn == -INFINITY ? 0.f : mn;
-            const float alpha = __builtin_amdgcn_exp2f(m[ct] - mref), eref = kLog2P - mref;
+            const float alpha = __builtin_amdgcn_exp2f(m[ct] - mref), eref = exponent_base(sa[ct], mx, mref, sc[ct]);
 #pragma unroll
             for (int tt = 0; tt < TPS; tt++) {
                 f16x2 e[4], r[4];
@@ -1004,6 +1028,7 @@ __global__ __launch_bounds__(256 * NSET) __attribute__((amdgpu_waves_per_eu(NSET
                 if constexpr (EXACT) l[ct] = mfma(ones, pg[ct][tt], l[ct]);
             }
         }
+        if (LATE) read(2 * TPS);
         constexpr int VG = 2 * TPS * W::VT;  // groups of the values' fragments: (tile, block, parity, term)
 #pragma unroll
         for (int u = 0; u < VG; u++) {
