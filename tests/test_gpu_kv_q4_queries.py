@@ -53,10 +53,12 @@ def test_large_scores(hip_ctx, heads, kv_heads, hd, tokens, start, sign, dtype, 
 @pytest.mark.parametrize("dtype", ["f32", "f16"])
 @pytest.mark.parametrize("value", [np.nan, np.inf])
 @pytest.mark.parametrize("heads,kv_heads,hd,tokens,start", SHAPES)
-def test_a_query_that_is_no_number_reaches_its_own_output_only(hip_ctx, heads, kv_heads, hd, tokens, start, value, dtype):
+def test_a_query_that_is_no_number_reaches_its_own_output_only(hip_ctx, heads, kv_heads, hd, tokens, start, value,
+                                                               dtype):
     rng = np.random.default_rng(heads + hd + start + 1)
     n = start + tokens
-    k, v, q = (rows(rng, m, h, hd, t) for m, h, t in ((n, kv_heads, "f32"), (n, kv_heads, "f32"), (tokens, heads, dtype)))
+    k, v = rows(rng, n, kv_heads, hd, "f32"), rows(rng, n, kv_heads, hd, "f32")
+    q = rows(rng, tokens, heads, hd, dtype)
     hit = (tokens // 2, heads // 2)
     bad = q.copy()
     bad[hit][hd - 3] = value

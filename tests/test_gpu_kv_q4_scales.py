@@ -19,9 +19,10 @@ def single_tokens(q, k, v, start, dtype):
     A probability p_k is off, relatively, by its score's hd products and sums and the query's two terms (half a float32
     step of the sum of magnitudes each), by the exponential's argument (base 2: its own rounding and that of what is
     taken out of it, the maximum and an exponent with 14 below 40; 2 ln 2 < 1.5 half steps) and by 2^-22 for the
-    exponential and for each of up to 8 rescalings; numerator and denominator both.  The sums lose half a step of the sum of magnitudes a key.  The products of p_k and its value's
-    scale d_k enter as two f16 terms: past their 2^-22, half of f16's smallest step, 2^-25, where the largest of the
-    block's products so far is at 2^13 or more; times a quant, at most 8."""
+    exponential and for each of up to 8 rescalings; numerator and denominator both.  The sums lose half a step of the
+    sum of magnitudes a key.  The products of p_k and its value's scale d_k enter as two f16 terms: past their 2^-22,
+    half of f16's smallest step, 2^-25, where the largest of the block's products so far is at 2^13 or more; times a
+    quant, at most 8."""
     T, H, hd = q.shape
     G = H // k.shape[1]
     out, bound = np.empty(q.shape), np.empty(q.shape)

@@ -84,7 +84,8 @@ OTHERS = {"not quantised": lambda x, y: x.astype(np.float64), "3% larger": lambd
 def references(parts, *model):
     """The logits of every call, those with any value near a border on its other side, and those of OTHERS."""
     c, w, prompt = build(*model)
-    passes = {"": Forward(c, w), "borders": Forward(c, w, True, CLEAR / 2), **{n: Other(c, w, f) for n, f in OTHERS.items()}}
+    passes = {"": Forward(c, w), "borders": Forward(c, w, True, CLEAR / 2)}
+    passes.update((name, Other(c, w, change)) for name, change in OTHERS.items())
     out, at = [], 0
     for n in parts:
         out.append({name: f(prompt[at:at + n]) for name, f in passes.items()})
@@ -116,6 +117,12 @@ def check(hip_ctx, parts, prec, *model):
 def test_session_logits(hip_ctx, prec, dtype):
     """A prompt, a second message, a short one of a few tokens, single tokens, and the rest."""
     check(hip_ctx, (40, 35, 7, 1, 1, 26), prec, 4, 2, 64, 3, 110, dtype)
+
+
+@pytest.mark.parametrize("prec", ["exact", "fast", "fast-f16"])
+@pytest.mark.parametrize("heads,kv_heads,hd", [(6, 3, 96), (16, 1, 32), (5, 1, 160), (4, 2, 256)])
+def test_session_logits_at_head_dims(hip_ctx, heads, kv_heads, hd, prec):
+    check(hip_ctx, (45, 9, 1, 1), prec, heads, kv_heads, hd, 2, 56, Q8_0)
 
 
 @pytest.mark.parametrize("prec,heads,kv_heads,hd", [("fast-f16", 32, 8, 64), ("fast-f16", 32, 4, 128),
