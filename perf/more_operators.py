@@ -304,6 +304,7 @@ def _cache(s):
             n = s["pages"] * c["page"]
             every = torch.arange(s["pages"], dtype=torch.int32, device="cuda")
             ends = torch.tensor([0, n, n], dtype=torch.int32, device="cuda")
+            torch.cuda.synchronize()  # (the context has a stream of its own)
             fill = PagedBatch(ends.data_ptr(), ends[1:].data_ptr(), every.data_ptr(), 1, s["pages"], n, n)
             s["cache"].append(fill, s["k_pages"].data_ptr(), s["v_pages"].data_ptr(), dtype="f16")
             torch.cuda.synchronize()
