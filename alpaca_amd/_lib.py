@@ -103,6 +103,28 @@ class NormRopeC(C.Structure):
                                           "interleaved", "start")] + [("eps", C.c_float)])
 
 
+class PagedKVC(C.Structure):
+    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("kv_heads", C.c_int32), ("head_dim", C.c_int32),
+                ("page_tokens", C.c_int32), ("pages", C.c_int32)]
+
+
+class PagedBatchC(C.Structure):
+    _fields_ = ([(n, C.c_void_p) for n in ("row_starts", "lengths", "table")] +
+                [(n, C.c_int32) for n in ("sequences", "table_stride", "rows", "max_rows")])
+
+
+class PagedRowsC(C.Structure):
+    _fields_ = ([(n, C.c_void_p) for n in ("q", "q_out", "k", "v")] +
+                [(n, C.c_int64) for n in ("q_stride", "q_out_stride", "k_stride", "v_stride")] + [("rope", C.c_void_p)] +
+                [(n, C.c_int32) for n in ("rope_positions", "interleaved", "dtype", "heads")])
+
+
+class LogprobsC(C.Structure):
+    _fields_ = ([("logits", C.c_void_p), ("stride", C.c_int64)] +
+                [(n, C.c_void_p) for n in ("tokens", "logprobs", "entropy", "top_tokens", "top_logprobs")] +
+                [(n, C.c_int32) for n in ("dtype", "rows", "vocab", "top")])
+
+
 EMIT_FN = C.CFUNCTYPE(C.c_int, C.c_void_p, C.c_int32)
 
 vp, fp, ip, dp = C.c_void_p, C.POINTER(C.c_float), C.POINTER(C.c_int32), C.POINTER(C.c_double)
@@ -173,6 +195,14 @@ SIGNATURES = {
     "ahip_attention_q4_workspace": (i, [vp, vp, i, i, i, i, i, i64p]),
     "ahip_attention_q4": (i, [vp, vp, i, vp, i64, i, i, i, vp, vp, i64, vp, i64, vp]),
     "ahip_qk_norm_rope": (i, [vp, vp, vp]),
+    "ahip_paged_kv_bytes": (i, [i, i, i, i, i64p]),
+    "ahip_paged_append": (i, [vp, vp, vp, vp, vp]),
+    "ahip_paged_load": (i, [vp, vp, vp, i, vp, i64, vp, i64, vp]),
+    "ahip_paged_attention_workspace": (i, [vp, i64p]),
+    "ahip_paged_attention": (i, [vp, vp, vp, i, vp, i64, i, i, i, vp, i64, vp, i64, vp]),
+    "ahip_token_logprobs_workspace": (i, [i64p]),
+    "ahip_token_logprobs": (i, [vp, vp, vp, i64, vp]),
+    "ahip_session_logprobs": (i, [vp, C.c_int32, i, fp, fp, ip, fp]),
     "ahip_rope_table": (i, [i, i, C.c_float, vp]),
     "ahip_quantize": (i, [i, fp, i64, vp]),
     "ahip_synth_uniform": (i, [C.c_uint64, C.c_uint64, i64, C.c_float, C.c_float, fp]),

@@ -1,0 +1,748 @@
+// Causal grouped-query attention of a batch of sequences over a cache in pages
+// (paged.h), of all positions or of a window with the first ones.
+//
+// A sequence's query at position p sees positions j <= p with j > p - window (where
+// there is a window) or j < sinks; query head h reads KV head h / G.  The (token, head
+// of the group) pairs of a KV head are its query columns c = t G + g, the columns of
+// the products S^T = K Q^T and O^T = V^T P^T, so that a lane's scores are all of one
+// column and its probabilities lie where the second product takes them.
+//
+// What is read of a batch is bounded here, whatever it holds: a step of keys ends
+// with the table, and a page outside the cache is not read; a column that sees a
+// position without a page gets NaN.
+#include "attn_parts.h"
+#include "paged.h"
+
+#include <algorithm>
+
+namespace {
+
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+
+__device__ __forceinline__ f32x16 mfma32(f16x8 a, f16x8 b, f32x16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
+}
+// The batch's arrays do not change while a kernel runs: scalar loads where the address is a wave's.
+template <typename T>
+__device__ __forceinline__ T uniform_load(const T* p) {
+    return *(const __attribute__((address_space(4))) T*)p;
+}
+
+struct AttnArgs {
+    PagedAttention a;
+    PagedSteps b;
+    PagedKV c;
+    int G, most;  // positions that the table can hold
+    Divisor by_group;
+    float scale_log2;
+    float* partials;
+    int* counters;
+    int wide_grid;   // workgroups of the many-column part
+    int few_columns; // sequences of more query columns are the many-column part's
+    int target;      // workgroups that the few-column part aims for
+    bool whole_q, whole_out;  // rows that lie on 16 bytes
+};
+
+constexpr int kFewCols = 16, kFewStep = 32;
+constexpr int kFewLeast = 16;      // steps of a workgroup, where columns are split
+constexpr int kManyColumns = 64;   // sequences of more columns take the many-column part
+constexpr int kMostTarget = kPagedCounters;       // split groups of columns at most
+constexpr int kMostSlots = 2 * kMostTarget + 64;  // their parts
+
+// The steps of `step` keys that queries at first..last see: the first tokens' ones, then a range.
+struct Steps {
+    int first_steps, lo, count;
+    __device__ __forceinline__ int operator[](int i) const { return i < first_steps ? i : lo + i - first_steps; }
+};
+__device__ __forceinline__ Steps steps_of(const AttnArgs& p, int first, int last, int step) {
+    Steps r{0, 0, 0};
+    if (last < 0) return r;
+    if (p.a.window) {
+        r.lo = max(0, first - p.a.window + 1) / step;
+        r.first_steps = min((int)(((int64_t)p.a.sinks + step - 1) / step), r.lo);
+    }
+    r.count = r.first_steps + max(0, min(last, p.most - 1) / step + 1 - r.lo);
+    return r;
+}
+// Whether a query at `pos` sees the key, and whether queries at first..last see all of [key0, key1], or any of it.
+__device__ __forceinline__ bool sees(const AttnArgs& p, int pos, int key) {
+    return key <= pos && (!p.a.window || key > pos - p.a.window || key < p.a.sinks);
+}
+__device__ __forceinline__ bool all_see(const AttnArgs& p, int first, int last, int key0, int key1) {
+    return key1 <= first && (!p.a.window || key0 > last - p.a.window || key1 < p.a.sinks);
+}
+__device__ __forceinline__ bool any_sees(const AttnArgs& p, int first, int last, int key0, int key1) {
+    return key0 <= last && (!p.a.window || key1 > first - p.a.window || key0 < p.a.sinks);
+}
+
+// The page of a tile, the same for the whole wave (-1: none).
+__device__ __forceinline__ int page_of(const AttnArgs& p, int s, int tile) {
+    const int i = tile >> p.c.tiles_log2;
+    if (i >= p.b.table_stride) return -1;
+    const int id = uniform_load(p.b.table + (int64_t)s * p.b.table_stride + i);
+    return (unsigned)id < (unsigned)p.c.pages ? id : -1;
+}
+
+// A column's queries as the lane takes them: dims of runs of 8, D apart, from q on.  float: scaled
+// into [-1, 1] by a power of two of the largest among the lanes that `over` joins, in two f16 terms, which so
+// hold any float32 range.  Returns what the products are to be scaled by for scores in base 2.
+template <int N, int D, typename T, typename Over>
+__device__ __forceinline__ float load_queries(const T* q, float scale_log2, bool whole, f16x8 (&qh)[N],
+                                              f16x8 (&ql)[sizeof(T) == 4 ? N : 1], Over over) {
+    if constexpr (sizeof(T) == 2) {
+#pragma unroll
+        for (int b = 0; b < N; b++) {
+            if (whole) {
+                qh[b] = *(const AS_GLOBAL f16x8*)(q + D * b);
+            } else {
+#pragma unroll
+                for (int e = 0; e < 8; e++) qh[b][e] = gptr(q)[D * b + e];
+            }
+        }
+        return scale_log2;
+    } else {
+        float x[N][8], most = 0.f;
+#pragma unroll
+        for (int b = 0; b < N; b++) {
+            if (whole) {
+                const f32x4 u = *(const AS_GLOBAL f32x4*)(q + D * b), v = *(const AS_GLOBAL f32x4*)(q + D * b + 4);
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    x[b][e] = u[e];
+                    x[b][4 + e] = v[e];
+                }
+            } else {
+#pragma unroll
+                for (int e = 0; e < 8; e++) x[b][e] = gptr(q)[D * b + e];
+            }
+        }
+#pragma unroll
+        for (int b = 0; b < N; b++)
+#pragma unroll
+            for (int e = 0; e < 8; e++) most = fmaxf(most, fabsf(x[b][e]));
+        most = over(most);
+        // (the bounds keep the scale itself, and a masked score's product with it, a number)
+        const int ex = most > 0.f && most < INFINITY ? max(-100, min(__builtin_amdgcn_frexp_expf(most), 120)) : 0;
+        const float down = ldexpf(1.f, -ex);
+#pragma unroll
+        for (int b = 0; b < N; b++) {
+            f16x2 hi[4], lo[4];
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const float u = x[b][2 * i] * down, v = x[b][2 * i + 1] * down;
+                hi[i] = round2(u, v);
+                lo[i] = round2(rest_low(hi[i], u), rest_high(hi[i], v));
+            }
+            qh[b] = frag(hi[0], hi[1], hi[2], hi[3]);
+            ql[b] = frag(lo[0], lo[1], lo[2], lo[3]);
+        }
+        return ldexpf(scale_log2, ex);
+    }
+}
+// 1 / sum of a column's probabilities, 0 where it sees nothing, NaN where it sees a position past the table.
+__device__ __forceinline__ float inverse(float l, bool past) { return past ? NAN : l == 0.f ? 0.f : 1.f / l; }
+
+// ------------------------------------------------------------------ few columns
+// Sequences of a few query columns, single tokens above all: bound by the pages' bytes.  16 columns of a
+// KV head are a workgroup's; each wave has steps of 32 keys of its own, whose tiles go from memory straight into
+// the products' operands, one step ahead.  The steps of one group of columns are split over workgroups, so that
+// all of them have like shares of the batch's work whatever its lengths, and the last one to arrive joins the parts.
+
+// A workgroup's work: a group of 16 columns of sequence s, part sp of `splits`.
+struct FewItem {
+    int s, kvh, group, sp, splits, counter, slot;
+};
+struct FewCount {
+    int groups, steps;  // of a sequence, of 16 columns of a KV head each
+};
+__device__ __forceinline__ FewCount few_count(const AttnArgs& p, const PagedSeq& q) {
+    const int64_t cols = (int64_t)q.n * p.G;
+    if (q.n == 0 || cols > p.few_columns) return {0, 0};
+    return {(int)((cols + kFewCols - 1) / kFewCols), steps_of(p, q.length - q.n, q.length - 1, kFewStep).count};
+}
+// Workgroup `w` of the few-column part, by a whole wave; splits = 0 past the last.
+__device__ __forceinline__ FewItem few_find(const AttnArgs& p, int w) {
+    const int lane = __lane_id(), S = p.b.sequences, KVH = p.c.kv_heads;
+    // steps a workgroup: all the batch's over the workgroups aimed for.  (float: the same sum in every wave)
+    float all = 0.f;
+    for (int s0 = 0; s0 < S; s0 += 64) {
+        if (s0 + lane < S) {
+            const FewCount f = few_count(p, paged_seq(p.b, s0 + lane));
+            all += (float)f.groups * (float)f.steps;
+        }
+    }
+    all = wave_sum(all) * (float)KVH;
+    const int share = max(kFewLeast, (int)fminf(all * 1.0001f / (float)p.target + 1.f, 1e9f));
+    FewItem r{0, 0, 0, 0, 0, 0, 0};
+    for (int s0 = 0; s0 < S; s0 += 64) {
+        int groups = 0, splits = 1;
+        if (s0 + lane < S) {
+            const FewCount f = few_count(p, paged_seq(p.b, s0 + lane));
+            groups = f.groups * KVH;
+            splits = max(1, (f.steps + share - 1) / share);
+        }
+        const int mine = groups * splits, upto = wave_scan(mine);
+        const int joint = splits > 1 ? groups : 0, joint_to = wave_scan(joint);
+        const int parts = joint * splits, parts_to = wave_scan(parts);
+        const uint64_t past = __builtin_amdgcn_ballot_w64(upto > w);
+        if (past) {
+            const int l = __builtin_ctzll(past);
+            const int i = w - __builtin_amdgcn_readlane(upto - mine, l);
+            r.s = s0 + l;
+            r.splits = __builtin_amdgcn_readlane(splits, l);
+            r.kvh = i % KVH;
+            r.sp = i / KVH % r.splits;
+            r.group = i / KVH / r.splits;
+            const int at = r.group * KVH + r.kvh;
+            r.counter += __builtin_amdgcn_readlane(joint_to - joint, l) + at;
+            r.slot += __builtin_amdgcn_readlane(parts_to - parts, l) + at * r.splits;
+            // (only row ranges that overlap could have more)
+            if (r.splits > 1 && (r.counter >= p.target || r.slot + r.splits > 2 * p.target + 64)) r.splits = 0;
+            return r;
+        }
+        w -= __builtin_amdgcn_readlane(upto, 63);
+        r.counter += __builtin_amdgcn_readlane(joint_to, 63);
+        r.slot += __builtin_amdgcn_readlane(parts_to, 63);
+    }
+    return r;
+}
+
+template <int NB>
+struct FewTile {
+    f16x8 k[2][NB], v[2 * NB];
+    int none;  // bits of the step's two tiles: those that have no page
+};
+template <int NB>
+constexpr int few_lds(int waves) {
+    return waves * kFewCols * (32 * NB + 4 + 2) * 4;
+}
+
+template <int NB, typename T>
+__device__ __forceinline__ void few_part(const AttnArgs& p, int w, uint8_t* lds) {
+    constexpr bool EXACT = sizeof(T) == 4;
+    constexpr int HD = 32 * NB, TILE = paged_tile_bytes(HD);
+    const int lane = threadIdx.x & 63, g = lane >> 4, c16 = lane & 15, waves = blockDim.x >> 6;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const FewItem it = few_find(p, w);
+    if (it.splits == 0) return;  // (the same for the whole workgroup)
+    const PagedSeq seq = paged_seq(p.b, it.s);
+    const int col0 = it.group * kFewCols, cols = min(seq.n * p.G - col0, kFewCols), pos0 = seq.length - seq.n;
+    const int first = pos0 + p.by_group(col0), last = pos0 + p.by_group(col0 + cols - 1);
+    const Steps steps = steps_of(p, first, last, kFewStep);
+    const int per = steps.count / it.splits, more = steps.count - per * it.splits;
+    const int t0 = per * it.sp + min(it.sp, more), t1 = t0 + per + (it.sp < more);
+
+    const uint8_t *kbase = p.c.k + (g * 16 + (lane & 7)) * 16, *vbase = p.c.v + ((g & 1) * HD + c16) * 16;
+    auto load = [&](FewTile<NB>& x, int i) {
+        const int tile = 2 * steps[min(i, t1 - 1)];  // (past the last step: that one, unused)
+        const int pa = page_of(p, it.s, tile), pb = p.c.tiles_log2 ? pa : page_of(p, it.s, tile + 1);
+        x.none = (pa < 0) | (pb < 0) << 1;
+        const int64_t a = paged_tile(p.c, max(pa, 0), it.kvh, tile) * TILE;
+        const int64_t b = paged_tile(p.c, max(pb, 0), it.kvh, tile + 1) * TILE;
+        const uint8_t *k = kbase + (lane & 8 ? b : a), *v = vbase + (lane & 32 ? b : a);
+#pragma unroll
+        for (int s = 0; s < 2; s++)
+#pragma unroll
+            for (int c = 0; c < NB; c++) x.k[s][c] = *(const AS_GLOBAL f16x8*)(k + c * 1024 + s * 128);
+#pragma unroll
+        for (int d = 0; d < 2 * NB; d++) x.v[d] = *(const AS_GLOBAL f16x8*)(v + d * 256);
+    };
+    FewTile<NB> xa, xb;
+    int j = t0 + wave;
+    if (j < t1) load(xa, j);
+
+    f16x8 qh[NB], ql[EXACT ? NB : 1];
+    const int col = col0 + min(c16, cols - 1), t = p.by_group(col), pos = pos0 + t;
+    const T* q = (const T*)p.a.q + (int64_t)(seq.row0 + t) * p.a.q_stride + (int64_t)(it.kvh * p.G + col - t * p.G) * HD + 8 * g;
+    const float sc = load_queries<NB, 32, T>(q, p.scale_log2, p.whole_q, qh, ql, [](float x) {
+        return xor32_combine(xor16_combine(x, MaxOp()), MaxOp());
+    });
+    float m = -INFINITY, l = 0.f;
+    f32x4 o[2 * NB];
+#pragma unroll
+    for (int d = 0; d < 2 * NB; d++) o[d] = f32x4{0.f, 0.f, 0.f, 0.f};
+
+    auto step = [&](FewTile<NB>& x, int i) {
+        f32x4 sa[2];  // S(key 8 g + 4 s + r, column c16)
+#pragma unroll
+        for (int s = 0; s < 2; s++) {
+            sa[s] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int c = 0; c < NB; c++) {
+                sa[s] = mfma(x.k[s][c], qh[c], sa[s]);
+                if constexpr (EXACT) sa[s] = mfma(x.k[s][c], ql[c], sa[s]);
+            }
+        }
+        const int key0 = steps[i] * kFewStep;
+        if (x.none || !all_see(p, first, last, key0, key0 + kFewStep - 1)) {
+            const bool none = x.none >> (g >> 1) & 1;
+            uint32_t keep[4] = {0u, 0u, 0u, 0u};
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+                const int key = key0 + 8 * g + e;
+                if (none) sa[e >> 2][e & 3] = NAN;
+                if (!sees(p, pos, key)) sa[e >> 2][e & 3] = -INFINITY;
+                if (!none && any_sees(p, first, last, key, key)) keep[e >> 1] |= 0xFFFFu << (16 * (e & 1));
+            }
+            // positions that may never have been written: values of 0, since 0 times what lies there may be NaN
+#pragma unroll
+            for (int d = 0; d < 2 * NB; d++) {
+                typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+                u32x4 u = __builtin_bit_cast(u32x4, x.v[d]);
+#pragma unroll
+                for (int e = 0; e < 4; e++) u[e] &= keep[e];
+                x.v[d] = __builtin_bit_cast(f16x8, u);
+            }
+        }
+        float mx = sa[0][0];
+#pragma unroll
+        for (int e = 1; e < 8; e++) mx = fmaxf(mx, sa[e >> 2][e & 3]);
+        mx = xor32_combine(xor16_combine(mx, MaxOp()), MaxOp());
+        const float mn = fmaxf(m, mx * sc);  // (sc > 0)
+        const float mref = mn == -INFINITY ? 0.f : mn;
+        const float alpha = __builtin_amdgcn_exp2f(m - mref), base = exponent_base(sa, mx, mref, sc);
+        f16x2 ph[4], pl[EXACT ? 4 : 1];
+        float sum = 0.f;
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            const float a = __builtin_amdgcn_exp2f(fmaf(sa[e >> 1][2 * (e & 1)], sc, base));
+            const float b = __builtin_amdgcn_exp2f(fmaf(sa[e >> 1][2 * (e & 1) + 1], sc, base));
+            sum += a + b;
+            ph[e] = round2(a, b);
+            if constexpr (EXACT) pl[e] = round2(rest_low(ph[e], a), rest_high(ph[e], b));
+        }
+        if (__builtin_amdgcn_ballot_w64(m != mn)) {
+#pragma unroll
+            for (int d = 0; d < 2 * NB; d++) o[d] *= alpha;
+            l *= alpha;
+            m = mn;
+        }
+        l += sum;
+        const f16x8 pf = frag(ph[0], ph[1], ph[2], ph[3]);
+#pragma unroll
+        for (int d = 0; d < 2 * NB; d++) {
+            o[d] = mfma(x.v[d], pf, o[d]);
+            if constexpr (EXACT) o[d] = mfma(x.v[d], frag(pl[0], pl[1], pl[2], pl[3]), o[d]);
+        }
+    };
+    if (j + waves < t1) load(xb, j + waves);
+    for (; j < t1; j += 2 * waves) {
+        step(xa, j);
+        if (j + waves >= t1) break;
+        load(xa, j + 2 * waves);
+        step(xb, j + waves);
+        load(xb, j + 3 * waves);
+    }
+
+    // o[d][r] = O(column c16, dim 16 d + 4 g + r); the waves' results meet in LDS
+    float (*xo)[kFewCols][HD + 4] = (float (*)[kFewCols][HD + 4])lds;
+    float (*xml)[2][kFewCols] = (float (*)[2][kFewCols])(lds + waves * kFewCols * (HD + 4) * 4);
+    l = xor32_combine(xor16_combine(l, AddOp()), AddOp());
+#pragma unroll
+    for (int d = 0; d < 2 * NB; d++) *(f32x4*)&xo[wave][c16][16 * d + 4 * g] = o[d];
+    if (g == 0) {
+        xml[wave][0][c16] = m;
+        xml[wave][1][c16] = l;
+    }
+    __syncthreads();
+    const int items = cols * (HD / 2), had = max(1, min(waves, t1 - t0));  // (a wave without a step adds nothing)
+    float* const part = p.partials + (int64_t)it.slot * kFewCols * (HD + 2);
+    auto put = [&](int c, int d, float a, float b, float sum) {
+        const int u = p.by_group(col0 + c), h = it.kvh * p.G + col0 + c - u * p.G;
+        const float inv = inverse(sum, pos0 + u >= p.most);
+        T* out = (T*)p.a.out + (int64_t)(seq.row0 + u) * p.a.out_stride + (int64_t)h * HD + d;
+        gptr(out)[0] = (T)(a * inv);
+        gptr(out)[1] = (T)(b * inv);
+    };
+    for (int i = threadIdx.x; i < items; i += blockDim.x) {
+        const int c = i / (HD / 2), d = 2 * (i % (HD / 2));
+        float top = xml[0][0][c];
+        for (int v = 1; v < had; v++) top = fmaxf(top, xml[v][0][c]);
+        float sum = 0.f, a = 0.f, b = 0.f;
+        for (int v = 0; v < had; v++) {
+            const float f = join_weight(xml[v][0][c], top);
+            sum += f * xml[v][1][c];
+            a += f * xo[v][c][d];
+            b += f * xo[v][c][d + 1];
+        }
+        if (it.splits == 1) {
+            put(c, d, a, b, sum);
+        } else {
+            float* x = part + (int64_t)(c * it.splits + it.sp) * (HD + 2);
+            put2(x + 2 + d, a, b);
+            if (d == 0) put2(x, top, sum);
+        }
+    }
+    if (it.splits == 1) return;
+    // the last part of the columns to arrive joins them all
+    int* arrived = (int*)lds;
+    __builtin_amdgcn_s_waitcnt(0);
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        int* counter = p.counters + it.counter;
+        *arrived = __hip_atomic_fetch_add(counter, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == it.splits - 1;
+        if (*arrived) __hip_atomic_store(counter, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    }
+    __syncthreads();
+    const bool mine = *arrived;
+    __syncthreads();  // (*arrived is read; the joining uses its place)
+    if (!mine) return;
+    auto at = [&](int c) { return part + (int64_t)c * it.splits * (HD + 2); };
+    if (2 * items > (int)blockDim.x) {
+        for (int i = threadIdx.x; i < items; i += blockDim.x) {
+            const int c = i / (HD / 2), d = 2 * (i % (HD / 2));
+            const Joined r = join<8>(at(c), HD, d, 0, 1, it.splits);
+            put(c, d, r.a, r.b, r.l);
+        }
+        return;
+    }
+    const int groups = blockDim.x / items, group = threadIdx.x / items, i = threadIdx.x - group * items;
+    const int c = i / (HD / 2), d = 2 * (i % (HD / 2));
+    const Joined r = join_groups<8>(at(c), HD, d, group, groups, items, i, it.splits, (float4*)lds);
+    if (group == 0) put(c, d, r.a, r.b, r.l);
+}
+
+template <int NB, typename T>
+__global__ __launch_bounds__(512) void paged_few_kernel(AttnArgs p) {
+    extern __shared__ __align__(16) uint8_t lds[];
+    few_part<NB, T>(p, blockIdx.x, lds);
+}
+
+// ------------------------------------------------------------------ many columns
+// 32 CW query columns a workgroup, 32 a wave; the keys' tiles go by DMA into LDS as they lie in memory, two buffers, one
+// barrier a step, and are read as operands without bank conflicts (16 bytes a lane in lane order).  SETS sets of CW
+// waves take consecutive ranges of the steps and join through LDS at the end.
+template <int NB, int CW, int SETS>
+struct Wide {
+    static constexpr int HD = 32 * NB, TILE = paged_tile_bytes(HD);
+    static constexpr int KEYS = NB <= 4 && SETS <= 2 ? 64 : 32;  // a step
+    static constexpr int TILES = KEYS / kPagedTile, SIDE = TILES * TILE, BUF = 2 * SIDE;
+    static constexpr int COLS = 32 * CW;
+    static constexpr int JOIN = SETS > 1 ? COLS * (HD + 4) * 4 + COLS * 8 : 0;  // a set's outputs and statistics
+    static constexpr int RING = 2 * SETS * BUF;
+    static constexpr int FEW = few_lds<NB>(CW * SETS);
+    static constexpr int LDS = RING > JOIN ? (RING > FEW ? RING : FEW) : (JOIN > FEW ? JOIN : FEW);
+    static constexpr bool FITS = LDS <= 160 << 10;
+};
+// P enters the products as P 2^9 and a column's reference follows its maximum only when that is 2^6 past it, which
+// few steps are.
+constexpr float kWideLog2P = 9.f, kSlack = 6.f;
+
+template <int NB, int CW, int SETS, typename T>
+__device__ __forceinline__ void wide_part(const AttnArgs& p, uint8_t* lds) {
+    typedef Wide<NB, CW, SETS> W;
+    constexpr bool EXACT = sizeof(T) == 4;
+    constexpr int HD = W::HD, TILE = W::TILE, KT = W::KEYS / 32;
+    const int lane = threadIdx.x & 63, half = lane >> 5, c32 = lane & 31;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), set = wave / CW, wl = wave % CW;
+    const int KVH = p.c.kv_heads, kvh = blockIdx.x % KVH;
+    const PagedItem it = paged_find(blockIdx.x / KVH, p.b.sequences, [&](int s) {
+        const int64_t cols = (int64_t)paged_seq(p.b, s).n * p.G;
+        return cols > p.few_columns ? (int)((cols + W::COLS - 1) / W::COLS) : 0;
+    });
+    if (it.s < 0) return;
+    const int s = __builtin_amdgcn_readfirstlane(it.s);
+    const PagedSeq seq = paged_seq(p.b, s);
+    const int cols = seq.n * p.G, pos0 = seq.length - seq.n;
+    // a sequence's last columns first: they see the most keys
+    const int col0 = ((cols + W::COLS - 1) / W::COLS - 1 - __builtin_amdgcn_readfirstlane(it.i)) * W::COLS;
+    const int first = pos0 + p.by_group(col0), last = pos0 + p.by_group(min(col0 + W::COLS, cols) - 1);
+    const int wcol0 = min(col0 + wl * 32, cols - 1);  // the wave's columns
+    const int w_first = pos0 + p.by_group(wcol0), w_last = pos0 + p.by_group(min(wcol0 + 31, cols - 1));
+    const Steps steps = steps_of(p, first, last, W::KEYS);
+    const int per = (steps.count + SETS - 1) / SETS, f0 = set * per, count = max(0, min(steps.count - f0, per));
+
+    const int col = min(col0 + wl * 32 + c32, cols - 1), t = p.by_group(col), pos = pos0 + t;
+    f16x8 qh[2 * NB], ql[EXACT ? 2 * NB : 1];
+    const T* q = (const T*)p.a.q + (int64_t)(seq.row0 + t) * p.a.q_stride + (int64_t)(kvh * p.G + col - t * p.G) * HD + 8 * half;
+    const float sc = load_queries<2 * NB, 16, T>(q, p.scale_log2, p.whole_q, qh, ql, [](float x) {
+        return xor32_combine(x, MaxOp());
+    });
+    float m = -INFINITY, l = 0.f;
+    f32x16 o[NB];
+#pragma unroll
+    for (int d = 0; d < NB; d++)
+#pragma unroll
+        for (int r = 0; r < 16; r++) o[d][r] = 0.f;
+
+    uint8_t* const ring = lds + set * 2 * W::BUF;
+    const uint32_t ring_at = lds_addr(ring);
+    constexpr int PARTS = 2 * W::TILES * NB;  // KB of a step: of keys, then of values, NB a tile
+    // Starts the loads of the set's step i into buffer i & 1; returns the bits of tiles without a page.
+    auto fetch = [&](int i) {
+        const int tile = steps[min(f0 + i, steps.count - 1)] * W::TILES;  // (past the last: that one, unused)
+        int64_t at[W::TILES];
+        int none = 0;
+#pragma unroll
+        for (int u = 0; u < W::TILES; u++) {
+            if (u == 0 || !((tile + u) & ((1 << p.c.tiles_log2) - 1))) {
+                const int page = page_of(p, s, tile + u);
+                none |= page < 0 ? 1 << u : 0;
+                at[u] = paged_tile(p.c, max(page, 0), kvh, tile + u) * TILE;
+            } else {
+                none |= (none >> (u - 1) & 1) << u;
+                at[u] = at[u - 1] + TILE;
+            }
+        }
+#pragma unroll
+        for (int k = 0; k < (PARTS + CW - 1) / CW; k++) {
+            const int c = wl + CW * k;
+            if (PARTS % CW && c >= PARTS) break;
+            const int side = c / (PARTS / 2), u = c % (PARTS / 2) / NB, part = c % NB;
+            int64_t from = at[0];
+#pragma unroll
+            for (int x = 1; x < W::TILES; x++) from = u == x ? at[x] : from;
+            dma16s((side ? p.c.v : p.c.k) + from + part * 1024, lane * 16,
+                   ring_at + (i & 1) * W::BUF + side * W::SIDE + u * TILE + part * 1024);
+        }
+        return none;
+    };
+    auto work = [&](int i, int none) {
+        const int key0 = steps[f0 + i] * W::KEYS;
+        if (!any_sees(p, w_first, w_last, key0, key0 + W::KEYS - 1)) return;
+        const uint8_t* kb = ring + (i & 1) * W::BUF + (c32 >> 4) * TILE + (half * 16 + (c32 & 15)) * 16;
+        const uint8_t* vb = ring + (i & 1) * W::BUF + W::SIDE + (half * HD + c32) * 16;
+        f32x16 x[KT];  // S(key 32 k + 16 (r / 8) + 8 half + r % 8, column c32)
+#pragma unroll
+        for (int k = 0; k < KT; k++) {
+#pragma unroll
+            for (int r = 0; r < 16; r++) x[k][r] = 0.f;
+#pragma unroll
+            for (int c = 0; c < 2 * NB; c++) {
+                const f16x8 a = *(const f16x8*)(kb + 2 * k * TILE + c * 512);
+                x[k] = mfma32(a, qh[c], x[k]);
+                if constexpr (EXACT) x[k] = mfma32(a, ql[c], x[k]);
+            }
+        }
+        const bool edge = none || !all_see(p, w_first, w_last, key0, key0 + W::KEYS - 1);
+        if (edge) {
+#pragma unroll
+            for (int k = 0; k < KT; k++)
+#pragma unroll
+                for (int r = 0; r < 16; r++) {
+                    if (none >> (2 * k + (r >> 3)) & 1) x[k][r] = NAN;
+                    if (!sees(p, pos, key0 + 32 * k + 16 * (r >> 3) + 8 * half + (r & 7))) x[k][r] = -INFINITY;
+                }
+        }
+        float mx = x[0][0];
+#pragma unroll
+        for (int e = 1; e < 16 * KT; e++) mx = fmaxf(mx, x[e >> 4][e & 15]);
+        mx = xor32_combine(mx, MaxOp());
+        const float mn = mx * sc;  // (sc > 0)
+        if (__builtin_amdgcn_ballot_w64(mn > m + kSlack)) {
+            const float top = fmaxf(m, mn), alpha = __builtin_amdgcn_exp2f(m - (top == -INFINITY ? 0.f : top));
+#pragma unroll
+            for (int d = 0; d < NB; d++) o[d] *= alpha;
+            l *= alpha;
+            m = top;
+        }
+        const float base = exponent_base(x, mx, m == -INFINITY ? 0.f : m, sc, kWideLog2P);
+        f16x8 pf[2 * KT], pg[EXACT ? 2 * KT : 1];
+        float sum = 0.f;
+#pragma unroll
+        for (int u = 0; u < 2 * KT; u++) {
+            f16x2 ph[4], pl[EXACT ? 4 : 1];
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                const float a = __builtin_amdgcn_exp2f(fmaf(x[u >> 1][8 * (u & 1) + 2 * e], sc, base));
+                const float b = __builtin_amdgcn_exp2f(fmaf(x[u >> 1][8 * (u & 1) + 2 * e + 1], sc, base));
+                sum += a + b;
+                ph[e] = round2(a, b);
+                if constexpr (EXACT) pl[e] = round2(rest_low(ph[e], a), rest_high(ph[e], b));
+            }
+            pf[u] = frag(ph[0], ph[1], ph[2], ph[3]);
+            if constexpr (EXACT) pg[u] = frag(pl[0], pl[1], pl[2], pl[3]);
+        }
+        l += sum;
+        if (edge) {
+            // positions that may never have been written: values of 0
+#pragma unroll
+            for (int u = 0; u < 2 * KT; u++) {
+                uint32_t keep[4] = {0u, 0u, 0u, 0u};
+#pragma unroll
+                for (int e = 0; e < 8; e++) {
+                    const int key = key0 + 16 * u + 8 * half + e;
+                    if (!(none >> u & 1) && any_sees(p, w_first, w_last, key, key)) keep[e >> 1] |= 0xFFFFu << (16 * (e & 1));
+                }
+#pragma unroll
+                for (int d = 0; d < NB; d++) {
+                    typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+                    u32x4 v = *(const u32x4*)(vb + u * TILE + d * 512);
+#pragma unroll
+                    for (int e = 0; e < 4; e++) v[e] &= keep[e];
+                    o[d] = mfma32(__builtin_bit_cast(f16x8, v), pf[u], o[d]);
+                    if constexpr (EXACT) o[d] = mfma32(__builtin_bit_cast(f16x8, v), pg[u], o[d]);
+                }
+            }
+        } else {
+#pragma unroll
+            for (int u = 0; u < 2 * KT; u++)
+#pragma unroll
+                for (int d = 0; d < NB; d++) {
+                    const f16x8 v = *(const f16x8*)(vb + u * TILE + d * 512);
+                    o[d] = mfma32(v, pf[u], o[d]);
+                    if constexpr (EXACT) o[d] = mfma32(v, pg[u], o[d]);
+                }
+        }
+    };
+    if (per > 0) {  // (the same for the whole workgroup)
+        int none = fetch(0);
+        for (int i = 0; i < per; i++) {
+            wait_stage_barrier<0>();
+            const int next = i + 1 < per ? fetch(i + 1) : 0;
+            if (i < count) work(i, none);
+            none = next;
+        }
+    }
+    // l: half the keys in either half of the wave
+    l = xor32_combine(l, AddOp());
+    if constexpr (SETS > 1) {
+        float* xo = (float*)lds;
+        float* xml = xo + W::COLS * (HD + 4);
+        const int c = wl * 32 + c32;
+        for (int other = 1; other < SETS; other++) {
+            __syncthreads();
+            if (set == other) {
+#pragma unroll
+                for (int d = 0; d < NB; d++)
+#pragma unroll
+                    for (int u = 0; u < 4; u++)
+                        *(f32x4*)&xo[c * (HD + 4) + 32 * d + 8 * u + 4 * half] =
+                            f32x4{o[d][4 * u], o[d][4 * u + 1], o[d][4 * u + 2], o[d][4 * u + 3]};
+                if (half == 0) {
+                    xml[2 * c] = m;
+                    xml[2 * c + 1] = l;
+                }
+            }
+            __syncthreads();
+            if (set == 0) {
+                const float mo = xml[2 * c], top = fmaxf(m, mo), fa = join_weight(m, top), fb = join_weight(mo, top);
+                m = top;
+                l = l * fa + xml[2 * c + 1] * fb;
+#pragma unroll
+                for (int d = 0; d < NB; d++)
+#pragma unroll
+                    for (int u = 0; u < 4; u++) {
+                        const f32x4 y = *(const f32x4*)&xo[c * (HD + 4) + 32 * d + 8 * u + 4 * half];
+#pragma unroll
+                        for (int r = 0; r < 4; r++) o[d][4 * u + r] = o[d][4 * u + r] * fa + y[r] * fb;
+                    }
+            }
+        }
+        if (set) return;
+    }
+    if (col0 + wl * 32 + c32 >= cols) return;
+    const float inv = inverse(l, pos >= p.most);
+    T* out = (T*)p.a.out + (int64_t)(seq.row0 + t) * p.a.out_stride + (int64_t)(kvh * p.G + col - t * p.G) * HD + 4 * half;
+#pragma unroll
+    for (int d = 0; d < NB; d++)
+#pragma unroll
+        for (int u = 0; u < 4; u++) {
+            typedef T T4 __attribute__((ext_vector_type(4)));
+            T4 y;
+#pragma unroll
+            for (int r = 0; r < 4; r++) y[r] = (T)(o[d][4 * u + r] * inv);
+            if (p.whole_out) {
+                *(AS_GLOBAL T4*)(out + 32 * d + 8 * u) = y;
+            } else {
+#pragma unroll
+                for (int r = 0; r < 4; r++) gptr(out)[32 * d + 8 * u + r] = y[r];
+            }
+        }
+}
+
+// The sequences of many columns, then those of few, in one launch.
+template <int NB, int CW, int SETS, typename T>
+__global__ __launch_bounds__(64 * CW * SETS) void paged_mixed_kernel(AttnArgs p) {
+    extern __shared__ __align__(16) uint8_t lds[];
+    if ((int)blockIdx.x < p.wide_grid) wide_part<NB, CW, SETS, T>(p, lds);
+    else few_part<NB, T>(p, blockIdx.x - p.wide_grid, lds);
+}
+
+template <auto* kernel>
+hipError_t launch_one(const AttnArgs& p, int64_t grid, int threads, int lds, hipStream_t st) {
+    static OncePerDevice once;
+    if (hipError_t e = allow_whole_lds(once, (const void*)kernel)) return e;
+    if (grid <= 0) return hipSuccess;
+    if (grid > INT32_MAX) return hipErrorInvalidConfiguration;
+    kernel<<<(unsigned)grid, threads, lds, st>>>(p);
+    return hipGetLastError();
+}
+
+// Workgroups that the few-column part may need for sequences of up to `cols` columns each.
+int64_t few_grid(const AttnArgs& p, int64_t cols) {
+    const int64_t tight = ((int64_t)p.b.rows * p.G + 15ll * p.b.sequences) / kFewCols;
+    const int64_t most = std::min<int64_t>((int64_t)p.b.rows * ((p.G + kFewCols - 1) / kFewCols),
+                                           std::min(tight, p.b.sequences * ((cols + kFewCols - 1) / kFewCols)));
+    return most * p.c.kv_heads + p.target + 1;
+}
+
+template <int NB, int CW, int SETS, typename T>
+hipError_t launch_mixed(AttnArgs& p, hipStream_t st) {
+    typedef Wide<NB, CW, SETS> W;
+    static_assert(W::FITS, "LDS");
+    p.few_columns = kManyColumns;
+    // sequences of many columns are at most rows G / kManyColumns, each with a group that is not full
+    const int64_t cols = (int64_t)p.b.rows * p.G;
+    const int64_t groups = cols / W::COLS + std::min<int64_t>(p.b.sequences, cols / kManyColumns);
+    if (groups * p.c.kv_heads > INT32_MAX) return hipErrorInvalidConfiguration;
+    p.wide_grid = (int)(groups * p.c.kv_heads);
+    return launch_one<paged_mixed_kernel<NB, CW, SETS, T>>(p, p.wide_grid + few_grid(p, kManyColumns), 64 * CW * SETS,
+                                                          W::LDS, st);
+}
+
+template <int NB, typename T>
+hipError_t launch_nb(AttnArgs& p, hipStream_t st) {
+    const int cus = device_cus();
+    const int64_t cols = (int64_t)p.b.rows * p.G;
+    const int64_t most = p.a.max_rows > 0 ? std::min<int64_t>(p.a.max_rows * (int64_t)p.G, cols) : cols;
+    auto groups = [&](int width) { return (cols + width - 1) / width * p.c.kv_heads; };
+    p.target = std::min(cus, kMostTarget);
+    if constexpr (NB <= 4)
+        if (most > kManyColumns) {
+            if (groups(256) >= cus) return launch_mixed<NB, 8, 1, T>(p, st);
+            if (groups(128) >= cus) return launch_mixed<NB, 4, 2, T>(p, st);
+            if (groups(64) >= cus / 2) return launch_mixed<NB, 2, 4, T>(p, st);
+        }
+    p.few_columns = INT32_MAX;
+    constexpr int waves = 8;
+    return launch_one<paged_few_kernel<NB, T>>(p, few_grid(p, cols), 64 * waves, few_lds<NB>(waves), st);
+}
+
+template <typename T>
+hipError_t launch(AttnArgs& p, hipStream_t st) {
+    switch (p.c.hd / 32) {
+    case 1: return launch_nb<1, T>(p, st);
+    case 2: return launch_nb<2, T>(p, st);
+    case 3: return launch_nb<3, T>(p, st);
+    case 4: return launch_nb<4, T>(p, st);
+    case 5: return launch_nb<5, T>(p, st);
+    case 6: return launch_nb<6, T>(p, st);
+    case 7: return launch_nb<7, T>(p, st);
+    default: return launch_nb<8, T>(p, st);
+    }
+}
+
+}  // namespace
+
+int64_t paged_attention_workspace(int hd) { return kMostTarget * 4 + (int64_t)kMostSlots * kFewCols * (hd + 2) * 4; }
+
+hipError_t launch_paged_attention(bool f16_rows, const PagedAttention& a, const PagedSteps& b, const PagedKV& c,
+                                  hipStream_t st) {
+    AttnArgs p;
+    p.a = a;
+    p.b = b;
+    p.c = c;
+    p.G = a.heads / c.kv_heads;
+    p.most = b.table_stride << (4 + c.tiles_log2);
+    p.by_group = Divisor(p.G);
+    p.scale_log2 = 1.4426950408889634f / sqrtf((float)c.hd);
+    p.counters = (int*)a.workspace;
+    p.partials = (float*)((uint8_t*)a.workspace + kMostTarget * 4);
+    p.wide_grid = 0;
+    const int size = f16_rows ? 2 : 4;
+    auto whole = [&](const void* x, int64_t stride) { return !(((uintptr_t)x | (uint64_t)stride * size) & 15); };
+    p.whole_q = whole(a.q, a.q_stride);
+    p.whole_out = whole(a.out, a.out_stride);
+    return f16_rows ? launch<f16>(p, st) : launch<float>(p, st);
+}

@@ -1,0 +1,351 @@
+// Writing a batch's keys and values into a cache in pages (paged.h), rotated to
+// their positions on the way, with its queries' rotation; and reading them back.
+//
+// A pair of dims (a, b) of a head at position p becomes (a cos - b sin, a sin + b cos)
+// with the table's angle of (p, pair); pairs are adjacent dims or halves of the head.
+//
+// A workgroup of 256 threads takes one tile of 16 positions of a sequence and, over
+// grid.y, as many KV heads as have 16 lanes of 16 dims a token (or that many query
+// heads, a few times): a thread rotates 16 dims of one token, its 8 angles in
+// registers, and turns 8 tokens by 2 dims of the values.  Keys of a tile's 16 tokens
+// are written 256 bytes at a time, values 16 bytes where all 8 tokens are new and 2
+// where a group is only partly so.  Bound by memory, short of the launch for few rows.
+#include "paged.h"
+
+namespace {
+
+constexpr int kThreads = 256;
+
+template <typename T>
+struct Lines;  // 8 dims at once
+template <>
+struct Lines<float> {
+    static __device__ __forceinline__ void load(const float* p, float (&x)[8], bool whole) {
+        if (whole) {
+            const int4 a = gload_i4(p), b = gload_i4(p + 4);
+            const int u[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+#pragma unroll
+            for (int e = 0; e < 8; e++) x[e] = __int_as_float(u[e]);
+        } else {
+#pragma unroll
+            for (int e = 0; e < 8; e++) x[e] = gptr(p)[e];
+        }
+    }
+    static __device__ __forceinline__ void store(float* p, const float (&x)[8], bool whole) {
+        if (whole) {
+            *(AS_GLOBAL f32x4*)p = f32x4{x[0], x[1], x[2], x[3]};
+            *(AS_GLOBAL f32x4*)(p + 4) = f32x4{x[4], x[5], x[6], x[7]};
+        } else {
+#pragma unroll
+            for (int e = 0; e < 8; e++) gptr(p)[e] = x[e];
+        }
+    }
+};
+__device__ __forceinline__ f16x8 rounded(const float (&x)[8]) {
+    return {(f16)x[0], (f16)x[1], (f16)x[2], (f16)x[3], (f16)x[4], (f16)x[5], (f16)x[6], (f16)x[7]};
+}
+template <>
+struct Lines<f16> {
+    static __device__ __forceinline__ void load(const f16* p, float (&x)[8], bool whole) {
+        if (whole) {
+            const f16x8 h = *(const AS_GLOBAL f16x8*)p;
+#pragma unroll
+            for (int e = 0; e < 8; e++) x[e] = (float)h[e];
+        } else {
+#pragma unroll
+            for (int e = 0; e < 8; e++) x[e] = (float)gptr(p)[e];
+        }
+    }
+    static __device__ __forceinline__ void store(f16* p, const float (&x)[8], bool whole) {
+        if (whole) {
+            *(AS_GLOBAL f16x8*)p = rounded(x);
+        } else {
+#pragma unroll
+            for (int e = 0; e < 8; e++) gptr(p)[e] = (f16)x[e];
+        }
+    }
+};
+// Two dims.
+template <typename T>
+__device__ __forceinline__ float2 load_two(const T* p, bool whole) {
+    typedef T T2 __attribute__((ext_vector_type(2)));
+    if (whole) {
+        const T2 x = *(const AS_GLOBAL T2*)p;
+        return make_float2((float)x[0], (float)x[1]);
+    }
+    return make_float2((float)gptr(p)[0], (float)gptr(p)[1]);
+}
+template <typename T>
+__device__ __forceinline__ void store_two(T* p, float a, float b, bool whole) {
+    typedef T T2 __attribute__((ext_vector_type(2)));
+    if (whole) {
+        *(AS_GLOBAL T2*)p = T2{(T)a, (T)b};
+    } else {
+        gptr(p)[0] = (T)a;
+        gptr(p)[1] = (T)b;
+    }
+}
+// An f16 that is a NaN or an infinity.
+__device__ __forceinline__ bool odd16(f16 x) { return (__builtin_bit_cast(uint16_t, x) & 0x7C00u) == 0x7C00u; }
+
+// What a workgroup works on: the tile, and its thread's token of it.
+struct Place {
+    PagedSeq seq;
+    int s, tile, pos0;  // pos0: the position of the sequence's first row
+    __device__ __forceinline__ int row(int pos) const {  // of a position, -1 where it is not new
+        const int i = pos - pos0;
+        return i >= 0 && i < seq.n ? seq.row0 + i : -1;
+    }
+};
+__device__ __forceinline__ bool find_place(const PagedSteps& b, Place& p) {
+    const PagedItem it = paged_find(blockIdx.x, b.sequences, [&](int s) {
+        const PagedSeq q = paged_seq(b, s);
+        // (>> rounds down: rows of negative positions have tiles too)
+        return q.n ? ((q.length - 1) >> 4) - ((q.length - q.n) >> 4) + 1 : 0;
+    });
+    if (it.s < 0) return false;
+    p.s = __builtin_amdgcn_readfirstlane(it.s);
+    p.seq = paged_seq(b, p.s);
+    p.pos0 = p.seq.length - p.seq.n;
+    p.tile = (p.pos0 >> 4) + __builtin_amdgcn_readfirstlane(it.i);
+    return true;
+}
+
+struct AppendArgs {
+    PagedRows r;
+    PagedSteps b;
+    PagedKV c;
+    int kv_slices, passes;            // of grid.y; of a query slice
+    int lanes, at_once;               // 16-dim lanes of a head, heads at once
+    bool q_whole, k_whole, v_whole, out_whole;  // rows that lie on 16 bytes
+};
+
+// The two runs of 8 dims that lane `u` of a head rotates.
+__device__ __forceinline__ void runs(int u, int hd, int interleaved, int (&d)[2]) {
+    d[0] = interleaved ? 16 * u : 8 * u;
+    d[1] = interleaved ? 16 * u + 8 : hd / 2 + 8 * u;
+}
+__device__ __forceinline__ void rotate(float (&x)[2][8], const float2 (&cs)[8], int interleaved) {
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+        float& a = interleaved ? x[i >> 2][2 * (i & 3)] : x[0][i];
+        float& b = interleaved ? x[i >> 2][2 * (i & 3) + 1] : x[1][i];
+        const float y = a * cs[i].x - b * cs[i].y, z = a * cs[i].y + b * cs[i].x;
+        a = y;
+        b = z;
+    }
+}
+
+template <typename T, bool INTERLEAVED>
+__global__ __launch_bounds__(kThreads) void paged_append_kernel(AppendArgs p) {
+    __shared__ uint32_t odd[16];  // a bit a head of the slice: tokens that have no form
+    Place at;
+    if (!find_place(p.b, at)) return;
+    const int hd = p.c.hd, tok = threadIdx.x & 15, u = threadIdx.x >> 4;
+    const int lane = u % p.lanes, sub = u / p.lanes;
+    const int pos = at.tile * 16 + tok, row = at.row(pos);
+    int d[2];
+    runs(lane, hd, INTERLEAVED, d);
+    float2 cs[8];
+    const bool turned = p.r.rope != nullptr;
+    if (turned) {
+        if (pos >= 0 && pos < p.r.rope_positions) {
+            const float2* t = p.r.rope + (int64_t)pos * (hd / 2) + 8 * lane;
+#pragma unroll
+            for (int i = 0; i < 8; i++) cs[i] = gload_f2(t + i);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; i++) cs[i] = make_float2(NAN, NAN);
+        }
+    }
+    if ((int)blockIdx.y >= p.kv_slices) {
+        if (row < 0 || sub >= p.at_once) return;
+        int h = ((int)blockIdx.y - p.kv_slices) * p.at_once * p.passes + sub;
+        for (int i = 0; i < p.passes && h < p.r.heads; i++, h += p.at_once) {
+            const T* q = (const T*)p.r.q + row * p.r.q_stride + (int64_t)h * hd;
+            T* out = (T*)p.r.q_out + row * p.r.q_out_stride + (int64_t)h * hd;
+            float x[2][8];
+            Lines<T>::load(q + d[0], x[0], p.q_whole);
+            Lines<T>::load(q + d[1], x[1], p.q_whole);
+            if (turned) rotate(x, cs, INTERLEAVED);
+            Lines<T>::store(out + d[0], x[0], p.out_whole);
+            Lines<T>::store(out + d[1], x[1], p.out_whole);
+        }
+        return;
+    }
+    const int page = paged_page(p.b, p.c, at.s, at.tile);  // (the same for the whole workgroup)
+    if (page < 0) return;
+    if (threadIdx.x < 16) odd[threadIdx.x] = 0;
+    __syncthreads();
+    const int h0 = blockIdx.y * p.at_once, kvh = h0 + sub;
+    const bool mine = row >= 0 && sub < p.at_once && kvh < p.c.kv_heads;
+    f16x8 key[2];
+    if (mine) {
+        const T* k = (const T*)p.r.k + row * p.r.k_stride + (int64_t)kvh * hd;
+        float x[2][8];
+        Lines<T>::load(k + d[0], x[0], p.k_whole);
+        Lines<T>::load(k + d[1], x[1], p.k_whole);
+        if (turned) rotate(x, cs, INTERLEAVED);
+        key[0] = rounded(x[0]);
+        key[1] = rounded(x[1]);
+        bool bad = false;
+#pragma unroll
+        for (int e = 0; e < 8; e++) bad = bad || odd16(key[0][e]) || odd16(key[1][e]);
+        if (bad) atomicOr(&odd[tok], 1u << sub);
+    }
+    // values: 2 dims of 8 tokens a thread
+    const int pairs = hd / 2, vi = threadIdx.x;
+    const int vsub = vi / (2 * pairs), half = (vi / pairs) & 1, dim = 2 * (vi % pairs);
+    const int vh = h0 + vsub, vpos = at.tile * 16 + 8 * half;
+    const bool values = vsub < p.at_once && vh < p.c.kv_heads;
+    f16x8 va = {}, vb = {};
+    int fresh = 0;
+    if (values) {
+        float2 x[8];
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+            const int r = at.row(vpos + e);
+            x[e] = make_float2(0.f, 0.f);
+            if (r < 0) continue;
+            fresh |= 1 << e;
+            x[e] = load_two((const T*)p.r.v + r * p.r.v_stride + (int64_t)vh * hd + dim, p.v_whole);
+        }
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+            va[e] = (f16)x[e].x;
+            vb[e] = (f16)x[e].y;
+            if (odd16(va[e]) || odd16(vb[e])) atomicOr(&odd[8 * half + e], 1u << vsub);
+        }
+    }
+    __syncthreads();
+    if (mine) {
+        if (odd[tok] >> sub & 1) {
+#pragma unroll
+            for (int e = 0; e < 8; e++) key[0][e] = key[1][e] = (f16)NAN;
+        }
+        uint8_t* t = p.c.k + paged_tile(p.c, page, kvh, at.tile) * paged_tile_bytes(hd) + paged_key_slot(tok) * 16;
+        *(AS_GLOBAL f16x8*)(t + d[0] / 8 * 256) = key[0];
+        *(AS_GLOBAL f16x8*)(t + d[1] / 8 * 256) = key[1];
+    }
+    if (values && fresh) {
+#pragma unroll
+        for (int e = 0; e < 8; e++)
+            if (odd[8 * half + e] >> vsub & 1) va[e] = vb[e] = (f16)0.f;
+        f16* t = (f16*)(p.c.v + paged_tile(p.c, page, vh, at.tile) * paged_tile_bytes(hd)) + (half * hd + dim) * 8;
+        if (fresh == 255) {
+            *(AS_GLOBAL f16x8*)t = va;
+            *(AS_GLOBAL f16x8*)(t + 8) = vb;
+        } else {
+#pragma unroll
+            for (int e = 0; e < 8; e++)
+                if (fresh >> e & 1) {
+                    gptr(t)[e] = va[e];
+                    gptr(t)[8 + e] = vb[e];
+                }
+        }
+    }
+}
+
+struct LoadArgs {
+    PagedSteps b;
+    PagedKV c;
+    void *k, *v;
+    int64_t k_stride, v_stride;
+    int lanes, at_once;
+    bool k_whole, v_whole;
+};
+
+template <typename T>
+__global__ __launch_bounds__(kThreads) void paged_load_kernel(LoadArgs p) {
+    Place at;
+    if (!find_place(p.b, at)) return;
+    const int hd = p.c.hd, tok = threadIdx.x & 15, u = threadIdx.x >> 4;
+    const int lane = u % p.lanes, sub = u / p.lanes, h0 = blockIdx.y * p.at_once;
+    const int page = paged_page(p.b, p.c, at.s, at.tile);  // (-1: NaN)
+    const int kvh = h0 + sub, row = at.row(at.tile * 16 + tok);
+    if (p.k && row >= 0 && sub < p.at_once && kvh < p.c.kv_heads) {
+        const uint8_t* t = p.c.k + paged_tile(p.c, max(page, 0), kvh, at.tile) * paged_tile_bytes(hd) + paged_key_slot(tok) * 16;
+        T* out = (T*)p.k + row * p.k_stride + (int64_t)kvh * hd + 16 * lane;
+#pragma unroll
+        for (int i = 0; i < 2; i++) {
+            float x[8];
+            const f16x8 y = *(const AS_GLOBAL f16x8*)(t + (2 * lane + i) * 256);
+#pragma unroll
+            for (int e = 0; e < 8; e++) x[e] = page < 0 ? NAN : (float)y[e];
+            Lines<T>::store(out + 8 * i, x, p.k_whole);
+        }
+    }
+    const int pairs = hd / 2, vsub = threadIdx.x / (2 * pairs), half = (threadIdx.x / pairs) & 1;
+    const int dim = 2 * (threadIdx.x % pairs), vh = h0 + vsub;
+    if (!p.v || vsub >= p.at_once || vh >= p.c.kv_heads) return;
+    const int64_t tile = paged_tile(p.c, max(page, 0), vh, at.tile) * paged_tile_bytes(hd);
+    const f16* t = (const f16*)(p.c.v + tile) + (half * hd + dim) * 8;
+    const f16x8 a = *(const AS_GLOBAL f16x8*)t, b = *(const AS_GLOBAL f16x8*)(t + 8);
+    uint16_t key[8];  // a token without a form has NaN keys
+#pragma unroll
+    for (int e = 0; e < 8; e++) key[e] = gptr((const uint16_t*)(p.c.k + tile))[paged_key_slot(8 * half + e) * 8];
+#pragma unroll
+    for (int e = 0; e < 8; e++) {
+        const int r = at.row(at.tile * 16 + 8 * half + e);
+        if (r < 0) continue;
+        const bool no = page < 0 || odd16(__builtin_bit_cast(f16, key[e]));
+        store_two((T*)p.v + r * p.v_stride + (int64_t)vh * hd + dim, no ? NAN : (float)a[e], no ? NAN : (float)b[e],
+                  p.v_whole);
+    }
+}
+
+bool whole(const void* p, int64_t stride, int size) { return !(((uintptr_t)p | (uint64_t)stride * size) & 15); }
+
+// Tiles that the batch can touch: a sequence of n new tokens lies in (n + 30) / 16 at most, and in n.
+unsigned tiles_bound(const PagedSteps& b) {
+    const int64_t t = ((int64_t)b.rows + 30ll * b.sequences) / 16;
+    return (unsigned)(t < b.rows ? t : b.rows);
+}
+
+}  // namespace
+
+hipError_t launch_paged_append(bool f16_rows, const PagedRows& r, const PagedSteps& b, const PagedKV& c, hipStream_t st) {
+    AppendArgs p;
+    const int size = f16_rows ? 2 : 4;
+    p.r = r;
+    p.b = b;
+    p.c = c;
+    p.lanes = c.hd / 16;
+    p.at_once = 16 / p.lanes;
+    p.kv_slices = (c.kv_heads + p.at_once - 1) / p.at_once;
+    p.passes = 1;
+    p.q_whole = whole(r.q, r.q_stride, size);
+    p.k_whole = whole(r.k, r.k_stride, size);
+    p.v_whole = whole(r.v, r.v_stride, size);
+    p.out_whole = whole(r.q_out, r.q_out_stride, size);
+    const int per = p.at_once * p.passes;
+    const dim3 grid(tiles_bound(b), p.kv_slices + (r.heads + per - 1) / per);
+    if (f16_rows) {
+        if (r.interleaved) paged_append_kernel<f16, true><<<grid, kThreads, 0, st>>>(p);
+        else paged_append_kernel<f16, false><<<grid, kThreads, 0, st>>>(p);
+    } else {
+        if (r.interleaved) paged_append_kernel<float, true><<<grid, kThreads, 0, st>>>(p);
+        else paged_append_kernel<float, false><<<grid, kThreads, 0, st>>>(p);
+    }
+    return hipGetLastError();
+}
+
+hipError_t launch_paged_load(bool f16_rows, const PagedSteps& b, const PagedKV& c, void* k, int64_t k_stride, void* v,
+                             int64_t v_stride, hipStream_t st) {
+    LoadArgs p;
+    const int size = f16_rows ? 2 : 4;
+    p.b = b;
+    p.c = c;
+    p.k = k;
+    p.v = v;
+    p.k_stride = k_stride;
+    p.v_stride = v_stride;
+    p.lanes = c.hd / 16;
+    p.at_once = 16 / p.lanes;
+    p.k_whole = whole(k, k_stride, size);
+    p.v_whole = whole(v, v_stride, size);
+    const dim3 grid(tiles_bound(b), (c.kv_heads + p.at_once - 1) / p.at_once);
+    if (f16_rows) paged_load_kernel<f16><<<grid, kThreads, 0, st>>>(p);
+    else paged_load_kernel<float><<<grid, kThreads, 0, st>>>(p);
+    return hipGetLastError();
+}

@@ -5,28 +5,13 @@
 
 #include <algorithm>
 #include <cmath>
-#include <string>
 
-#include "../../include/alpaca_hip.h"
-#include "host.h"
+#include "checks.h"
 
 namespace {
 
-int bad(const std::string& what) { return ahip_fail(AHIP_ERR_INVALID_ARGUMENT, what); }
-
-int launched(hipError_t e) {
-    if (e == hipSuccess) return AHIP_OK;
-    (void)hipGetLastError();
-    return ahip_fail(AHIP_ERR_COMMAND_FAILED, std::string("kernel launch: ") + hipGetErrorString(e));
-}
-
 // Head counts and dims, and the sizes that the kernels' grids and 32-bit token indexes hold.
 constexpr int kMostHeads = 65535, kMostTokens = 1 << 30;
-
-int check_dim(int hd) {
-    if (hd <= 0 || hd % 32 || hd > 256) return bad("head dimension must be a multiple of 32 up to 256");
-    return AHIP_OK;
-}
 
 int check_shape(int kv_heads, int hd, int capacity) {
     if (kv_heads <= 0 || kv_heads > kMostHeads || capacity <= 0 || capacity > kMostTokens) return bad("cache shape");
@@ -39,35 +24,12 @@ int check_cache(const ahip_kv_q4* c) {
     return check_shape(c->kv_heads, c->head_dim, c->capacity);
 }
 
-int check_dtype(int dtype) {
-    if (dtype != AHIP_F32 && dtype != AHIP_F16) return bad("rows must be f32 or f16");
-    return AHIP_OK;
-}
-
-// Rows of `width` elements, `stride` elements apart.
-int check_rows(const char* what, const void* p, int64_t stride, int64_t width, int dtype) {
-    if (!p) return bad(std::string("null ") + what);
-    if ((uintptr_t)p % (dtype == AHIP_F32 ? 4 : 2)) return bad(std::string(what) + ": misaligned");
-    if (stride < width) return bad(std::string(what) + ": stride below the row's width");
-    if (stride > (int64_t)1 << 32) return bad(std::string(what) + ": implausibly large stride");
-    return AHIP_OK;
-}
-
 // start .. start + tokens inside the capacity; a start on the device is checked there.
 int check_range(int start, const int32_t* start_dev, int tokens, int capacity) {
     if (tokens < 0 || tokens > capacity) return bad("more tokens than the cache holds");
     if (start_dev) return (uintptr_t)start_dev & 3 ? bad("misaligned start_dev") : (int)AHIP_OK;
     if (start < 0 || start > capacity - tokens)
-        return bad("positions " + std::to_string(start) + " to " + std::to_string((int64_t)start + tokens) +
-                   " exceed the capacity " + std::to_string(capacity));
-    return AHIP_OK;
-}
-
-int stream_of(ahip_context* ctx, ahip_stream* stream, hipStream_t* out) {
-    if (stream && stream->device != ctx->device) return bad("stream and context belong to different devices");
-    (void)hipGetLastError();  // a launch's own failure is read back through it
-    if (hipSetDevice(ctx->device) != hipSuccess) return ahip_fail(AHIP_ERR_COMMAND_FAILED, "hipSetDevice");
-    *out = stream ? stream->st : ctx->stream;
+        return bad("positions %d to %lld exceed the capacity %d", start, (long long)start + tokens, capacity);
     return AHIP_OK;
 }
 
@@ -128,7 +90,7 @@ static int check_queries(const ahip_kv_q4* c, int tokens, int heads) {
     if (heads <= 0 || heads > kMostHeads || heads % c->kv_heads)
         return bad("query heads must be a multiple of the KV heads");
     if (tokens < 0 || tokens > c->capacity) return bad("more tokens than the cache holds");
-    if ((int64_t)tokens * heads > kMostTokens) return ahip_fail(AHIP_ERR_UNSUPPORTED, "more than 2^30 queries a call");
+    if ((int64_t)tokens * heads > kMostTokens) return failed(AHIP_ERR_UNSUPPORTED, "more than 2^30 queries a call");
     return AHIP_OK;
 }
 
@@ -176,8 +138,8 @@ extern "C" int ahip_attention_q4(ahip_context* ctx, const ahip_kv_q4* cache, int
     const Q4Plan plan = plan_of(cache, dtype, tokens, heads, start, start_dev);
     const int64_t need = q4_attention_workspace(tokens, heads, cache->head_dim, plan);
     if (need && (!workspace || workspace_bytes < need || ((uintptr_t)workspace & 15)))
-        return bad("the attention needs " + std::to_string(need) + " bytes of 16-byte aligned workspace, got " +
-                   std::to_string(workspace ? workspace_bytes : 0));
+        return bad("the attention needs %lld bytes of 16-byte aligned workspace, got %lld", (long long)need,
+                   workspace ? (long long)workspace_bytes : 0);
     Q4Attention a;
     a.q = q;
     a.out = out;
@@ -199,7 +161,7 @@ extern "C" int ahip_qk_norm_rope(ahip_context* ctx, const ahip_norm_rope* args, 
     if (n.heads < 0 || n.heads > kMostHeads || n.kv_heads < 0 || n.kv_heads > kMostHeads) return bad("head counts");
     if (n.tokens < 0 || n.tokens > kMostTokens) return bad("token count");
     if ((int64_t)n.tokens * (n.heads + n.kv_heads) > kMostTokens)
-        return ahip_fail(AHIP_ERR_UNSUPPORTED, "more than 2^30 heads a call");
+        return failed(AHIP_ERR_UNSUPPORTED, "more than 2^30 heads a call");
     if ((n.q_gain || n.k_gain) && !(n.eps >= 0 && std::isfinite(n.eps))) return bad("eps must be finite and >= 0");
     if (((uintptr_t)n.q_gain | (uintptr_t)n.k_gain) & 3) return bad("misaligned gain");
     if (n.rope) {

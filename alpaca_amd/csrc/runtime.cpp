@@ -26,6 +26,7 @@
 #include "common.h"
 #include "host.h"
 #include "kv_q4.h"
+#include "logprobs.h"
 
 // ------------------------------------------------------------------ errors
 
@@ -706,6 +707,8 @@ struct ahip_session {
     int prefill_generic_attention = 0, prefill_f32_gemm = 0;
     bool logits_ready = false;  // `logits` holds the last forward's logits (for ahip_session_sample)
     DevBuf sample_idx, sample_p, sample_out;  // sampler scratch, allocated on first use
+    DevBuf logprobs;                          // workspace and results of ahip_session_logprobs, likewise
+    bool logprobs_clear = false;              // the workspace has been cleared
     hipStream_t stream = nullptr;
     // Streams of a split prefill (part 0 on `stream`, the other part on the
     // device's split stream, shared by all sessions) and this session's events:
@@ -2056,6 +2059,56 @@ extern "C" int ahip_session_sample(ahip_session* s, float temperature, int top_k
     return run_sample(s->logits.as<float>(), s->m->c.vocab_size, temperature, top_k, top_p, u, s->sample_idx,
                       s->sample_p, s->sample_out, s->stream, token);
 }
+
+extern "C" int ahip_session_logprobs(ahip_session* s, int32_t token, int top, float* logprob, float* entropy,
+                                     int32_t* top_tokens, float* top_logprobs) {
+    if (!s) return fail(AHIP_ERR_INVALID_ARGUMENT, "null argument");
+    drop_stale_error();
+    const int vocab = s->m->c.vocab_size;
+    if (token < 0 || token >= vocab) return fail(AHIP_ERR_INVALID_ARGUMENT, "token id outside vocabulary");
+    if (top < 0 || top > kLogprobsMostTop || top > vocab) return fail(AHIP_ERR_INVALID_ARGUMENT, "count of top tokens");
+    if (top && (!top_tokens || !top_logprobs)) return fail(AHIP_ERR_INVALID_ARGUMENT, "null top outputs");
+    BusyGuard guard(s);
+    if (!guard.ok) return fail(AHIP_ERR_BUSY, "session is already executing a forward pass");
+    if (!s->logits_ready) return fail(AHIP_ERR_INVALID_ARGUMENT, "no logits: call forward or decode first");
+    HIP_OR(hipSetDevice(s->m->device), "hipSetDevice");
+    struct Results {
+        int32_t token;
+        float logprob, entropy;
+        int32_t top_tokens[kLogprobsMostTop];
+        float top_logprobs[kLogprobsMostTop];
+    } host = {};
+    const int64_t work = logprobs_workspace();
+    if (!s->logprobs_clear) {
+        if (!s->logprobs.p)
+            if (int rc = s->logprobs.alloc(work + sizeof(Results))) return rc;
+        HIP_OR(hipMemsetAsync(s->logprobs.p, 0, work, s->stream), "clear workspace");
+        s->logprobs_clear = true;
+    }
+    auto* dev = (Results*)((uint8_t*)s->logprobs.p + work);
+    host.token = token;
+    HIP_OR(hipMemcpyAsync(&dev->token, &host.token, 4, hipMemcpyHostToDevice, s->stream), "token upload");
+    LogprobsArgs a;
+    a.logits = s->logits.p;
+    a.stride = vocab;
+    a.rows = 1;
+    a.vocab = vocab;
+    a.top = top;
+    a.tokens = &dev->token;
+    a.logprobs = &dev->logprob;
+    a.entropy = &dev->entropy;
+    a.top_tokens = dev->top_tokens;
+    a.top_logprobs = dev->top_logprobs;
+    LAUNCH(launch_logprobs(false, a, s->logprobs.p, s->stream));
+    HIP_OR(hipMemcpyAsync(&host, dev, sizeof(host), hipMemcpyDeviceToHost, s->stream), "log probabilities download");
+    HIP_OR(hipStreamSynchronize(s->stream), "log probabilities");
+    if (logprob) *logprob = host.logprob;
+    if (entropy) *entropy = host.entropy;
+    std::copy(host.top_tokens, host.top_tokens + top, top_tokens);
+    std::copy(host.top_logprobs, host.top_logprobs + top, top_logprobs);
+    return AHIP_OK;
+}
+
 extern "C" int ahip_session_length(const ahip_session* s, int* v) {
     if (!s || !v) return fail(AHIP_ERR_INVALID_ARGUMENT, "null argument");
     *v = s->length;

@@ -222,6 +222,15 @@ class HIPLlamaSession:
         L.check(L.lib().ahip_session_sample(self.handle, temperature, top_k, top_p, u, C.byref(r)))
         return r.value
 
+    def logprobs(self, token: int, top: int = 0):
+        """(log probability of ``token``, entropy, [(token, log probability)] of the ``top`` likeliest) under the last
+        forward/decode logits (ahip_session_logprobs)."""
+        lp, entropy = C.c_float(), C.c_float()
+        tokens, lps = np.empty(max(top, 1), np.int32), np.empty(max(top, 1), np.float32)
+        L.check(L.lib().ahip_session_logprobs(self.handle, token, top, C.byref(lp), C.byref(entropy),
+                                              tokens.ctypes.data_as(L.ip), lps.ctypes.data_as(L.fp)))
+        return lp.value, entropy.value, [(int(t), float(x)) for t, x in zip(tokens[:max(top, 0)], lps)]
+
     def reset(self) -> None:
         L.check(L.lib().ahip_session_reset(self.handle))
         self.gpu_seconds = 0.0

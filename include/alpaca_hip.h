@@ -282,6 +282,10 @@ int ahip_session_decode_greedy(ahip_session* s, int32_t start, int max_steps, in
  * (:21-25).  NaN logits are AHIP_ERR_INVALID_ARGUMENT (the Swift code throws).
  * After a greedy chain or a reset there are no logits to sample. */
 int ahip_session_sample(ahip_session* s, float temperature, int top_k, float top_p, double u, int32_t* token);
+/* No counterpart in the reference: ahip_token_logprobs of the same logits, for a token (the sampled one, say) and
+ * the `top` likeliest, into host memory; any output may be null, the top ones if top is 0. */
+int ahip_session_logprobs(ahip_session* s, int32_t token, int top, float* logprob, float* entropy,
+                          int32_t* top_tokens, float* top_logprobs);
 
 int ahip_session_reset(ahip_session* s);
 int ahip_session_length(const ahip_session* s, int* length);
@@ -451,6 +455,126 @@ int ahip_qk_norm_rope(ahip_context* ctx, const ahip_norm_rope* args, ahip_stream
 /* The table, into host memory: angles in double, rounded once to float (CPUOps.rope,
  * CPUOps.swift:196-201); positions * head_dim floats. */
 int ahip_rope_table(int positions, int head_dim, float theta, float* table);
+
+/* ------------------------------------------------------------ KV cache in pages
+ * No counterpart in the reference.  One layer's f16 KV cache for many sequences at
+ * once: pages of page_tokens tokens, which a table gives to every sequence in the
+ * order of its positions, and the operators of a step over a batch of them.  As
+ * with the 4-bit cache, every call takes device pointers, queues its kernels on
+ * `stream` (null: the context stream) without waiting, allocates nothing and may be
+ * captured into a HIP graph; `dtype` is the type of the rows, AHIP_F32 or AHIP_F16,
+ * a row one token's heads side by side, [heads][head_dim], `*_stride` elements from
+ * one to the next.  head_dim is a multiple of 32 up to 256, page_tokens a power of
+ * two from 16 to 1024.
+ *
+ * A cache's k and v are buffers of ahip_paged_kv_bytes each, 16-byte aligned, laid
+ * out for the kernels within a page (ahip_paged_load gives the values); page i is
+ * the i-th of `pages` equal parts of either, so that a page is copied by copying
+ * those bytes.  They need no clearing: only positions that were written are read. */
+typedef struct {
+    void* k;
+    void* v;
+    int32_t kv_heads, head_dim, page_tokens, pages;
+} ahip_paged_kv;
+/* Bytes of a cache's k, and of its v. */
+int ahip_paged_kv_bytes(int kv_heads, int head_dim, int page_tokens, int pages, int64_t* bytes);
+
+/* A step's batch.  The arrays are on the device and are read when the kernels run.
+ * Sequence s has rows row_starts[s] .. row_starts[s + 1] - 1 of the `rows` there
+ * are, its new tokens, the last ones of its lengths[s] (these included): its i-th row
+ * has position lengths[s] - its rows + i.  A sequence may have none; rows that belong to no
+ * sequence (behind the last, say) are neither read nor written.  Position p lies in
+ * page table[s * table_stride + p / page_tokens]; entries that no query sees and no row
+ * is written to may hold anything.  Two sequences may share a page (a common beginning), but
+ * positions that are written belong to one row.
+ *
+ * max_rows says how many rows a sequence has at most, 0 if that is not known; it chooses
+ * between kernels and changes no result beyond rounding.
+ *
+ * Row starts must not fall.  A row of a negative position (more rows than the length
+ * says) stores nothing and sees nothing.  A position past the table's row, or in a page
+ * below 0 or past the last, stores nothing; a query that sees one gets NaN. */
+typedef struct {
+    const int32_t* row_starts; /* [sequences + 1] */
+    const int32_t* lengths;    /* [sequences] */
+    const int32_t* table;      /* [sequences][table_stride] */
+    int32_t sequences, table_stride, rows, max_rows;
+} ahip_paged_batch;
+
+/* Writes the batch's keys and values, rotated to their positions and rounded to f16,
+ * and its queries' rotation, in one launch; other positions keep their bytes.  rope is a
+ * table as ahip_rope_table makes it (null: no rotation; a position outside it gets NaN); values
+ * are not rotated.  heads 0: no queries.  q_out may be q with the same stride, or else may
+ * not overlap an input.
+ * A token whose keys or values of a KV head, in f16, hold a NaN or an infinity (a magnitude
+ * past 65,504) reads back as NaN in that head, keys and values, and gives NaN to the
+ * queries that see it and to no others. */
+typedef struct {
+    const void* q;     /* rows [rows][heads][head_dim] */
+    void* q_out;
+    const void* k;     /* rows [rows][kv_heads][head_dim] */
+    const void* v;
+    int64_t q_stride, q_out_stride, k_stride, v_stride;
+    const float* rope; /* (cos, sin) [rope_positions][head_dim / 2] */
+    int32_t rope_positions, interleaved, dtype, heads;
+} ahip_paged_rows;
+int ahip_paged_append(ahip_context* ctx, const ahip_paged_kv* cache, const ahip_paged_batch* batch,
+                      const ahip_paged_rows* rows, ahip_stream* stream);
+/* The cache's values at the positions of the batch's rows, as rows (NaN where a position
+ * has no page); k or v may be null. */
+int ahip_paged_load(ahip_context* ctx, const ahip_paged_kv* cache, const ahip_paged_batch* batch, int dtype, void* k,
+                    int64_t k_stride, void* v, int64_t v_stride, ahip_stream* stream);
+/* Causal grouped-query attention (as ahip_op_attention) of the batch's queries over the
+ * cache, which already holds their keys and values.  With window > 0 a query at position
+ * p sees the positions p - window + 1 .. p and 0 .. sinks - 1 of those up to p; pages of
+ * other positions are not read, and may be another sequence's by then.  A query that sees nothing gets
+ * zeros.  out may not overlap q.
+ *
+ * The cached keys and values enter the products exactly, sums are float32.  With
+ * AHIP_F32 a query's value is held to 2^-22 of itself or 2^-24 of the largest in its
+ * head, a probability to 2^-22 of itself or 2^-33 of its row's largest, whichever is
+ * more; with AHIP_F16 probabilities are rounded to f16.
+ *
+ * `workspace` (16-byte aligned, ahip_paged_attention_workspace bytes, which depends on the
+ * cache's head_dim only) holds the partial results of key ranges and the counters of their
+ * arrival.  Its first AHIP_PAGED_WORKSPACE_ZERO bytes are zero before its first call,
+ * and every call leaves them so: clear them once, and let one workspace serve any calls that
+ * come one after another.  Calls that may run at the same time, captured graphs among them,
+ * need workspaces of their own. */
+#define AHIP_PAGED_WORKSPACE_ZERO 4096
+int ahip_paged_attention_workspace(const ahip_paged_kv* cache, int64_t* bytes);
+int ahip_paged_attention(ahip_context* ctx, const ahip_paged_kv* cache, const ahip_paged_batch* batch, int dtype,
+                         const void* q, int64_t q_stride, int heads, int window, int sinks, void* out,
+                         int64_t out_stride, void* workspace, int64_t workspace_bytes, ahip_stream* stream);
+
+/* ------------------------------------------------------------ log probabilities
+ * No counterpart in the reference.  Of rows of logits (AHIP_F32 or AHIP_F16) on the
+ * device, row r `stride` elements from row r - 1: the log probability of tokens[r] under
+ * their softmax (NaN for a token outside the vocabulary), the entropy in nats, and the
+ * `top` likeliest tokens (larger logits first, the lower index of equal ones, NaN behind every
+ * number) with their log probabilities.  logprobs (with tokens), entropy or the top arrays (top 0) may be null.
+ * A masked token's logit is -inf.  A row that holds a NaN or +inf, or nothing above -inf, has NaN for every
+ * probability and entropy.  Sums are float32.
+ *
+ * Queued on `stream` (null: the context stream) without waiting; allocates nothing.
+ * `workspace` (16-byte aligned, ahip_token_logprobs_workspace bytes) lets few rows be split over
+ * the device; null: a row is one workgroup's.  Its first AHIP_LOGPROBS_WORKSPACE_ZERO bytes are zero before
+ * its first call, and every call leaves them so; calls that may run at the same time need their own. */
+#define AHIP_LOGPROBS_MOST_TOP 32
+#define AHIP_LOGPROBS_WORKSPACE_ZERO 2048
+typedef struct {
+    const void* logits;
+    int64_t stride;
+    const int32_t* tokens;  /* [rows] */
+    float* logprobs;        /* [rows] */
+    float* entropy;         /* [rows] */
+    int32_t* top_tokens;    /* [rows][top] */
+    float* top_logprobs;    /* [rows][top] */
+    int32_t dtype, rows, vocab, top;
+} ahip_logprobs;
+int ahip_token_logprobs_workspace(int64_t* bytes);
+int ahip_token_logprobs(ahip_context* ctx, const ahip_logprobs* args, void* workspace, int64_t workspace_bytes,
+                        ahip_stream* stream);
 
 /* Host block quantiser, Quantization.swift:39-73 (ggml quantize_row_*_ref):
  * count must be a multiple of 32; writes count/32 blocks into out. */
