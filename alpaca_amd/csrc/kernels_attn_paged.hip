@@ -44,7 +44,8 @@ struct AttnArgs {
 };
 
 constexpr int kFewCols = 16, kFewStep = 32;
-constexpr int kFewLeast = 16;      // steps of a workgroup, where columns are split
+constexpr int kFewLeast = 8;       // steps of a workgroup, where columns are split
+constexpr int kFewWaves = 4;       // of a workgroup of the few-column part alone
 constexpr int kManyColumns = 64;   // sequences of more columns take the many-column part
 constexpr int kMostTarget = kPagedCounters;       // split groups of columns at most
 constexpr int kMostSlots = 2 * kMostTarget + 64;  // their parts
@@ -233,19 +234,33 @@ __device__ __forceinline__ void few_part(const AttnArgs& p, int w, uint8_t* lds)
     const int t0 = per * it.sp + min(it.sp, more), t1 = t0 + per + (it.sp < more);
 
     const uint8_t *kbase = p.c.k + (g * 16 + (lane & 7)) * 16, *vbase = p.c.v + ((g & 1) * HD + c16) * 16;
-    auto load = [&](FewTile<NB>& x, int i) {
+    constexpr bool AHEAD = NB <= 4;  // two tiles in registers, where those allow; else one, refilled as it is used
+    struct Place {
+        const uint8_t *k, *v;
+        int none;
+    };
+    auto place = [&](int i) {
         const int tile = 2 * steps[min(i, t1 - 1)];  // (past the last step: that one, unused)
         const int pa = page_of(p, it.s, tile), pb = p.c.tiles_log2 ? pa : page_of(p, it.s, tile + 1);
-        x.none = (pa < 0) | (pb < 0) << 1;
         const int64_t a = paged_tile(p.c, max(pa, 0), it.kvh, tile) * TILE;
         const int64_t b = paged_tile(p.c, max(pb, 0), it.kvh, tile + 1) * TILE;
-        const uint8_t *k = kbase + (lane & 8 ? b : a), *v = vbase + (lane & 32 ? b : a);
+        return Place{kbase + (lane & 8 ? b : a), vbase + (lane & 32 ? b : a), (pa < 0) | (pb < 0) << 1};
+    };
+    auto load_k = [&](FewTile<NB>& x, const Place& at) {
 #pragma unroll
         for (int s = 0; s < 2; s++)
 #pragma unroll
-            for (int c = 0; c < NB; c++) x.k[s][c] = *(const AS_GLOBAL f16x8*)(k + c * 1024 + s * 128);
+            for (int c = 0; c < NB; c++) x.k[s][c] = *(const AS_GLOBAL f16x8*)(at.k + c * 1024 + s * 128);
+    };
+    auto load_v = [&](FewTile<NB>& x, const Place& at) {
+        x.none = at.none;
 #pragma unroll
-        for (int d = 0; d < 2 * NB; d++) x.v[d] = *(const AS_GLOBAL f16x8*)(v + d * 256);
+        for (int d = 0; d < 2 * NB; d++) x.v[d] = *(const AS_GLOBAL f16x8*)(at.v + d * 256);
+    };
+    auto load = [&](FewTile<NB>& x, int i) {
+        const Place at = place(i);
+        load_k(x, at);
+        load_v(x, at);
     };
     FewTile<NB> xa, xb;
     int j = t0 + wave;
@@ -272,6 +287,11 @@ __device__ __forceinline__ void few_part(const AttnArgs& p, int w, uint8_t* lds)
                 sa[s] = mfma(x.k[s][c], qh[c], sa[s]);
                 if constexpr (EXACT) sa[s] = mfma(x.k[s][c], ql[c], sa[s]);
             }
+        }
+        Place next;
+        if constexpr (!AHEAD) {
+            next = place(i + waves);
+            load_k(x, next);
         }
         const int key0 = steps[i] * kFewStep;
         if (x.none || !all_see(p, first, last, key0, key0 + kFewStep - 1)) {
@@ -324,14 +344,19 @@ __device__ __forceinline__ void few_part(const AttnArgs& p, int w, uint8_t* lds)
             o[d] = mfma(x.v[d], pf, o[d]);
             if constexpr (EXACT) o[d] = mfma(x.v[d], frag(pl[0], pl[1], pl[2], pl[3]), o[d]);
         }
+        if constexpr (!AHEAD) load_v(x, next);
     };
-    if (j + waves < t1) load(xb, j + waves);
-    for (; j < t1; j += 2 * waves) {
-        step(xa, j);
-        if (j + waves >= t1) break;
-        load(xa, j + 2 * waves);
-        step(xb, j + waves);
-        load(xb, j + 3 * waves);
+    if constexpr (AHEAD) {
+        if (j + waves < t1) load(xb, j + waves);
+        for (; j < t1; j += 2 * waves) {
+            step(xa, j);
+            if (j + waves >= t1) break;
+            load(xa, j + 2 * waves);
+            step(xb, j + waves);
+            load(xb, j + 3 * waves);
+        }
+    } else {
+        for (; j < t1; j += waves) step(xa, j);
     }
 
     // o[d][r] = O(column c16, dim 16 d + 4 g + r); the waves' results meet in LDS
@@ -403,23 +428,26 @@ __device__ __forceinline__ void few_part(const AttnArgs& p, int w, uint8_t* lds)
 }
 
 template <int NB, typename T>
-__global__ __launch_bounds__(512) void paged_few_kernel(AttnArgs p) {
+__global__ __launch_bounds__(64 * kFewWaves) void paged_few_kernel(AttnArgs p) {
     extern __shared__ __align__(16) uint8_t lds[];
     few_part<NB, T>(p, blockIdx.x, lds);
 }
 
 // ------------------------------------------------------------------ many columns
-// 32 CW query columns a workgroup, 32 a wave; the keys' tiles go by DMA into LDS as they lie in memory, two buffers, one
-// barrier a step, and are read as operands without bank conflicts (16 bytes a lane in lane order).  SETS sets of CW
-// waves take consecutive ranges of the steps and join through LDS at the end.
+// 32 CW query columns a workgroup, 32 a wave; the keys' tiles go by DMA into LDS as they lie in memory and are read as operands
+// without bank conflicts (16 bytes a lane in lane order).  Steps are of 32 keys, and a wave is one ahead with its scores: the
+// products of step i + 1's keys run beside the exponentials of step i, those of step i's values beside the maximum of step
+// i + 1's scores.  A stage of STEPS steps has one barrier; while its values and the keys of the step ahead of each are at
+// work, the next one's are under way.  SETS sets of CW waves take consecutive ranges of the steps and join through LDS at the
+// end.
 template <int NB, int CW, int SETS>
 struct Wide {
-    static constexpr int HD = 32 * NB, TILE = paged_tile_bytes(HD);
-    static constexpr int KEYS = NB <= 4 && SETS <= 2 ? 64 : 32;  // a step
-    static constexpr int TILES = KEYS / kPagedTile, SIDE = TILES * TILE, BUF = 2 * SIDE;
+    static constexpr int HD = 32 * NB, TILE = paged_tile_bytes(HD), KEYS = 32, STEP = 2 * TILE;
+    static constexpr int STEPS = NB <= 4 && SETS <= 2 ? 2 : 1;  // of a stage
     static constexpr int COLS = 32 * CW;
     static constexpr int JOIN = SETS > 1 ? COLS * (HD + 4) * 4 + COLS * 8 : 0;  // a set's outputs and statistics
-    static constexpr int RING = 2 * SETS * BUF;
+    static constexpr int SIDE = 2 * STEPS * STEP;  // two stages of keys, or of values
+    static constexpr int RING = 2 * SETS * SIDE;
     static constexpr int FEW = few_lds<NB>(CW * SETS);
     static constexpr int LDS = RING > JOIN ? (RING > FEW ? RING : FEW) : (JOIN > FEW ? JOIN : FEW);
     static constexpr bool FITS = LDS <= 160 << 10;
@@ -432,7 +460,8 @@ template <int NB, int CW, int SETS, typename T>
 __device__ __forceinline__ void wide_part(const AttnArgs& p, uint8_t* lds) {
     typedef Wide<NB, CW, SETS> W;
     constexpr bool EXACT = sizeof(T) == 4;
-    constexpr int HD = W::HD, TILE = W::TILE, KT = W::KEYS / 32;
+    constexpr int HD = W::HD, TILE = W::TILE, KEYS = W::KEYS, U = W::STEPS;
+    typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
     const int lane = threadIdx.x & 63, half = lane >> 5, c32 = lane & 31;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), set = wave / CW, wl = wave % CW;
     const int KVH = p.c.kv_heads, kvh = blockIdx.x % KVH;
@@ -449,8 +478,10 @@ __device__ __forceinline__ void wide_part(const AttnArgs& p, uint8_t* lds) {
     const int first = pos0 + p.by_group(col0), last = pos0 + p.by_group(min(col0 + W::COLS, cols) - 1);
     const int wcol0 = min(col0 + wl * 32, cols - 1);  // the wave's columns
     const int w_first = pos0 + p.by_group(wcol0), w_last = pos0 + p.by_group(min(wcol0 + 31, cols - 1));
-    const Steps steps = steps_of(p, first, last, W::KEYS);
-    const int per = (steps.count + SETS - 1) / SETS, f0 = set * per, count = max(0, min(steps.count - f0, per));
+    const Steps steps = steps_of(p, first, last, KEYS);
+    const int per = (steps.count + SETS - 1) / SETS, f0 = set * per;
+    // the wave's steps: of its set's those that one of its columns sees
+    const int count = max(0, min(min(steps.count, steps_of(p, first, w_last, KEYS).count) - f0, per));
 
     const int col = min(col0 + wl * 32 + c32, cols - 1), t = p.by_group(col), pos = pos0 + t;
     f16x8 qh[2 * NB], ql[EXACT ? 2 * NB : 1];
@@ -458,75 +489,127 @@ __device__ __forceinline__ void wide_part(const AttnArgs& p, uint8_t* lds) {
     const float sc = load_queries<2 * NB, 16, T>(q, p.scale_log2, p.whole_q, qh, ql, [](float x) {
         return xor32_combine(x, MaxOp());
     });
-    float m = -INFINITY, l = 0.f;
+    // (the queries are here before the loop: a wait for them inside it would wait for the tiles under way)
+#pragma unroll
+    for (int c = 0; c < 2 * NB; c++) {
+        asm volatile("" : "+v"(qh[c]));
+        if constexpr (EXACT) asm volatile("" : "+v"(ql[c]));
+    }
+    float m = -INFINITY, l = 0.f, base = 0.f;
     f32x16 o[NB];
 #pragma unroll
     for (int d = 0; d < NB; d++)
 #pragma unroll
         for (int r = 0; r < 16; r++) o[d][r] = 0.f;
 
-    uint8_t* const ring = lds + set * 2 * W::BUF;
+    // Whether a position that one of the workgroup's columns sees has no page (then every step looks again).
+    bool holes = false;
+    if (steps.count) {
+        auto missing = [&](int from, int to) {
+            for (int i = (from >> 4 >> p.c.tiles_log2) + lane; i <= to >> 4 >> p.c.tiles_log2; i += 64)
+                if (i < p.b.table_stride)
+                    holes |= (unsigned)gptr(p.b.table)[(int64_t)s * p.b.table_stride + i] >= (unsigned)p.c.pages;
+        };
+        missing(p.a.window ? max(0, first - p.a.window + 1) : 0, min(last, p.most - 1));
+        if (steps.first_steps) missing(0, min(p.a.sinks, p.most) - 1);
+        holes = __builtin_amdgcn_ballot_w64(holes);
+    }
+    // The set's steps i that are plain: all of i + 1 is seen by all columns of the wave, and all of i by one of the workgroup's.
+    const int plain0 = holes ? INT32_MAX
+                       : p.a.window ? steps.first_steps + (last >= p.a.window ? (last - p.a.window) / KEYS + 1 : 0) - steps.lo - f0
+                                    : -f0;
+    const int plain1 = min(count, steps.first_steps + max(0, w_first + 1) / KEYS - steps.lo - f0) - 1;
+
+    // keys of step i at ring + ((i - 1) % 2U) STEP, values of step i at ring + SIDE + (i % 2U) STEP
+    uint8_t* const ring = lds + set * 2 * W::SIDE;
     const uint32_t ring_at = lds_addr(ring);
-    constexpr int PARTS = 2 * W::TILES * NB;  // KB of a step: of keys, then of values, NB a tile
-    // Starts the loads of the set's step i into buffer i & 1; returns the bits of tiles without a page.
-    auto fetch = [&](int i) {
-        const int tile = steps[min(f0 + i, steps.count - 1)] * W::TILES;  // (past the last: that one, unused)
-        int64_t at[W::TILES];
-        int none = 0;
-#pragma unroll
-        for (int u = 0; u < W::TILES; u++) {
-            if (u == 0 || !((tile + u) & ((1 << p.c.tiles_log2) - 1))) {
-                const int page = page_of(p, s, tile + u);
-                none |= page < 0 ? 1 << u : 0;
-                at[u] = paged_tile(p.c, max(page, 0), kvh, tile + u) * TILE;
-            } else {
-                none |= (none >> (u - 1) & 1) << u;
-                at[u] = at[u - 1] + TILE;
-            }
-        }
-#pragma unroll
-        for (int k = 0; k < (PARTS + CW - 1) / CW; k++) {
-            const int c = wl + CW * k;
-            if (PARTS % CW && c >= PARTS) break;
-            const int side = c / (PARTS / 2), u = c % (PARTS / 2) / NB, part = c % NB;
-            int64_t from = at[0];
-#pragma unroll
-            for (int x = 1; x < W::TILES; x++) from = u == x ? at[x] : from;
-            dma16s((side ? p.c.v : p.c.k) + from + part * 1024, lane * 16,
-                   ring_at + (i & 1) * W::BUF + side * W::SIDE + u * TILE + part * 1024);
-        }
-        return none;
+    // the wave's share of a stage's loads: tiles u0, u0 + CW, ... and KB p0, p0 + P, ... of them
+    constexpr int TILES = 2 * U, MINE = TILES > CW ? TILES / CW : 1, P = CW > TILES ? CW / TILES : 1;
+    const int u0 = wl % TILES, p0 = wl / TILES;
+    struct Places {
+        int64_t at[MINE];
     };
-    auto work = [&](int i, int none) {
-        const int key0 = steps[f0 + i] * W::KEYS;
-        if (!any_sees(p, w_first, w_last, key0, key0 + W::KEYS - 1)) return;
-        const uint8_t* kb = ring + (i & 1) * W::BUF + (c32 >> 4) * TILE + (half * 16 + (c32 & 15)) * 16;
-        const uint8_t* vb = ring + (i & 1) * W::BUF + W::SIDE + (half * HD + c32) * 16;
-        f32x16 x[KT];  // S(key 32 k + 16 (r / 8) + 8 half + r % 8, column c32)
+    auto places = [&](int i) {  // of the stage that begins with step i (past the last step: that one, unused)
+        Places r;
 #pragma unroll
-        for (int k = 0; k < KT; k++) {
+        for (int k = 0; k < MINE; k++) {
+            const int u = u0 + CW * k, tile = 2 * steps[max(0, min(f0 + i + (u >> 1), steps.count - 1))] + (u & 1);
+            r.at[k] = paged_tile(p.c, max(page_of(p, s, tile), 0), kvh, tile) * TILE;
+        }
+        return r;
+    };
+    auto fetch = [&](const uint8_t* from, const Places& r, uint32_t to) {
 #pragma unroll
-            for (int r = 0; r < 16; r++) x[k][r] = 0.f;
+        for (int k = 0; k < MINE; k++)
 #pragma unroll
-            for (int c = 0; c < 2 * NB; c++) {
-                const f16x8 a = *(const f16x8*)(kb + 2 * k * TILE + c * 512);
-                x[k] = mfma32(a, qh[c], x[k]);
-                if constexpr (EXACT) x[k] = mfma32(a, ql[c], x[k]);
+            for (int part = 0; part < NB; part += P)
+                if (P == 1 || NB % P == 0 || part + p0 < NB)
+                    dma16s(from + r.at[k] + (part + p0) * 1024, lane * 16, to + (u0 + CW * k) * TILE + (part + p0) * 1024);
+    };
+    const uint32_t k_lane = (c32 >> 4) * TILE + (half * 16 + (c32 & 15)) * 16, v_lane = W::SIDE + (half * HD + c32) * 16;
+    // S(key 16 (r / 8) + 8 half + r % 8, column c32) of step i, `beside` a product
+    auto scores = [&](int i, f32x16& x, auto beside) {
+        const uint8_t* kb = ring + ((i - 1) & (2 * U - 1)) * W::STEP + k_lane;
+#pragma unroll
+        for (int r = 0; r < 16; r++) x[r] = 0.f;
+#pragma unroll
+        for (int c = 0; c < 2 * NB; c++) {
+            const f16x8 a = *(const f16x8*)(kb + c * 512);
+            x = mfma32(a, qh[c], x);
+            if constexpr (EXACT) x = mfma32(a, ql[c], x);
+            beside(c);
+        }
+    };
+    // Hides what a column does not see.
+    auto hide = [&](int i, f32x16& x) {
+        const int key0 = steps[f0 + i] * KEYS;
+        if (!holes && all_see(p, w_first, w_last, key0, key0 + KEYS - 1)) return;
+        if (holes) {
+#pragma unroll
+            for (int u = 0; u < 2; u++)
+                if (page_of(p, s, key0 / 16 + u) < 0)
+#pragma unroll
+                    for (int r = 0; r < 8; r++) x[8 * u + r] = NAN;
+        }
+        if (!p.a.window) {
+            const int at = pos - key0 - 8 * half;  // the lane's key 16 u + r is seen up to this one
+#pragma unroll
+            for (int r = 0; r < 16; r++)
+                if (16 * (r >> 3) + (r & 7) > at) x[r] = -INFINITY;
+        } else {
+#pragma unroll
+            for (int r = 0; r < 16; r++)
+                if (!sees(p, pos, key0 + 8 * half + 16 * (r >> 3) + (r & 7))) x[r] = -INFINITY;
+        }
+    };
+    // Values of 0 at positions that no column of the workgroup sees, where they may never have been written or be another
+    // sequence's: 0 times what lies there may be NaN.  (The waves of a set write the same.)
+    auto clear = [&](int i) {
+        const int key0 = steps[f0 + i] * KEYS, key1 = key0 + KEYS - 1;
+        if (!holes && key1 < seq.length && (!p.a.window || key0 > first - p.a.window || key1 < p.a.sinks)) return;
+        for (int u = 0; u < 2; u++) {
+            const bool none = holes && page_of(p, s, key0 / 16 + u) < 0;
+            for (int c = lane; c < 2 * HD; c += 64) {
+                uint32_t keep[4] = {0u, 0u, 0u, 0u};
+#pragma unroll
+                for (int e = 0; e < 8; e++) {
+                    const int key = key0 + 16 * u + (c >= HD ? 8 : 0) + e;
+                    if (!none && any_sees(p, first, last, key, key)) keep[e >> 1] |= 0xFFFFu << (16 * (e & 1));
+                }
+                u32x4* at = (u32x4*)(ring + W::SIDE + (i & (2 * U - 1)) * W::STEP + u * TILE + c * 16);
+                u32x4 v = *at;
+#pragma unroll
+                for (int e = 0; e < 4; e++) v[e] &= keep[e];
+                *at = v;
             }
         }
-        const bool edge = none || !all_see(p, w_first, w_last, key0, key0 + W::KEYS - 1);
-        if (edge) {
+    };
+    // The reference follows the scores to come, where they are past it.
+    bool large = false;  // (a column's reference is: exponent_base has something to do)
+    auto follow = [&](f32x16& x) {
+        float mx = x[0];
 #pragma unroll
-            for (int k = 0; k < KT; k++)
-#pragma unroll
-                for (int r = 0; r < 16; r++) {
-                    if (none >> (2 * k + (r >> 3)) & 1) x[k][r] = NAN;
-                    if (!sees(p, pos, key0 + 32 * k + 16 * (r >> 3) + 8 * half + (r & 7))) x[k][r] = -INFINITY;
-                }
-        }
-        float mx = x[0][0];
-#pragma unroll
-        for (int e = 1; e < 16 * KT; e++) mx = fmaxf(mx, x[e >> 4][e & 15]);
+        for (int e = 1; e < 16; e++) mx = fmaxf(mx, x[e]);
         mx = xor32_combine(mx, MaxOp());
         const float mn = mx * sc;  // (sc > 0)
         if (__builtin_amdgcn_ballot_w64(mn > m + kSlack)) {
@@ -536,62 +619,105 @@ __device__ __forceinline__ void wide_part(const AttnArgs& p, uint8_t* lds) {
             l *= alpha;
             m = top;
         }
-        const float base = exponent_base(x, mx, m == -INFINITY ? 0.f : m, sc, kWideLog2P);
-        f16x8 pf[2 * KT], pg[EXACT ? 2 * KT : 1];
-        float sum = 0.f;
+        f32x16(&y)[1] = reinterpret_cast<f32x16(&)[1]>(x);
+        base = exponent_base(y, mx, m == -INFINITY ? 0.f : m, sc, kWideLog2P);
+        large = __builtin_amdgcn_ballot_w64(fabsf(m) > kLargeScore && m != -INFINITY);
+    };
+    // Step i, its scores in x; those of step i + 1 into next.  Slots of a product (two in float32), the next operand's
+    // read and what runs beside it, in this order: operands AHEAD slots before their use, exponentials beside the keys'
+    // products, maxima beside the values'.
+    auto step = [&](int i, f32x16& x, f32x16& next) {
+        const bool plain = i >= plain0 && i < plain1;
+        constexpr int SLOTS = 2 * NB, AHEAD = NB == 1 ? 2 : 4, RING = AHEAD + 1;
+        f16x2 ph[8], pl[EXACT ? 8 : 1];
+        float sum[2] = {0.f, 0.f}, part[5];
+        uint64_t past = 0;
+        auto at = [](int k) { return min(k, SLOTS - 1); };
+        if (!plain) clear(i);
+        const uint8_t* kb = ring + (i & (2 * U - 1)) * W::STEP + k_lane;
+        const uint8_t* vb = ring + (i & (2 * U - 1)) * W::STEP + v_lane;
+        f16x8 fr[RING];
+        auto read = [&](int k) {  // value operands tile by tile
+            fr[k % RING] = *(const f16x8*)(k < SLOTS ? kb + k * 512 : vb + (k - SLOTS) / NB * TILE + (k - SLOTS) % NB * 512);
+        };
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-        for (int u = 0; u < 2 * KT; u++) {
-            f16x2 ph[4], pl[EXACT ? 4 : 1];
+        for (int k = 0; k < AHEAD; k++) read(k);
 #pragma unroll
-            for (int e = 0; e < 4; e++) {
-                const float a = __builtin_amdgcn_exp2f(fmaf(x[u >> 1][8 * (u & 1) + 2 * e], sc, base));
-                const float b = __builtin_amdgcn_exp2f(fmaf(x[u >> 1][8 * (u & 1) + 2 * e + 1], sc, base));
-                sum += a + b;
+        for (int r = 0; r < 16; r++) next[r] = 0.f;
+#pragma unroll
+        for (int k = 0; k < SLOTS; k++) {
+            read(k + AHEAD);
+            next = mfma32(fr[k % RING], qh[k], next);
+            if constexpr (EXACT) next = mfma32(fr[k % RING], ql[k], next);
+#pragma unroll
+            for (int e = k * 8 / SLOTS; e < (k + 1) * 8 / SLOTS; e++) {
+                const float a = __builtin_amdgcn_exp2f(fmaf(x[2 * e], sc, base));
+                const float b = __builtin_amdgcn_exp2f(fmaf(x[2 * e + 1], sc, base));
+                sum[0] += a;
+                sum[1] += b;
                 ph[e] = round2(a, b);
                 if constexpr (EXACT) pl[e] = round2(rest_low(ph[e], a), rest_high(ph[e], b));
             }
-            pf[u] = frag(ph[0], ph[1], ph[2], ph[3]);
-            if constexpr (EXACT) pg[u] = frag(pl[0], pl[1], pl[2], pl[3]);
+            asm volatile("" : "+v"(sum[0]), "+v"(sum[1]));
+            __builtin_amdgcn_sched_barrier(0);
         }
-        l += sum;
-        if (edge) {
-            // positions that may never have been written: values of 0
 #pragma unroll
-            for (int u = 0; u < 2 * KT; u++) {
-                uint32_t keep[4] = {0u, 0u, 0u, 0u};
+        for (int k = 0; k < SLOTS; k++) {
+            const int u = k / NB, d = k % NB;
+            if (k + AHEAD < SLOTS) read(SLOTS + k + AHEAD);
+            const f16x8 v = fr[(SLOTS + k) % RING];
+            o[d] = mfma32(v, frag(ph[4 * u], ph[4 * u + 1], ph[4 * u + 2], ph[4 * u + 3]), o[d]);
+            if constexpr (EXACT) o[d] = mfma32(v, frag(pl[4 * u], pl[4 * u + 1], pl[4 * u + 2], pl[4 * u + 3]), o[d]);
+            if (k == 0) l += sum[0] + sum[1];
+            // the largest score, and whether it is past the reference: a part of the chain a slot
+            if (k == at(1)) {
 #pragma unroll
-                for (int e = 0; e < 8; e++) {
-                    const int key = key0 + 16 * u + 8 * half + e;
-                    if (!(none >> u & 1) && any_sees(p, w_first, w_last, key, key)) keep[e >> 1] |= 0xFFFFu << (16 * (e & 1));
-                }
-#pragma unroll
-                for (int d = 0; d < NB; d++) {
-                    typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
-                    u32x4 v = *(const u32x4*)(vb + u * TILE + d * 512);
-#pragma unroll
-                    for (int e = 0; e < 4; e++) v[e] &= keep[e];
-                    o[d] = mfma32(__builtin_bit_cast(f16x8, v), pf[u], o[d]);
-                    if constexpr (EXACT) o[d] = mfma32(__builtin_bit_cast(f16x8, v), pg[u], o[d]);
-                }
+                for (int e = 0; e < 5; e++) part[e] = fmaxf(fmaxf(next[3 * e], next[3 * e + 1]), next[3 * e + 2]);
             }
-        } else {
-#pragma unroll
-            for (int u = 0; u < 2 * KT; u++)
-#pragma unroll
-                for (int d = 0; d < NB; d++) {
-                    const f16x8 v = *(const f16x8*)(vb + u * TILE + d * 512);
-                    o[d] = mfma32(v, pf[u], o[d]);
-                    if constexpr (EXACT) o[d] = mfma32(v, pg[u], o[d]);
-                }
+            if (k == at(2)) part[0] = fmaxf(fmaxf(fmaxf(part[0], part[1]), part[2]), fmaxf(fmaxf(part[3], part[4]), next[15]));
+            if (k == at(3)) part[0] = xor32_combine(part[0], MaxOp());
+            if (k == at(4)) past = __builtin_amdgcn_ballot_w64(part[0] * sc > m + kSlack);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        if (__builtin_expect(!plain || large || past, 0)) {
+            if (i + 1 >= count) return;
+            if (!plain) hide(i + 1, next);
+            follow(next);
         }
     };
     if (per > 0) {  // (the same for the whole workgroup)
-        int none = fetch(0);
-        for (int i = 0; i < per; i++) {
+        const Places a = places(1 - U);  // keys of step 0, at the end of a stage
+        fetch(p.c.k, a, ring_at + U * W::STEP);
+        Places kp = places(1), vp = places(0);
+        wait_stage_barrier<0>();
+        fetch(p.c.k, kp, ring_at);
+        fetch(p.c.v, vp, ring_at + W::SIDE);
+        kp = places(1 + U);
+        vp = places(U);
+        f32x16 x, y;
+        if (count > 0) {
+            scores(0, x, [](int) {});
+            hide(0, x);
+            follow(x);
+        }
+        auto stage = [&](int i) {  // that begins with step i: the next one's loads on their way
             wait_stage_barrier<0>();
-            const int next = i + 1 < per ? fetch(i + 1) : 0;
-            if (i < count) work(i, none);
-            none = next;
+            if (i + U >= per) return;
+            const uint32_t to = ring_at + ((i + U) & (2 * U - 1)) * W::STEP;
+            fetch(p.c.k, kp, to);
+            fetch(p.c.v, vp, to + W::SIDE);
+            kp = places(i + 1 + 2 * U);
+            vp = places(i + 2 * U);
+        };
+        for (int i = 0; i < per; i += 2) {
+            stage(i);
+            if (i < count) step(i, x, y);
+            if (U == 1) {
+                if (i + 1 >= per) break;
+                stage(i + 1);
+            }
+            if (i + 1 < count) step(i + 1, y, x);
         }
     }
     // l: half the keys in either half of the wave
@@ -651,9 +777,12 @@ __device__ __forceinline__ void wide_part(const AttnArgs& p, uint8_t* lds) {
         }
 }
 
+// Waves of a SIMD: two where a half of its registers holds what a wave needs.
+constexpr int wide_waves(int nb, bool exact) { return nb <= (exact ? 4 : 6) ? 2 : 1; }
+
 // The sequences of many columns, then those of few, in one launch.
 template <int NB, int CW, int SETS, typename T>
-__global__ __launch_bounds__(64 * CW * SETS) void paged_mixed_kernel(AttnArgs p) {
+__global__ __launch_bounds__(64 * CW * SETS) __attribute__((amdgpu_waves_per_eu(wide_waves(NB, sizeof(T) == 4), 2))) void paged_mixed_kernel(AttnArgs p) {
     extern __shared__ __align__(16) uint8_t lds[];
     if ((int)blockIdx.x < p.wide_grid) wide_part<NB, CW, SETS, T>(p, lds);
     else few_part<NB, T>(p, blockIdx.x - p.wide_grid, lds);
@@ -691,22 +820,45 @@ hipError_t launch_mixed(AttnArgs& p, hipStream_t st) {
                                                           W::LDS, st);
 }
 
+// How a call runs, by the workgroups that the batch's columns make; the lengths are on the device, and the shares of the
+// few-column part are chosen there.  us, one card:
+//
+// The many-column part, where its workgroups nearly fill the chip.  Of 128 columns and one set of waves, two a CU, from one a
+// CU on (two sets: 1,000 tokens and 31 single ones, 32/8 heads of 128, f16: 114 and 131; 2,048 tokens 60 and 58); of 128 and two
+// sets, where workgroups of 64 are more than the CUs (600 tokens at 4,096: 74, of 64 columns 96; 1,000: 82 and 98); of 64 and four
+// sets from 1.6 CUs of them on, in units of 32 dims (300 tokens at 4,096: 53, the few-column part 65; 512 of 32/32 heads of 64:
+// 41 and 46; but 1,000 of 9/3 heads of 64: 39 and 33).  Where most workgroups are of sequences of few columns, one set of 128
+// leaves them the most room (512 tokens of 32/32 heads of 64 and 31 single ones: 97, two sets 106, 64 columns 125).
+// One sequence's 256 columns, one workgroup a CU, where the short ones of their second round fill it behind the long ones
+// of the first (32/8 heads of 128, f16: 4,096 tokens 160 and 170, 3,500 126 and 132; but 3,000 104 and 98, 5,000 256 and 242).
+//
+// The few-column part alone: four waves a workgroup (one token of 9/3 heads of 64 at 2,000 positions 8.1, eight waves 8.6), a workgroup a CU where
+// there are not as many groups of columns, else two (64 sequences of 32/8 heads of 128: 163 and 178; one at 131,072: 102 and 99).
 template <int NB, typename T>
 hipError_t launch_nb(AttnArgs& p, hipStream_t st) {
-    const int cus = device_cus();
-    const int64_t cols = (int64_t)p.b.rows * p.G;
-    const int64_t most = p.a.max_rows > 0 ? std::min<int64_t>(p.a.max_rows * (int64_t)p.G, cols) : cols;
-    auto groups = [&](int width) { return (cols + width - 1) / width * p.c.kv_heads; };
-    p.target = std::min(cus, kMostTarget);
-    if constexpr (NB <= 4)
-        if (most > kManyColumns) {
-            if (groups(256) >= cus) return launch_mixed<NB, 8, 1, T>(p, st);
-            if (groups(128) >= cus) return launch_mixed<NB, 4, 2, T>(p, st);
-            if (groups(64) >= cus / 2) return launch_mixed<NB, 2, 4, T>(p, st);
-        }
+    const int64_t cus = device_cus(), cols = (int64_t)p.b.rows * p.G, KVH = p.c.kv_heads;
+    const int64_t max_rows = p.a.max_rows > 0 ? std::min(p.a.max_rows, p.b.rows) : p.b.rows;
+    auto groups = [&](int width) { return (cols + width - 1) / width * KVH; };
+    p.target = (int)std::min<int64_t>(cus, kMostTarget);
+    if (max_rows * p.G > kManyColumns) {
+        constexpr bool two = wide_waves(NB, sizeof(T) == 4) == 2;
+        // sequences that have one row whatever the others have
+        const int64_t more = std::max<int64_t>(1, max_rows - 1);
+        const int64_t single = p.b.sequences - (p.b.rows - p.b.sequences + more - 1) / more;
+        if constexpr (NB == 3 || NB == 4)
+            if (p.b.sequences == 1 && !p.a.window && 3 * groups(256) >= 5 * cus && groups(256) <= 2 * cus)
+                return launch_mixed<NB, 8, 1, T>(p, st);
+        if (groups(128) > cus || (groups(64) * NB > 8 * cus / 5 && (!two || single * KVH >= 4 * groups(128))))
+            return launch_mixed<NB, 4, 1, T>(p, st);
+        if constexpr (two)
+            if (groups(64) > cus) return launch_mixed<NB, 4, 2, T>(p, st);
+        if constexpr (NB <= 4)
+            if (5 * groups(64) * NB >= 8 * cus) return launch_mixed<NB, 2, 4, T>(p, st);
+    }
     p.few_columns = INT32_MAX;
-    constexpr int waves = 8;
-    return launch_one<paged_few_kernel<NB, T>>(p, few_grid(p, cols), 64 * waves, few_lds<NB>(waves), st);
+    const int64_t grid = few_grid(p, cols);
+    if (grid - p.target - 1 >= cus) p.target = (int)std::min<int64_t>(2 * cus, kMostTarget);
+    return launch_one<paged_few_kernel<NB, T>>(p, few_grid(p, cols), 64 * kFewWaves, few_lds<NB>(kFewWaves), st);
 }
 
 template <typename T>
