@@ -7,9 +7,10 @@
 //
 // The top n (at most 32): the row falls to 64 groups of 4 threads, and the n-th largest of
 // the groups' maxima is a bound that n values reach, so that of a row in any but a contrived
-// order little more than n do.  The threads whose maximum reaches it read their part of the row
-// again (it is a cache's by then) and put what reaches it into LDS, where its rank is the
-// number of better ones: larger, or as large and of a lower index.
+// order little more than n do.  A thread keeps where its two largest groups of lines were:
+// where those reach the bound they are read again (a thread that has more such groups: all of its
+// part, by its whole wave; a short slice is still in registers), and what reaches it goes into LDS, where its
+// rank is the number of better ones: larger, or as large and of a lower index.
 //
 // Few rows are split over workgroups, whose triples and best tokens the last one to arrive
 // joins in the same launch.
@@ -78,64 +79,97 @@ struct Slice {
         const int e = head + lines * V + i;
         return e < n ? e : -1;
     }
+    // Line k, which is thread k % kThreads's.
+    __device__ __forceinline__ void load_line(int k, float (&y)[V]) const {
+        typedef T TV __attribute__((ext_vector_type(V)));
+        const TV u = ((const AS_GLOBAL TV*)(x + head))[min(k, lines - 1)];
+#pragma unroll
+        for (int e = 0; e < V; e++) y[e] = (float)u[e];
+    }
     // f(value, element) for all of thread i's.
     template <typename F>
     __device__ __forceinline__ void each(int i, F f) const {
-        constexpr int U = 32 / V;
-        for (int k = i; k < lines; k += U * kThreads) {
-            float y[U * V];
-            load<U>(k, y);
+        for (int k = i; k < lines; k += kThreads) {
+            float y[V];
+            load_line(k, y);
 #pragma unroll
-            for (int j = 0; j < U; j++)
-                if (k + j * kThreads < lines) {
-#pragma unroll
-                    for (int e = 0; e < V; e++) f(y[j * V + e], head + (k + j * kThreads) * V + e);
-                }
+            for (int e = 0; e < V; e++) f(y[e], head + k * V + e);
         }
+        ends(i, f);
+    }
+    // Of the elements outside the lines.
+    template <typename F>
+    __device__ __forceinline__ void ends(int i, F f) const {
         if (before(i) >= 0) f((float)gptr(x)[before(i)], before(i));
         if (behind(i) >= 0) f((float)gptr(x)[behind(i)], behind(i));
     }
+    // f(value, element) for all of the threads of this wave that `take`, the lanes sharing each one's lines, AT threads a
+    // round trip to memory.
+    template <typename F>
+    __device__ __forceinline__ void each_of(bool take, F f) const {
+        constexpr int AT = 4;
+        const int lane = __lane_id(), first = threadIdx.x - lane;
+        if (take) ends(threadIdx.x, f);
+        uint64_t left = __builtin_amdgcn_ballot_w64(take);
+        while (left) {
+            int of[AT];
+#pragma unroll
+            for (int a = 0; a < AT; a++) {
+                of[a] = left ? first + __builtin_ctzll(left) : -1;
+                left &= left - 1;
+            }
+            for (int j = lane; j * kThreads < lines; j += 64) {
+                float y[AT][V];
+#pragma unroll
+                for (int a = 0; a < AT; a++) load_line(max(of[a], 0) + j * kThreads, y[a]);
+#pragma unroll
+                for (int a = 0; a < AT; a++) {
+                    const int k = of[a] + j * kThreads;
+                    if (of[a] < 0 || k >= lines) continue;
+#pragma unroll
+                    for (int e = 0; e < V; e++) f(y[a][e], head + k * V + e);
+                }
+            }
+        }
+    }
 };
 
-// Whether (a, i) ranks before (b, j): numbers before NaN, larger ones first, then the lower index.
-__device__ __forceinline__ bool before(float a, int i, float b, int j) {
-    if (a > b) return true;
-    if (a < b) return false;
-    const bool an = a != a, bn = b != b;
-    return an == bn ? i < j : bn;
+// A token as a number that is larger the better it ranks: numbers before NaN, larger ones first (-0 as 0), then the lower
+// index.
+typedef unsigned long long Key;
+__device__ __forceinline__ Key key_of(float x, int token) {
+    const uint32_t u = __float_as_uint(x + 0.f), up = u >> 31 ? ~u : u | 0x80000000u;
+    return (Key)(x != x ? 0u : up) << 32 | (uint32_t)~token;
 }
+__device__ __forceinline__ float value_of(Key k) {
+    const uint32_t up = (uint32_t)(k >> 32);
+    return up == 0 ? NAN : __uint_as_float(up >> 31 ? up & 0x7FFFFFFFu : ~up);
+}
+__device__ __forceinline__ int token_of(Key k) { return (int)~(uint32_t)k; }
 
 struct Shared {
     float m[kWaves], s[kWaves], t[kWaves];
     float group[kGroups];
-    float value[kListed];
-    int index[kListed];
-    float best[kMostTop];
-    int token[kMostTop];
+    Key key[kListed];
+    Key best[kMostTop];
+    Key next;
     float bound;
     int above, equal, last;
-    float wave_value[kWaves];
-    int wave_index[kWaves];
 };
 
 // The n-th largest of the groups' maxima; by one wave.
 __device__ __forceinline__ float nth_largest(const Shared& sh, int n) {
-    const int lane = __lane_id();
-    const float mine = sh.group[lane];
-    int rank = 0;
-#pragma unroll 8
-    for (int i = 0; i < kGroups; i++) {
-        const float other = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(mine), i));
-        rank += other > mine || (other == mine && i < lane);
-    }
-    const uint64_t at = __builtin_amdgcn_ballot_w64(rank == n - 1);
-    return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(mine), __builtin_ctzll(at | 1ull << 63)));
+    const float mine = sh.group[__lane_id()];
+    int larger = 0;
+#pragma unroll
+    for (int i = 0; i < kGroups; i++)
+        larger += __int_as_float(__builtin_amdgcn_readlane(__float_as_int(mine), i)) > mine;
+    return -wave_max(larger < n ? -mine : -INFINITY);  // (-inf only where that is a maximum)
 }
 
-// The first `need` elements of the slice, in order, for which f holds, into best / token from `at` on; returns how
-// many there were.  By one wave.
+// The first `need` elements of the slice, in order, for which f holds, into best from `at` on.  By one wave.
 template <typename T, typename F>
-__device__ __forceinline__ int fill(const Slice<T>& sl, Shared& sh, int at, int need, F f) {
+__device__ __forceinline__ void fill(const Slice<T>& sl, Shared& sh, int at, int need, F f) {
     const int lane = __lane_id();
     int got = 0;
     for (int e0 = 0; e0 < sl.n && got < need; e0 += 64) {
@@ -144,33 +178,27 @@ __device__ __forceinline__ int fill(const Slice<T>& sl, Shared& sh, int at, int 
         const bool take = e < sl.n && f(x);
         const uint64_t all = __builtin_amdgcn_ballot_w64(take);
         const int place = got + __builtin_popcountll(all & ((1ull << lane) - 1));
-        if (take && place < need) {
-            sh.best[at + place] = x;
-            sh.token[at + place] = sl.begin + e;
-        }
+        if (take && place < need) sh.best[at + place] = key_of(x, sl.begin + e);
         got += __builtin_popcountll(all);
     }
-    return min(got, need);
 }
 
 // The n best of `count` candidates in LDS; the threads have met behind their writing.
 __device__ __forceinline__ void rank_listed(Shared& sh, int first, int count, int at, int n) {
     for (int i = threadIdx.x; i < count; i += kThreads) {
-        const float x = sh.value[first + i];
-        const int e = sh.index[first + i];
+        const Key mine = sh.key[first + i];
         int rank = 0;
-        for (int j = 0; j < count; j++) rank += before(sh.value[first + j], sh.index[first + j], x, e);
-        if (rank < n) {
-            sh.best[at + rank] = x;
-            sh.token[at + rank] = e;
-        }
+#pragma unroll 8
+        for (int j = 0; j < count; j++) rank += sh.key[first + j] > mine;
+        if (rank < n) sh.best[at + rank] = mine;
     }
 }
 
-// The n best of a slice into best / token, whoever reads them having met the others afterwards; sh.group holds the groups'
-// maxima, `mine` is the thread's own.  Places that the slice is too short for hold (NaN, INT32_MAX).
-template <typename T>
-__device__ void top_of_slice(const Slice<T>& sl, Shared& sh, int n, float mine) {
+// The n best of a slice into best, whoever reads them having met the others afterwards; sh.group holds the groups'
+// maxima.  Places that the slice is too short for hold (NaN, INT32_MAX).
+// `all`(f) calls f(value, element) for what the wave's threads that have something to offer hold.
+template <typename T, typename All>
+__device__ __forceinline__ void top_of_slice(const Slice<T>& sl, Shared& sh, int n, All all) {
     const int tid = threadIdx.x;
     if (tid < 64) {
         const float b = nth_largest(sh, n);
@@ -178,29 +206,19 @@ __device__ void top_of_slice(const Slice<T>& sl, Shared& sh, int n, float mine) 
             sh.bound = b;
             sh.above = sh.equal = 0;
         }
-        if (tid < n) {
-            sh.best[tid] = NAN;
-            sh.token[tid] = INT32_MAX;
-        }
+        if (tid < n) sh.best[tid] = key_of(NAN, INT32_MAX);
     }
     __syncthreads();
     const float bound = sh.bound;
-    if (mine >= bound)
-        sl.each(tid, [&](float x, int e) {
-            if (x > bound) {
-                const int i = atomicAdd(&sh.above, 1);
-                if (i < kAbove) {
-                    sh.value[i] = x;
-                    sh.index[i] = sl.begin + e;
-                }
-            } else if (x == bound) {
-                const int i = atomicAdd(&sh.equal, 1);
-                if (i < kEqual) {
-                    sh.value[kAbove + i] = x;
-                    sh.index[kAbove + i] = sl.begin + e;
-                }
-            }
-        });
+    all([&](float x, int e) {
+        if (x > bound) {
+            const int i = atomicAdd(&sh.above, 1);
+            if (i < kAbove) sh.key[i] = key_of(x, sl.begin + e);
+        } else if (x == bound) {
+            const int i = atomicAdd(&sh.equal, 1);
+            if (i < kEqual) sh.key[kAbove + i] = key_of(x, sl.begin + e);
+        }
+    });
     __syncthreads();
     const int above = sh.above, equal = sh.equal;
     if (above <= kAbove) {
@@ -217,46 +235,33 @@ __device__ void top_of_slice(const Slice<T>& sl, Shared& sh, int n, float mine) 
         return;
     }
     // a row in an order that hides the bound: the best, then the best behind it, n times
-    float last = INFINITY;
-    int last_e = -1;
+    Key last = ~(Key)0;
     for (int r = 0; r < n; r++) {
-        float b = -INFINITY;
-        int be = INT32_MAX;
+        if (tid == 0) sh.next = 0;
+        __syncthreads();
+        Key mine = 0;
         sl.each(tid, [&](float x, int e) {
-            if (x == x && before(last, last_e, x, e) && before(x, e, b, be)) {
-                b = x;
-                be = e;
-            }
+            const Key k = key_of(x, sl.begin + e);
+            if (k < last && k > mine) mine = k;
         });
-        wave_argmax(b, be);
-        if ((tid & 63) == 0) {
-            sh.wave_value[tid >> 6] = b;
-            sh.wave_index[tid >> 6] = be;
-        }
+        atomicMax(&sh.next, mine);
         __syncthreads();
-        for (int w = 0; w < kWaves; w++)
-            if (w == 0 || before(sh.wave_value[w], sh.wave_index[w], last, last_e)) {
-                last = sh.wave_value[w];
-                last_e = sh.wave_index[w];
-            }
+        last = sh.next;
+        if (tid == 0) sh.best[r] = last;
         __syncthreads();
-        if (tid == 0) {
-            sh.best[r] = last;
-            sh.token[r] = sl.begin + last_e;
-        }
     }
 }
 
 template <typename T>
-__global__ __launch_bounds__(kThreads, 6) void logprobs_kernel(LogprobsArgs p) {
+__global__ __launch_bounds__(kThreads, 8) void logprobs_kernel(LogprobsArgs p) {
     __shared__ Shared sh;
     const int tid = threadIdx.x, row = blockIdx.x / p.splits, part = blockIdx.x - row * p.splits, n = p.top;
     const T* x = (const T*)p.logits + (int64_t)row * p.stride;
     const Slice<T> sl(x, min((int64_t)p.vocab, (int64_t)part * p.each), min((int64_t)p.vocab, (part + 1ll) * p.each));
-    constexpr int U = 4, N = U * Slice<T>::V;
+    constexpr int U = 16 / Slice<T>::V, N = U * Slice<T>::V;
 
     Sums sum;
-    auto add = [&](auto& y) {
+    auto add = [&](auto& y) {  // returns the largest
         constexpr int K = sizeof(y) / sizeof(float);
         float top = y[0];
 #pragma unroll
@@ -269,17 +274,27 @@ __global__ __launch_bounds__(kThreads, 6) void logprobs_kernel(LogprobsArgs p) {
             sum.s += e;
             sum.t = fmaf(e, fmaxf(d, -1000.f), sum.t);  // (a token masked by -inf adds 0)
         }
+        return top;
     };
+    float y[N];
+    // the thread's groups of U lines with the largest values, and the largest of the others
+    float top[3] = {-INFINITY, -INFINITY, -INFINITY};
+    int at[2] = {tid, tid};
     for (int k = tid; k < sl.lines; k += U * kThreads) {
-        float y[N];
         sl.template load<U>(k, y);
-        add(y);
+        const float x = add(y);
+        const bool first = x > top[0], second = x > top[1];
+        top[2] = fmaxf(top[2], second ? top[1] : x);
+        top[1] = first ? top[0] : second ? x : top[1];
+        at[1] = first ? at[0] : second ? k : at[1];
+        top[0] = first ? x : top[0];
+        at[0] = first ? k : at[0];
     }
     if (sl.before(tid) >= 0 || sl.behind(tid) >= 0) {
-        float y[2];
-        y[0] = sl.before(tid) >= 0 ? (float)gptr(sl.x)[sl.before(tid)] : -INFINITY;
-        y[1] = sl.behind(tid) >= 0 ? (float)gptr(sl.x)[sl.behind(tid)] : -INFINITY;
-        add(y);
+        float z[2];
+        z[0] = sl.before(tid) >= 0 ? (float)gptr(sl.x)[sl.before(tid)] : -INFINITY;
+        z[1] = sl.behind(tid) >= 0 ? (float)gptr(sl.x)[sl.behind(tid)] : -INFINITY;
+        add(z);
     }
     const float mine = sum.m;
     float group = fmaxf(mine, dpp_mov<0xB1>(mine));
@@ -311,13 +326,36 @@ __global__ __launch_bounds__(kThreads, 6) void logprobs_kernel(LogprobsArgs p) {
         return y;
     });
     if (n) {
-        top_of_slice(sl, sh, n, mine);
+        top_of_slice(sl, sh, n, [&](auto f) {
+            const float bound = sh.bound;
+            auto offer = [&](int k) {
+#pragma unroll
+                for (int i = 0; i < N; i++) {
+                    const int line = k + i / Slice<T>::V * kThreads;
+                    if (line < sl.lines) f(y[i], sl.head + line * Slice<T>::V + i % Slice<T>::V);
+                }
+            };
+            if (sl.lines <= U * kThreads) {  // still in registers
+                if (tid < sl.lines && mine >= bound) offer(tid);
+                if (mine >= bound) sl.ends(tid, f);
+                return;
+            }
+            const bool whole = top[2] >= bound;
+#pragma unroll
+            for (int i = 0; i < 2; i++)
+                if (!whole && top[i] >= bound && (i == 0 || at[1] != at[0])) {
+                    sl.template load<U>(at[i], y);
+                    offer(at[i]);
+                }
+            if (!whole && mine >= bound) sl.ends(tid, f);
+            sl.each_of(whole, f);
+        });
         __syncthreads();
     }
     if (p.splits > 1) {
         float* const at = p.parts + (int64_t)row * p.splits * kPart;
         float* const to = at + part * kPart;
-        if (tid < n) put2(to + 4 + 2 * tid, sh.best[tid], __int_as_float(sh.token[tid]));
+        if (tid < n) put2(to + 4 + 2 * tid, __uint_as_float((uint32_t)sh.best[tid]), __uint_as_float((uint32_t)(sh.best[tid] >> 32)));
         if (tid == 64) {
             put2(to, sum.m, sum.s);
             put2(to + 2, sum.t, 0.f);
@@ -350,8 +388,7 @@ __global__ __launch_bounds__(kThreads, 6) void logprobs_kernel(LogprobsArgs p) {
         const int listed = p.splits * n;
         for (int i = tid; i < listed; i += kThreads) {
             const float2 y = get2(at + i / n * kPart + 4 + 2 * (i % n));
-            sh.value[i] = y.x;
-            sh.index[i] = __float_as_int(y.y);
+            sh.key[i] = (Key)__float_as_uint(y.y) << 32 | __float_as_uint(y.x);
         }
         __syncthreads();
         sum.m = sh.m[0];
@@ -361,7 +398,7 @@ __global__ __launch_bounds__(kThreads, 6) void logprobs_kernel(LogprobsArgs p) {
             // the parts' tokens are in order: a bound from the first ones of each
             if (tid < kGroups) {
                 const int s = tid % p.splits, r = tid / p.splits;
-                sh.group[tid] = r < n ? fmaxf(-INFINITY, sh.value[s * n + r]) : -INFINITY;
+                sh.group[tid] = r < n ? fmaxf(-INFINITY, value_of(sh.key[s * n + r])) : -INFINITY;
             }
             __syncthreads();
             if (tid < 64) {
@@ -373,23 +410,18 @@ __global__ __launch_bounds__(kThreads, 6) void logprobs_kernel(LogprobsArgs p) {
             }
             __syncthreads();
             constexpr int PER = kListed / kThreads;
-            float y[PER];
-            int e[PER];
+            Key mine[PER];
 #pragma unroll
             for (int k = 0; k < PER; k++) {
                 const int i = tid + k * kThreads;
-                y[k] = i < listed ? sh.value[i] : NAN;
-                e[k] = i < listed ? sh.index[i] : INT32_MAX;
+                mine[k] = i < listed ? sh.key[i] : 0;
             }
             const float bound = sh.bound;
             __syncthreads();
 #pragma unroll
             for (int k = 0; k < PER; k++)
-                if (tid + k * kThreads < listed && (y[k] >= bound || bound == -INFINITY)) {
-                    const int i = atomicAdd(&sh.above, 1);
-                    sh.value[i] = y[k];
-                    sh.index[i] = e[k];
-                }
+                if (tid + k * kThreads < listed && (value_of(mine[k]) >= bound || bound == -INFINITY))
+                    sh.key[atomicAdd(&sh.above, 1)] = mine[k];
             __syncthreads();
             rank_listed(sh, 0, sh.above, 0, n);
             __syncthreads();
@@ -397,8 +429,8 @@ __global__ __launch_bounds__(kThreads, 6) void logprobs_kernel(LogprobsArgs p) {
     }
     const float log_s = logf(sum.s);
     if (tid < n) {
-        gptr(p.top_tokens)[(int64_t)row * n + tid] = sh.token[tid];
-        gptr(p.top_logprobs)[(int64_t)row * n + tid] = (sh.best[tid] - sum.m) - log_s;
+        gptr(p.top_tokens)[(int64_t)row * n + tid] = token_of(sh.best[tid]);
+        gptr(p.top_logprobs)[(int64_t)row * n + tid] = (value_of(sh.best[tid]) - sum.m) - log_s;
     }
     if (tid == 64 && p.entropy) gptr(p.entropy)[row] = log_s - sum.t / sum.s;
     if (tid == 128 && p.logprobs) {

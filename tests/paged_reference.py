@@ -121,7 +121,7 @@ def logprobs(x, tokens, top):
         t = np.where(e == 0, 0, e * np.where(e == 0, 0, d)).sum(-1, keepdims=True) / s
         lp = d - ls
         # (a number before a NaN, larger ones first, then the lower index)
-        order = [sorted(range(vocab), key=lambda j: (np.isnan(r[j]), 0 if np.isnan(r[j]) else -r[j], j))[:top] for r in x64]
+        order = [np.lexsort((np.arange(vocab), np.where(np.isnan(r), 0, -r), np.isnan(r)))[:top] for r in x64]
         best = np.array(order, np.int64).reshape(rows, top)
         sums = (vocab / 256 + 64) * EPS32 + 2.0 ** -22
         off = sums + 2 * EPS32 * np.abs(ls) + 2 * EPS32 * (np.abs(np.where(np.isfinite(d), d, 0)) + np.abs(ls))
