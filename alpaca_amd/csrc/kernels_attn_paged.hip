@@ -465,16 +465,16 @@ __device__ __forceinline__ void wide_part(const AttnArgs& p, uint8_t* lds) {
     const int lane = threadIdx.x & 63, half = lane >> 5, c32 = lane & 31;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), set = wave / CW, wl = wave % CW;
     const int KVH = p.c.kv_heads, kvh = blockIdx.x % KVH;
-    const PagedItem it = paged_find(blockIdx.x / KVH, p.b.sequences, [&](int s) {
-        const int64_t cols = (int64_t)paged_seq(p.b, s).n * p.G;
+    const PagedItem it = paged_find(p.b, blockIdx.x / KVH, [&](const PagedSeq& q) {
+        const int64_t cols = (int64_t)q.n * p.G;
         return cols > p.few_columns ? (int)((cols + W::COLS - 1) / W::COLS) : 0;
     });
     if (it.s < 0) return;
-    const int s = __builtin_amdgcn_readfirstlane(it.s);
-    const PagedSeq seq = paged_seq(p.b, s);
+    const int s = it.s;
+    const PagedSeq seq = it.seq;
     const int cols = seq.n * p.G, pos0 = seq.length - seq.n;
     // a sequence's last columns first: they see the most keys
-    const int col0 = ((cols + W::COLS - 1) / W::COLS - 1 - __builtin_amdgcn_readfirstlane(it.i)) * W::COLS;
+    const int col0 = ((cols + W::COLS - 1) / W::COLS - 1 - it.i) * W::COLS;
     const int first = pos0 + p.by_group(col0), last = pos0 + p.by_group(min(col0 + W::COLS, cols) - 1);
     const int wcol0 = min(col0 + wl * 32, cols - 1);  // the wave's columns
     const int w_first = pos0 + p.by_group(wcol0), w_last = pos0 + p.by_group(min(wcol0 + 31, cols - 1));

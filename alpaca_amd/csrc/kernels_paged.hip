@@ -98,16 +98,15 @@ struct Place {
     }
 };
 __device__ __forceinline__ bool find_place(const PagedSteps& b, Place& p) {
-    const PagedItem it = paged_find(blockIdx.x, b.sequences, [&](int s) {
-        const PagedSeq q = paged_seq(b, s);
+    const PagedItem it = paged_find(b, blockIdx.x, [&](const PagedSeq& q) {
         // (>> rounds down: rows of negative positions have tiles too)
-        return q.n ? ((q.length - 1) >> 4) - ((q.length - q.n) >> 4) + 1 : 0;
+        return ((q.length - 1) >> 4) - ((q.length - q.n) >> 4) + 1;
     });
     if (it.s < 0) return false;
-    p.s = __builtin_amdgcn_readfirstlane(it.s);
-    p.seq = paged_seq(b, p.s);
+    p.s = it.s;
+    p.seq = it.seq;
     p.pos0 = p.seq.length - p.seq.n;
-    p.tile = (p.pos0 >> 4) + __builtin_amdgcn_readfirstlane(it.i);
+    p.tile = (p.pos0 >> 4) + it.i;
     return true;
 }
 
@@ -115,9 +114,9 @@ struct AppendArgs {
     PagedRows r;
     PagedSteps b;
     PagedKV c;
-    int kv_slices, passes;            // of grid.y; of a query slice
+    int kv_slices;                    // of grid.y, query slices behind them
     int lanes, at_once;               // 16-dim lanes of a head, heads at once
-    bool q_whole, k_whole, v_whole, out_whole;  // rows that lie on 16 bytes
+    bool q_whole, k_whole, v_whole, out_whole, rope_whole;  // rows that lie on 16 bytes
 };
 
 // The two runs of 8 dims that lane `u` of a head rotates.
@@ -136,12 +135,14 @@ __device__ __forceinline__ void rotate(float (&x)[2][8], const float2 (&cs)[8], 
     }
 }
 
-template <typename T, bool INTERLEAVED>
+template <typename T, bool INTERLEAVED, int PASSES>
 __global__ __launch_bounds__(kThreads) void paged_append_kernel(AppendArgs p) {
     __shared__ uint32_t odd[16];  // a bit a head of the slice: tokens that have no form
     Place at;
     if (!find_place(p.b, at)) return;
-    const int hd = p.c.hd, tok = threadIdx.x & 15, u = threadIdx.x >> 4;
+    // queries: the lanes of a token side by side, as their rows lie; keys: the tokens, as the pages do
+    const bool queries = (int)blockIdx.y >= p.kv_slices;
+    const int hd = p.c.hd, lo = threadIdx.x & 15, hi = threadIdx.x >> 4, tok = queries ? hi : lo, u = queries ? lo : hi;
     const int lane = u % p.lanes, sub = u / p.lanes;
     const int pos = at.tile * 16 + tok, row = at.row(pos);
     int d[2];
@@ -151,26 +152,42 @@ __global__ __launch_bounds__(kThreads) void paged_append_kernel(AppendArgs p) {
     if (turned) {
         if (pos >= 0 && pos < p.r.rope_positions) {
             const float2* t = p.r.rope + (int64_t)pos * (hd / 2) + 8 * lane;
+            if (p.rope_whole) {
 #pragma unroll
-            for (int i = 0; i < 8; i++) cs[i] = gload_f2(t + i);
+                for (int i = 0; i < 4; i++) {
+                    const int4 y = gload_i4(t + 2 * i);
+                    cs[2 * i] = make_float2(__int_as_float(y.x), __int_as_float(y.y));
+                    cs[2 * i + 1] = make_float2(__int_as_float(y.z), __int_as_float(y.w));
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < 8; i++) cs[i] = gload_f2(t + i);
+            }
         } else {
 #pragma unroll
             for (int i = 0; i < 8; i++) cs[i] = make_float2(NAN, NAN);
         }
     }
-    if ((int)blockIdx.y >= p.kv_slices) {
+    if (queries) {
         if (row < 0 || sub >= p.at_once) return;
-        int h = ((int)blockIdx.y - p.kv_slices) * p.at_once * p.passes + sub;
-        for (int i = 0; i < p.passes && h < p.r.heads; i++, h += p.at_once) {
-            const T* q = (const T*)p.r.q + row * p.r.q_stride + (int64_t)h * hd;
-            T* out = (T*)p.r.q_out + row * p.r.q_out_stride + (int64_t)h * hd;
-            float x[2][8];
-            Lines<T>::load(q + d[0], x[0], p.q_whole);
-            Lines<T>::load(q + d[1], x[1], p.q_whole);
-            if (turned) rotate(x, cs, INTERLEAVED);
-            Lines<T>::store(out + d[0], x[0], p.out_whole);
-            Lines<T>::store(out + d[1], x[1], p.out_whole);
-        }
+        const int h = ((int)blockIdx.y - p.kv_slices) * p.at_once * PASSES + sub;
+        const T* q = (const T*)p.r.q + row * p.r.q_stride + (int64_t)h * hd;
+        T* out = (T*)p.r.q_out + row * p.r.q_out_stride + (int64_t)h * hd;
+        const int64_t next = (int64_t)p.at_once * hd;
+        float x[PASSES][2][8];
+#pragma unroll
+        for (int i = 0; i < PASSES; i++)
+            if (h + i * p.at_once < p.r.heads) {
+                Lines<T>::load(q + i * next + d[0], x[i][0], p.q_whole);
+                Lines<T>::load(q + i * next + d[1], x[i][1], p.q_whole);
+            }
+#pragma unroll
+        for (int i = 0; i < PASSES; i++)
+            if (h + i * p.at_once < p.r.heads) {
+                if (turned) rotate(x[i], cs, INTERLEAVED);
+                Lines<T>::store(out + i * next + d[0], x[i][0], p.out_whole);
+                Lines<T>::store(out + i * next + d[1], x[i][1], p.out_whole);
+            }
         return;
     }
     const int page = paged_page(p.b, p.c, at.s, at.tile);  // (the same for the whole workgroup)
@@ -203,15 +220,14 @@ __global__ __launch_bounds__(kThreads) void paged_append_kernel(AppendArgs p) {
     if (values) {
         float2 x[8];
 #pragma unroll
-        for (int e = 0; e < 8; e++) {
-            const int r = at.row(vpos + e);
-            x[e] = make_float2(0.f, 0.f);
-            if (r < 0) continue;
-            fresh |= 1 << e;
+        for (int e = 0; e < 8; e++) {  // (a token that is not new: another's row, unused)
+            const int i = vpos + e - at.pos0, r = at.seq.row0 + min(max(i, 0), at.seq.n - 1);
+            fresh |= (i >= 0 && i < at.seq.n) << e;
             x[e] = load_two((const T*)p.r.v + r * p.r.v_stride + (int64_t)vh * hd + dim, p.v_whole);
         }
 #pragma unroll
         for (int e = 0; e < 8; e++) {
+            if (!(fresh >> e & 1)) continue;
             va[e] = (f16)x[e].x;
             vb[e] = (f16)x[e].y;
             if (odd16(va[e]) || odd16(vb[e])) atomicOr(&odd[8 * half + e], 1u << vsub);
@@ -302,6 +318,17 @@ unsigned tiles_bound(const PagedSteps& b) {
     return (unsigned)(t < b.rows ? t : b.rows);
 }
 
+constexpr int64_t kManyValues = 1 << 21;
+
+template <typename T, int PASSES>
+hipError_t launch_append(const AppendArgs& p, hipStream_t st) {
+    const int per = p.at_once * PASSES;
+    const dim3 grid(tiles_bound(p.b), p.kv_slices + (p.r.heads + per - 1) / per);
+    if (p.r.interleaved) paged_append_kernel<T, true, PASSES><<<grid, kThreads, 0, st>>>(p);
+    else paged_append_kernel<T, false, PASSES><<<grid, kThreads, 0, st>>>(p);
+    return hipGetLastError();
+}
+
 }  // namespace
 
 hipError_t launch_paged_append(bool f16_rows, const PagedRows& r, const PagedSteps& b, const PagedKV& c, hipStream_t st) {
@@ -313,21 +340,16 @@ hipError_t launch_paged_append(bool f16_rows, const PagedRows& r, const PagedSte
     p.lanes = c.hd / 16;
     p.at_once = 16 / p.lanes;
     p.kv_slices = (c.kv_heads + p.at_once - 1) / p.at_once;
-    p.passes = 1;
     p.q_whole = whole(r.q, r.q_stride, size);
     p.k_whole = whole(r.k, r.k_stride, size);
     p.v_whole = whole(r.v, r.v_stride, size);
     p.out_whole = whole(r.q_out, r.q_out_stride, size);
-    const int per = p.at_once * p.passes;
-    const dim3 grid(tiles_bound(b), p.kv_slices + (r.heads + per - 1) / per);
-    if (f16_rows) {
-        if (r.interleaved) paged_append_kernel<f16, true><<<grid, kThreads, 0, st>>>(p);
-        else paged_append_kernel<f16, false><<<grid, kThreads, 0, st>>>(p);
-    } else {
-        if (r.interleaved) paged_append_kernel<float, true><<<grid, kThreads, 0, st>>>(p);
-        else paged_append_kernel<float, false><<<grid, kThreads, 0, st>>>(p);
-    }
-    return hipGetLastError();
+    p.rope_whole = whole(r.rope, 0, 8);
+    // Several heads a thread one after the other, their angles read once and their rows under way together, where that
+    // leaves enough workgroups.
+    if (r.heads > 2 * p.at_once && (int64_t)b.rows * r.heads * c.hd >= kManyValues)
+        return f16_rows ? launch_append<f16, 4>(p, st) : launch_append<float, 4>(p, st);
+    return f16_rows ? launch_append<f16, 1>(p, st) : launch_append<float, 1>(p, st);
 }
 
 hipError_t launch_paged_load(bool f16_rows, const PagedSteps& b, const PagedKV& c, void* k, int64_t k_stride, void* v,

@@ -92,24 +92,28 @@ __device__ __forceinline__ int wave_scan(int x) {
     return x;
 }
 
-// The sequence that has item `w` where sequence s has items(s) of them, in order: {s, w - those
-// before}; s = -1 past the last.  By a whole wave.
+// The sequence that has item `w` where one of rows q has items(q) of them, in order, and w - those before; s = -1 past
+// the last.  By a whole wave, the same in all lanes.
 struct PagedItem {
     int s, i;
+    PagedSeq seq;
 };
 template <typename F>
-__device__ __forceinline__ PagedItem paged_find(int w, int sequences, F items) {
+__device__ __forceinline__ PagedItem paged_find(const PagedSteps& b, int w, F items) {
     const int lane = __lane_id();
-    for (int s0 = 0; s0 < sequences; s0 += 64) {
-        const int mine = s0 + lane < sequences ? items(s0 + lane) : 0, upto = wave_scan(mine);
+    for (int s0 = 0; s0 < b.sequences; s0 += 64) {
+        PagedSeq q{0, 0, 0};
+        if (s0 + lane < b.sequences) q = paged_seq(b, s0 + lane);
+        const int mine = q.n ? items(q) : 0, upto = wave_scan(mine);
         const uint64_t past = __builtin_amdgcn_ballot_w64(upto > w);
         if (past) {
             const int l = __builtin_ctzll(past);
-            return {s0 + l, w - __builtin_amdgcn_readlane(upto - mine, l)};
+            auto of = [&](int x) { return __builtin_amdgcn_readlane(x, l); };
+            return {s0 + l, w - of(upto - mine), {of(q.row0), of(q.n), of(q.length)}};
         }
         w -= __builtin_amdgcn_readlane(upto, 63);
     }
-    return {-1, 0};
+    return {-1, 0, {0, 0, 0}};
 }
 
 // The page that holds tile `tile` (positions 16 tile ..) of sequence s, or -1; and the tile's place among all tiles
