@@ -152,6 +152,7 @@ __device__ __forceinline__ float inverse(float l, bool past) { return past ? NAN
 // A workgroup's work: a group of 16 columns of sequence s, part sp of `splits`.
 struct FewItem {
     int s, kvh, group, sp, splits, counter, slot;
+    PagedSeq seq;
 };
 struct FewCount {
     int groups, steps;  // of a sequence, of 16 columns of a KV head each
@@ -164,39 +165,43 @@ __device__ __forceinline__ FewCount few_count(const AttnArgs& p, const PagedSeq&
 // Workgroup `w` of the few-column part, by a whole wave; splits = 0 past the last.
 __device__ __forceinline__ FewItem few_find(const AttnArgs& p, int w) {
     const int lane = __lane_id(), S = p.b.sequences, KVH = p.c.kv_heads;
+    auto seq_of = [&](int s0) { return s0 + lane < S ? paged_seq(p.b, s0 + lane) : PagedSeq{0, 0, 0}; };
     // steps a workgroup: all the batch's over the workgroups aimed for.  (float: the same sum in every wave)
-    float all = 0.f;
-    for (int s0 = 0; s0 < S; s0 += 64) {
-        if (s0 + lane < S) {
-            const FewCount f = few_count(p, paged_seq(p.b, s0 + lane));
-            all += (float)f.groups * (float)f.steps;
-        }
+    const PagedSeq front = seq_of(0);  // (all of a batch of up to 64)
+    const FewCount front_count = few_count(p, front);
+    float all = (float)front_count.groups * (float)front_count.steps;
+    for (int s0 = 64; s0 < S; s0 += 64) {
+        const FewCount f = few_count(p, seq_of(s0));
+        all += (float)f.groups * (float)f.steps;
     }
     all = wave_sum(all) * (float)KVH;
     const int share = max(kFewLeast, (int)fminf(all * 1.0001f / (float)p.target + 1.f, 1e9f));
-    FewItem r{0, 0, 0, 0, 0, 0, 0};
+    FewItem r{0, 0, 0, 0, 0, 0, 0, {0, 0, 0}};
     for (int s0 = 0; s0 < S; s0 += 64) {
-        int groups = 0, splits = 1;
-        if (s0 + lane < S) {
-            const FewCount f = few_count(p, paged_seq(p.b, s0 + lane));
-            groups = f.groups * KVH;
-            splits = max(1, (f.steps + share - 1) / share);
+        PagedSeq q = front;
+        FewCount f = front_count;
+        if (s0) {
+            q = seq_of(s0);
+            f = few_count(p, q);
         }
+        const int groups = f.groups * KVH, splits = max(1, (f.steps + share - 1) / share);
         const int mine = groups * splits, upto = wave_scan(mine);
         const int joint = splits > 1 ? groups : 0, joint_to = wave_scan(joint);
         const int parts = joint * splits, parts_to = wave_scan(parts);
         const uint64_t past = __builtin_amdgcn_ballot_w64(upto > w);
         if (past) {
             const int l = __builtin_ctzll(past);
-            const int i = w - __builtin_amdgcn_readlane(upto - mine, l);
+            auto of = [&](int x) { return __builtin_amdgcn_readlane(x, l); };
+            const int i = w - of(upto - mine);
             r.s = s0 + l;
-            r.splits = __builtin_amdgcn_readlane(splits, l);
+            r.seq = {of(q.row0), of(q.n), of(q.length)};
+            r.splits = of(splits);
             r.kvh = i % KVH;
             r.sp = i / KVH % r.splits;
             r.group = i / KVH / r.splits;
             const int at = r.group * KVH + r.kvh;
-            r.counter += __builtin_amdgcn_readlane(joint_to - joint, l) + at;
-            r.slot += __builtin_amdgcn_readlane(parts_to - parts, l) + at * r.splits;
+            r.counter += of(joint_to - joint) + at;
+            r.slot += of(parts_to - parts) + at * r.splits;
             // (only row ranges that overlap could have more)
             if (r.splits > 1 && (r.counter >= p.target || r.slot + r.splits > 2 * p.target + 64)) r.splits = 0;
             return r;
@@ -226,7 +231,7 @@ __device__ __forceinline__ void few_part(const AttnArgs& p, int w, uint8_t* lds)
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const FewItem it = few_find(p, w);
     if (it.splits == 0) return;  // (the same for the whole workgroup)
-    const PagedSeq seq = paged_seq(p.b, it.s);
+    const PagedSeq& seq = it.seq;
     const int col0 = it.group * kFewCols, cols = min(seq.n * p.G - col0, kFewCols), pos0 = seq.length - seq.n;
     const int first = pos0 + p.by_group(col0), last = pos0 + p.by_group(col0 + cols - 1);
     const Steps steps = steps_of(p, first, last, kFewStep);
