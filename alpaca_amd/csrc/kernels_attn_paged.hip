@@ -837,8 +837,9 @@ hipError_t launch_mixed(AttnArgs& p, hipStream_t st) {
 // One sequence's 256 columns, one workgroup a CU, where the short ones of their second round fill it behind the long ones
 // of the first (32/8 heads of 128, f16: 4,096 tokens 160 and 170, 3,500 126 and 132; but 3,000 104 and 98, 5,000 256 and 242).
 //
-// The few-column part alone: four waves a workgroup (one token of 9/3 heads of 64 at 2,000 positions 8.1, eight waves 8.6), a workgroup a CU where
-// there are not as many groups of columns, else two (64 sequences of 32/8 heads of 128: 163 and 178; one at 131,072: 102 and 99).
+// The few-column part alone: four waves a workgroup (one token of 9/3 heads of 64 at 2,000 positions 8.1, eight waves 8.6), a
+// workgroup a CU, or two where groups of columns are half as many (64 sequences of 32/8 heads of 128: 163 and 178; 16 of 16/8
+// heads of 256 at 4,096 49 and 53; one of 32/8 heads of 128 at 131,072: 102 and 99, of 16/8 heads of 256 at 30,000 54 and 51).
 template <int NB, typename T>
 hipError_t launch_nb(AttnArgs& p, hipStream_t st) {
     const int64_t cus = device_cus(), cols = (int64_t)p.b.rows * p.G, KVH = p.c.kv_heads;
@@ -862,7 +863,7 @@ hipError_t launch_nb(AttnArgs& p, hipStream_t st) {
     }
     p.few_columns = INT32_MAX;
     const int64_t grid = few_grid(p, cols);
-    if (grid - p.target - 1 >= cus) p.target = (int)std::min<int64_t>(2 * cus, kMostTarget);
+    if (2 * (grid - p.target - 1) >= cus) p.target = (int)std::min<int64_t>(2 * cus, kMostTarget);
     return launch_one<paged_few_kernel<NB, T>>(p, few_grid(p, cols), 64 * kFewWaves, few_lds<NB>(kFewWaves), st);
 }
 
