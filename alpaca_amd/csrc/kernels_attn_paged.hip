@@ -516,7 +516,7 @@ __device__ __forceinline__ void wide_part(const AttnArgs& p, uint8_t* lds) {
                     holes |= (unsigned)gptr(p.b.table)[(int64_t)s * p.b.table_stride + i] >= (unsigned)p.c.pages;
         };
         missing(p.a.window ? max(0, first - p.a.window + 1) : 0, min(last, p.most - 1));
-        if (steps.first_steps) missing(0, min(p.a.sinks, p.most) - 1);
+        if (steps.first_steps) missing(0, min(p.a.sinks - 1, min(last, p.most - 1)));
         holes = __builtin_amdgcn_ballot_w64(holes);
     }
     // The set's steps i that are plain: all of i + 1 is seen by all columns of the wave, and all of i by one of the workgroup's.
@@ -552,8 +552,8 @@ __device__ __forceinline__ void wide_part(const AttnArgs& p, uint8_t* lds) {
                     dma16s(from + r.at[k] + (part + p0) * 1024, lane * 16, to + (u0 + CW * k) * TILE + (part + p0) * 1024);
     };
     const uint32_t k_lane = (c32 >> 4) * TILE + (half * 16 + (c32 & 15)) * 16, v_lane = W::SIDE + (half * HD + c32) * 16;
-    // S(key 16 (r / 8) + 8 half + r % 8, column c32) of step i, `beside` a product
-    auto scores = [&](int i, f32x16& x, auto beside) {
+    // S(key 16 (r / 8) + 8 half + r % 8, column c32) of step i
+    auto scores = [&](int i, f32x16& x) {
         const uint8_t* kb = ring + ((i - 1) & (2 * U - 1)) * W::STEP + k_lane;
 #pragma unroll
         for (int r = 0; r < 16; r++) x[r] = 0.f;
@@ -562,7 +562,6 @@ __device__ __forceinline__ void wide_part(const AttnArgs& p, uint8_t* lds) {
             const f16x8 a = *(const f16x8*)(kb + c * 512);
             x = mfma32(a, qh[c], x);
             if constexpr (EXACT) x = mfma32(a, ql[c], x);
-            beside(c);
         }
     };
     // Hides what a column does not see.
@@ -591,7 +590,7 @@ __device__ __forceinline__ void wide_part(const AttnArgs& p, uint8_t* lds) {
     // sequence's: 0 times what lies there may be NaN.  (The waves of a set write the same.)
     auto clear = [&](int i) {
         const int key0 = steps[f0 + i] * KEYS, key1 = key0 + KEYS - 1;
-        if (!holes && key1 < seq.length && (!p.a.window || key0 > first - p.a.window || key1 < p.a.sinks)) return;
+        if (!holes && key1 < min(seq.length, p.most) && (!p.a.window || key0 > first - p.a.window || key1 < p.a.sinks)) return;
         for (int u = 0; u < 2; u++) {
             const bool none = holes && page_of(p, s, key0 / 16 + u) < 0;
             for (int c = lane; c < 2 * HD; c += 64) {
@@ -599,7 +598,7 @@ __device__ __forceinline__ void wide_part(const AttnArgs& p, uint8_t* lds) {
 #pragma unroll
                 for (int e = 0; e < 8; e++) {
                     const int key = key0 + 16 * u + (c >= HD ? 8 : 0) + e;
-                    if (!none && any_sees(p, first, last, key, key)) keep[e >> 1] |= 0xFFFFu << (16 * (e & 1));
+                    if (!none && key < p.most && any_sees(p, first, last, key, key)) keep[e >> 1] |= 0xFFFFu << (16 * (e & 1));
                 }
                 u32x4* at = (u32x4*)(ring + W::SIDE + (i & (2 * U - 1)) * W::STEP + u * TILE + c * 16);
                 u32x4 v = *at;
@@ -702,7 +701,7 @@ __device__ __forceinline__ void wide_part(const AttnArgs& p, uint8_t* lds) {
         vp = places(U);
         f32x16 x, y;
         if (count > 0) {
-            scores(0, x, [](int) {});
+            scores(0, x);
             hide(0, x);
             follow(x);
         }
@@ -798,7 +797,7 @@ hipError_t launch_one(const AttnArgs& p, int64_t grid, int threads, int lds, hip
     static OncePerDevice once;
     if (hipError_t e = allow_whole_lds(once, (const void*)kernel)) return e;
     if (grid <= 0) return hipSuccess;
-    if (grid > INT32_MAX) return hipErrorInvalidConfiguration;
+    if (grid * threads > UINT32_MAX) return hipErrorInvalidConfiguration;  // (a launch holds no more threads)
     kernel<<<(unsigned)grid, threads, lds, st>>>(p);
     return hipGetLastError();
 }
@@ -893,6 +892,9 @@ hipError_t launch_paged_attention(bool f16_rows, const PagedAttention& a, const 
     p.c = c;
     p.G = a.heads / c.kv_heads;
     p.most = b.table_stride << (4 + c.tiles_log2);
+    // a window of all positions is none; so bounded, differences of positions are 32-bit numbers
+    if (a.window >= p.most) p.a.window = 0;
+    p.a.sinks = std::min(a.sinks, p.most);
     p.by_group = Divisor(p.G);
     p.scale_log2 = 1.4426950408889634f / sqrtf((float)c.hd);
     p.counters = (int*)a.workspace;

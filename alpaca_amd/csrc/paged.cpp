@@ -9,7 +9,9 @@
 namespace {
 
 constexpr int kMostHeads = 32767;        // of either kind: both lie in one dimension of a grid
-constexpr int kMostRows = 1 << 30;       // and (row, head) pairs
+constexpr int kMostRows = 1 << 26;       // (a launch holds 2^32 threads)
+constexpr int kMostPairs = 1 << 30;      // of a row and a head; positions of a table's row
+constexpr int kMostLogits = 1 << 30;     // of a row
 constexpr int kMostSequences = 1 << 20;
 
 int log2_of(int x) {
@@ -39,7 +41,7 @@ int check_batch(const ahip_paged_batch* b, const ahip_paged_kv* c) {
     if (b->rows == 0 || b->sequences == 0) return AHIP_OK;  // (nothing runs)
     if (!b->row_starts || !b->lengths || !b->table) return bad("null batch array");
     if (((uintptr_t)b->row_starts | (uintptr_t)b->lengths | (uintptr_t)b->table) & 3) return bad("misaligned batch array");
-    if (b->table_stride <= 0 || (int64_t)b->table_stride * c->page_tokens > kMostRows)
+    if (b->table_stride <= 0 || (int64_t)b->table_stride * c->page_tokens > kMostPairs)
         return bad("a table's row must hold 1 to 2^30 tokens");
     return AHIP_OK;
 }
@@ -70,7 +72,7 @@ PagedSteps steps_of(const ahip_paged_batch& a) {
 
 int check_heads(const ahip_paged_batch& b, int heads) {
     if (heads > kMostHeads) return bad("query head count");
-    if ((int64_t)b.rows * heads > kMostRows) return failed(AHIP_ERR_UNSUPPORTED, "more than 2^30 queries a call");
+    if ((int64_t)b.rows * heads > kMostPairs) return failed(AHIP_ERR_UNSUPPORTED, "more than 2^30 queries a call");
     return AHIP_OK;
 }
 
@@ -97,6 +99,7 @@ extern "C" int ahip_paged_append(ahip_context* ctx, const ahip_paged_kv* cache, 
         if ((uintptr_t)rows->rope & 7) return bad("misaligned rotation table");
         if (rows->rope_positions <= 0) return bad("empty rotation table");
     }
+    if (rows->heads == 0 && (rows->q || rows->q_out)) return bad("queries of no heads");
     if (nothing(*batch)) return AHIP_OK;
     const int64_t width = (int64_t)cache->kv_heads * cache->head_dim, q_width = (int64_t)rows->heads * cache->head_dim;
     if (int rc = check_rows("keys", rows->k, rows->k_stride, width, rows->dtype)) return rc;
@@ -197,7 +200,7 @@ extern "C" int ahip_token_logprobs(ahip_context* ctx, const ahip_logprobs* args,
     if (!ctx || !args) return bad(ctx ? "null arguments" : "null context");
     const ahip_logprobs& a = *args;
     if (int rc = check_dtype(a.dtype)) return rc;
-    if (a.rows < 0 || a.vocab <= 0 || a.vocab > kMostRows) return bad("logits' shape");
+    if (a.rows < 0 || a.rows >= 1 << 24 || a.vocab <= 0 || a.vocab > kMostLogits) return bad("logits' shape");
     if (a.top < 0 || a.top > AHIP_LOGPROBS_MOST_TOP || a.top > a.vocab)
         return bad("top must be 0 to %d and at most the vocabulary", AHIP_LOGPROBS_MOST_TOP);
     if (a.rows == 0 || (!a.logprobs && !a.entropy && !a.top)) return AHIP_OK;

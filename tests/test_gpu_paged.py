@@ -467,6 +467,53 @@ def test_positions_without_a_page(hip_ctx, heads, tokens, dtype):
     assert (np.abs(got[3 * tokens:3 * tokens + 1].astype(np.float64) - want) <= bound).all()
 
 
+@pytest.mark.parametrize("dtype", ["f32", "f16"])
+@pytest.mark.parametrize("heads,kv_heads,new,n", [(4, 4, 3, 70), (64, 64, 300, 350), (16, 2, 300, 350)])
+def test_the_table_ends_inside_a_step(hip_ctx, heads, kv_heads, new, n, dtype):
+    """Queries past a table of an odd number of pages of 16 get NaN, those before it what they see; the other pages hold NaN."""
+    rng = np.random.default_rng(31)
+    b = Batch(rng, 16, [new], [n])
+    q = rows(rng, new, heads, 64, dtype)
+    cache = make(hip_ctx, b, kv_heads, 64)
+    with Device(hip_ctx) as dev:
+        data = fill(dev, cache, rng, b)
+        cut = n // 16 - 1 - (n // 16) % 2  # (odd: half a step)
+        assert cut % 2 == 1 and cut * 16 > n - new or new == 3
+        b.table, b.stride = np.ascontiguousarray(b.table[:, :cut]), cut
+        for i in set(range(b.pages)) - set(b.table.ravel().tolist()):
+            for buf in (cache._desc.k, cache._desc.v):
+                size = cache.bytes // 2 // b.pages
+                L.check(L.lib().ahip_memset(hip_ctx.handle, buf + i * size, 0xFF, size))
+        # (page 0 stands in for one that there is not: NaN there too, where the sequence does not have it)
+        got = attend(dev, cache, b.on(dev), q, dtype)
+    cache.close()
+    past = np.arange(n - new, n) >= cut * 16
+    assert np.array_equal(np.isnan(got).all((1, 2)), past) and np.isfinite(got[~past]).all()
+    if (~past).any():
+        some = [0, heads - 1]
+        want, bound = ref.attention(q, *data[0], n - new, dtype, heads=some)
+        assert (np.abs(got.astype(np.float64) - want) <= bound)[:, some][~past].all()
+
+
+@pytest.mark.parametrize("window", [0, 40, 2**30, 2**31 - 1])
+@pytest.mark.parametrize("heads,rows_more", [(4, 5), (64, 200)])
+def test_rows_of_negative_positions_beside_others(hip_ctx, heads, rows_more, window):
+    """More rows than the length says: zeros for those, the others' attention as it is, under any window."""
+    rng = np.random.default_rng(32)
+    n = 60 if heads == 4 else 150
+    b = Batch(rng, 16, [n + rows_more], [n])
+    q = rows(rng, b.rows, heads, 64, "f32")
+    cache = make(hip_ctx, b, heads, 64)
+    with Device(hip_ctx) as dev:
+        data = fill(dev, cache, rng, b)
+        got = attend(dev, cache, b.on(dev), q, "f32", window=window, sinks=window and 3)
+    cache.close()
+    assert (got[:rows_more] == 0).all()
+    some = [0, heads - 1]
+    want, bound = ref.attention(q[rows_more:], *data[0], 0, "f32", window, window and 3, heads=some)
+    assert (np.abs(got[rows_more:].astype(np.float64) - want) <= bound)[:, some].all()
+
+
 @pytest.mark.parametrize("heads,tokens", [(4, 3), (64, 300)])
 def test_batches_that_say_too_much_stay_inside_their_arrays(hip_ctx, heads, tokens):
     """Row starts past the rows or falling, lengths below 0 and far past the table: no row outside the arrays is touched,

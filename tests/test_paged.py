@@ -61,7 +61,7 @@ def refusals_of_a_batch(call):
     refused(call(lengths=None), "null batch array")
     refused(call(table=P + 2), "misaligned batch array")
     refused(call(rows=-1), "batch shape")
-    refused(call(rows=2**30 + 1), "batch shape")
+    refused(call(rows=2**26 + 1), "batch shape")
     refused(call(sequences=-1), "batch shape")
     refused(call(sequences=2**20 + 1), "batch shape")
     refused(call(max_rows=-1), "batch shape")
@@ -96,6 +96,7 @@ def test_append_refusals():
     refused(append(vs=1 << 40), "values: implausibly")
     refused(append(q=None), "null queries")
     refused(append(qo=None), "null query output")
+    refused(append(heads=0), "queries of no heads")
     refused(append(qos=255), "query output: stride")
 
 
@@ -149,6 +150,7 @@ def test_logprobs_refusals():
     refused(L.lib().ahip_token_logprobs(ctx, None, None, 0, None), "null arguments")
     refused(logprobs(dtype=L.Q4_0), "rows must be")
     refused(logprobs(rows=-1), "shape")
+    refused(logprobs(rows=2**24), "shape")
     refused(logprobs(vocab=0), "shape")
     refused(logprobs(vocab=2**30 + 1, stride=2**30 + 1), "shape")
     refused(logprobs(top=33), "top must be")
