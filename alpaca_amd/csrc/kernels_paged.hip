@@ -4,12 +4,17 @@
 // A pair of dims (a, b) of a head at position p becomes (a cos - b sin, a sin + b cos)
 // with the table's angle of (p, pair); pairs are adjacent dims or halves of the head.
 //
-// A workgroup of 256 threads takes one tile of 16 positions of a sequence and, over
-// grid.y, as many KV heads as have 16 lanes of 16 dims a token (or that many query
-// heads, a few times): a thread rotates 16 dims of one token, its 8 angles in
-// registers, and turns 8 tokens by 2 dims of the values.  Keys of a tile's 16 tokens
-// are written 256 bytes at a time, values 16 bytes where all 8 tokens are new and 2
-// where a group is only partly so.  Bound by memory, short of the launch for few rows.
+// A workgroup of 256 threads takes as many heads as have 16 lanes of 16 dims a token: KV
+// heads of one tile of 16 positions of a sequence, or query heads of 16 rows (one or four
+// times that many).  A thread rotates 16 dims of one token, its 8 angles in registers, and
+// turns 8 tokens by 2 dims of the values.  Keys of a tile's 16 tokens are written 256
+// bytes at a time, values 16 bytes where all 8 tokens are new and 2 where a group is
+// only partly so.
+//
+// Bound by memory: 4,096 f16 tokens of 32/8 heads of 128 with what reads them back 33 us (4.1
+// TB/s; 38 with a tile's workgroups on all XCDs, each of which then fetches its angles, and with
+// rows read one after the other).  Few rows: a chain of five round trips to memory, the
+// batch, the page, the angles, the rows and the stores, 4.3 us for one token of 9/3 heads of 64.
 #include "paged.h"
 
 namespace {
@@ -97,8 +102,8 @@ struct Place {
         return i >= 0 && i < seq.n ? seq.row0 + i : -1;
     }
 };
-__device__ __forceinline__ bool find_place(const PagedSteps& b, Place& p) {
-    const PagedItem it = paged_find(b, blockIdx.x, [&](const PagedSeq& q) {
+__device__ __forceinline__ bool find_place(const PagedSteps& b, int tile, Place& p) {
+    const PagedItem it = paged_find(b, tile, [&](const PagedSeq& q) {
         // (>> rounds down: rows of negative positions have tiles too)
         return ((q.length - 1) >> 4) - ((q.length - q.n) >> 4) + 1;
     });
@@ -114,8 +119,10 @@ struct AppendArgs {
     PagedRows r;
     PagedSteps b;
     PagedKV c;
-    int kv_slices;                    // of grid.y, query slices behind them
-    int lanes, at_once;               // 16-dim lanes of a head, heads at once
+    int tiles, kv_slices;  // workgroups: KV heads of tiles of positions, then
+    int blocks, q_slices;  // query heads of blocks of 16 rows
+    bool together;         // those of the same tokens on one XCD, whose cache then has their angles
+    int lanes, at_once;    // 16-dim lanes of a head, heads at once
     bool q_whole, k_whole, v_whole, out_whole, rope_whole;  // rows that lie on 16 bytes
 };
 
@@ -135,16 +142,55 @@ __device__ __forceinline__ void rotate(float (&x)[2][8], const float2 (&cs)[8], 
     }
 }
 
+// The position of each lane's row, 16 lanes a row; INT_MIN for a row of no sequence.
+__device__ __forceinline__ int position_of(const PagedSteps& b, int row) {
+    const int lane = __lane_id();
+    int pos = INT32_MIN;
+    for (int s0 = 0; s0 < b.sequences; s0 += 64) {
+        PagedSeq q{0, 0, 0};
+        if (s0 + lane < b.sequences) q = paged_seq(b, s0 + lane);
+#pragma unroll
+        for (int t = 0; t < 4; t++) {
+            const int r = __builtin_amdgcn_readlane(row, 16 * t);
+            const uint64_t has = __builtin_amdgcn_ballot_w64(r >= q.row0 && r < q.row0 + q.n);
+            if (!has) continue;
+            const int p = __builtin_amdgcn_readlane(q.length - q.n - q.row0, __builtin_ctzll(has)) + r;
+            if (lane >> 4 == t) pos = p;
+        }
+    }
+    return pos;
+}
+
 template <typename T, bool INTERLEAVED, int PASSES>
 __global__ __launch_bounds__(kThreads) void paged_append_kernel(AppendArgs p) {
     __shared__ uint32_t odd[16];  // a bit a head of the slice: tokens that have no form
-    Place at;
-    if (!find_place(p.b, at)) return;
+    int unit, slice;
+    bool queries;
+    if (p.together) {  // workgroups go round the 8 XCDs
+        const int slices = p.kv_slices + p.q_slices, eight = blockIdx.x / (8 * slices), i = blockIdx.x - eight * 8 * slices;
+        unit = 8 * eight + (i & 7), slice = i >> 3;
+        queries = slice >= p.kv_slices;
+        if (queries) slice -= p.kv_slices;
+    } else {
+        const int kv = p.tiles * p.kv_slices, units = (int)blockIdx.x < kv ? p.tiles : p.blocks;
+        queries = (int)blockIdx.x >= kv;
+        const int w = blockIdx.x - (queries ? kv : 0);
+        slice = w / units, unit = w - slice * units;
+    }
     // queries: the lanes of a token side by side, as their rows lie; keys: the tokens, as the pages do
-    const bool queries = (int)blockIdx.y >= p.kv_slices;
     const int hd = p.c.hd, lo = threadIdx.x & 15, hi = threadIdx.x >> 4, tok = queries ? hi : lo, u = queries ? lo : hi;
     const int lane = u % p.lanes, sub = u / p.lanes;
-    const int pos = at.tile * 16 + tok, row = at.row(pos);
+    Place at;
+    int pos, row;
+    if (queries) {
+        row = unit * 16 + tok;
+        pos = position_of(p.b, row);
+        if (pos == INT32_MIN) row = -1;
+    } else {
+        if (!find_place(p.b, unit, at)) return;
+        pos = at.tile * 16 + tok;
+        row = at.row(pos);
+    }
     int d[2];
     runs(lane, hd, INTERLEAVED, d);
     float2 cs[8];
@@ -170,7 +216,7 @@ __global__ __launch_bounds__(kThreads) void paged_append_kernel(AppendArgs p) {
     }
     if (queries) {
         if (row < 0 || sub >= p.at_once) return;
-        const int h = ((int)blockIdx.y - p.kv_slices) * p.at_once * PASSES + sub;
+        const int h = slice * p.at_once * PASSES + sub;
         const T* q = (const T*)p.r.q + row * p.r.q_stride + (int64_t)h * hd;
         T* out = (T*)p.r.q_out + row * p.r.q_out_stride + (int64_t)h * hd;
         const int64_t next = (int64_t)p.at_once * hd;
@@ -194,8 +240,23 @@ __global__ __launch_bounds__(kThreads) void paged_append_kernel(AppendArgs p) {
     if (page < 0) return;
     if (threadIdx.x < 16) odd[threadIdx.x] = 0;
     __syncthreads();
-    const int h0 = blockIdx.y * p.at_once, kvh = h0 + sub;
+    const int h0 = slice * p.at_once, kvh = h0 + sub;
     const bool mine = row >= 0 && sub < p.at_once && kvh < p.c.kv_heads;
+    // values: 2 dims of 8 tokens a thread
+    const int pairs = hd / 2, vi = threadIdx.x;
+    const int vsub = vi / (2 * pairs), half = (vi / pairs) & 1, dim = 2 * (vi % pairs);
+    const int vh = h0 + vsub, vpos = at.tile * 16 + 8 * half;
+    const bool values = vsub < p.at_once && vh < p.c.kv_heads;
+    float2 v[8];
+    int fresh = 0;
+    if (values) {
+#pragma unroll
+        for (int e = 0; e < 8; e++) {  // (a token that is not new: another's row, unused)
+            const int i = vpos + e - at.pos0, r = at.seq.row0 + min(max(i, 0), at.seq.n - 1);
+            fresh |= (i >= 0 && i < at.seq.n) << e;
+            v[e] = load_two((const T*)p.r.v + r * p.r.v_stride + (int64_t)vh * hd + dim, p.v_whole);
+        }
+    }
     f16x8 key[2];
     if (mine) {
         const T* k = (const T*)p.r.k + row * p.r.k_stride + (int64_t)kvh * hd;
@@ -210,26 +271,13 @@ __global__ __launch_bounds__(kThreads) void paged_append_kernel(AppendArgs p) {
         for (int e = 0; e < 8; e++) bad = bad || odd16(key[0][e]) || odd16(key[1][e]);
         if (bad) atomicOr(&odd[tok], 1u << sub);
     }
-    // values: 2 dims of 8 tokens a thread
-    const int pairs = hd / 2, vi = threadIdx.x;
-    const int vsub = vi / (2 * pairs), half = (vi / pairs) & 1, dim = 2 * (vi % pairs);
-    const int vh = h0 + vsub, vpos = at.tile * 16 + 8 * half;
-    const bool values = vsub < p.at_once && vh < p.c.kv_heads;
     f16x8 va = {}, vb = {};
-    int fresh = 0;
     if (values) {
-        float2 x[8];
-#pragma unroll
-        for (int e = 0; e < 8; e++) {  // (a token that is not new: another's row, unused)
-            const int i = vpos + e - at.pos0, r = at.seq.row0 + min(max(i, 0), at.seq.n - 1);
-            fresh |= (i >= 0 && i < at.seq.n) << e;
-            x[e] = load_two((const T*)p.r.v + r * p.r.v_stride + (int64_t)vh * hd + dim, p.v_whole);
-        }
 #pragma unroll
         for (int e = 0; e < 8; e++) {
             if (!(fresh >> e & 1)) continue;
-            va[e] = (f16)x[e].x;
-            vb[e] = (f16)x[e].y;
+            va[e] = (f16)v[e].x;
+            vb[e] = (f16)v[e].y;
             if (odd16(va[e]) || odd16(vb[e])) atomicOr(&odd[8 * half + e], 1u << vsub);
         }
     }
@@ -273,39 +321,49 @@ struct LoadArgs {
 
 template <typename T>
 __global__ __launch_bounds__(kThreads) void paged_load_kernel(LoadArgs p) {
+    __shared__ uint32_t odd[16];  // a bit a head of the slice: tokens without a form, whose keys are NaN
     Place at;
-    if (!find_place(p.b, at)) return;
+    if (!find_place(p.b, blockIdx.x, at)) return;
     const int hd = p.c.hd, tok = threadIdx.x & 15, u = threadIdx.x >> 4;
     const int lane = u % p.lanes, sub = u / p.lanes, h0 = blockIdx.y * p.at_once;
     const int page = paged_page(p.b, p.c, at.s, at.tile);  // (-1: NaN)
     const int kvh = h0 + sub, row = at.row(at.tile * 16 + tok);
-    if (p.k && row >= 0 && sub < p.at_once && kvh < p.c.kv_heads) {
+    if (threadIdx.x < 16) odd[threadIdx.x] = page < 0 ? ~0u : 0u;
+    __syncthreads();
+    const int pairs = hd / 2, vsub = threadIdx.x / (2 * pairs), half = (threadIdx.x / pairs) & 1;
+    const int dim = 2 * (threadIdx.x % pairs), vh = h0 + vsub;
+    const bool values = p.v && vsub < p.at_once && vh < p.c.kv_heads;
+    f16x8 va, vb, key[2];
+    if (values) {
+        const uint8_t* t = p.c.v + paged_tile(p.c, max(page, 0), vh, at.tile) * paged_tile_bytes(hd);
+        va = *(const AS_GLOBAL f16x8*)(t + (half * hd + dim) * 16);
+        vb = *(const AS_GLOBAL f16x8*)(t + (half * hd + dim) * 16 + 16);
+    }
+    const bool mine = row >= 0 && sub < p.at_once && kvh < p.c.kv_heads;
+    if (mine) {
         const uint8_t* t = p.c.k + paged_tile(p.c, max(page, 0), kvh, at.tile) * paged_tile_bytes(hd) + paged_key_slot(tok) * 16;
+#pragma unroll
+        for (int i = 0; i < 2; i++) key[i] = *(const AS_GLOBAL f16x8*)(t + (2 * lane + i) * 256);
+        if (lane == 0 && odd16(key[0][0])) atomicOr(&odd[tok], 1u << sub);
+    }
+    __syncthreads();
+    if (mine && p.k) {
         T* out = (T*)p.k + row * p.k_stride + (int64_t)kvh * hd + 16 * lane;
 #pragma unroll
         for (int i = 0; i < 2; i++) {
             float x[8];
-            const f16x8 y = *(const AS_GLOBAL f16x8*)(t + (2 * lane + i) * 256);
 #pragma unroll
-            for (int e = 0; e < 8; e++) x[e] = page < 0 ? NAN : (float)y[e];
+            for (int e = 0; e < 8; e++) x[e] = page < 0 ? NAN : (float)key[i][e];
             Lines<T>::store(out + 8 * i, x, p.k_whole);
         }
     }
-    const int pairs = hd / 2, vsub = threadIdx.x / (2 * pairs), half = (threadIdx.x / pairs) & 1;
-    const int dim = 2 * (threadIdx.x % pairs), vh = h0 + vsub;
-    if (!p.v || vsub >= p.at_once || vh >= p.c.kv_heads) return;
-    const int64_t tile = paged_tile(p.c, max(page, 0), vh, at.tile) * paged_tile_bytes(hd);
-    const f16* t = (const f16*)(p.c.v + tile) + (half * hd + dim) * 8;
-    const f16x8 a = *(const AS_GLOBAL f16x8*)t, b = *(const AS_GLOBAL f16x8*)(t + 8);
-    uint16_t key[8];  // a token without a form has NaN keys
-#pragma unroll
-    for (int e = 0; e < 8; e++) key[e] = gptr((const uint16_t*)(p.c.k + tile))[paged_key_slot(8 * half + e) * 8];
+    if (!values) return;
 #pragma unroll
     for (int e = 0; e < 8; e++) {
         const int r = at.row(at.tile * 16 + 8 * half + e);
         if (r < 0) continue;
-        const bool no = page < 0 || odd16(__builtin_bit_cast(f16, key[e]));
-        store_two((T*)p.v + r * p.v_stride + (int64_t)vh * hd + dim, no ? NAN : (float)a[e], no ? NAN : (float)b[e],
+        const bool no = odd[8 * half + e] >> vsub & 1;
+        store_two((T*)p.v + r * p.v_stride + (int64_t)vh * hd + dim, no ? NAN : (float)va[e], no ? NAN : (float)vb[e],
                   p.v_whole);
     }
 }
@@ -321,11 +379,18 @@ unsigned tiles_bound(const PagedSteps& b) {
 constexpr int64_t kManyValues = 1 << 21;
 
 template <typename T, int PASSES>
-hipError_t launch_append(const AppendArgs& p, hipStream_t st) {
+hipError_t launch_append(AppendArgs& p, hipStream_t st) {
     const int per = p.at_once * PASSES;
-    const dim3 grid(tiles_bound(p.b), p.kv_slices + (p.r.heads + per - 1) / per);
-    if (p.r.interleaved) paged_append_kernel<T, true, PASSES><<<grid, kThreads, 0, st>>>(p);
-    else paged_append_kernel<T, false, PASSES><<<grid, kThreads, 0, st>>>(p);
+    p.tiles = (int)tiles_bound(p.b);
+    p.blocks = (p.b.rows + 15) / 16;
+    p.q_slices = (p.r.heads + per - 1) / per;
+    p.together = p.r.rope && p.blocks >= 64 && p.b.rows >= 8ll * p.b.sequences;
+    // (there are at least as many tiles as blocks)
+    const int64_t grid = p.together ? (p.tiles + 7ll) / 8 * 8 * (p.kv_slices + p.q_slices)
+                                    : (int64_t)p.tiles * p.kv_slices + (int64_t)p.blocks * p.q_slices;
+    if (grid * kThreads > UINT32_MAX) return hipErrorInvalidConfiguration;  // (a launch holds no more threads)
+    if (p.r.interleaved) paged_append_kernel<T, true, PASSES><<<(unsigned)grid, kThreads, 0, st>>>(p);
+    else paged_append_kernel<T, false, PASSES><<<(unsigned)grid, kThreads, 0, st>>>(p);
     return hipGetLastError();
 }
 
