@@ -5,16 +5,15 @@
 // with the table's angle of (p, pair); pairs are adjacent dims or halves of the head.
 //
 // A workgroup of 256 threads takes as many heads as have 16 lanes of 16 dims a token: KV
-// heads of one tile of 16 positions of a sequence, or query heads of 16 rows (one or four
-// times that many).  A thread rotates 16 dims of one token, its 8 angles in registers, and
+// heads of one tile of 16 positions of a sequence, or query heads of 16 rows (once or
+// twice that many).  A thread rotates 16 dims of one token, its 8 angles in registers, and
 // turns 8 tokens by 2 dims of the values.  Keys of a tile's 16 tokens are written 256
 // bytes at a time, values 16 bytes where all 8 tokens are new and 2 where a group is
 // only partly so.
 //
 // Bound by memory: 4,096 f16 tokens of 32/8 heads of 128 with what reads them back 33 us (4.1
-// TB/s; 38 with a tile's workgroups on all XCDs, each of which then fetches its angles, and with
-// rows read one after the other).  Few rows: a chain of five round trips to memory, the
-// batch, the page, the angles, the rows and the stores, 4.3 us for one token of 9/3 heads of 64.
+// TB/s over both launches).  Few rows: a chain of five round trips to memory, the batch, the
+// page, the angles, the rows and the stores, 4.3 us for one token of 9/3 heads of 64.
 #include "paged.h"
 
 namespace {
@@ -376,6 +375,10 @@ unsigned tiles_bound(const PagedSteps& b) {
     return (unsigned)(t < b.rows ? t : b.rows);
 }
 
+// Two query heads a thread (f16), their angles read once and their rows under way together, from so many values on: 2,048
+// tokens of 32/8 heads of 128, written and read back, 17.9 us, of one head a thread 19.2; 4,096 of 32/32 heads of 64 46.7 and
+// 46.2; four heads as two.  f32, whose rows are twice as long: 4,096 of 32/8 heads of 128 56.4 and 55.4, of 32/32 heads of 64
+// 61.4 and 58.4 (four: 61.6 and 65.0); one.
 constexpr int64_t kManyValues = 1 << 21;
 
 template <typename T, int PASSES>
@@ -384,6 +387,8 @@ hipError_t launch_append(AppendArgs& p, hipStream_t st) {
     p.tiles = (int)tiles_bound(p.b);
     p.blocks = (p.b.rows + 15) / 16;
     p.q_slices = (p.r.heads + per - 1) / per;
+    // Where an XCD has several tiles of a sequence: 4,096 tokens as above 33.8 us, a tile's workgroups all over the chip
+    // 35.5, f32 of 32/32 heads of 64 57.2 and 61.2.  128 single tokens, each a tile and an eighth of a block: 13.8 and 10.7.
     p.together = p.r.rope && p.blocks >= 64 && p.b.rows >= 8ll * p.b.sequences;
     // (there are at least as many tiles as blocks)
     const int64_t grid = p.together ? (p.tiles + 7ll) / 8 * 8 * (p.kv_slices + p.q_slices)
@@ -410,11 +415,9 @@ hipError_t launch_paged_append(bool f16_rows, const PagedRows& r, const PagedSte
     p.v_whole = whole(r.v, r.v_stride, size);
     p.out_whole = whole(r.q_out, r.q_out_stride, size);
     p.rope_whole = whole(r.rope, 0, 8);
-    // Several heads a thread one after the other, their angles read once and their rows under way together, where that
-    // leaves enough workgroups.
-    if (r.heads > 2 * p.at_once && (int64_t)b.rows * r.heads * c.hd >= kManyValues)
-        return f16_rows ? launch_append<f16, 4>(p, st) : launch_append<float, 4>(p, st);
-    return f16_rows ? launch_append<f16, 1>(p, st) : launch_append<float, 1>(p, st);
+    if (!f16_rows) return launch_append<float, 1>(p, st);
+    const bool many = r.heads > p.at_once && (int64_t)b.rows * r.heads * c.hd >= kManyValues;
+    return many ? launch_append<f16, 2>(p, st) : launch_append<f16, 1>(p, st);
 }
 
 hipError_t launch_paged_load(bool f16_rows, const PagedSteps& b, const PagedKV& c, void* k, int64_t k_stride, void* v,
