@@ -91,7 +91,19 @@ SHAPES = [  # new, lengths
                                                     (160, 128, 2, 2), (192, 16, 1, 16), (224, 256, 3, 3), (256, 1024, 2, 4)])
 @pytest.mark.parametrize("case", range(len(SHAPES)))
 def test_append_rotates_and_load_reads_back(hip_ctx, case, hd, page, kv_heads, heads, dtype):
-    new, lengths = SHAPES[case]
+    check_append(hip_ctx, case, *SHAPES[case], hd, page, kv_heads, heads, dtype)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16"])
+@pytest.mark.parametrize("hd,page,kv_heads,heads,new,lengths", [
+    (64, 32, 32, 32, [1100], [1500]), (128, 16, 8, 40, [700, 0, 333, 90], [700, 5, 1000, 99]), (160, 64, 3, 7, [2100], [2101]),
+    (256, 16, 1, 9, [1030], [1030]), (128, 16, 8, 33, [1] * 520, [1 + i % 70 for i in range(520)])])
+def test_append_of_many_tokens(hip_ctx, hd, page, kv_heads, heads, new, lengths, dtype):
+    for case in range(3):
+        check_append(hip_ctx, case, new, lengths, hd, page, kv_heads, heads, dtype)
+
+
+def check_append(hip_ctx, case, new, lengths, hd, page, kv_heads, heads, dtype):
     rng = np.random.default_rng(100 * hd + case)
     b = Batch(rng, page, new, lengths, spare_rows=case % 3, lead=case % 2)
     extra, lead = [(0, 0), (16, 0), (3, 1)][case % 3]  # rows on 16 bytes, apart, and at any element
