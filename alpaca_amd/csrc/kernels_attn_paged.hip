@@ -144,10 +144,16 @@ __device__ __forceinline__ float load_queries(const T* q, float scale_log2, bool
 __device__ __forceinline__ float inverse(float l, bool past) { return past ? NAN : l == 0.f ? 0.f : 1.f / l; }
 
 // ------------------------------------------------------------------ few columns
-// Sequences of a few query columns, single tokens above all: bound by the pages' bytes.  16 columns of a
-// KV head are a workgroup's; each wave has steps of 32 keys of its own, whose tiles go from memory straight into
-// the products' operands, one step ahead.  The steps of one group of columns are split over workgroups, so that
-// all of them have like shares of the batch's work whatever its lengths, and the last one to arrive joins the parts.
+// Sequences of a few query columns, single tokens above all: bound by the pages' bytes.  16 columns of a KV head are a
+// workgroup's, the products 16x16x32 of which a single token of G query heads uses G columns: the matrix unit has room for
+// that, and nothing is read twice.  Each wave has steps of 32 keys of its own, whose tiles go from memory straight into the
+// products' operands, one step ahead; LDS would only add a trip.  The steps of one group of columns are split over
+// workgroups, so that all of them have like shares of the batch's work whatever its lengths, and the last one to arrive
+// joins the parts.
+//
+// 64 sequences of 32/8 heads of 128, 868 MB of pages, f16: 162 us, 5.3 TB/s (a copy reaches 5.0, a sum 5.8), matrix unit 4%
+// busy; one of 131,072 positions 99 us, 5.4 TB/s; 24 sequences with windows, 126 MB: 30.6 us, 4.1 TB/s, of which 5 are the
+// launch, the look for the work and the join.  A token of 9/3 heads of 64 at 2,000 positions: 8.1 us, a chain of such trips.
 
 // A workgroup's work: a group of 16 columns of sequence s, part sp of `splits`.
 struct FewItem {
@@ -439,12 +445,20 @@ __global__ __launch_bounds__(64 * kFewWaves) void paged_few_kernel(AttnArgs p) {
 }
 
 // ------------------------------------------------------------------ many columns
-// 32 CW query columns a workgroup, 32 a wave; the keys' tiles go by DMA into LDS as they lie in memory and are read as operands
-// without bank conflicts (16 bytes a lane in lane order).  Steps are of 32 keys, and a wave is one ahead with its scores: the
-// products of step i + 1's keys run beside the exponentials of step i, those of step i's values beside the maximum of step
-// i + 1's scores.  A stage of STEPS steps has one barrier; while its values and the keys of the step ahead of each are at
-// work, the next one's are under way.  SETS sets of CW waves take consecutive ranges of the steps and join through LDS at the
-// end.
+// 32 CW query columns a workgroup, 32 a wave, products 32x32x16; the keys' tiles go by DMA into LDS as they lie in memory and
+// are read as operands without bank conflicts (16 bytes a lane in lane order).  Steps are of 32 keys, and a wave is one ahead
+// with its scores: the products of step i + 1's keys run beside the exponentials of step i, those of step i's values beside the
+// maximum of step i + 1's scores.  A stage of STEPS steps has one barrier; while its values and the keys of the step ahead of
+// each are at work, the next one's are under way.  SETS sets of CW waves take consecutive ranges of the steps and join through
+// LDS at the end.  KV heads are the fastest index of the grid, so that the workgroups of 8 of them have an XCD's L2 each for
+// their pages.
+//
+// Bound by the two units that share a SIMD's issue.  4,096 f16 tokens of 32/8 heads of 128: 157-171 us on different cards,
+// 800-870 TFLOP/s (a library product of 8,192: 1,176), matrix unit 42% busy and vector unit 45% of the cycles, 7.4 vector
+// instructions a matrix one, no bank conflicts; without its LDS reads it would take 0.93 of that, without its exponentials
+// 0.91, without its loads 0.85, with none of them 0.73.  float32 has two products for each of these (two f16 terms of the
+// queries, two of the probabilities): three chunks of 2,500 tokens with windows of 1,024, 24/8 heads of 128, 185-199 us, 78
+// GFLOP once and 156 as they are done, 790-840 TFLOP/s, matrix unit 50% busy.
 template <int NB, int CW, int SETS>
 struct Wide {
     static constexpr int HD = 32 * NB, TILE = paged_tile_bytes(HD), KEYS = 32, STEP = 2 * TILE;
@@ -786,7 +800,8 @@ constexpr int wide_waves(int nb, bool exact) { return nb <= (exact ? 4 : 6) ? 2 
 
 // The sequences of many columns, then those of few, in one launch.
 template <int NB, int CW, int SETS, typename T>
-__global__ __launch_bounds__(64 * CW * SETS) __attribute__((amdgpu_waves_per_eu(wide_waves(NB, sizeof(T) == 4), 2))) void paged_mixed_kernel(AttnArgs p) {
+__global__ __launch_bounds__(64 * CW * SETS)
+__attribute__((amdgpu_waves_per_eu(wide_waves(NB, sizeof(T) == 4), 2))) void paged_mixed_kernel(AttnArgs p) {
     extern __shared__ __align__(16) uint8_t lds[];
     if ((int)blockIdx.x < p.wide_grid) wide_part<NB, CW, SETS, T>(p, lds);
     else few_part<NB, T>(p, blockIdx.x - p.wide_grid, lds);
@@ -827,18 +842,20 @@ hipError_t launch_mixed(AttnArgs& p, hipStream_t st) {
 // How a call runs, by the workgroups that the batch's columns make; the lengths are on the device, and the shares of the
 // few-column part are chosen there.  us, one card:
 //
-// The many-column part, where its workgroups nearly fill the chip.  Of 128 columns and one set of waves, two a CU, from one a
-// CU on (two sets: 1,000 tokens and 31 single ones, 32/8 heads of 128, f16: 114 and 131; 2,048 tokens 60 and 58); of 128 and two
-// sets, where workgroups of 64 are more than the CUs (600 tokens at 4,096: 74, of 64 columns 96; 1,000: 82 and 98); of 64 and four
-// sets from 1.6 CUs of them on, in units of 32 dims (300 tokens at 4,096: 53, the few-column part 65; 512 of 32/32 heads of 64:
-// 41 and 46; but 1,000 of 9/3 heads of 64: 39 and 33).  Where most workgroups are of sequences of few columns, one set of 128
-// leaves them the most room (512 tokens of 32/32 heads of 64 and 31 single ones: 97, two sets 106, 64 columns 125).
-// One sequence's 256 columns, one workgroup a CU, where the short ones of their second round fill it behind the long ones
-// of the first (32/8 heads of 128, f16: 4,096 tokens 160 and 170, 3,500 126 and 132; but 3,000 104 and 98, 5,000 256 and 242).
+// The many-column part, where its workgroups nearly fill the chip. Of 128 columns and one set of waves, two a CU, from one a
+// CU on (two sets: 1,000 tokens and 31 single ones, 32/8 heads of 128, f16: 114 and 131; 2,048 tokens 60 and 58); of 128 and
+// two sets, where workgroups of 64 are more than the CUs (600 tokens at 4,096: 74, of 64 columns 96; 1,000: 82 and 98); of
+// 64 and four sets from 1.6 CUs of them on, in units of 32 dims (300 tokens at 4,096: 53, the few-column part 65; 512 of
+// 32/32 heads of 64: 41 and 46; but 1,000 of 9/3 heads of 64: 39 and 33). Where most workgroups are of sequences of few
+// columns, one set of 128 leaves them the most room (512 tokens of 32/32 heads of 64 and 31 single ones: 97, two sets 106,
+// 64 columns 125). One sequence's 256 columns, one workgroup a CU, where the short ones of their second round fill it behind
+// the long ones of the first (32/8 heads of 128, f16: 4,096 tokens 160 and 170, 3,500 126 and 132; but 3,000 104 and 98,
+// 5,000 256 and 242).
 //
-// The few-column part alone: four waves a workgroup (one token of 9/3 heads of 64 at 2,000 positions 8.1, eight waves 8.6), a
-// workgroup a CU, or two where groups of columns are half as many (64 sequences of 32/8 heads of 128: 163 and 178; 16 of 16/8
-// heads of 256 at 4,096 49 and 53; one of 32/8 heads of 128 at 131,072: 102 and 99, of 16/8 heads of 256 at 30,000 54 and 51).
+// The few-column part alone: four waves a workgroup (one token of 9/3 heads of 64 at 2,000 positions 8.1, eight waves 8.6),
+// a workgroup a CU, or two where groups of columns are half as many (64 sequences of 32/8 heads of 128: 163 and 178; 16 of
+// 16/8 heads of 256 at 4,096 49 and 53; one of 32/8 heads of 128 at 131,072: 102 and 99, of 16/8 heads of 256 at 30,000 54
+// and 51).
 template <int NB, typename T>
 hipError_t launch_nb(AttnArgs& p, hipStream_t st) {
     const int64_t cus = device_cus(), cols = (int64_t)p.b.rows * p.G, KVH = p.c.kv_heads;

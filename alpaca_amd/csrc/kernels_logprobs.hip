@@ -14,6 +14,11 @@
 //
 // Few rows are split over workgroups, whose triples and best tokens the last one to arrive
 // joins in the same launch.
+//
+// 2,048 float32 rows of 49,152, 403 MB: 70 us without top tokens (5.8 TB/s, what a plain sum
+// reaches), 81 with 20, for which 5% more is read and a workgroup's memory idles while it ranks
+// them.  One row: 8.4 us with 5 of them, 5.0 without, the launch, one trip to memory and the
+// chain of joins.
 #include "logprobs.h"
 
 #include <algorithm>

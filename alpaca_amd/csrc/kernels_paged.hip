@@ -13,7 +13,7 @@
 //
 // Bound by memory: 4,096 f16 tokens of 32/8 heads of 128 with what reads them back 33 us (4.1
 // TB/s over both launches).  Few rows: a chain of five round trips to memory, the batch, the
-// page, the angles, the rows and the stores, 4.3 us for one token of 9/3 heads of 64.
+// page, the angles, the rows and the stores, 4.5 us for one token of 9/3 heads of 64.
 #include "paged.h"
 
 namespace {
@@ -318,6 +318,8 @@ struct LoadArgs {
     bool k_whole, v_whole;
 };
 
+// Back into rows: a tile a workgroup as above, all its loads under way before the first is used; 4,096 tokens of 8 heads of
+// 128 into f16 8.4 us, the bytes of 6.7.
 template <typename T>
 __global__ __launch_bounds__(kThreads) void paged_load_kernel(LoadArgs p) {
     __shared__ uint32_t odd[16];  // a bit a head of the slice: tokens without a form, whose keys are NaN
