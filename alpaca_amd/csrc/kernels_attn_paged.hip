@@ -152,7 +152,7 @@ __device__ __forceinline__ float inverse(float l, bool past) { return past ? NAN
 // joins the parts.
 //
 // 64 sequences of 32/8 heads of 128, 868 MB of pages, f16: 162 us, 5.3 TB/s (a copy reaches 5.0, a sum 5.8), matrix unit 4%
-// busy; one of 131,072 positions 99 us, 5.4 TB/s; 24 sequences with windows, 126 MB: 30.6 us, 4.1 TB/s, of which 5 are the
+// busy; one of 131,072 positions 99 us, 5.4 TB/s; 24 sequences with windows, 126 MB: 29.1 us, 4.3 TB/s, of which 5 are the
 // launch, the look for the work and the join.  A token of 9/3 heads of 64 at 2,000 positions: 8.1 us, a chain of such trips.
 
 // A workgroup's work: a group of 16 columns of sequence s, part sp of `splits`.
@@ -175,13 +175,32 @@ __device__ __forceinline__ FewItem few_find(const AttnArgs& p, int w) {
     // steps a workgroup: all the batch's over the workgroups aimed for.  (float: the same sum in every wave)
     const PagedSeq front = seq_of(0);  // (all of a batch of up to 64)
     const FewCount front_count = few_count(p, front);
-    float all = (float)front_count.groups * (float)front_count.steps;
+    float all = (float)front_count.groups * (float)front_count.steps, groups_all = (float)front_count.groups;
     for (int s0 = 64; s0 < S; s0 += 64) {
         const FewCount f = few_count(p, seq_of(s0));
         all += (float)f.groups * (float)f.steps;
+        groups_all += (float)f.groups;
     }
-    all = wave_sum(all) * (float)KVH;
-    const int share = max(kFewLeast, (int)fminf(all * 1.0001f / (float)p.target + 1.f, 1e9f));
+    all = wave_sum(all) * (float)KVH * 1.0001f;
+    const float target = (float)p.target;
+    int share = (int)fminf(all / target + 1.f, 1e9f);
+    if (share <= kFewLeast) {
+        share = kFewLeast;
+    } else if (groups_all = wave_sum(groups_all) * (float)KVH; 2.f * groups_all <= target) {
+        // Last parts that are not full make these up to groups_all more than aimed for, and a CU that has one more ends last.
+        // So the least share that makes no more (of a batch of more than 64 sequences, one that makes no more): 8 of 32/8 heads
+        // of 128 at up to 16,000 47 us and not 58, two at up to 60,000 76 and 99.  Of more groups that would leave too few to
+        // split: 96 sequences of 8/4 heads of 64, 384 groups of 512, 46 and not 37.6.
+        int most = max(share, (int)fminf(all / (target - groups_all) + 1.f, 1e9f));
+        for (int i = 0; i < 5 && share < most && S <= 64; i++) {
+            const int mid = (share + most) >> 1;
+            const float parts = ceilf((float)front_count.steps * (0.999999f / (float)mid));
+            const bool fits = wave_sum((float)front_count.groups * parts) * (float)KVH <= target;
+            most = fits ? mid : most;
+            share = fits ? share : mid + 1;
+        }
+        share = most;
+    }
     FewItem r{0, 0, 0, 0, 0, 0, 0, {0, 0, 0}};
     for (int s0 = 0; s0 < S; s0 += 64) {
         PagedSeq q = front;
@@ -853,9 +872,9 @@ hipError_t launch_mixed(AttnArgs& p, hipStream_t st) {
 // 5,000 256 and 242).
 //
 // The few-column part alone: four waves a workgroup (one token of 9/3 heads of 64 at 2,000 positions 8.1, eight waves 8.6),
-// a workgroup a CU, or two where groups of columns are half as many (64 sequences of 32/8 heads of 128: 163 and 178; 16 of
-// 16/8 heads of 256 at 4,096 49 and 53; one of 32/8 heads of 128 at 131,072: 102 and 99, of 16/8 heads of 256 at 30,000 54
-// and 51).
+// a workgroup a CU, or two where groups of columns are half as many (64 sequences of 32/8 heads of 128: 162 and 178; 24 at
+// up to 4,000 39 and 45; 12 at up to 12,000, 96 groups, 50 and 50; two at up to 60,000 78.6 and 76.3; one at 131,072 102 and
+// 99, of 16/8 heads of 256 at 30,000 54 and 51).
 template <int NB, typename T>
 hipError_t launch_nb(AttnArgs& p, hipStream_t st) {
     const int64_t cus = device_cus(), cols = (int64_t)p.b.rows * p.G, KVH = p.c.kv_heads;

@@ -334,6 +334,16 @@ def test_attention_of_many_sequences(hip_ctx, dtype):
     attention_case(hip_ctx, 4, 2, 64, 16, new, lengths, dtype, hint=False, window=50, sinks=3)
 
 
+@pytest.mark.parametrize("dtype", ["f32", "f16"])
+@pytest.mark.parametrize("sequences,kv_heads,longest", [(2, 2, 20000), (20, 1, 8000), (64, 1, 3000), (65, 1, 3000), (100, 1, 2500),
+                                                        (140, 1, 2000)])
+def test_attention_split_evenly_whatever_the_lengths(hip_ctx, sequences, kv_heads, longest, dtype):
+    """Shares of more than a few steps, below and above a wave's lanes and half of the workgroups."""
+    rng = np.random.default_rng(sequences)
+    lengths = [longest] + [int(n) for n in rng.integers(longest // 3, longest, sequences - 1)]
+    attention_case(hip_ctx, 2 * kv_heads, kv_heads, 64, 32, [1] * sequences, lengths, dtype)
+
+
 # (heads, kv_heads, hd, page, new, lengths): chips full of workgroups of 256, 128 and 64 columns, with sequences of few
 # columns among them
 WIDE = [(64, 64, 64, 16, [700, 1, 513], [700, 300, 600]), (96, 96, 32, 64, [300, 5, 410], [431, 6, 410]),
