@@ -38,6 +38,7 @@ struct AttnArgs {
     float* partials;
     int* counters;
     int wide_grid;   // workgroups of the many-column part
+    int wide_parts;  // that a group of its columns may be split into
     int few_columns; // sequences of more query columns are the many-column part's
     int target;      // workgroups that the few-column part aims for
     bool whole_q, whole_out;  // rows that lie on 16 bytes
@@ -49,6 +50,7 @@ constexpr int kFewWaves = 4;       // of a workgroup of the few-column part alon
 constexpr int kManyColumns = 64;   // sequences of more columns take the many-column part
 constexpr int kMostTarget = kPagedCounters;       // split groups of columns at most
 constexpr int kMostSlots = 2 * kMostTarget + 64;  // their parts
+constexpr __host__ __device__ int few_slots(int target) { return 2 * target + 64; }  // of them, the few-column part's
 
 // The steps of `step` keys that queries at first..last see: the first tokens' ones, then a range.
 struct Steps {
@@ -228,7 +230,7 @@ __device__ __forceinline__ FewItem few_find(const AttnArgs& p, int w) {
             r.counter += of(joint_to - joint) + at;
             r.slot += of(parts_to - parts) + at * r.splits;
             // (only row ranges that overlap could have more)
-            if (r.splits > 1 && (r.counter >= p.target || r.slot + r.splits > 2 * p.target + 64)) r.splits = 0;
+            if (r.splits > 1 && (r.counter >= p.target || r.slot + r.splits > few_slots(p.target))) r.splits = 0;
             return r;
         }
         w -= __builtin_amdgcn_readlane(upto, 63);
@@ -469,8 +471,9 @@ __global__ __launch_bounds__(64 * kFewWaves) void paged_few_kernel(AttnArgs p) {
 // with its scores: the products of step i + 1's keys run beside the exponentials of step i, those of step i's values beside the
 // maximum of step i + 1's scores.  A stage of STEPS steps has one barrier; while its values and the keys of the step ahead of
 // each are at work, the next one's are under way.  SETS sets of CW waves take consecutive ranges of the steps and join through
-// LDS at the end.  KV heads are the fastest index of the grid, so that the workgroups of 8 of them have an XCD's L2 each for
-// their pages.
+// LDS at the end; those of four sets may be workgroups' parts of the steps, which the last one to arrive joins, as the
+// few-column part's are.  KV heads are the fastest index of the grid, so that the workgroups of 8 of them have an XCD's L2
+// each for their pages.
 //
 // Bound by the two units that share a SIMD's issue.  4,096 f16 tokens of 32/8 heads of 128: 157-171 us on different cards,
 // 800-870 TFLOP/s (a library product of 8,192: 1,176), matrix unit 42% busy and vector unit 45% of the cycles, 7.4 vector
@@ -483,6 +486,7 @@ struct Wide {
     static constexpr int HD = 32 * NB, TILE = paged_tile_bytes(HD), KEYS = 32, STEP = 2 * TILE;
     static constexpr int STEPS = NB <= 4 && SETS <= 2 ? 2 : 1;  // of a stage
     static constexpr int COLS = 32 * CW;
+    static constexpr bool SPLIT = SETS == 4 && NB >= 3;  // the steps over workgroups, where columns make too few
     static constexpr int JOIN = SETS > 1 ? COLS * (HD + 4) * 4 + COLS * 8 : 0;  // a set's outputs and statistics
     static constexpr int SIDE = 2 * STEPS * STEP;  // two stages of keys, or of values
     static constexpr int RING = 2 * SETS * SIDE;
@@ -493,6 +497,8 @@ struct Wide {
 // P enters the products as P 2^9 and a column's reference follows its maximum only when that is 2^6 past it, which
 // few steps are.
 constexpr float kWideLog2P = 9.f, kSlack = 6.f;
+// Parts of the steps: a part and the joining cost about 6 us, so that 600 positions (19 steps) stay whole: 18 us, in two 25.
+constexpr int kWideLeast = 16;  // steps of a part
 
 template <int NB, int CW, int SETS, typename T>
 __device__ __forceinline__ void wide_part(const AttnArgs& p, uint8_t* lds) {
@@ -502,8 +508,9 @@ __device__ __forceinline__ void wide_part(const AttnArgs& p, uint8_t* lds) {
     typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
     const int lane = threadIdx.x & 63, half = lane >> 5, c32 = lane & 31;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), set = wave / CW, wl = wave % CW;
-    const int KVH = p.c.kv_heads, kvh = blockIdx.x % KVH;
-    const PagedItem it = paged_find(p.b, blockIdx.x / KVH, [&](const PagedSeq& q) {
+    const int KVH = p.c.kv_heads, kvh = blockIdx.x % KVH, w = blockIdx.x / KVH;
+    const int sp = W::SPLIT ? w % p.wide_parts : 0, item = W::SPLIT ? w / p.wide_parts : w;
+    const PagedItem it = paged_find(p.b, item, [&](const PagedSeq& q) {
         const int64_t cols = (int64_t)q.n * p.G;
         return cols > p.few_columns ? (int)((cols + W::COLS - 1) / W::COLS) : 0;
     });
@@ -517,9 +524,13 @@ __device__ __forceinline__ void wide_part(const AttnArgs& p, uint8_t* lds) {
     const int wcol0 = min(col0 + wl * 32, cols - 1);  // the wave's columns
     const int w_first = pos0 + p.by_group(wcol0), w_last = pos0 + p.by_group(min(wcol0 + 31, cols - 1));
     const Steps steps = steps_of(p, first, last, KEYS);
-    const int per = (steps.count + SETS - 1) / SETS, f0 = set * per;
+    // the workgroup's part of the steps, and the set's of those
+    const int parts = W::SPLIT ? max(1, min(p.wide_parts, steps.count / kWideLeast)) : 1;
+    const int each = (steps.count + parts - 1) / parts, end = min(steps.count, (sp + 1) * each);
+    if (W::SPLIT && sp >= parts) return;
+    const int per = max(0, end - sp * each + SETS - 1) / SETS, f0 = sp * each + set * per;
     // the wave's steps: of its set's those that one of its columns sees
-    const int count = max(0, min(min(steps.count, steps_of(p, first, w_last, KEYS).count) - f0, per));
+    const int count = max(0, min(min(end, steps_of(p, first, w_last, KEYS).count) - f0, per));
 
     const int col = min(col0 + wl * 32 + c32, cols - 1), t = p.by_group(col), pos = pos0 + t;
     f16x8 qh[2 * NB], ql[EXACT ? 2 * NB : 1];
@@ -792,8 +803,56 @@ __device__ __forceinline__ void wide_part(const AttnArgs& p, uint8_t* lds) {
                     }
             }
         }
-        if (set) return;
+        if (parts == 1 && set) return;
     }
+    if constexpr (W::SPLIT)
+        if (parts > 1) {
+            // the last part of the columns to arrive joins them all
+            const int group = item * KVH + kvh, here = min(cols - col0, W::COLS), c = wl * 32 + c32;
+            const int64_t slot = few_slots(p.target) + (int64_t)group * p.wide_parts * (W::COLS / kFewCols);
+            float* const part = p.partials + slot * kFewCols * (HD + 2);
+            float* xo = (float*)lds;  // rows by way of LDS, so that a wave's stores lie side by side
+            float* xml = xo + W::COLS * (HD + 4);
+            if (set == 0) {
+#pragma unroll
+                for (int d = 0; d < NB; d++)
+#pragma unroll
+                    for (int u = 0; u < 4; u++)
+                        *(f32x4*)&xo[c * (HD + 4) + 32 * d + 8 * u + 4 * half] =
+                            f32x4{o[d][4 * u], o[d][4 * u + 1], o[d][4 * u + 2], o[d][4 * u + 3]};
+                if (half == 0) {
+                    xml[2 * c] = m;
+                    xml[2 * c + 1] = l;
+                }
+            }
+            __syncthreads();
+            for (int i = threadIdx.x; i < here * (HD / 2); i += 64 * CW * SETS) {
+                const int jc = i / (HD / 2), d = 2 * (i % (HD / 2));
+                float* x = part + (int64_t)(jc * parts + sp) * (HD + 2);
+                put2(x + 2 + d, xo[jc * (HD + 4) + d], xo[jc * (HD + 4) + d + 1]);
+                if (d == 0) put2(x, xml[2 * jc], xml[2 * jc + 1]);
+            }
+            int* arrived = (int*)lds;
+            __builtin_amdgcn_s_waitcnt(0);
+            __syncthreads();
+            if (threadIdx.x == 0) {
+                int* counter = p.counters + p.target + group;
+                *arrived = __hip_atomic_fetch_add(counter, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == parts - 1;
+                if (*arrived) __hip_atomic_store(counter, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            }
+            __syncthreads();
+            if (!*arrived) return;
+            for (int i = threadIdx.x; i < here * (HD / 2); i += 64 * CW * SETS) {
+                const int jc = i / (HD / 2), d = 2 * (i % (HD / 2));
+                const Joined r = join<4>(part + (int64_t)jc * parts * (HD + 2), HD, d, 0, 1, parts);
+                const int u = p.by_group(col0 + jc), h = kvh * p.G + col0 + jc - u * p.G;
+                const float inv = inverse(r.l, pos0 + u >= p.most);
+                T* out = (T*)p.a.out + (int64_t)(seq.row0 + u) * p.a.out_stride + (int64_t)h * HD + d;
+                gptr(out)[0] = (T)(r.a * inv);
+                gptr(out)[1] = (T)(r.b * inv);
+            }
+            return;
+        }
     if (col0 + wl * 32 + c32 >= cols) return;
     const float inv = inverse(l, pos >= p.most);
     T* out = (T*)p.a.out + (int64_t)(seq.row0 + t) * p.a.out_stride + (int64_t)(kvh * p.G + col - t * p.G) * HD + 4 * half;
@@ -854,6 +913,13 @@ hipError_t launch_mixed(AttnArgs& p, hipStream_t st) {
     const int64_t groups = cols / W::COLS + std::min<int64_t>(p.b.sequences, cols / kManyColumns);
     if (groups * p.c.kv_heads > INT32_MAX) return hipErrorInvalidConfiguration;
     p.wide_grid = (int)(groups * p.c.kv_heads);
+    p.wide_parts = 1;
+    if constexpr (W::SPLIT)
+        if (p.wide_grid > 0 && p.wide_grid <= kMostTarget - p.target) {
+            const int most = (kMostSlots - few_slots(p.target)) / (W::COLS / kFewCols);
+            p.wide_parts = std::max(1, std::min(device_cus(), most) / p.wide_grid);
+            p.wide_grid *= p.wide_parts;
+        }
     return launch_one<paged_mixed_kernel<NB, CW, SETS, T>>(p, p.wide_grid + few_grid(p, kManyColumns), 64 * CW * SETS,
                                                           W::LDS, st);
 }
@@ -865,7 +931,10 @@ hipError_t launch_mixed(AttnArgs& p, hipStream_t st) {
 // CU on (two sets: 1,000 tokens and 31 single ones, 32/8 heads of 128, f16: 114 and 131; 2,048 tokens 60 and 58); of 128 and
 // two sets, where workgroups of 64 are more than the CUs (600 tokens at 4,096: 74, of 64 columns 96; 1,000: 82 and 98); of
 // 64 and four sets from 1.6 CUs of them on, in units of 32 dims (300 tokens at 4,096: 53, the few-column part 65; 512 of
-// 32/32 heads of 64: 41 and 46; but 1,000 of 9/3 heads of 64: 39 and 33). Where most workgroups are of sequences of few
+// 32/32 heads of 64: 41 and 46; but 1,000 of 9/3 heads of 64: 39 and 33); from 1.1 where heads of 96 and more have tables of
+// 2,048 positions and more, whose steps are split (150 tokens at 4,096: 33, the few-column part 52, at 16,000 75 and 122;
+// 100 beside 31 single ones 68 and 83; but 140 at 600: 25 and 23, and of 32/32 heads of 64, where nothing is left to split,
+// 140 at 2,500: 28 and 23). 200 tokens at 4,096, in two parts: 39, in one 52. Where most workgroups are of sequences of few
 // columns, one set of 128 leaves them the most room (512 tokens of 32/32 heads of 64 and 31 single ones: 97, two sets 106,
 // 64 columns 125). One sequence's 256 columns, one workgroup a CU, where the short ones of their second round fill it behind
 // the long ones of the first (32/8 heads of 128, f16: 4,096 tokens 160 and 170, 3,500 126 and 132; but 3,000 104 and 98,
@@ -894,7 +963,7 @@ hipError_t launch_nb(AttnArgs& p, hipStream_t st) {
         if constexpr (two)
             if (groups(64) > cus) return launch_mixed<NB, 4, 2, T>(p, st);
         if constexpr (NB <= 4)
-            if (5 * groups(64) * NB >= 8 * cus) return launch_mixed<NB, 2, 4, T>(p, st);
+            if (10 * groups(64) * NB >= (NB >= 3 && p.most >= 2048 ? 11 : 16) * cus) return launch_mixed<NB, 2, 4, T>(p, st);
     }
     p.few_columns = INT32_MAX;
     const int64_t grid = few_grid(p, cols);
@@ -936,6 +1005,7 @@ hipError_t launch_paged_attention(bool f16_rows, const PagedAttention& a, const 
     p.counters = (int*)a.workspace;
     p.partials = (float*)((uint8_t*)a.workspace + kMostTarget * 4);
     p.wide_grid = 0;
+    p.wide_parts = 1;
     const int size = f16_rows ? 2 : 4;
     auto whole = [&](const void* x, int64_t stride) { return !(((uintptr_t)x | (uint64_t)stride * size) & 15); };
     p.whole_q = whole(a.q, a.q_stride);

@@ -363,6 +363,22 @@ def test_attention_of_many_columns(hip_ctx, case, dtype):
                    some_heads=some)
 
 
+# turns of a long context, whose keys workgroups share, with shorter sequences among them
+TURNS = [(32, 8, 128, 64, [200], [4200]), (32, 8, 128, 16, [150, 1, 1], [3000, 2100, 7]), (16, 4, 96, 32, [400], [2500]),
+         (24, 8, 96, 16, [180, 17], [2048, 1700]), (32, 8, 128, 128, [100] + [1] * 31, [4000] + [9] * 31),
+         (64, 8, 128, 16, [90], [90]), (16, 16, 128, 16, [70, 70, 70], [70, 1100, 2200])]
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16"])
+@pytest.mark.parametrize("window,sinks", [(0, 0), (1500, 4), (20, 0)])
+@pytest.mark.parametrize("case", range(len(TURNS)))
+def test_attention_of_turns_of_a_long_context(hip_ctx, case, window, sinks, dtype):
+    heads, kv_heads, hd, page, new, lengths = TURNS[case]
+    some = [0, heads // 2, heads - 1]
+    attention_case(hip_ctx, heads, kv_heads, hd, page, new, lengths, dtype, extra=[0, 8, 3][case % 3], lead=case % 2,
+                   window=window, sinks=sinks, some_heads=some)
+
+
 @pytest.mark.parametrize("dtype", ["f32", "f16"])
 @pytest.mark.parametrize("hd", [160, 192, 224, 256])
 def test_attention_of_many_columns_of_wide_heads(hip_ctx, hd, dtype):
@@ -605,6 +621,27 @@ def test_attention_twice_gives_the_same_bits(hip_ctx):
             attend(dev, cache, on, q, "f32", workspace=(mine[0], need - 1))
     cache.close()
     assert np.array_equal(a.view(np.uint32), c.view(np.uint32))
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16"])
+def test_one_workspace_serves_turns_and_single_tokens_in_turn(hip_ctx, dtype):
+    rng = np.random.default_rng(20)
+    full = Batch(rng, 64, [0] * 3, [5000, 3000, 100])
+    cache = make(hip_ctx, full, 8, 128)
+    with Device(hip_ctx) as dev:
+        fill(dev, cache, rng, full)
+        need = cache.workspace_bytes()
+        one = dev.empty(need, 0xFF)
+        L.check(L.lib().ahip_memset(hip_ctx.handle, one, 0, PAGED_WORKSPACE_ZERO))
+        for new, lengths in [([200], [5000]), ([1, 1], [5000, 2999]), ([150, 1, 1], [5000, 3000, 100]), ([200], [5000])] * 2:
+            b = Batch(rng, 64, new, lengths, full.pages, stride=full.stride)
+            b.table = full.table[:len(new)].copy()
+            q = rows(rng, b.rows, 32, 128, dtype)
+            a = attend(dev, cache, b.on(dev), q, dtype, workspace=(one, need))
+            c = attend(dev, cache, b.on(dev), q, dtype)
+            assert np.isfinite(a).all() and np.array_equal(a.view(np.uint8), c.view(np.uint8)), (new, lengths)
+            assert not dev.get(one, PAGED_WORKSPACE_ZERO, np.uint8).any()
+    cache.close()
 
 
 def test_one_workspace_serves_batches_of_every_shape_in_turn(hip_ctx):
