@@ -630,11 +630,15 @@ __device__ __forceinline__ void wide_part(const AttnArgs& p, uint8_t* lds) {
                 if (!sees(p, pos, key0 + 8 * half + 16 * (r >> 3) + (r & 7))) x[r] = -INFINITY;
         }
     };
-    // Values of 0 at positions that no column of the workgroup sees, where they may never have been written or be another
-    // sequence's: 0 times what lies there may be NaN.  (The waves of a set write the same.)
+    // Values of 0 at positions that no column of the workgroup sees, where they may never have been written, be another
+    // sequence's or stand for a page that there is not: 0 times what lies there may be NaN.  (The waves of a set write the
+    // same.)  A step past `last`, where `holes` has not looked, is left as it is if all of it has pages and is the
+    // sequence's: cleared in any case, three chunks of 2,500 f32 tokens with windows took 193 us and not 187.
     auto clear = [&](int i) {
         const int key0 = steps[f0 + i] * KEYS, key1 = key0 + KEYS - 1;
-        if (!holes && key1 < min(seq.length, p.most) && (!p.a.window || key0 > first - p.a.window || key1 < p.a.sinks)) return;
+        const bool lies = key1 <= last || (page_of(p, s, key0 / 16) >= 0 && page_of(p, s, key0 / 16 + 1) >= 0);
+        if (!holes && lies && key1 < min(seq.length, p.most) && (!p.a.window || key0 > first - p.a.window || key1 < p.a.sinks))
+            return;
         for (int u = 0; u < 2; u++) {
             const bool none = holes && page_of(p, s, key0 / 16 + u) < 0;
             for (int c = lane; c < 2 * HD; c += 64) {
