@@ -34,6 +34,7 @@ constexpr int kMostSplits = 32;
 static_assert(kMostSplits * kMostTop <= kListed, "the parts' tokens in LDS");
 constexpr int kPart = 4 + 2 * kMostTop;  // floats of a part in the workspace
 constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kFarthest = -1000.f;  // e to this power is 0 in float32: distances below it weigh nothing either
 
 struct Sums {
     float m = -INFINITY, s = 0.f, t = 0.f;
@@ -41,7 +42,9 @@ struct Sums {
     __device__ __forceinline__ void move(float to) {
         if (m == to) return;
         const float f = __builtin_amdgcn_exp2f((m - to) * kLog2e);
-        t = m == -INFINITY ? s * f : (t + s * (m - to)) * f;  // (nothing yet, but perhaps a NaN in s)
+        // (nothing yet, but perhaps a NaN in s; a reference of tokens masked by a large negative number is so far below that
+        // f is 0: bounded as in the sums, s times the distance stays a number)
+        t = m == -INFINITY ? s * f : (t + s * fmaxf(m - to, kFarthest)) * f;
         s *= f;
         m = to;
     }
@@ -277,7 +280,7 @@ __global__ __launch_bounds__(kThreads, 8) void logprobs_kernel(LogprobsArgs p) {
         for (int i = 0; i < K; i++) {
             const float d = y[i] - ref, e = __builtin_amdgcn_exp2f(d * kLog2e);
             sum.s += e;
-            sum.t = fmaf(e, fmaxf(d, -1000.f), sum.t);  // (a token masked by -inf adds 0)
+            sum.t = fmaf(e, fmaxf(d, kFarthest), sum.t);  // (a masked token adds 0)
         }
         return top;
     };
