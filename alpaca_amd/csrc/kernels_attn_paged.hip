@@ -495,7 +495,8 @@ struct Wide {
     static constexpr bool FITS = LDS <= 160 << 10;
 };
 // P enters the products as P 2^9 and a column's reference follows its maximum only when that is 2^6 past it, which
-// few steps are.
+// few steps are.  By their difference, exact for neighbouring numbers: m + 6 rounds to m + 8 where those are 4 or 8 apart, and
+// P would be past f16.
 constexpr float kWideLog2P = 9.f, kSlack = 6.f;
 // Parts of the steps: a part and the joining cost about 6 us, so that 600 positions (19 steps) stay whole: 18 us, in two 25.
 constexpr int kWideLeast = 16;  // steps of a part
@@ -659,12 +660,13 @@ __device__ __forceinline__ void wide_part(const AttnArgs& p, uint8_t* lds) {
     // The reference follows the scores to come, where they are past it.
     bool large = false;  // (a column's reference is: exponent_base has something to do)
     auto follow = [&](f32x16& x) {
+#pragma clang fp contract(off)  // (mn - m of the rounded mn, as exponent_base has it)
         float mx = x[0];
 #pragma unroll
         for (int e = 1; e < 16; e++) mx = fmaxf(mx, x[e]);
         mx = xor32_combine(mx, MaxOp());
         const float mn = mx * sc;  // (sc > 0)
-        if (__builtin_amdgcn_ballot_w64(mn > m + kSlack)) {
+        if (__builtin_amdgcn_ballot_w64(mn - m > kSlack)) {
             const float top = fmaxf(m, mn), alpha = __builtin_amdgcn_exp2f(m - (top == -INFINITY ? 0.f : top));
 #pragma unroll
             for (int d = 0; d < NB; d++) o[d] *= alpha;
@@ -729,7 +731,7 @@ __device__ __forceinline__ void wide_part(const AttnArgs& p, uint8_t* lds) {
             }
             if (k == at(2)) part[0] = fmaxf(fmaxf(fmaxf(part[0], part[1]), part[2]), fmaxf(fmaxf(part[3], part[4]), next[15]));
             if (k == at(3)) part[0] = xor32_combine(part[0], MaxOp());
-            if (k == at(4)) past = __builtin_amdgcn_ballot_w64(part[0] * sc > m + kSlack);
+            if (k == at(4)) past = __builtin_amdgcn_ballot_w64(part[0] * sc - m > kSlack);
             __builtin_amdgcn_sched_barrier(0);
         }
         if (__builtin_expect(!plain || large || past, 0)) {
