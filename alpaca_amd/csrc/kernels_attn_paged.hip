@@ -968,7 +968,8 @@ hipError_t launch_nb(AttnArgs& p, hipStream_t st) {
             return launch_mixed<NB, 4, 1, T>(p, st);
         if constexpr (two)
             if (groups(64) > cus) return launch_mixed<NB, 4, 2, T>(p, st);
-        if constexpr (NB <= 4)
+        // (heads of 32 cannot have 1.6 CUs of these units and no more than a CU of workgroups)
+        if constexpr (NB >= 2 && NB <= 4)
             if (10 * groups(64) * NB >= (NB >= 3 && p.most >= 2048 ? 11 : 16) * cus) return launch_mixed<NB, 2, 4, T>(p, st);
     }
     p.few_columns = INT32_MAX;

@@ -344,8 +344,8 @@ def test_attention_split_evenly_whatever_the_lengths(hip_ctx, sequences, kv_head
     attention_case(hip_ctx, 2 * kv_heads, kv_heads, 64, 32, [1] * sequences, lengths, dtype)
 
 
-# (heads, kv_heads, hd, page, new, lengths): chips full of workgroups of 256, 128 and 64 columns, with sequences of few
-# columns among them
+# (heads, kv_heads, hd, page, new, lengths): chips full of workgroups of 128 and 64 columns, with sequences of few
+# columns among them (tests/paged_shapes.py has shapes for every kernel, those of 256 columns too)
 WIDE = [(64, 64, 64, 16, [700, 1, 513], [700, 300, 600]), (96, 96, 32, 64, [300, 5, 410], [431, 6, 410]),
         (80, 80, 96, 32, [1, 900], [700, 901]), (64, 32, 128, 16, [550, 1, 2], [1100, 33, 64]),
         (64, 32, 128, 1024, [1100], [1100]), (32, 32, 64, 32, [512, 1, 1], [900, 44, 1000]),
