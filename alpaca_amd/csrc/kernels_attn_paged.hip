@@ -564,6 +564,9 @@ __device__ __forceinline__ void wide_part(const AttnArgs& p, uint8_t* lds) {
         if (steps.first_steps) missing(0, min(p.a.sinks - 1, min(last, p.most - 1)));
         holes = __builtin_amdgcn_ballot_w64(holes);
     }
+    // Whether the second tile of the step that `last` is in has none.  (Further steps are not run, and where `last` is in that
+    // tile itself the search above has found it.)
+    const bool behind = last >= 0 && page_of(p, s, (last / 16) | 1) < 0;
     // The set's steps i that are plain: all of i + 1 is seen by all columns of the wave, and all of i by one of the workgroup's.
     const int plain0 = holes ? INT32_MAX
                        : p.a.window ? steps.first_steps + (last >= p.a.window ? (last - p.a.window) / KEYS + 1 : 0) - steps.lo - f0
@@ -633,12 +636,12 @@ __device__ __forceinline__ void wide_part(const AttnArgs& p, uint8_t* lds) {
     };
     // Values of 0 at positions that no column of the workgroup sees, where they may never have been written, be another
     // sequence's or stand for a page that there is not: 0 times what lies there may be NaN.  (The waves of a set write the
-    // same.)  A step past `last`, where `holes` has not looked, is left as it is if all of it has pages and is the
-    // sequence's: cleared in any case, three chunks of 2,500 f32 tokens with windows took 193 us and not 187.
+    // same.)  Positions behind `last` that are the sequence's and have a page are left: cleared too, three chunks of 2,500
+    // f32 tokens with windows took 193 us and not 187.
     auto clear = [&](int i) {
         const int key0 = steps[f0 + i] * KEYS, key1 = key0 + KEYS - 1;
-        const bool lies = key1 <= last || (page_of(p, s, key0 / 16) >= 0 && page_of(p, s, key0 / 16 + 1) >= 0);
-        if (!holes && lies && key1 < min(seq.length, p.most) && (!p.a.window || key0 > first - p.a.window || key1 < p.a.sinks))
+        if (!holes && key1 < min(seq.length, p.most) && (!p.a.window || key0 > first - p.a.window || key1 < p.a.sinks) &&
+            !(behind && key1 > last))
             return;
         for (int u = 0; u < 2; u++) {
             const bool none = holes && page_of(p, s, key0 / 16 + u) < 0;
