@@ -496,7 +496,9 @@ struct Wide {
 };
 // P enters the products as P 2^9 and a column's reference follows its maximum only when that is 2^6 past it, which
 // few steps are.  By their difference, exact for neighbouring numbers: m + 6 rounds to m + 8 where those are 4 or 8 apart, and
-// P would be past f16.
+// P would be past f16.  In f16 P is one term, rounded by 2^-11 at most, here and in the few-column part (2^14 there): rows of
+// f16 are rounded by as much at the end, so that a prompt's error against 64 bits is 2.5e-4 of its norm where that rounding alone
+// is 2.1e-4; a second term is a second product for every value.
 constexpr float kWideLog2P = 9.f, kSlack = 6.f;
 // Parts of the steps: a part and the joining cost about 6 us, so that 600 positions (19 steps) stay whole: 18 us, in two 25.
 constexpr int kWideLeast = 16;  // steps of a part
@@ -943,11 +945,14 @@ hipError_t launch_mixed(AttnArgs& p, hipStream_t st) {
 // 32/32 heads of 64: 41 and 46; but 1,000 of 9/3 heads of 64: 39 and 33); from 1.1 where heads of 96 and more have tables of
 // 2,048 positions and more, whose steps are split (150 tokens at 4,096: 33, the few-column part 52, at 16,000 75 and 122;
 // 100 beside 31 single ones 68 and 83; but 140 at 600: 25 and 23, and of 32/32 heads of 64, where nothing is left to split,
-// 140 at 2,500: 28 and 23). 200 tokens at 4,096, in two parts: 39, in one 52. Where most workgroups are of sequences of few
+// 280 at 2,500: 28 and 23). 200 tokens at 4,096, in two parts: 39, in one 52. Where most workgroups are of sequences of few
 // columns, one set of 128 leaves them the most room (512 tokens of 32/32 heads of 64 and 31 single ones: 97, two sets 106,
 // 64 columns 125). One sequence's 256 columns, one workgroup a CU, where the short ones of their second round fill it behind
-// the long ones of the first (32/8 heads of 128, f16: 4,096 tokens 160 and 170, 3,500 126 and 132; but 3,000 104 and 98,
-// 5,000 256 and 242).
+// the long ones of the first (32/8 heads of 128, f16: 4,096 tokens 159 and 168, 3,500 122 and 127; but 3,000 104 and 98,
+// 5,000 256 and 242; 24/8 heads, 5,000 176 and 187). Far into a context, where all are alike long, it gains as much (4,096
+// behind 28,672 others 1,947 and 2,009, 3,500 behind 29,268 1,784 and 1,890, f32 4,096 3,065 and 3,100); at twice the prompt's
+// length little (4,096 of 8,192 419 and 424, f32 650 and 651), and of many KV heads it may lose there (3,800 of 7,600, 32/32
+// heads of 96, f16 330 and 317; 1,700 of 3,400, 64/64 of 128, f32 290 and 275).
 //
 // The few-column part alone: four waves a workgroup (one token of 9/3 heads of 64 at 2,000 positions 8.1, eight waves 8.6),
 // a workgroup a CU, or two where groups of columns are half as many (64 sequences of 32/8 heads of 128: 162 and 178; 24 at

@@ -489,7 +489,9 @@ int ahip_paged_kv_bytes(int kv_heads, int head_dim, int page_tokens, int pages, 
  * positions that are written belong to one row.
  *
  * max_rows says how many rows a sequence has at most, 0 if that is not known; it chooses
- * between kernels and changes no result beyond rounding.
+ * between kernels and changes no result beyond rounding.  A batch has up to 2^20 sequences (every
+ * workgroup looks through them for its own: up to a thousand cost little) and 2^26 rows, with up to
+ * 2^30 queries, and a table's row holds up to 2^30 tokens; more is refused.
  *
  * Row starts must not fall.  A row of a negative position (more rows than the length
  * says) stores nothing and sees nothing.  A position past the table's row, or in a page
@@ -553,8 +555,8 @@ int ahip_paged_attention(ahip_context* ctx, const ahip_paged_kv* cache, const ah
  * their softmax (NaN for a token outside the vocabulary), the entropy in nats, and the
  * `top` likeliest tokens (larger logits first, the lower index of equal ones, NaN behind every
  * number) with their log probabilities.  logprobs (with tokens), entropy or the top arrays (top 0) may be null.
- * A masked token's logit is -inf.  A row that holds a NaN or +inf, or nothing above -inf, has NaN for every
- * probability and entropy.  Sums are float32.
+ * A masked token's logit is -inf or a large negative number, the type's lowest too.  A row that holds a NaN or +inf, or nothing above -inf, has NaN for every
+ * probability and entropy.  Sums are float32.  Up to 2^24 - 1 rows of up to 2^30 logits.
  *
  * Queued on `stream` (null: the context stream) without waiting; allocates nothing.
  * `workspace` (16-byte aligned, ahip_token_logprobs_workspace bytes) lets few rows be split over
