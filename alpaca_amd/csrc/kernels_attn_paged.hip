@@ -476,7 +476,7 @@ __global__ __launch_bounds__(64 * kFewWaves) void paged_few_kernel(AttnArgs p) {
 // each for their pages.
 //
 // Bound by the two units that share a SIMD's issue.  4,096 f16 tokens of 32/8 heads of 128: 157-171 us on different cards,
-// 800-870 TFLOP/s (a library product of 8,192: 1,176), matrix unit 42% busy and vector unit 45% of the cycles, 7.4 vector
+// 800-870 TFLOP/s (a library product of 8,192: 1,176), matrix unit 41% busy and vector unit 44% of the cycles, 7.4 vector
 // instructions a matrix one, no bank conflicts; without its LDS reads it would take 0.93 of that, without its exponentials
 // 0.91, without its loads 0.85, with none of them 0.73.  float32 has two products for each of these (two f16 terms of the
 // queries, two of the probabilities): three chunks of 2,500 tokens with windows of 1,024, 24/8 heads of 128, 185-199 us, 78
